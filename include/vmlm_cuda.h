@@ -284,6 +284,99 @@ VMLM_API int vmlm_pool_find_slot(const vmlm_pool *pool, const char *name, size_t
  * on the pool's device slots: vmlm_op_gemm_dev with scale = slot dt when dt < n_slots. */
 VMLM_API int vmlm_pool_gemm(vmlm_pool *pool, const void *ins, void *stream);
 
+/* --------------------------------------- a 4-bit key/value cache for decode
+ * What a decode step needs between its q/k/v projections and its output
+ * projection, no reference counterpart: the norm and rotation of queries and
+ * keys, a cache that holds keys and values in 4 bits, attention over it, and
+ * eviction from it. Device pointers only (a cache lives on the device); all
+ * activations f32, in rows of heads * d values with a row stride ld (in
+ * values), so q, k and v may be slices of one projection's output. Rows whose
+ * pointer or stride is not a multiple of 16 bytes are read value by value.
+ * Lengths and positions are device arrays, so that a captured step can be
+ * replayed; what cannot be checked on the host is checked on the device and
+ * reported by vmlm_sync (VMLM_ERR_OPERATOR).
+ *
+ * A cache holds [n_seq][n_kv][cap] rows (slots) of d = 64, 128 or 256 values,
+ * keys and values alike: codes d/2 bytes (column p in byte p/2, the low nibble
+ * when p is even), and for every 32 columns two halves (step, base). A code c
+ * stands for half(step * (16 + c) + base). A group x of 32 columns becomes, in
+ * f32 operations rounded one by one, after |x| is clamped to 16384:
+ *   step = half((max - min) * (1/15)), base = half(min - 16 * step),
+ *   c = clamp(rint((x - base) * (1 / step)) - 16, 0, 15), or 0 where step = 0.
+ * A NaN makes its whole group NaN. Buffers belong to the caller (16-byte
+ * aligned): k and v n_seq * n_kv * cap * d/2 bytes, ks and vs
+ * n_seq * n_kv * cap * d/32 * 4 bytes. Slots at or behind a sequence's length
+ * are never read: they may hold anything. */
+typedef struct vmlm_kv4 {
+  void *k, *v;   /* codes */
+  void *ks, *vs; /* (step, base) */
+  size_t n_seq, n_kv, cap, d;
+} vmlm_kv4;
+
+/* The rotation of a head's first `rot` columns (a multiple of 16, at most d):
+ * (a, b) -> (a cos - b sin, b cos + a sin) on the pairs (i, i + rot/2), or
+ * (2i, 2i + 1) when interleaved != 0, with row pos[token] of the tables
+ * [n_pos][rot/2]. A position outside [0, n_pos) leaves the token's rows
+ * unwritten and is reported by vmlm_sync. */
+typedef struct vmlm_rope {
+  const float *cos_t, *sin_t;
+  const int32_t *pos;
+  size_t n_pos, rot;
+  int interleaved;
+} vmlm_rope;
+
+/* Queries and keys after their projections: for each head
+ * y = x * (1 / sqrt(sum(x^2) / d + eps)) * g (g = gq or gk, [d]; NULL: no
+ * norm), then the rotation (rope NULL: none). qo and ko may be q and k (same
+ * stride). n_q = 0 or n_kv = 0 leaves that part out. */
+VMLM_API int vmlm_qk_norm_rope_dev(const float *q, size_t ldq, const float *k, size_t ldk, const float *gq,
+                                   const float *gk, float eps, const vmlm_rope *rope, float *qo, size_t ldqo,
+                                   float *ko, size_t ldko, size_t tokens, size_t n_q, size_t n_kv, size_t d,
+                                   void *stream);
+
+/* The same for q (n_q = 0: none) and k, and the m new tokens of each sequence
+ * (rows b * m + t) written to slots len[b] + t in 4 bits, v as it is. len is
+ * not changed; len[b] < 0 marks an idle sequence, for which nothing is
+ * written to the cache. A slot behind cap is not written and is reported by
+ * vmlm_sync. */
+VMLM_API int vmlm_kv4_append_dev(const vmlm_kv4 *cache, const float *q, size_t ldq, float *qo, size_t ldqo,
+                                 size_t n_q, const float *k, size_t ldk, const float *v, size_t ldv, const float *gq,
+                                 const float *gk, float eps, const vmlm_rope *rope, const int32_t *len, size_t m,
+                                 void *stream);
+
+/* Values of `count` rows from slot start[b] of each sequence and kv head, as
+ * halves (bits): k, v [n_seq][n_kv][count][d], 16-byte aligned. Rows at or
+ * behind end[b] read as zeros; a row before end[b] outside the cache reads as
+ * zeros and is reported by vmlm_sync. */
+VMLM_API int vmlm_kv4_read_dev(const vmlm_kv4 *cache, const int32_t *start, const int32_t *end, size_t count,
+                               uint16_t *k, uint16_t *v, void *stream);
+
+/* Attention of the m newest tokens of each sequence (rows b * m + t of q and
+ * out, n_q heads, n_q / n_kv of them to a kv head): token t sees the slots
+ * j < len[b] - (m - 1 - t), len[b] counting the m tokens themselves.
+ *   out = sum_j p_j v_j, p = softmax(scale * q . k_j); no visible slot: zeros.
+ * With w_out ([n_seq][n_kv][cap]), the weight that each slot received is
+ * accumulated: w_out[j] = w_in[j] + the sum of p_j over the tokens and the kv
+ * head's query heads for j < len[b] (w_in counts as 0 for the m newest slots
+ * and where it is NULL; w_in and w_out may be the same). Other slots of w_out
+ * are not written. A len above cap is taken as cap and reported by vmlm_sync.
+ * Sums are f32; products with cached values are exact. */
+VMLM_API int vmlm_kv4_attn_dev(const vmlm_kv4 *cache, const float *q, size_t ldq, const int32_t *len, float *out,
+                               size_t ldo, size_t m, size_t n_q, float scale, const float *w_in, float *w_out,
+                               void *stream);
+
+/* Keep `keep` slots of each sequence and kv head and copy them, in slot order,
+ * to slots 0 .. of another cache with the same n_seq, n_kv and d: the first
+ * `first` and the last `recent` slots, and of the others those with the
+ * largest w ([n_seq][n_kv][cap]; of equal ones the lower slots, a NaN last). A
+ * sequence with len[b] <= keep keeps all. idx [n_seq][n_kv][keep] receives the
+ * kept slots (-1 behind them), w_out (may be NULL) their weights (0 behind
+ * them), len_out[b] = min(len[b], keep) (0 for a negative len). src is not
+ * changed. */
+VMLM_API int vmlm_kv4_evict_dev(const vmlm_kv4 *src, const vmlm_kv4 *dst, const float *w, const int32_t *len,
+                                size_t keep, size_t first, size_t recent, int32_t *idx, float *w_out,
+                                int32_t *len_out, void *stream);
+
 /* ------------------------------------------------- device-pointer GEMMs
  * Same arithmetic as the host entry points; pointers are device memory of the
  * current CUDA device; `stream` is a cudaStream_t. NULL selects the library's

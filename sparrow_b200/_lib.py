@@ -28,6 +28,19 @@ class Slot(ctypes.Structure):
 
 SP = ctypes.POINTER(Slot)
 
+
+class Kv4(ctypes.Structure):
+    """vmlm_kv4: a 4-bit key/value cache (device pointers)."""
+    _fields_ = [("k", P), ("v", P), ("ks", P), ("vs", P), ("n_seq", S), ("n_kv", S), ("cap", S), ("d", S)]
+
+
+class RopeTable(ctypes.Structure):
+    """vmlm_rope: cos / sin tables and the tokens' positions (device pointers)."""
+    _fields_ = [("cos_t", P), ("sin_t", P), ("pos", P), ("n_pos", S), ("rot", S), ("interleaved", I)]
+
+
+KP, RP, F = ctypes.POINTER(Kv4), ctypes.POINTER(RopeTable), ctypes.c_float
+
 # name -> (restype, argtypes); must list every symbol the header declares.
 SIGNATURES = {
     "vmlm_version": (I, []),
@@ -86,6 +99,11 @@ SIGNATURES = {
     "vmlm_gemm_nt_int8_outlier": (I, [P, P, P, P, P, S, P, S, S, S]),
     "vmlm_gemm_nt_int8_outlier_dev": (I, [P, P, P, P, I, P, S, P, S, S, S, P]),
     "vmlm_gather_columns_dev": (I, [P, P, S, S, S, P, P]),
+    "vmlm_qk_norm_rope_dev": (I, [P, S, P, S, P, P, F, RP, P, S, P, S, S, S, S, S, P]),
+    "vmlm_kv4_append_dev": (I, [KP, P, S, P, S, S, P, S, P, S, P, P, F, RP, P, S, P]),
+    "vmlm_kv4_read_dev": (I, [KP, P, P, S, P, P, P]),
+    "vmlm_kv4_attn_dev": (I, [KP, P, S, P, P, S, S, S, F, P, P, P]),
+    "vmlm_kv4_evict_dev": (I, [KP, KP, P, P, S, S, S, P, P, P, P]),
     "vmlm_op_gemm_dev": (I, [ctypes.c_uint, SP, SP, SP, SP, P]),
 }
 

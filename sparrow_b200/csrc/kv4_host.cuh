@@ -1,0 +1,251 @@
+// kv4_host.cuh -- host side of the 4-bit cache's entry points: argument checks,
+// kernel choice and launches. Included by vmlm_cuda.cu behind the contexts and
+// launch helpers.
+#pragma once
+
+namespace {
+
+constexpr size_t kKv4MaxDim = static_cast<size_t>(1) << 31;
+
+int kv4_check(const char* what, const vmlm_kv4* c) {
+  if (!c) return fail(VMLM_ERR_ARG, "%s: null cache", what);
+  if (c->d != 64 && c->d != 128 && c->d != 256)
+    return fail(VMLM_ERR_SHAPE, "%s: head size %zu (64, 128 and 256 are built)", what, c->d);
+  if (c->n_kv == 0) return fail(VMLM_ERR_ARG, "%s: no kv heads", what);
+  if (c->n_seq >= kKv4MaxDim || c->n_kv >= kKv4MaxDim || c->cap >= kKv4MaxDim ||
+      c->n_seq * c->n_kv >= kKv4MaxDim)
+    return fail(VMLM_ERR_SHAPE, "%s: n_seq * n_kv and cap must be < 2^31", what);
+  if (c->n_seq > 0 && c->cap > 0) {
+    if (!c->k || !c->v || !c->ks || !c->vs) return fail(VMLM_ERR_ARG, "%s: null pointer in the cache", what);
+    if (!aligned16(c->k) || !aligned16(c->v) || !aligned16(c->ks) || !aligned16(c->vs))
+      return fail(VMLM_ERR_ARG, "%s: the cache's buffers must start on a 16-byte boundary", what);
+  }
+  return VMLM_OK;
+}
+
+Kv4View kv4_view(const vmlm_kv4* c) {
+  Kv4View v;
+  v.k = static_cast<uint8_t*>(c->k);
+  v.v = static_cast<uint8_t*>(c->v);
+  v.ks = static_cast<uint32_t*>(c->ks);
+  v.vs = static_cast<uint32_t*>(c->vs);
+  v.cap = static_cast<long long>(c->cap);
+  v.n_seq = static_cast<int>(c->n_seq);
+  v.n_kv = static_cast<int>(c->n_kv);
+  return v;
+}
+
+// A [tokens] x [heads * d] activation argument with row stride ld.
+int kv4_check_rows(const char* what, const char* name, const float* x, size_t ld, size_t heads, size_t d) {
+  if (!x) return fail(VMLM_ERR_ARG, "%s: %s is null", what, name);
+  if (ld < heads * d) return fail(VMLM_ERR_ARG, "%s: row stride of %s is %zu, below %zu", what, name, ld, heads * d);
+  return VMLM_OK;
+}
+
+bool kv4_vec(const float* x, size_t ld) { return !x || (aligned16(x) && ld % 4 == 0); }
+
+bool kv4_overlap(const void* a, size_t na, const void* b, size_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return na > 0 && nb > 0 && x < y + nb && y < x + na;
+}
+
+int kv4_check_rope(const char* what, const vmlm_rope* r, size_t d) {
+  if (!r) return VMLM_OK;
+  if (!r->cos_t || !r->sin_t || !r->pos) return fail(VMLM_ERR_ARG, "%s: null pointer in the rotation", what);
+  if (r->rot == 0 || r->rot % 16 != 0 || r->rot > d)
+    return fail(VMLM_ERR_ARG, "%s: rot is %zu: a multiple of 16 up to %zu is wanted", what, r->rot, d);
+  if (r->n_pos == 0 || r->n_pos >= kKv4MaxDim) return fail(VMLM_ERR_ARG, "%s: n_pos is %zu", what, r->n_pos);
+  return VMLM_OK;
+}
+
+template <bool kCache>
+int kv4_launch_rows(Ctx* ctx, const Kv4Rows& p, const Kv4View& v, size_t d, cudaStream_t st) {
+  const long long rows = p.tokens * (p.n_q + p.n_kv + (kCache ? p.n_kv : 0));
+  if (rows == 0) return VMLM_OK;
+  if (cdiv(rows, 8) >= static_cast<long long>(kKv4MaxDim))
+    return fail(VMLM_ERR_SHAPE, "tokens x heads is too large (%lld rows)", rows);
+  const dim3 grid(static_cast<unsigned>(cdiv(rows, 8)));
+  if (d == 64) return launch(kv4_rows_kernel<64, kCache>, grid, dim3(256), 0, st, false, p, v, ctx->err);
+  if (d == 128) return launch(kv4_rows_kernel<128, kCache>, grid, dim3(256), 0, st, false, p, v, ctx->err);
+  return launch(kv4_rows_kernel<256, kCache>, grid, dim3(256), 0, st, false, p, v, ctx->err);
+}
+
+void kv4_set_rope(Kv4Rows* p, const vmlm_rope* r) {
+  if (!r) return;
+  p->cos_t = r->cos_t;
+  p->sin_t = r->sin_t;
+  p->pos = r->pos;
+  p->n_pos = static_cast<long long>(r->n_pos);
+  p->rot = static_cast<int>(r->rot);
+  p->interleaved = r->interleaved;
+}
+
+template <int D>
+int kv4_launch_attn(Ctx* ctx, Kv4Attn p, const Kv4View& v, cudaStream_t st) {
+  const long long rows = static_cast<long long>(v.n_seq) * p.m * p.n_q;
+  if (p.w_out) {
+    VMLM_TRY(ensure(ctx->kv4_lse, static_cast<size_t>(rows) * 4));
+    p.lse = static_cast<float*>(ctx->kv4_lse.p);
+  }
+  VMLM_TRY(launch(kv4_attn_kernel<D>, dim3(static_cast<unsigned>(cdiv(rows, 4))), dim3(128), 0, st, false, p, v,
+                  ctx->err));
+  if (!p.w_out || v.cap == 0) return VMLM_OK;
+  const long long slots = static_cast<long long>(v.n_seq) * v.n_kv * v.cap;
+  return launch(kv4_weights_kernel<D>, dim3(static_cast<unsigned>(cdiv(slots, 4))), dim3(128), 0, st, false, p, v);
+}
+
+}  // namespace
+
+extern "C" {
+
+int vmlm_qk_norm_rope_dev(const float* q, size_t ldq, const float* k, size_t ldk, const float* gq, const float* gk,
+                          float eps, const vmlm_rope* rope, float* qo, size_t ldqo, float* ko, size_t ldko,
+                          size_t tokens, size_t n_q, size_t n_kv, size_t d, void* stream) {
+  std::lock_guard<std::recursive_mutex> lk(g_mu);
+  const char* what = "qk_norm_rope_dev";
+  if (d != 64 && d != 128 && d != 256)
+    return fail(VMLM_ERR_SHAPE, "%s: head size %zu (64, 128 and 256 are built)", what, d);
+  if (tokens >= kKv4MaxDim || n_q >= 65536 || n_kv >= 65536)
+    return fail(VMLM_ERR_SHAPE, "%s: tokens must be < 2^31 and heads < 65536", what);
+  VMLM_TRY(kv4_check_rope(what, rope, d));
+  if (tokens == 0 || n_q + n_kv == 0) return VMLM_OK;
+  if (n_q > 0) {
+    VMLM_TRY(kv4_check_rows(what, "q", q, ldq, n_q, d));
+    VMLM_TRY(kv4_check_rows(what, "qo", qo, ldqo, n_q, d));
+  }
+  if (n_kv > 0) {
+    VMLM_TRY(kv4_check_rows(what, "k", k, ldk, n_kv, d));
+    VMLM_TRY(kv4_check_rows(what, "ko", ko, ldko, n_kv, d));
+  }
+  Ctx* ctx = nullptr;
+  VMLM_TRY(current_ctx(&ctx));
+  cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
+  Kv4Rows p = {};
+  p.q = q, p.k = k, p.qo = qo, p.ko = ko, p.gq = gq, p.gk = gk, p.eps = eps;
+  p.ldq = ldq, p.ldk = ldk, p.ldqo = ldqo, p.ldko = ldko;
+  p.tokens = tokens, p.m = tokens;
+  p.n_q = static_cast<int>(n_q), p.n_kv = static_cast<int>(n_kv);
+  kv4_set_rope(&p, rope);
+  p.vec = (n_q == 0 || (kv4_vec(q, ldq) && kv4_vec(qo, ldqo))) && (n_kv == 0 || (kv4_vec(k, ldk) && kv4_vec(ko, ldko)));
+  return kv4_launch_rows<false>(ctx, p, Kv4View{}, d, st);
+}
+
+int vmlm_kv4_append_dev(const vmlm_kv4* cache, const float* q, size_t ldq, float* qo, size_t ldqo, size_t n_q,
+                        const float* k, size_t ldk, const float* v, size_t ldv, const float* gq, const float* gk,
+                        float eps, const vmlm_rope* rope, const int32_t* len, size_t m, void* stream) {
+  std::lock_guard<std::recursive_mutex> lk(g_mu);
+  const char* what = "kv4_append_dev";
+  VMLM_TRY(kv4_check(what, cache));
+  VMLM_TRY(kv4_check_rope(what, rope, cache->d));
+  if (m >= kKv4MaxDim || cache->n_seq * m >= kKv4MaxDim || n_q >= 65536 || cache->n_kv >= 65536)
+    return fail(VMLM_ERR_SHAPE, "%s: tokens must be < 2^31 and heads < 65536", what);
+  if (m == 0 || cache->n_seq == 0) return VMLM_OK;
+  if (cache->cap == 0) return fail(VMLM_ERR_ARG, "%s: the cache has no slots", what);
+  if (!len) return fail(VMLM_ERR_ARG, "%s: len is null", what);
+  VMLM_TRY(kv4_check_rows(what, "k", k, ldk, cache->n_kv, cache->d));
+  VMLM_TRY(kv4_check_rows(what, "v", v, ldv, cache->n_kv, cache->d));
+  if (n_q > 0) {
+    VMLM_TRY(kv4_check_rows(what, "q", q, ldq, n_q, cache->d));
+    VMLM_TRY(kv4_check_rows(what, "qo", qo, ldqo, n_q, cache->d));
+  }
+  Ctx* ctx = nullptr;
+  VMLM_TRY(current_ctx(&ctx));
+  cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
+  Kv4Rows p = {};
+  p.q = q, p.k = k, p.v = v, p.qo = qo, p.gq = gq, p.gk = gk, p.eps = eps;
+  p.ldq = ldq, p.ldk = ldk, p.ldv = ldv, p.ldqo = ldqo;
+  p.tokens = cache->n_seq * m, p.m = m, p.len = len;
+  p.n_q = static_cast<int>(n_q), p.n_kv = static_cast<int>(cache->n_kv);
+  kv4_set_rope(&p, rope);
+  p.vec = (n_q == 0 || (kv4_vec(q, ldq) && kv4_vec(qo, ldqo))) && kv4_vec(k, ldk) && kv4_vec(v, ldv);
+  return kv4_launch_rows<true>(ctx, p, kv4_view(cache), cache->d, st);
+}
+
+int vmlm_kv4_read_dev(const vmlm_kv4* cache, const int32_t* start, const int32_t* end, size_t count, uint16_t* k,
+                      uint16_t* v, void* stream) {
+  std::lock_guard<std::recursive_mutex> lk(g_mu);
+  const char* what = "kv4_read_dev";
+  VMLM_TRY(kv4_check(what, cache));
+  if (count >= kKv4MaxDim) return fail(VMLM_ERR_SHAPE, "%s: count must be < 2^31", what);
+  if (count == 0 || cache->n_seq == 0) return VMLM_OK;
+  if (!start || !end || !k || !v) return fail(VMLM_ERR_ARG, "%s: null pointer", what);
+  if (!aligned16(k) || !aligned16(v)) return fail(VMLM_ERR_ARG, "%s: k and v must start on a 16-byte boundary", what);
+  Ctx* ctx = nullptr;
+  VMLM_TRY(current_ctx(&ctx));
+  cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
+  const Kv4View c = kv4_view(cache);
+  const long long work = static_cast<long long>(c.n_seq) * c.n_kv * static_cast<long long>(count) * (cache->d / 8) * 2;
+  const dim3 grid(static_cast<unsigned>(std::min<long long>(cdiv(work, 256), 1 << 30)));
+  const long long n = static_cast<long long>(count);
+  __half *ko = reinterpret_cast<__half*>(k), *vo = reinterpret_cast<__half*>(v);
+  if (cache->d == 64) return launch(kv4_read_kernel<64>, grid, dim3(256), 0, st, false, c, start, end, n, ko, vo, ctx->err);
+  if (cache->d == 128) return launch(kv4_read_kernel<128>, grid, dim3(256), 0, st, false, c, start, end, n, ko, vo, ctx->err);
+  return launch(kv4_read_kernel<256>, grid, dim3(256), 0, st, false, c, start, end, n, ko, vo, ctx->err);
+}
+
+int vmlm_kv4_attn_dev(const vmlm_kv4* cache, const float* q, size_t ldq, const int32_t* len, float* out, size_t ldo,
+                      size_t m, size_t n_q, float scale, const float* w_in, float* w_out, void* stream) {
+  std::lock_guard<std::recursive_mutex> lk(g_mu);
+  const char* what = "kv4_attn_dev";
+  VMLM_TRY(kv4_check(what, cache));
+  if (n_q % cache->n_kv != 0)
+    return fail(VMLM_ERR_SHAPE, "%s: %zu query heads do not share %zu kv heads evenly", what, n_q, cache->n_kv);
+  if (n_q >= 65536 || m >= kKv4MaxDim || cache->n_seq * m * n_q >= kKv4MaxDim)
+    return fail(VMLM_ERR_SHAPE, "%s: n_seq * m * n_q must be < 2^31 and n_q < 65536", what);
+  if (m == 0 || n_q == 0 || cache->n_seq == 0) return VMLM_OK;
+  if (!len) return fail(VMLM_ERR_ARG, "%s: len is null", what);
+  if (w_in && !w_out) return fail(VMLM_ERR_ARG, "%s: w_in without w_out", what);
+  VMLM_TRY(kv4_check_rows(what, "q", q, ldq, n_q, cache->d));
+  VMLM_TRY(kv4_check_rows(what, "out", out, ldo, n_q, cache->d));
+  Ctx* ctx = nullptr;
+  VMLM_TRY(current_ctx(&ctx));
+  cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
+  Kv4Attn p = {};
+  p.q = q, p.out = out, p.ldq = ldq, p.ldo = ldo, p.len = len, p.w_in = w_in, p.w_out = w_out;
+  p.scale2 = scale * 1.44269504088896340736f;
+  p.m = static_cast<int>(m), p.n_q = static_cast<int>(n_q);
+  const Kv4View v = kv4_view(cache);
+  if (cache->d == 64) return kv4_launch_attn<64>(ctx, p, v, st);
+  if (cache->d == 128) return kv4_launch_attn<128>(ctx, p, v, st);
+  return kv4_launch_attn<256>(ctx, p, v, st);
+}
+
+int vmlm_kv4_evict_dev(const vmlm_kv4* src, const vmlm_kv4* dst, const float* w, const int32_t* len, size_t keep,
+                       size_t first, size_t recent, int32_t* idx, float* w_out, int32_t* len_out, void* stream) {
+  std::lock_guard<std::recursive_mutex> lk(g_mu);
+  const char* what = "kv4_evict_dev";
+  VMLM_TRY(kv4_check(what, src));
+  VMLM_TRY(kv4_check(what, dst));
+  if (src->n_seq != dst->n_seq || src->n_kv != dst->n_kv || src->d != dst->d)
+    return fail(VMLM_ERR_SHAPE, "%s: the two caches differ in n_seq, n_kv or d", what);
+  if (keep > dst->cap) return fail(VMLM_ERR_SHAPE, "%s: keep is %zu, dst holds %zu slots", what, keep, dst->cap);
+  if (first > keep || recent > keep - first)
+    return fail(VMLM_ERR_ARG, "%s: first + recent is above keep (%zu + %zu, %zu)", what, first, recent, keep);
+  if (src->n_seq == 0) return VMLM_OK;
+  if (!len || !len_out || (keep > 0 && (!w || !idx))) return fail(VMLM_ERR_ARG, "%s: null pointer", what);
+  const size_t rows[2] = {src->n_seq * src->n_kv * src->cap, dst->n_seq * dst->n_kv * dst->cap};
+  const void* from[4] = {src->k, src->v, src->ks, src->vs};
+  const void* to[4] = {dst->k, dst->v, dst->ks, dst->vs};
+  for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < 4; ++j)
+      if (kv4_overlap(from[i], rows[0] * (i < 2 ? src->d / 2 : src->d / 8), to[j],
+                      rows[1] * (j < 2 ? src->d / 2 : src->d / 8)))
+        return fail(VMLM_ERR_ARG, "%s: src and dst overlap", what);
+  Ctx* ctx = nullptr;
+  VMLM_TRY(current_ctx(&ctx));
+  cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
+  const Kv4View s = kv4_view(src), d = kv4_view(dst);
+  VMLM_TRY(launch(kv4_select_kernel, dim3(static_cast<unsigned>(s.n_seq) * s.n_kv), dim3(kEvictThreads), 0, st, false,
+                  w, len, s.cap, s.n_kv, static_cast<int>(keep), static_cast<int>(first), static_cast<int>(recent),
+                  idx, w_out, len_out, ctx->err));
+  const long long work = static_cast<long long>(s.n_seq) * s.n_kv * static_cast<long long>(keep) * (src->d / 32) * 2;
+  if (work == 0) return VMLM_OK;
+  const dim3 grid(static_cast<unsigned>(std::min<long long>(cdiv(work, 256), 1 << 30)));
+  const int kp = static_cast<int>(keep);
+  const int32_t* ci = idx;
+  if (src->d == 64) return launch(kv4_move_kernel<64>, grid, dim3(256), 0, st, false, s, d, ci, kp);
+  if (src->d == 128) return launch(kv4_move_kernel<128>, grid, dim3(256), 0, st, false, s, d, ci, kp);
+  return launch(kv4_move_kernel<256>, grid, dim3(256), 0, st, false, s, d, ci, kp);
+}
+
+}  // extern "C"

@@ -19,6 +19,8 @@
 #include "probe.cuh"
 #include "decode.cuh"
 #include "decode_sk.cuh"
+#include "kv4.cuh"
+#include "kv4_attn.cuh"
 #include "tc2_gemm.cuh"
 #include "tc_gemm.cuh"
 #include "variants.cuh"
@@ -129,6 +131,7 @@ struct Ctx {
   int* err_host = nullptr;  // pinned copy read after host-API calls
   DevBuf h_a, h_c, h_w, h_s, h_acc, h_b, h_g;  // host-API staging
   DevBuf xn;  // RMSNorm-fused Q8 calls: the normalised activations [M][K]
+  DevBuf kv4_lse;     // attention over a 4-bit cache: log2 of each row's softmax denominator
   DevBuf grp_planes;  // grouped Q8 batches in planes mode: every problem's planes, exponents and flags
   // host-pointer calls pipelined by row chunks: copies in and out on streams of
   // their own, ordered against the compute stream by events
@@ -1805,6 +1808,8 @@ int run_outlier(Ctx* c, const float* a, const int8_t* q, const float* scale, con
 int device_error(int code) {
   if (code == kDevEmbRange) return fail(VMLM_ERR_OPERATOR, "EMB: row index out of range");
   if (code == kDevEmbFraction) return fail(VMLM_ERR_OPERATOR, "EMB: row index is not an integer");
+  if (code == kDevKv4Slot) return fail(VMLM_ERR_OPERATOR, "KV4: slot outside the cache");
+  if (code == kDevRopePos) return fail(VMLM_ERR_OPERATOR, "ROPE: position outside the table");
   if (code == kDevIdxRange) return fail(VMLM_ERR_ARG, "an outlier column index is >= k");
   return fail(VMLM_ERR_DEVICE_TIMEOUT, "a kernel gave up a bounded wait (device code %d)", code);
 }
@@ -2138,7 +2143,7 @@ int vmlm_shutdown(void) {
     for (DevBuf* b : {&c->act, &c->small, &c->slots, &c->counters, &c->shard_done, &c->sync, &c->norm_terms,
                       &c->norm_dirty, &c->norm_flags, &c->f32_ta, &c->f32_tb, &c->f32_da, &c->f32_db, &c->f32_nfa,
                       &c->f32_nfb, &c->f32_nft, &c->f32_flags, &c->h_a, &c->h_c, &c->h_w, &c->h_s, &c->h_acc, &c->h_b, &c->h_g, &c->xn,
-                      &c->grp_planes})
+                      &c->grp_planes, &c->kv4_lse})
       if (b->p) cudaFree(b->p);
     cudaFree(c->err);
     cudaFreeHost(c->err_host);
@@ -2906,6 +2911,8 @@ int vmlm_sync(void* stream) {
 }
 
 }  // extern "C"
+
+#include "kv4_host.cuh"
 
 // ====================================================== allocation-free Q8
 //

@@ -19,7 +19,7 @@ import ctypes
 
 import numpy as np
 
-from ._lib import Slot, check, lib
+from ._lib import Kv4, RopeTable, Slot, check, lib
 
 
 def _host_ptr(x, dtype, count, name):
@@ -412,6 +412,128 @@ def emb_dev(table, idx, out, stream=None) -> None:
     check(lib().vmlm_emb_dev(_dev_ptr(table, name, rows * cols, "table"), dt, rows, cols,
                              _dev_ptr(idx, "float32", m, "idx"), m, _dev_ptr(out, "float32", m * cols, "out"),
                              _stream_ptr(stream)))
+
+
+# ------------------------------------- a 4-bit key/value cache for decode
+
+def _rows_ptr(x, rows, width, name):
+    """(address, row stride) of a [rows, >= width] float32 CUDA tensor whose rows may be slices of wider ones."""
+    if str(x.dtype) != "torch.float32" or not x.is_cuda:
+        raise ValueError(f"{name}: expected a float32 CUDA tensor")
+    if x.dim() != 2 or x.shape[0] < rows or x.shape[1] < width or (x.shape[1] > 1 and x.stride(1) != 1):
+        raise ValueError(f"{name}: needs {rows} rows of {width} values with unit column stride, has {tuple(x.shape)}")
+    return x.data_ptr(), x.stride(0) if x.shape[0] > 1 else max(x.stride(0), x.shape[1])
+
+
+class Rope:
+    """The rotation of a head's first 2 * cos.shape[1] columns: cos, sin [n_pos, rot/2] float32, pos [tokens] int32
+    (vmlm_rope). `pos` may be set again for other tokens."""
+
+    def __init__(self, cos, sin, pos, interleaved=False):
+        n_pos, half = cos.shape
+        self._keep = [cos, sin, pos]
+        self.table = RopeTable(_dev_ptr(cos, "float32", n_pos * half, "cos"), _dev_ptr(sin, "float32", n_pos * half, "sin"),
+                               _dev_ptr(pos, "int32", 0, "pos"), n_pos, 2 * half, int(bool(interleaved)))
+        self.tokens = pos.numel()
+        self.ref = ctypes.byref(self.table)
+
+    def set_positions(self, pos) -> None:
+        self.table.pos = _dev_ptr(pos, "int32", 0, "pos")
+        self._keep[2], self.tokens = pos, pos.numel()
+
+
+class Kv4Cache:
+    """A 4-bit key/value cache over caller-owned CUDA tensors (vmlm_kv4): codes k, v uint8 [n_seq, n_kv, cap, d/2] and
+    ks, vs float16 [n_seq, n_kv, cap, d/32, 2] (step, base). `Kv4Cache.empty` allocates them."""
+
+    def __init__(self, k, v, ks, vs):
+        n_seq, n_kv, cap, half = k.shape
+        self.n_seq, self.n_kv, self.cap, self.d = n_seq, n_kv, cap, 2 * half
+        n = n_seq * n_kv * cap
+        if tuple(v.shape) != tuple(k.shape) or ks.numel() != n * half // 8 or vs.numel() != n * half // 8:
+            raise ValueError("Kv4Cache: k, v, ks and vs differ in shape")
+        self.k, self.v, self.ks, self.vs = k, v, ks, vs
+        self.struct = Kv4(_dev_ptr(k, "uint8", n * half, "k"), _dev_ptr(v, "uint8", n * half, "v"),
+                          _dev_ptr(ks, "float16", n * half // 8, "ks"), _dev_ptr(vs, "float16", n * half // 8, "vs"),
+                          n_seq, n_kv, cap, 2 * half)
+        self.ref = ctypes.byref(self.struct)
+
+    @classmethod
+    def empty(cls, n_seq, n_kv, cap, d, device="cuda"):
+        import torch
+        codes = [torch.empty((n_seq, n_kv, cap, d // 2), dtype=torch.uint8, device=device) for _ in range(2)]
+        sb = [torch.empty((n_seq, n_kv, cap, d // 32, 2), dtype=torch.float16, device=device) for _ in range(2)]
+        return cls(*codes, *sb)
+
+
+def _gain_ptr(g, d, name):
+    return None if g is None else _dev_ptr(g, "float32", d, name)
+
+
+def _rope_ref(rope, tokens):
+    if rope is None:
+        return None
+    if rope.tokens < tokens:
+        raise ValueError(f"rope: {rope.tokens} positions for {tokens} tokens")
+    return rope.ref
+
+
+def qk_norm_rope_dev(q, k, gq, gk, eps, rope, qo, ko, tokens, n_q, n_kv, d, stream=None) -> None:
+    """RMSNorm of each query and key head (gains gq, gk [d] or None) and the rotation (rope or None), in one pass: q, qo
+    [tokens, n_q * d], k, ko [tokens, n_kv * d], rows may be slices of wider ones."""
+    pq, ldq = _rows_ptr(q, tokens, n_q * d, "q") if n_q else (None, 0)
+    pqo, ldqo = _rows_ptr(qo, tokens, n_q * d, "qo") if n_q else (None, 0)
+    pk, ldk = _rows_ptr(k, tokens, n_kv * d, "k") if n_kv else (None, 0)
+    pko, ldko = _rows_ptr(ko, tokens, n_kv * d, "ko") if n_kv else (None, 0)
+    check(lib().vmlm_qk_norm_rope_dev(pq, ldq, pk, ldk, _gain_ptr(gq, d, "gq"), _gain_ptr(gk, d, "gk"), eps,
+                                      _rope_ref(rope, tokens), pqo, ldqo, pko, ldko, tokens, n_q, n_kv, d,
+                                      _stream_ptr(stream)))
+
+
+def kv4_append_dev(cache, k, v, length, m, q=None, qo=None, n_q=0, gq=None, gk=None, eps=0.0, rope=None,
+                   stream=None) -> None:
+    """Write the m new tokens of each sequence (rows b * m + t of k and v) to slots length[b] + t in 4 bits, the keys
+    normalised and rotated where gk and rope are given, and the queries with them (q -> qo)."""
+    tokens, d = cache.n_seq * m, cache.d
+    pk, ldk = _rows_ptr(k, tokens, cache.n_kv * d, "k")
+    pv, ldv = _rows_ptr(v, tokens, cache.n_kv * d, "v")
+    pq, ldq = _rows_ptr(q, tokens, n_q * d, "q") if n_q else (None, 0)
+    pqo, ldqo = _rows_ptr(qo, tokens, n_q * d, "qo") if n_q else (None, 0)
+    check(lib().vmlm_kv4_append_dev(cache.ref, pq, ldq, pqo, ldqo, n_q, pk, ldk, pv, ldv, _gain_ptr(gq, d, "gq"),
+                                    _gain_ptr(gk, d, "gk"), eps, _rope_ref(rope, tokens),
+                                    _dev_ptr(length, "int32", cache.n_seq, "length"), m, _stream_ptr(stream)))
+
+
+def kv4_read_dev(cache, start, end, count, k, v, stream=None) -> None:
+    """Rows start[b] .. start[b] + count - 1 of each sequence and kv head as the values they stand for: k, v float16
+    [n_seq, n_kv, count, d]; rows at or behind end[b] are zeros."""
+    n = cache.n_seq * cache.n_kv * count * cache.d
+    check(lib().vmlm_kv4_read_dev(cache.ref, _dev_ptr(start, "int32", cache.n_seq, "start"),
+                                  _dev_ptr(end, "int32", cache.n_seq, "end"), count, _dev_ptr(k, "float16", n, "k"),
+                                  _dev_ptr(v, "float16", n, "v"), _stream_ptr(stream)))
+
+
+def kv4_attn_dev(cache, q, length, out, m, n_q, scale, w_in=None, w_out=None, stream=None) -> None:
+    """Attention of the m newest tokens of each sequence (rows b * m + t of q and out) over the cache; length[b] counts
+    them. w_out [n_seq, n_kv, cap] receives w_in plus the weight that each slot got."""
+    tokens, width = cache.n_seq * m, n_q * cache.d
+    pq, ldq = _rows_ptr(q, tokens, width, "q")
+    po, ldo = _rows_ptr(out, tokens, width, "out")
+    slots = cache.n_seq * cache.n_kv * cache.cap
+    check(lib().vmlm_kv4_attn_dev(cache.ref, pq, ldq, _dev_ptr(length, "int32", cache.n_seq, "length"), po, ldo, m, n_q,
+                                  scale, _dev_ptr(w_in, "float32", slots, "w_in"),
+                                  _dev_ptr(w_out, "float32", slots, "w_out"), _stream_ptr(stream)))
+
+
+def kv4_evict_dev(src, dst, w, length, keep, first, recent, idx, w_out, len_out, stream=None) -> None:
+    """Copy the `keep` slots of each sequence and kv head with the most weight w [n_seq, n_kv, src.cap] (the first `first`
+    and the last `recent` always among them) from src to dst, in slot order; idx, w_out [n_seq, n_kv, keep] and len_out
+    [n_seq] say which they are. w_out may be None."""
+    out = src.n_seq * src.n_kv * keep
+    check(lib().vmlm_kv4_evict_dev(src.ref, dst.ref, _dev_ptr(w, "float32", src.n_seq * src.n_kv * src.cap, "w"),
+                                   _dev_ptr(length, "int32", src.n_seq, "length"), keep, first, recent,
+                                   _dev_ptr(idx, "int32", out, "idx"), _dev_ptr(w_out, "float32", out, "w_out"),
+                                   _dev_ptr(len_out, "int32", src.n_seq, "len_out"), _stream_ptr(stream)))
 
 
 # ------------------------------------------------------ the OP_GEMM operator
