@@ -80,18 +80,45 @@ void kv4_set_rope(Kv4Rows* p, const vmlm_rope* r) {
   p->interleaved = r->interleaved;
 }
 
-template <int D>
+template <int D, int NT, bool kW>
 int kv4_launch_attn(Ctx* ctx, Kv4Attn p, const Kv4View& v, cudaStream_t st) {
-  const long long rows = static_cast<long long>(v.n_seq) * p.m * p.n_q;
-  if (p.w_out) {
-    VMLM_TRY(ensure(ctx->kv4_lse, static_cast<size_t>(rows) * 4));
-    p.lse = static_cast<float*>(ctx->kv4_lse.p);
+  constexpr int kSmem = attn_smem_bytes(D, NT);
+  static bool set[64] = {};
+  if (ctx->dev < 64 && !set[ctx->dev]) {
+    VMLM_CUDA(cudaFuncSetAttribute(kv4_attn_kernel<D, NT, kW>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    set[ctx->dev] = true;
   }
-  VMLM_TRY(launch(kv4_attn_kernel<D>, dim3(static_cast<unsigned>(cdiv(rows, 4))), dim3(128), 0, st, false, p, v,
-                  ctx->err));
-  if (!p.w_out || v.cap == 0) return VMLM_OK;
-  const long long slots = static_cast<long long>(v.n_seq) * v.n_kv * v.cap;
-  return launch(kv4_weights_kernel<D>, dim3(static_cast<unsigned>(cdiv(slots, 4))), dim3(128), 0, st, false, p, v);
+  const size_t heads = static_cast<size_t>(v.n_seq) * v.n_kv;
+  p.chunks = static_cast<int>(cdiv(p.rows, 4 * NT));
+  const int grid = 2 * ctx->sms;
+  VMLM_TRY(ensure(ctx->kv4_part, static_cast<size_t>(grid) * 2 * 4 * NT * (D + 2) * 4));
+  VMLM_TRY(ensure_zeroed(ctx->kv4_arrived, heads * p.chunks * 4, st));
+  p.part = static_cast<float*>(ctx->kv4_part.p);
+  p.arrived = static_cast<int*>(ctx->kv4_arrived.p);
+  p.min_units = D == 64 ? 8 : D == 128 ? 4 : 2;
+  if (kW) {
+    VMLM_TRY(ensure(ctx->kv4_lse, heads * p.rows * 4));
+    VMLM_TRY(ensure(ctx->kv4_score, heads * p.rows * static_cast<size_t>(v.cap) * 4));
+    p.lse = static_cast<float*>(ctx->kv4_lse.p);
+    p.score = static_cast<float*>(ctx->kv4_score.p);
+  }
+  VMLM_TRY(launch(kv4_attn_kernel<D, NT, kW>, dim3(grid), dim3(kAttnWarps * 32), kSmem, st, false, p, v, ctx->err));
+  if (!kW || v.cap == 0) return VMLM_OK;
+  if (heads >= 65536) return fail(VMLM_ERR_SHAPE, "kv4_attn_dev: n_seq * n_kv must be < 65536 with w_out");
+  return launch(kv4_weights_kernel, dim3(static_cast<unsigned>(cdiv(v.cap, 256)), static_cast<unsigned>(heads)), dim3(256),
+                0, st, false, p, v);
+}
+
+// Rows of a chunk: 4 where that holds them all, else 8, or (d = 64) 16. A chunk's
+// rows share the unpacked values; more than 256 / d * 4 do not fit the registers.
+template <int D, bool kW>
+int kv4_pick_attn(Ctx* ctx, const Kv4Attn& p, const Kv4View& v, cudaStream_t st) {
+  if (p.rows <= 4 || D == 256) return kv4_launch_attn<D, 1, kW>(ctx, p, v, st);
+  if constexpr (D != 256) {
+    if (p.rows <= 8 || D == 128) return kv4_launch_attn<D, 2, kW>(ctx, p, v, st);
+    if constexpr (D == 64) return kv4_launch_attn<D, 4, kW>(ctx, p, v, st);
+  }
+  return VMLM_OK;
 }
 
 }  // namespace
@@ -204,10 +231,13 @@ int vmlm_kv4_attn_dev(const vmlm_kv4* cache, const float* q, size_t ldq, const i
   p.q = q, p.out = out, p.ldq = ldq, p.ldo = ldo, p.len = len, p.w_in = w_in, p.w_out = w_out;
   p.scale2 = scale * 1.44269504088896340736f;
   p.m = static_cast<int>(m), p.n_q = static_cast<int>(n_q);
+  p.group = static_cast<int>(n_q / cache->n_kv);
+  p.rows = p.m * p.group;
+  p.vec = kv4_vec(q, ldq);
   const Kv4View v = kv4_view(cache);
-  if (cache->d == 64) return kv4_launch_attn<64>(ctx, p, v, st);
-  if (cache->d == 128) return kv4_launch_attn<128>(ctx, p, v, st);
-  return kv4_launch_attn<256>(ctx, p, v, st);
+  if (cache->d == 64) return w_out ? kv4_pick_attn<64, true>(ctx, p, v, st) : kv4_pick_attn<64, false>(ctx, p, v, st);
+  if (cache->d == 128) return w_out ? kv4_pick_attn<128, true>(ctx, p, v, st) : kv4_pick_attn<128, false>(ctx, p, v, st);
+  return w_out ? kv4_pick_attn<256, true>(ctx, p, v, st) : kv4_pick_attn<256, false>(ctx, p, v, st);
 }
 
 int vmlm_kv4_evict_dev(const vmlm_kv4* src, const vmlm_kv4* dst, const float* w, const int32_t* len, size_t keep,
