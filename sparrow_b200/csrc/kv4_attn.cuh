@@ -42,24 +42,30 @@ struct Kv4Attn {
   int* arrived;       // [n_seq][n_kv][chunks]: partial results written, zero between calls
   float scale2;       // scale * log2(e)
   int m, n_q, group, rows, chunks;  // rows = m * group query rows a kv head, in chunks
-  int min_units;      // work of a CTA, in units of kAttnUnit slots, below which fewer CTAs are used
   int vec;            // q rows start on 16-byte boundaries
+  uint32_t mul4, mul64;  // 4 and 64, as values that the compiler does not know: see kv4_pair
 };
 
-constexpr int kAttnWarps = 8;
-constexpr int kAttnUnit = 64;            // slots: the grain in which work is shared out
 constexpr int kAttnStageBytes = 5120;    // 4096 values of K and of V with their steps and bases
-constexpr float kAttnShift = 14.f;       // weights are held as 2^14 times their value, so that their halves keep 2^-25 of 2^-14
+constexpr float kAttnShift = 14.f;       // weights are held as 2^14 times their value: their halves keep 2^-39 of the largest
 constexpr float kAttnSlack = 1.f;        // a running maximum may lag by this (log2): 2^15 is still a half
+constexpr int kAttnAlone = 4;            // tiles a warp up to which a CTA takes an item alone
 
-// Dynamic shared memory: the warps' rings, then the merge buffer.
-__host__ __device__ constexpr int attn_merge_floats(int D, int NT) {
-  return kAttnWarps * NT * 4 * (NT * D > 128 ? D / 2 : D);
-}
+// Warps of the one CTA on an SM. A chunk of rows takes D/8 registers a four rows
+// for its queries and as many for its output; 256 values of d x fours fit 168
+// registers (12 warps), 128 fit 128 (16 warps).
+__host__ __device__ constexpr int attn_warps(int D, int NT) { return NT * D > 128 ? 12 : 16; }
+// Dynamic shared memory: the warps' rings, a partial result and two (m, l) lists a warp.
 __host__ __device__ constexpr int attn_smem_bytes(int D, int NT) {
-  return kAttnWarps * 2 * kAttnStageBytes + attn_merge_floats(D, NT) * 4 + kAttnWarps * NT * 4 * 8;
+  return attn_warps(D, NT) * (2 * kAttnStageBytes + 4 * NT * D * 4 + 2 * 4 * NT * 8);
 }
 
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async8(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
   const int n = on ? 16 : 0;  // 0: the destination is filled with zeros
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
@@ -81,6 +87,14 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// The same with a zero accumulator: no registers to clear.
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -94,15 +108,15 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
 __device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
 
-// Nibble I (0..3) of both 16-bit halves of u as the halves of their values.
-template <int I>
-__device__ __forceinline__ uint32_t kv4_pair(uint32_t u, __half2 step, __half2 base) {
-  const uint32_t t = I == 0 ? u << 6 : I == 1 ? u << 2 : I == 2 ? u >> 2 : u >> 6;
-  return h2_bits(__hfma2(bits_h2((t & 0x03C003C0u) | 0x4C004C00u), step, base));
-}
-__device__ __forceinline__ uint32_t kv4_pair_at(int i, uint32_t u, __half2 step, __half2 base) {
-  return i == 0 ? kv4_pair<0>(u, step, base) : i == 1 ? kv4_pair<1>(u, step, base)
-       : i == 2 ? kv4_pair<2>(u, step, base) : kv4_pair<3>(u, step, base);
+// The low (kHigh = false) or high nibbles of bits 0..7 of both halves of u as the halves of their values. The mask keeps
+// the nibble where it is and a multiply-add moves it to the mantissa's top and puts 16.0 under it: one LOP3 and two
+// operations of the FMA pipe for two values. With a shift and a LOP3 instead, three of four operations are the ALU
+// pipe's, and it was the first to fill up (58% busy at 131071 slots, 32/8 heads of 128, where the FMA pipe had 20%).
+// The factors come from the caller: a constant power of two would be turned into a shift on the ALU pipe.
+template <bool kHigh>
+__device__ __forceinline__ uint32_t kv4_pair(uint32_t u, uint32_t mul, __half2 step, __half2 base) {
+  const uint32_t t = (u & (kHigh ? 0x00F000F0u : 0x000F000Fu)) * mul + 0x4C004C00u;  // mul: 4 (high) or 64
+  return h2_bits(__hfma2(bits_h2(t), step, base));
 }
 
 // Where a slot's 16-byte chunk c of codes lies in its row in shared memory: the
@@ -115,59 +129,121 @@ __device__ __forceinline__ int attn_swizzle(int slot, int c) {
   return c;
 }
 
-// A run of slots [s0, s1) of one item (sequence, kv head, chunk of rows).
-struct AttnSeg {
+// The work is the tiles of TS = 4096 / d slots of every item (sequence, kv head,
+// chunk of rows), in that order, in equal contiguous shares for the CTAs and,
+// within a CTA, for its warps, whatever the lengths are: a warp's share is a few
+// runs, each a part of an item or all of it. Few and short items (one a CTA, at
+// most kAttnAlone tiles a warp) get a CTA each instead: joining the parts of an
+// item across CTAs costs about 4 us, which such a call does not otherwise last.
+struct AttnRun {
   int b, hc;          // sequence, kv head * chunks + chunk
-  int s0, s1, n;      // n: the sequence's length
-  long long first;    // the item's first unit
-  int units;          // the item's units
-  bool whole;         // the run is the whole item
+  int head, r0;       // kv head, the chunk's first row
+  int s0, s1, n;      // slots [s0, s1) of the n of the sequence
+  int first, units;   // the item's first tile among all, and its number of tiles
+  bool enter, leave;  // the item has tiles before, behind this run
 };
 
-// Walks the runs of one CTA: units [pos, end) of all items in order of
-// sequence, kv head and chunk. Every warp walks alone and sees the same.
+template <int TS>
 struct AttnWalk {
   const int32_t* len;
-  int n_seq, hc_count;
-  long long cap, pos, end, base;  // base: the first unit of sequence b
+  int n_seq, hc_count, chunks, chunk_rows;
+  long long cap;
+  int pos, end, base;  // tiles [pos, end); base: the first tile of sequence b
   int b;
 
   __device__ __forceinline__ int length(int i) const {
     const long long n = __ldg(len + i);
     return static_cast<int>(n > cap ? cap : n < 0 ? 0 : n);
   }
-  __device__ __forceinline__ bool next(AttnSeg& s) {
+  __device__ __forceinline__ int tiles(int i) const { return (length(i) + TS - 1) / TS; }
+  // Moves (b, base) to the sequence that holds tile `at`; with kItems, to the one that holds the at-th item.
+  template <bool kItems>
+  __device__ __forceinline__ int seek(int at) {
+    const int lane = threadIdx.x & 31;
+    int before = 0, tile = 0;
+    #pragma unroll 1
+    for (int i0 = 0; i0 < n_seq; i0 += 32) {
+      const int t = i0 + lane < n_seq ? tiles(i0 + lane) * hc_count : 0;
+      const int w = kItems ? (t > 0 ? hc_count : 0) : t;
+      int sum = w, sum_t = t;
+      #pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, sum, o), y = __shfl_up_sync(0xffffffffu, sum_t, o);
+        if (lane >= o) sum += x, sum_t += y;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, before + sum > at);
+      if (past) {
+        const int l = __ffs(past) - 1;
+        b = i0 + l;
+        base = tile + __shfl_sync(0xffffffffu, sum_t - t, l);
+        return before + __shfl_sync(0xffffffffu, sum - w, l);
+      }
+      before += __shfl_sync(0xffffffffu, sum, 31);
+      tile += __shfl_sync(0xffffffffu, sum_t, 31);
+    }
+    return before;
+  }
+  __device__ __forceinline__ bool next(AttnRun& s) {
     if (pos >= end) return false;
     int n, u;
     while (true) {
       n = length(b);
-      u = (n + kAttnUnit - 1) / kAttnUnit;
-      const long long all = static_cast<long long>(u) * hc_count;
-      if (pos < base + all) break;
-      base += all;
+      u = (n + TS - 1) / TS;
+      if (pos < base + u * hc_count) break;
+      base += u * hc_count;
       ++b;
     }
-    const long long at = pos - base;
+    const int at = pos - base;
     s.b = b;
-    s.hc = static_cast<int>(at / u);
-    const int off = static_cast<int>(at - static_cast<long long>(s.hc) * u);
-    const long long left = end - pos;
-    const int take = static_cast<int>(left < u - off ? left : u - off);
+    s.hc = hc_count == 1 ? 0 : at / u;
+    s.head = chunks == 1 ? s.hc : s.hc / chunks;
+    s.r0 = (s.hc - s.head * chunks) * chunk_rows;
+    const int off = at - s.hc * u, take = min(end - pos, u - off);
     s.n = n;
-    s.s0 = off * kAttnUnit;
-    s.s1 = min(n, (off + take) * kAttnUnit);
+    s.s0 = off * TS;
+    s.s1 = min(n, (off + take) * TS);
     s.first = pos - off;
     s.units = u;
-    s.whole = take == u;
+    s.enter = off > 0;
+    s.leave = off + take < u;
     pos += take;
     return true;
   }
 };
 
+// The output's fragments: element x of a chunk is tile x / (64 NT), half, four of rows, lane (gid, row of the four).
+// Its column:
+template <int D, int NT>
+__device__ __forceinline__ int attn_col(int x) {
+  const int g = (x & 31) >> 2, h = x / (32 * NT) & 1, ti = x / (64 * NT);
+  if constexpr (D == 64) return 8 * g + 4 * h + ti;
+  return 8 * (g * (D / 64) + ti / 8 * 2 + h) + ti % 8;
+}
+template <int NT>
+__device__ __forceinline__ int attn_row(int x) { return x / 32 % NT * 4 + (x & 3); }
+// Where a column lies: tile, half, lane group.
+template <int D>
+__device__ __forceinline__ void attn_place(int col, int& ti, int& h, int& g) {
+  if constexpr (D == 64) {
+    g = col >> 3, h = (col >> 2) & 1, ti = col & 3;
+  } else {
+    constexpr int VW = D / 64;
+    const int w = col >> 3, in = w % VW;
+    g = w / VW, h = in & 1, ti = in / 2 * 8 + (col & 7);
+  }
+}
+
+// (m, l, v) joined with another part's: the larger maximum, scaled sums.
+__device__ __forceinline__ void attn_join(float& m, float& l, float& v, float pm, float pl, float pv) {
+  const float mm = fmaxf(m, pm), f = ex2(m - mm), fp = ex2(pm - mm);
+  l = fmaf(l, f, pl * fp), v = fmaf(v, f, pv * fp), m = mm;
+}
+
 // D: head size. NT: chunks hold 4 * NT rows. kW: scores are kept for w_out.
 template <int D, int NT, bool kW>
-__global__ void __launch_bounds__(kAttnWarps * 32, 2) kv4_attn_kernel(const Kv4Attn p, const Kv4View c,
-                                                                       int* __restrict__ err) {
+__global__ void __launch_bounds__(attn_warps(D, NT) * 32, 1) kv4_attn_kernel(const Kv4Attn p, const Kv4View c,
+                                                                             int* __restrict__ err) {
+  constexpr int kWarps = attn_warps(D, NT), kThreads = kWarps * 32;
   constexpr int TS = 4096 / D;      // slots of a tile
   constexpr int ST = TS / 16;       // its 16-slot steps
   constexpr int KW = D / 32;        // code words of a K row that a lane takes
@@ -175,108 +251,166 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 2) kv4_attn_kernel(const Kv4A
   constexpr int RC = 4 * NT;        // rows of a chunk
   constexpr int OT = D / 16;        // 16-column tiles of the output
   constexpr int kCh = D / 32;       // 16-byte chunks of a row of codes
-  constexpr int kHalves = NT * D > 128 ? 2 : 1;  // the merge buffer holds this part of the output at a time
+  constexpr int kPart = RC * (D + 2);
   extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ float s_mul[RC][2 * kWarps];  // the factors of the parts that are joined, and where they lie
+  __shared__ int s_at[2 * kWarps];
+  // Parts of items that the warps leave for each other, in the order of the work: 2 w of warp w is the end of an item
+  // that other warps began, 2 w + 1 the beginning of one that others end.
+  __shared__ int s_state[2 * kWarps];  // 0: none, 1: the item ends here, 2: it goes on
+  __shared__ int s_from[2 * kWarps];   // the output part: bytes into smem
+  __shared__ AttnRun s_run[2 * kWarps], s_part[2];
+  __shared__ int s_last[2], s_c0[2], s_parts;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int gid = lane >> 2, tig = lane & 3;
   unsigned char* ring = smem + warp * 2 * kAttnStageBytes;
-  float* merge = reinterpret_cast<float*>(smem + kAttnWarps * 2 * kAttnStageBytes);
-  float* ml = merge + attn_merge_floats(D, NT);  // [warp][row][m, l]
-  __shared__ int s_last;
+  float* heads = reinterpret_cast<float*>(smem + kWarps * 2 * kAttnStageBytes);  // [warp][RC * D]
+  float* ml = heads + kWarps * RC * D;                                           // [warp][head, tail][row][m, l]
 
-  // All units, and this CTA's share of them.
-  AttnWalk walk;
+  // All tiles, this CTA's share of them, and this warp's share of those.
+  AttnWalk<TS> walk;
   walk.len = p.len, walk.n_seq = c.n_seq, walk.hc_count = c.n_kv * p.chunks, walk.cap = c.cap;
-  long long units = 0;
+  walk.chunks = p.chunks, walk.chunk_rows = RC;
+  int units = 0, longest = 0, used = 0;
+  #pragma unroll 1
   for (int i = lane; i < c.n_seq; i += 32) {
     if (__ldg(p.len + i) > c.cap && tid == lane) atomicCAS(err, 0, kDevKv4Slot);
-    units += (walk.length(i) + kAttnUnit - 1) / kAttnUnit;
+    const int u = walk.tiles(i);
+    units += u, longest = max(longest, u), used += u > 0;
   }
-  #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) units += __shfl_xor_sync(0xffffffffu, units, o);
-  units *= walk.hc_count;
-  const long long want = units / p.min_units;
-  const int ctas = static_cast<int>(want < 1 ? 1 : want < gridDim.x ? want : gridDim.x);
-  const int cta = blockIdx.x;
+  units = __reduce_add_sync(0xffffffffu, units) * walk.hc_count;
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  used = __reduce_add_sync(0xffffffffu, used) * walk.hc_count;
+  const int cta = blockIdx.x, grid = gridDim.x;
+  const bool alone = used <= grid && longest <= kWarps * kAttnAlone;
+  const int ctas = alone ? used : max(1, min(grid, units / kWarps));
+  const int each = units / max(1, ctas), extra = units - each * ctas;  // the first `extra` CTAs have one tile more
 
   // Sequences without a slot: zeros.
-  for (int i = cta; i < c.n_seq; i += gridDim.x) {
+  #pragma unroll 1
+  for (int i = cta; i < c.n_seq; i += grid) {
     if (walk.length(i) > 0) continue;
-    for (long long x = tid; x < static_cast<long long>(p.m) * p.n_q * D; x += kAttnWarps * 32) {
+    #pragma unroll 1
+    for (long long x = tid; x < static_cast<long long>(p.m) * p.n_q * D; x += kThreads) {
       const long long t = x / (p.n_q * D);
       p.out[(static_cast<long long>(i) * p.m + t) * p.ldo + (x - t * p.n_q * D)] = 0.f;
     }
   }
   if (cta >= ctas) return;
-  walk.pos = units * cta / ctas;
-  walk.end = units * (cta + 1) / ctas;
-  walk.b = 0, walk.base = 0;
+  int lo, hi;
+  if (alone) {
+    const int before = walk.template seek<true>(cta);
+    const int u = walk.tiles(walk.b);
+    lo = walk.base + (cta - before) * u, hi = lo + u;
+  } else {
+    lo = cta * each + min(cta, extra), hi = lo + each + (cta < extra);
+  }
+  walk.pos = lo + (hi - lo) * warp / kWarps;
+  walk.end = lo + (hi - lo) * (warp + 1) / kWarps;
+  if (!alone) walk.template seek<false>(walk.pos);
 
-  // The part of a run that this warp takes, and its first tile's loads.
-  auto share = [&](const AttnSeg& s, int& w0, int& w1) {
-    const int per = ((s.s1 - s.s0 + kAttnWarps - 1) / kAttnWarps + 15) & ~15;
-    w0 = min(s.s1, s.s0 + warp * per);
-    w1 = min(s.s1, w0 + per);
-  };
-  auto fetch = [&](const AttnSeg& s, int at, int end, int stage) {
-    const int head = s.hc / p.chunks;
-    const long long row = (static_cast<long long>(s.b) * c.n_kv + head) * c.cap + at;
-    const uint32_t dst = smem_u32(ring + stage * kAttnStageBytes);
-    const int left = end - at;  // rows of the tile that exist
-    const uint8_t *k = c.k + row * (D / 2), *v = c.v + row * (D / 2);
-    #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int x = lane + 32 * i, slot = x / kCh, ch = x % kCh;
-      const uint32_t to = slot * (D / 2) + attn_swizzle<D>(slot, ch) * 16;
-      const long long from = slot < left ? x * 16 : 0;
-      cp_async16(dst + to, k + from, slot < left);
-      cp_async16(dst + 2048 + to, v + from, slot < left);
+  // Lane-constant places in a stage: the lane's chunks as they arrive (source bytes lane * 16 + 512 i of the tile) ...
+  uint32_t put[4];
+  #pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int x = lane + 32 * i, slot = x / kCh;
+    put[i] = smem_u32(ring) + slot * (D / 2) + attn_swizzle<D>(slot, x % kCh) * 16;
+  }
+  const uint32_t put_sb = smem_u32(ring) + 4096 + lane * (D == 64 ? 8 : 16);
+  // ... and what it reads: its words of K slot gid, of V slots 2 tig and 2 tig + 1, and their steps and bases.
+  const int k_at = gid * (D / 2) + (D == 64 ? tig * 8 : D == 128 ? attn_swizzle<D>(gid, tig) * 16 : 0);
+  const int v_in = gid * VW * 4;
+  const int va_at = 2048 + 2 * tig * (D / 2) + attn_swizzle<D>(2 * tig, v_in / 16) * 16 + v_in % 16;
+  const int vb_at = 2048 + (2 * tig + 1) * (D / 2) + attn_swizzle<D>(2 * tig + 1, v_in / 16) * 16 + v_in % 16;
+  const int ks_at = 4096 + gid * (D / 8) + (D == 64 ? (tig >> 1) * 4 : tig * (D / 32));
+  const int vs_at = 4608 + 2 * tig * (D / 8) + gid * VW / 4 * 4;
+
+  auto fetch = [&](long long row, int left, int stage) {  // row: of the tile's first slot; left: rows that exist
+    const uint32_t off = stage * kAttnStageBytes;
+    const uint8_t *k = c.k + row * (D / 2) + lane * 16, *v = c.v + row * (D / 2) + lane * 16;
+    constexpr int kSb = D == 64 ? 8 : 16;  // a d = 64 row has 8 bytes of steps and bases, and no more alignment
+    const uint8_t* ks = reinterpret_cast<const uint8_t*>(c.ks) + row * (D / 8) + lane * kSb;
+    const uint8_t* vs = reinterpret_cast<const uint8_t*>(c.vs) + row * (D / 8) + lane * kSb;
+    if (left >= TS) {
+      #pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        cp_async16(put[i] + off, k + 512 * i);
+        cp_async16(put[i] + off + 2048, v + 512 * i);
+      }
+      if constexpr (D == 64) {
+        #pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          cp_async8(put_sb + off + 256 * i, ks + 256 * i);
+          cp_async8(put_sb + off + 512 + 256 * i, vs + 256 * i);
+        }
+      } else {
+        cp_async16(put_sb + off, ks);
+        cp_async16(put_sb + off + 512, vs);
+      }
+      return;
     }
-    const uint8_t *ks = reinterpret_cast<const uint8_t*>(c.ks) + row * (D / 8);
-    const uint8_t *vs = reinterpret_cast<const uint8_t*>(c.vs) + row * (D / 8);
-    if constexpr (D == 64) {  // 8 bytes a row: no more alignment than that
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) {  // rows that do not exist become zeros: finite values, whatever lies there
+      const bool on = (lane + 32 * i) / kCh < left;
+      cp_async16(put[i] + off, on ? k + 512 * i : c.k, on);
+      cp_async16(put[i] + off + 2048, on ? v + 512 * i : c.v, on);
+    }
+    if constexpr (D == 64) {
       #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int x = lane + 32 * i;
-        cp_async8(dst + 4096 + x * 8, ks + (x < left ? x * 8 : 0), x < left);
-        cp_async8(dst + 4608 + x * 8, vs + (x < left ? x * 8 : 0), x < left);
+        const bool on = lane + 32 * i < left;
+        cp_async8(put_sb + off + 256 * i, on ? static_cast<const void*>(ks + 256 * i) : c.ks, on);
+        cp_async8(put_sb + off + 512 + 256 * i, on ? static_cast<const void*>(vs + 256 * i) : c.vs, on);
       }
     } else {
-      const int slot = lane * 16 / (D / 8);
-      cp_async16(dst + 4096 + lane * 16, ks + (slot < left ? lane * 16 : 0), slot < left);
-      cp_async16(dst + 4608 + lane * 16, vs + (slot < left ? lane * 16 : 0), slot < left);
+      const bool on = lane * 16 / (D / 8) < left;
+      cp_async16(put_sb + off, on ? static_cast<const void*>(ks) : c.ks, on);
+      cp_async16(put_sb + off + 512, on ? static_cast<const void*>(vs) : c.vs, on);
     }
   };
+  auto first_row = [&](const AttnRun& s) { return (static_cast<long long>(s.b) * c.n_kv + s.head) * c.cap; };
+  // A query row's token; its place in q and in the output; where its log2 sum goes.
+  auto token = [&](int row) { return p.m == 1 ? 0 : row / p.group; };
+  auto row_at = [&](const AttnRun& s, int row, long long ld) {
+    const int t = token(row);
+    return (static_cast<long long>(s.b) * p.m + t) * ld + static_cast<long long>(s.head * p.group + row - t * p.group) * D;
+  };
+  auto put_lse = [&](const AttnRun& s, int row, float m, float l) {
+    p.lse[(static_cast<long long>(s.b) * c.n_kv + s.head) * p.rows + row] = m - kAttnShift + log2f(l);
+  };
 
-  AttnSeg seg, nxt;
-  if (!walk.next(seg)) return;
-  int w0, w1;
-  share(seg, w0, w1);
-  if (w0 < w1) fetch(seg, w0, w1, 0);
+  if (lane < 2) s_state[2 * warp + lane] = 0;
+  __syncwarp();
+  AttnRun run, nxt;
+  bool have = walk.next(run);
+  long long row0 = 0;
+  if (have) {
+    row0 = first_row(run);
+    fetch(row0 + run.s0, run.s1 - run.s0, 0);
+  }
   cp_async_commit();
   int stage = 0;
 
-  while (true) {
+  while (have) {
     const bool more = walk.next(nxt);
-    int x0 = 0, x1 = 0;
-    if (more) share(nxt, x0, x1);
-    const int head = seg.hc / p.chunks, r0 = (seg.hc - head * p.chunks) * RC;
+    long long row1 = 0;  // the next run's first slot, and its slots
+    int left1 = 0;
+    if (more) row1 = first_row(nxt) + nxt.s0, left1 = nxt.s1 - nxt.s0;
+    const int r0 = run.r0;
 
     // The chunk's rows: B fragments of their halves, a power of two apart from
     // the row so that its largest value lies in [1, 2). Lane (gid, tig) has row
     // gid / 2 of each four, hi for even gid and lo for odd.
     uint32_t qb[NT][2 * KW][2];
-    float sc[NT];  // what a score has to be multiplied by (log2 units), of row tig
+    float sc[NT];  // what a score has to be multiplied by to be in log2 units, of row tig; not negative
     int vis[NT];   // slots that row tig sees
+    int all_see = 0x7fffffff;  // slots that every row sees
     #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int r = r0 + nt * 4 + (gid >> 1);
       float x[D / 4];
       if (r < p.rows) {
-        const int t = r / p.group;
-        const float* src = p.q + (static_cast<long long>(seg.b) * p.m + t) * p.ldq +
-                           static_cast<long long>(head * p.group + r - t * p.group) * D + tig * (D / 4);
-        load_row<D / 4>(src, p.vec, x);
+        load_row<D / 4>(p.q + row_at(run, r, p.ldq) + tig * (D / 4), p.vec, x);
       } else {
         #pragma unroll
         for (int i = 0; i < D / 4; ++i) x[i] = 0.f;
@@ -287,21 +421,22 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 2) kv4_attn_kernel(const Kv4A
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const int e = min(max(static_cast<int>((__float_as_uint(top) >> 23) & 255) - 127, -120), 120);
-      const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-      sc[nt] = __shfl_sync(0xffffffffu, __uint_as_float(static_cast<uint32_t>(127 + e) << 23), 8 * tig) * p.scale2;
+      const float down = copysignf(__uint_as_float(static_cast<uint32_t>(127 - e) << 23), p.scale2);
+      sc[nt] = __shfl_sync(0xffffffffu, __uint_as_float(static_cast<uint32_t>(127 + e) << 23), 8 * tig) * fabsf(p.scale2);
       #pragma unroll
       for (int w = 0; w < KW; ++w) {
         #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float a = x[8 * w + i] * down, b = x[8 * w + i + 4] * down;
-          const __half2 hi = __floats2half2_rn(a, b);
-          const __half2 lo = __floats2half2_rn(a - __low2float(hi), b - __high2float(hi));
-          qb[nt][2 * w + (i >> 1)][i & 1] = (gid & 1) ? h2_bits(lo) : h2_bits(hi);
+          const __half2 top2 = __floats2half2_rn(a, b);
+          const __half2 low2 = __floats2half2_rn(a - __low2float(top2), b - __high2float(top2));
+          qb[nt][2 * w + (i >> 1)][i & 1] = (gid & 1) ? h2_bits(low2) : h2_bits(top2);
         }
       }
       const int rt = r0 + nt * 4 + tig;
-      vis[nt] = rt < p.rows ? seg.n - (p.m - 1 - rt / p.group) : 0;
+      vis[nt] = rt < p.rows ? run.n - (p.m - 1 - token(rt)) : 0;
     }
+    all_see = r0 + RC > p.rows ? 0 : run.n - (p.m - 1 - token(r0));
 
     float top[NT], sum[NT], o[OT][2][NT];
     #pragma unroll
@@ -311,298 +446,392 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 2) kv4_attn_kernel(const Kv4A
       for (int i = 0; i < OT; ++i) o[i][0][nt] = 0.f, o[i][1][nt] = 0.f;
     }
 
-    int at = w0;
-    do {
-      if (at + TS < w1) {
-        fetch(seg, at + TS, w1, stage ^ 1);
-      } else if (more && x0 < x1) {
-        fetch(nxt, x0, x1, stage ^ 1);
-      }
+    #pragma unroll 1
+    for (int at = run.s0; at < run.s1; at += TS) {
+      const bool same = at + TS < run.s1;
+      if (same || more) fetch(same ? row0 + at + TS : row1, same ? run.s1 - at - TS : left1, stage ^ 1);
       cp_async_commit();
       cp_async_wait<1>();
       __syncwarp();
       const unsigned char* st = ring + stage * kAttnStageBytes;
-      const int left = w1 - at;
-      if (left > 0) {
-        // scores, in log2 units
-        float s[ST][2][NT];
-        #pragma unroll
-        for (int u = 0; u < ST; ++u) {
-          float acc[NT][4];
-          #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
-          if (u * 16 < left) {
-            const int ja = u * 16 + gid, jb = ja + 8;
-            uint32_t wa[KW], wb[KW];
-            if constexpr (D == 64) {
-              const uint2 a = *reinterpret_cast<const uint2*>(st + ja * 32 + tig * 8);
-              const uint2 b = *reinterpret_cast<const uint2*>(st + jb * 32 + tig * 8);
-              wa[0] = a.x, wa[1] = a.y, wb[0] = b.x, wb[1] = b.y;
-            } else {
-              #pragma unroll
-              for (int h = 0; h < KW / 4; ++h) {
-                const int ch = tig * (KW / 4) + h;
-                const uint4 a = *reinterpret_cast<const uint4*>(st + ja * (D / 2) + attn_swizzle<D>(ja, ch) * 16);
-                const uint4 b = *reinterpret_cast<const uint4*>(st + jb * (D / 2) + attn_swizzle<D>(jb, ch) * 16);
-                wa[4 * h] = a.x, wa[4 * h + 1] = a.y, wa[4 * h + 2] = a.z, wa[4 * h + 3] = a.w;
-                wb[4 * h] = b.x, wb[4 * h + 1] = b.y, wb[4 * h + 2] = b.z, wb[4 * h + 3] = b.w;
-              }
-            }
-            const uint32_t* sb = reinterpret_cast<const uint32_t*>(st + 4096);
+      const int left = run.s1 - at;
+      // scores (times sc: in log2 units)
+      float s[ST][2][NT];
+      #pragma unroll
+      for (int u = 0; u < ST; ++u) {
+        float acc[NT][4];
+        {
+          const unsigned char* pk = st + k_at + u * 16 * (D / 2);
+          uint32_t wa[KW], wb[KW];
+          if constexpr (D == 64) {
+            const uint2 a = *reinterpret_cast<const uint2*>(pk), b = *reinterpret_cast<const uint2*>(pk + 8 * (D / 2));
+            wa[0] = a.x, wa[1] = a.y, wb[0] = b.x, wb[1] = b.y;
+          } else {
             #pragma unroll
-            for (int w = 0; w < KW; ++w) {
-              const int g = D == 64 ? tig >> 1 : tig * (KW / 4) + w / 4;
-              const __half2 sa = bits_h2(sb[ja * (D / 32) + g]), sbb = bits_h2(sb[jb * (D / 32) + g]);
-              __half2 ha[4], hb[4];
-              kv4_unpack(wa[w], __low2half2(sa), __high2half2(sa), ha);
-              kv4_unpack(wb[w], __low2half2(sbb), __high2half2(sbb), hb);
-              #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                mma_f16(acc[nt], h2_bits(ha[0]), h2_bits(hb[0]), h2_bits(ha[1]), h2_bits(hb[1]), qb[nt][2 * w][0],
-                        qb[nt][2 * w][1]);
-                mma_f16(acc[nt], h2_bits(ha[2]), h2_bits(hb[2]), h2_bits(ha[3]), h2_bits(hb[3]), qb[nt][2 * w + 1][0],
-                        qb[nt][2 * w + 1][1]);
-              }
+            for (int h = 0; h < KW / 4; ++h) {
+              const int ch = D == 128 ? 0 : attn_swizzle<D>(gid, tig * 2 + h) * 16;
+              const uint4 a = *reinterpret_cast<const uint4*>(pk + ch), b = *reinterpret_cast<const uint4*>(pk + 8 * (D / 2) + ch);
+              wa[4 * h] = a.x, wa[4 * h + 1] = a.y, wa[4 * h + 2] = a.z, wa[4 * h + 3] = a.w;
+              wb[4 * h] = b.x, wb[4 * h + 1] = b.y, wb[4 * h + 2] = b.z, wb[4 * h + 3] = b.w;
+            }
+          }
+          const unsigned char* ps = st + ks_at + u * 16 * (D / 8);
+          #pragma unroll
+          for (int w = 0; w < KW; ++w) {
+            const __half2 sa = *reinterpret_cast<const __half2*>(ps + w / 4 * 4);
+            const __half2 sb = *reinterpret_cast<const __half2*>(ps + 8 * (D / 8) + w / 4 * 4);
+            const __half2 sta = __low2half2(sa), bsa = __high2half2(sa), stb = __low2half2(sb), bsb = __high2half2(sb);
+            const uint32_t a0 = kv4_pair<false>(wa[w], p.mul64, sta, bsa), b0 = kv4_pair<false>(wb[w], p.mul64, stb, bsb);
+            const uint32_t a1 = kv4_pair<true>(wa[w], p.mul4, sta, bsa), b1 = kv4_pair<true>(wb[w], p.mul4, stb, bsb);
+            const uint32_t xa = wa[w] >> 8, xb = wb[w] >> 8;
+            const uint32_t a2 = kv4_pair<false>(xa, p.mul64, sta, bsa), b2 = kv4_pair<false>(xb, p.mul64, stb, bsb);
+            const uint32_t a3 = kv4_pair<true>(xa, p.mul4, sta, bsa), b3 = kv4_pair<true>(xb, p.mul4, stb, bsb);
+            #pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              if (w == 0)
+                mma_f16_first(acc[nt], a0, b0, a1, b1, qb[nt][0][0], qb[nt][0][1]);
+              else
+                mma_f16(acc[nt], a0, b0, a1, b1, qb[nt][2 * w][0], qb[nt][2 * w][1]);
+              mma_f16(acc[nt], a2, b2, a3, b3, qb[nt][2 * w + 1][0], qb[nt][2 * w + 1][1]);
             }
           }
           #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            s[u][0][nt] = (acc[nt][0] + acc[nt][1]) * sc[nt];
-            s[u][1][nt] = (acc[nt][2] + acc[nt][3]) * sc[nt];
+            s[u][0][nt] = acc[nt][0] + acc[nt][1];
+            s[u][1][nt] = acc[nt][2] + acc[nt][3];
           }
         }
-        if (kW) {
-          #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const int r = r0 + nt * 4 + tig;
-            if (r < p.rows) {
-              float* to = p.score + ((static_cast<long long>(seg.b) * c.n_kv + head) * p.rows + r) * c.cap + at;
-              #pragma unroll
-              for (int u = 0; u < ST; ++u) {
-                if (u * 16 + gid < left) to[u * 16 + gid] = s[u][0][nt];
-                if (u * 16 + gid + 8 < left) to[u * 16 + gid + 8] = s[u][1][nt];
-              }
-            }
-          }
-        }
-        // slots that a row does not see; then the running maximum
-        uint32_t pb[ST][NT][2];
+      }
+      if (kW) {
         #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          const int see = min(left, vis[nt] - at);
-          if (__any_sync(0xffffffffu, see < TS)) {
+          const int r = r0 + nt * 4 + tig;
+          if (r < p.rows) {
+            float* to = p.score + ((static_cast<long long>(run.b) * c.n_kv + run.head) * p.rows + r) * c.cap + at;
             #pragma unroll
             for (int u = 0; u < ST; ++u) {
-              if (u * 16 + gid >= see) s[u][0][nt] = -INFINITY;
-              if (u * 16 + gid + 8 >= see) s[u][1][nt] = -INFINITY;
-            }
-          }
-          float best = s[0][0][nt];
-          #pragma unroll
-          for (int u = 0; u < ST; ++u) best = fmaxf(best, fmaxf(s[u][0][nt], s[u][1][nt]));
-          if (__any_sync(0xffffffffu, best > top[nt] + kAttnSlack)) {
-            best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 4));
-            best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 8));
-            best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 16));
-            best = fmaxf(best, top[nt]);
-            const float f = ex2(top[nt] - best);
-            top[nt] = best;
-            sum[nt] *= f;
-            #pragma unroll
-            for (int i = 0; i < OT; ++i) o[i][0][nt] *= f, o[i][1][nt] *= f;
-          }
-          const float off = kAttnShift - top[nt];
-          #pragma unroll
-          for (int u = 0; u < ST; ++u) {
-            #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float e = ex2(s[u][h][nt] + off);
-              sum[nt] += e;
-              const float hi = __uint_as_float(__float_as_uint(e) & 0xFFFFE000u);
-              pb[u][nt][h] = transpose8x8(h2_bits(__floats2half2_rn(hi, e - hi)));
+              if (u * 16 + gid < left) to[u * 16 + gid] = s[u][0][nt] * sc[nt];
+              if (u * 16 + gid + 8 < left) to[u * 16 + gid + 8] = s[u][1][nt] * sc[nt];
             }
           }
         }
-        // output: nibble by nibble of the V words
-        const unsigned char* sv = st + 2048;
-        const uint32_t* sb = reinterpret_cast<const uint32_t*>(st + 4608);
-        uint32_t ul[ST][2][VW], uh[ST][2][VW];  // low and high 16 bits of two slots' words
-        __half2 stp[ST][2], bas[ST][2];
+      }
+      // slots that a row does not see; then the running maximum, and the weights as split halves
+      const bool some_hidden = left < TS || at + TS > all_see;
+      uint32_t pb[ST][NT][2];
+      #pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        if (some_hidden) {
+          const int see = min(left, vis[nt] - at);
+          #pragma unroll
+          for (int u = 0; u < ST; ++u) {
+            if (u * 16 + gid >= see) s[u][0][nt] = -INFINITY;
+            if (u * 16 + gid + 8 >= see) s[u][1][nt] = -INFINITY;
+          }
+        }
+        float best = s[0][0][nt];
+        #pragma unroll
+        for (int u = 0; u < ST; ++u) best = fmaxf(best, fmaxf(s[u][0][nt], s[u][1][nt]));
+        best *= sc[nt];
+        if (__any_sync(0xffffffffu, best > top[nt] + kAttnSlack)) {
+          best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 4));
+          best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 8));
+          best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 16));
+          best = fmaxf(best, top[nt]);
+          const float f = ex2(top[nt] - best);
+          top[nt] = best;
+          sum[nt] *= f;
+          #pragma unroll
+          for (int i = 0; i < OT; ++i) o[i][0][nt] *= f, o[i][1][nt] *= f;
+        }
+        const float off = kAttnShift - top[nt];
         #pragma unroll
         for (int u = 0; u < ST; ++u) {
           #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const int ja = u * 16 + 8 * h + 2 * tig, jb = ja + 1;
-            uint32_t wa[VW], wb[VW];
-            const int byte = gid * VW * 4, ch = byte / 16, in = byte % 16;
-            const unsigned char* pa = sv + ja * (D / 2) + attn_swizzle<D>(ja, ch) * 16 + in;
-            const unsigned char* pq = sv + jb * (D / 2) + attn_swizzle<D>(jb, ch) * 16 + in;
-            if constexpr (VW == 1) {
-              wa[0] = *reinterpret_cast<const uint32_t*>(pa), wb[0] = *reinterpret_cast<const uint32_t*>(pq);
-            } else if constexpr (VW == 2) {
-              const uint2 a = *reinterpret_cast<const uint2*>(pa), b = *reinterpret_cast<const uint2*>(pq);
-              wa[0] = a.x, wa[1] = a.y, wb[0] = b.x, wb[1] = b.y;
-            } else {
-              const uint4 a = *reinterpret_cast<const uint4*>(pa), b = *reinterpret_cast<const uint4*>(pq);
-              wa[0] = a.x, wa[1] = a.y, wa[2] = a.z, wa[3] = a.w;
-              wb[0] = b.x, wb[1] = b.y, wb[2] = b.z, wb[3] = b.w;
+            const float e = ex2(fmaf(s[u][h][nt], sc[nt], off));
+            sum[nt] += e;
+            const float big = __uint_as_float(__float_as_uint(e) & 0xFFFFE000u);
+            pb[u][nt][h] = transpose8x8(h2_bits(__floats2half2_rn(big, e - big)));
+          }
+        }
+      }
+      // output: byte by byte of the V words
+      uint32_t wa[ST][2][VW], wb[ST][2][VW];  // two slots' words
+      __half2 stp[ST][2], bas[ST][2];
+      #pragma unroll
+      for (int u = 0; u < ST; ++u) {
+        #pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const unsigned char* pa = st + va_at + (u * 16 + h * 8) * (D / 2);
+          const unsigned char* pq = st + vb_at + (u * 16 + h * 8) * (D / 2);
+          if constexpr (VW == 1) {
+            wa[u][h][0] = *reinterpret_cast<const uint32_t*>(pa), wb[u][h][0] = *reinterpret_cast<const uint32_t*>(pq);
+          } else if constexpr (VW == 2) {
+            const uint2 a = *reinterpret_cast<const uint2*>(pa), b = *reinterpret_cast<const uint2*>(pq);
+            wa[u][h][0] = a.x, wa[u][h][1] = a.y, wb[u][h][0] = b.x, wb[u][h][1] = b.y;
+          } else {
+            const uint4 a = *reinterpret_cast<const uint4*>(pa), b = *reinterpret_cast<const uint4*>(pq);
+            wa[u][h][0] = a.x, wa[u][h][1] = a.y, wa[u][h][2] = a.z, wa[u][h][3] = a.w;
+            wb[u][h][0] = b.x, wb[u][h][1] = b.y, wb[u][h][2] = b.z, wb[u][h][3] = b.w;
+          }
+          const unsigned char* ps = st + vs_at + (u * 16 + h * 8) * (D / 8);
+          const uint32_t x = *reinterpret_cast<const uint32_t*>(ps), y = *reinterpret_cast<const uint32_t*>(ps + D / 8);
+          stp[u][h] = bits_h2(__byte_perm(x, y, 0x5410));
+          bas[u][h] = bits_h2(__byte_perm(x, y, 0x7632));
+        }
+      }
+      // Tiles 2 y and 2 y + 1 are the low and the high nibbles of one byte of the words: d = 64, columns 8 gid + n and
+      // 8 gid + 4 + n of the lane's word (n = tile); else columns n of words 2 w and 2 w + 1 of the lane's words
+      // (tile = 8 w + n).
+      #pragma unroll
+      for (int y = 0; y < OT / 2; ++y) {
+        float acc[2][NT][4];
+        #pragma unroll
+        for (int u = 0; u < ST; ++u) {
+          {
+            uint32_t ln[4], hn[4];
+            #pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              #pragma unroll
+              for (int z = 0; z < 2; ++z) {
+                const int w = VW == 1 ? 0 : y / 4 * 2 + z, byte = VW == 1 ? y + 2 * z : y % 4;
+                const uint32_t both = __byte_perm(wa[u][h][w], wb[u][h][w], byte | (byte + 4) << 8);
+                ln[2 * h + z] = kv4_pair<false>(both, p.mul64, stp[u][h], bas[u][h]);
+                hn[2 * h + z] = kv4_pair<true>(both, p.mul4, stp[u][h], bas[u][h]);
+              }
             }
             #pragma unroll
-            for (int w = 0; w < VW; ++w) {
-              ul[u][h][w] = __byte_perm(wa[w], wb[w], 0x5410);
-              uh[u][h][w] = __byte_perm(wa[w], wb[w], 0x7632);
+            for (int nt = 0; nt < NT; ++nt) {
+              if (u == 0) {
+                mma_f16_first(acc[0][nt], ln[0], ln[1], ln[2], ln[3], pb[u][nt][0], pb[u][nt][1]);
+                mma_f16_first(acc[1][nt], hn[0], hn[1], hn[2], hn[3], pb[u][nt][0], pb[u][nt][1]);
+              } else {
+                mma_f16(acc[0][nt], ln[0], ln[1], ln[2], ln[3], pb[u][nt][0], pb[u][nt][1]);
+                mma_f16(acc[1][nt], hn[0], hn[1], hn[2], hn[3], pb[u][nt][0], pb[u][nt][1]);
+              }
             }
-            const int g = gid * VW / 4;
-            const uint32_t x = sb[ja * (D / 32) + g], y = sb[jb * (D / 32) + g];
-            stp[u][h] = bits_h2(__byte_perm(x, y, 0x5410));
-            bas[u][h] = bits_h2(__byte_perm(x, y, 0x7632));
           }
         }
         #pragma unroll
-        for (int i = 0; i < OT; ++i) {
-          float acc[NT][4];
-          #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
-          #pragma unroll
-          for (int u = 0; u < ST; ++u) {
-            if (u * 16 < left) {
-              uint32_t a[4];
-              #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                if constexpr (VW == 1) {  // tile i: columns 8 gid + i and 8 gid + 4 + i
-                  a[2 * h] = kv4_pair_at(i, ul[u][h][0], stp[u][h], bas[u][h]);
-                  a[2 * h + 1] = kv4_pair_at(i, uh[u][h][0], stp[u][h], bas[u][h]);
-                } else {  // tile (pair, n): columns n of words 2 pair and 2 pair + 1 of the lane's words
-                  const int w = i / 8 * 2, n = i % 8;
-                  a[2 * h] = kv4_pair_at(n & 3, n < 4 ? ul[u][h][w] : uh[u][h][w], stp[u][h], bas[u][h]);
-                  a[2 * h + 1] = kv4_pair_at(n & 3, n < 4 ? ul[u][h][w + 1] : uh[u][h][w + 1], stp[u][h], bas[u][h]);
-                }
-              }
-              #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) mma_f16(acc[nt], a[0], a[1], a[2], a[3], pb[u][nt][0], pb[u][nt][1]);
-            }
-          }
+        for (int z = 0; z < 2; ++z) {
           #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            o[i][0][nt] += acc[nt][0] + acc[nt][1];
-            o[i][1][nt] += acc[nt][2] + acc[nt][3];
+            o[2 * y + z][0][nt] += acc[z][nt][0] + acc[z][nt][1];
+            o[2 * y + z][1][nt] += acc[z][nt][2] + acc[z][nt][3];
           }
         }
       }
       __syncwarp();
       stage ^= 1;
-      at += TS;
-    } while (at < w1);
+    }
 
-    // The warps' results become one: largest maximum, then scaled sums.
+    // The run's result. All of an item: the output, through the stage that was just used up. A part of one: left in
+    // shared memory for the CTA; the end of an item that others began comes first in the share and lies apart from the
+    // ring, which goes on; the beginning of one that others end comes last and stays in the used-up stage.
+    float* fr = run.enter ? heads + warp * RC * D : reinterpret_cast<float*>(ring + (stage ^ 1) * kAttnStageBytes);
+    const int which = 2 * warp + (run.enter ? 0 : 1);
     #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       #pragma unroll
       for (int x = 4; x < 32; x <<= 1) sum[nt] += __shfl_xor_sync(0xffffffffu, sum[nt], x);
-      if (gid == 0) {
-        ml[(warp * RC + nt * 4 + tig) * 2] = top[nt];
-        ml[(warp * RC + nt * 4 + tig) * 2 + 1] = sum[nt];
+      if (gid == 0 && (run.enter || run.leave)) {
+        float* to = ml + (which * RC + nt * 4 + tig) * 2;
+        to[0] = top[nt], to[1] = sum[nt];
       }
-    }
-    const long long item = static_cast<long long>(seg.b) * walk.hc_count + seg.hc;
-    const bool starts = seg.s0 == 0;
-    float* part = p.part + (static_cast<long long>(cta) * 2 + (starts ? 1 : 0)) * (RC * (D + 2));
-    #pragma unroll
-    for (int hv = 0; hv < kHalves; ++hv) {
-      constexpr int OH = OT / kHalves;
-      __syncthreads();
       #pragma unroll
-      for (int i = 0; i < OH; ++i)
+      for (int i = 0; i < OT; ++i)
         #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < 2; ++h) fr[((i * 2 + h) * NT + nt) * 32 + lane] = o[i][h][nt];
+    }
+    if (!run.enter && !run.leave) {
+      __syncwarp();
+      #pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float inv = sum[nt] != 0.f ? 1.f / sum[nt] : 0.f;
+        #pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const int r = nt * 4 + r4;
+          const float f = __shfl_sync(0xffffffffu, inv, r4), tp = __shfl_sync(0xffffffffu, top[nt], r4),
+                      sm = __shfl_sync(0xffffffffu, sum[nt], r4);
+          if (r0 + r >= p.rows) continue;
+          float* to = p.out + row_at(run, r0 + r, p.ldo);
           #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-            merge[((warp * OH + i) * 2 + h) * NT * 32 + nt * 32 + lane] = o[hv * OH + i][h][nt];
-      __syncthreads();
-      for (int x = tid; x < RC * D / kHalves; x += kAttnWarps * 32) {
-        // x -> (row, a column of this part): lanes take neighbouring columns
-        const int r = x / (D / kHalves), y = x % (D / kHalves);
-        int col, ti, h, g;
-        if constexpr (D == 64) {
-          constexpr int per = 8 / kHalves;  // columns of a lane's word in this part
-          g = y / per;
-          const int z = y % per;            // (h, i within the part)
-          h = z / OH, ti = z % OH;
-          col = 8 * g + 4 * h + hv * OH + ti;
-        } else {
-          constexpr int words = VW / kHalves > 1 ? VW / kHalves : 1;  // words of a lane in this part
-          if constexpr (VW / kHalves >= 2) {
-            const int w = y / 8, n = y % 8;
-            g = w / words;
-            const int ww = w % words;
-            h = ww & 1, ti = ww / 2 * 8 + n;
-            col = 8 * (g * VW + hv * words + ww) + n;
-          } else {  // d = 128 in two parts: nibbles 4 hv .. 4 hv + 3 of both words
-            const int w = y / 4, n = y % 4;
-            g = w / 2, h = w & 1, ti = n;
-            col = 8 * (g * VW + h) + 4 * hv + n;
+          for (int x = 0; x < D; x += 32) {
+            int ti, h, g;
+            attn_place<D>(x + lane, ti, h, g);
+            to[x + lane] = fr[((ti * 2 + h) * NT + nt) * 32 + g * 4 + r4] * f;
           }
-        }
-        float m = -1e30f;
-        #pragma unroll
-        for (int k = 0; k < kAttnWarps; ++k) m = fmaxf(m, ml[(k * RC + r) * 2]);
-        float v = 0.f, l = 0.f;
-        #pragma unroll
-        for (int k = 0; k < kAttnWarps; ++k) {
-          const float f = ex2(ml[(k * RC + r) * 2] - m);
-          l = fmaf(f, ml[(k * RC + r) * 2 + 1], l);
-          v = fmaf(f, merge[((k * OH + ti) * 2 + h) * NT * 32 + (r >> 2) * 32 + g * 4 + (r & 3)], v);
-        }
-        const int row = r0 + r;
-        if (seg.whole) {
-          if (row < p.rows) {
-            const int t = row / p.group;
-            p.out[(static_cast<long long>(seg.b) * p.m + t) * p.ldo +
-                  static_cast<long long>(head * p.group + row - t * p.group) * D + col] = l != 0.f ? v / l : 0.f;
-            if (kW && col == 0)
-              p.lse[(static_cast<long long>(seg.b) * c.n_kv + head) * p.rows + row] = m - kAttnShift + log2f(l);
-          }
-        } else {
-          part[2 * RC + r * D + col] = v;
-          if (col == 0) part[r] = m, part[RC + r] = l;
+          if (kW && lane == 0) put_lse(run, r0 + r, tp, sm);
         }
       }
+      __syncwarp();
+    } else if (lane == 0) {
+      s_state[which] = run.leave ? 2 : 1;
+      s_from[which] = static_cast<int>(reinterpret_cast<unsigned char*>(fr) - smem);
+      s_run[which] = run;
     }
-    if (!seg.whole) {
-      // The CTA that finds every other part of the item written joins them.
-      __threadfence();
-      __syncthreads();
-      const long long last_unit = seg.first + seg.units - 1;
-      const int c0 = static_cast<int>(((seg.first + 1) * ctas - 1) / units);
-      const int c1 = static_cast<int>(((last_unit + 1) * ctas - 1) / units);
-      if (tid == 0) s_last = atom_add_acq_rel_gpu(p.arrived + item, 1) == c1 - c0;
-      __syncthreads();
-      if (s_last) {
-        __threadfence();
-        for (int x = tid; x < RC * D; x += kAttnWarps * 32) {
-          const int r = x / D, col = x % D, row = r0 + r;
-          if (row >= p.rows) continue;
-          float m = -1e30f, v = 0.f, l = 0.f;
-          for (int k = c0; k <= c1; ++k) {
-            const float* from = p.part + (static_cast<long long>(k) * 2 + (k == c0 ? 1 : 0)) * (RC * (D + 2));
-            const float mk = __ldcg(from + r), lk = __ldcg(from + RC + r), vk = __ldcg(from + 2 * RC + r * D + col);
-            const float mm = fmaxf(m, mk), f = ex2(m - mm), fk = ex2(mk - mm);
-            l = fmaf(l, f, lk * fk), v = fmaf(v, f, vk * fk), m = mm;
-          }
-          const int t = row / p.group;
-          p.out[(static_cast<long long>(seg.b) * p.m + t) * p.ldo +
-                static_cast<long long>(head * p.group + row - t * p.group) * D + col] = l != 0.f ? v / l : 0.f;
-          if (kW && col == 0)
-            p.lse[(static_cast<long long>(seg.b) * c.n_kv + head) * p.rows + row] = m - kAttnShift + log2f(l);
-        }
-        if (tid == 0) p.arrived[item] = 0;
-      }
-    }
-    if (!more) break;
-    __syncthreads();  // ml and merge are read before the next run writes them
-    seg = nxt, w0 = x0, w1 = x1;
+    have = more;
+    row0 = row1 - nxt.s0;
+    run = nxt;
   }
   cp_async_wait<0>();
+  __syncthreads();
+
+  // Parts of one item left by neighbouring warps become one result: all of the item, or this CTA's part of it, of which
+  // there are at most two (kind 0: it began in an earlier CTA; kind 1: it began here and goes on).
+  uint32_t part_on = 0;  // bit: kind
+  int next = 0;
+  while (true) {
+    while (next < 2 * kWarps && !s_state[next]) ++next;
+    if (next >= 2 * kWarps) break;
+    const int first = next, kind = first & 1;  // a list that begins with a head: the item entered this CTA
+    int last = first;
+    bool open = s_state[first] == 2;
+    while (open) {
+      int k = last + 1;
+      while (k < 2 * kWarps && !s_state[k]) ++k;
+      if (k >= 2 * kWarps) break;
+      last = k, open = s_state[k] == 2;
+    }
+    next = last + 1;
+    const AttnRun it = s_run[first];
+    const bool final_here = kind == 1 && !open;
+    float* part = p.part + (static_cast<long long>(cta) * 2 + kind) * kPart;
+    // A warp a row: lane k has part k, and its factor.
+    #pragma unroll 1
+    for (int r = warp; r < RC; r += kWarps) {
+      const int k = first + lane;
+      const bool on = k <= last && s_state[k];
+      const float mk = on ? ml[(k * RC + r) * 2] : -1e30f, lk = on ? ml[(k * RC + r) * 2 + 1] : 0.f;
+      float m = mk;
+      #pragma unroll
+      for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+      const float f = ex2(mk - m);
+      float l = f * lk;
+      #pragma unroll
+      for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+      const uint32_t parts = __ballot_sync(0xffffffffu, on);
+      const int at = __popc(parts & ((1u << lane) - 1u));
+      if (on) {
+        s_mul[r][at] = final_here ? (l != 0.f ? f / l : 0.f) : f;
+        if (r == 0) s_at[at] = s_from[k];
+      }
+      if (lane == 0) {
+        if (r == 0) s_parts = __popc(parts);
+        if (!final_here)
+          part[r] = m, part[RC + r] = l;
+        else if (kW && it.r0 + r < p.rows)
+          put_lse(it, it.r0 + r, m, l);
+      }
+    }
+    __syncthreads();
+    #pragma unroll
+    for (int x0 = 0; x0 < RC * D; x0 += kThreads) {
+      const int x = x0 + tid, r = attn_row<NT>(x);
+      if (x >= RC * D) break;
+      float v = 0.f;
+      const int parts = s_parts;
+      #pragma unroll 4
+      for (int k = 0; k < parts; ++k) v = fmaf(s_mul[r][k], reinterpret_cast<const float*>(smem + s_at[k])[x], v);
+      if (!final_here)
+        part[2 * RC + x] = v;
+      else if (it.r0 + r < p.rows)
+        p.out[row_at(it, it.r0 + r, p.ldo) + attn_col<D, NT>(x)] = v;
+    }
+    if (next < 2 * kWarps) __syncthreads();  // s_mul is used again
+    if (!final_here) {
+      part_on |= 1u << kind;
+      if (tid == 0) s_part[kind] = it;
+    }
+  }
+  if (!part_on) return;
+
+  // The CTA that finds every other part of an item written joins them. The barrier orders the CTA's stores before the
+  // counting thread's release, and its acquire before the other threads' loads.
+  __syncthreads();
+  auto cta_of = [&](int u) {
+    const int big = (each + 1) * extra;
+    return u < big ? u / (each + 1) : extra + (u - big) / each;
+  };
+  if (tid < 2 && (part_on >> tid & 1)) {
+    const AttnRun& it = s_part[tid];
+    const int c0 = cta_of(it.first), c1 = cta_of(it.first + it.units - 1);
+    const int item = it.b * walk.hc_count + it.hc;
+    s_c0[tid] = c0;
+    s_last[tid] = atom_add_acq_rel_gpu(p.arrived + item, 1) == c1 - c0 ? c1 - c0 + 1 : 0;
+  }
+  __syncthreads();
+  #pragma unroll 1
+  for (int kind = 0; kind < 2; ++kind) {
+    if (!(part_on >> kind & 1) || s_last[kind] == 0) continue;
+    const AttnRun it = s_part[kind];
+    const int parts = s_last[kind], c0 = s_c0[kind];
+    // Thread groups that cover the chunk once take turns with the parts, four values a thread (the four rows of a
+    // column), each with its own running maximum and sum: one round of loads.
+    const float* from = p.part + static_cast<long long>(c0) * 2 * kPart;
+    constexpr int kFour = RC * D / 4, kGroups = kThreads / kFour;
+    const int x = tid % kFour * 4, grp = tid / kFour, r = attn_row<NT>(x);
+    float m[4] = {-1e30f, -1e30f, -1e30f, -1e30f}, l[4] = {}, v[4] = {};
+    if (grp < kGroups) {
+      constexpr int kAhead = 5;
+      #pragma unroll 1
+      for (int k0 = grp; k0 < parts; k0 += kAhead * kGroups) {
+        float4 pm[kAhead], pl[kAhead], pv[kAhead];
+        #pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          const int k = k0 + i * kGroups;
+          if (k >= parts) continue;
+          const float* at = from + static_cast<long long>(k) * 2 * kPart + (k == 0 ? kPart : 0);
+          pm[i] = __ldcg(reinterpret_cast<const float4*>(at + r));
+          pl[i] = __ldcg(reinterpret_cast<const float4*>(at + RC + r));
+          pv[i] = __ldcg(reinterpret_cast<const float4*>(at + 2 * RC + x));
+        }
+        #pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          if (k0 + i * kGroups >= parts) continue;
+          const float am[4] = {pm[i].x, pm[i].y, pm[i].z, pm[i].w}, al[4] = {pl[i].x, pl[i].y, pl[i].z, pl[i].w},
+                      av[4] = {pv[i].x, pv[i].y, pv[i].z, pv[i].w};
+          #pragma unroll
+          for (int j = 0; j < 4; ++j) attn_join(m[j], l[j], v[j], am[j], al[j], av[j]);
+        }
+      }
+    }
+    if constexpr (kGroups > 1) {
+      static_assert((kGroups - 1) * kFour * 48 <= kWarps * 2 * kAttnStageBytes, "the joins' values lie in the rings");
+      float4* other = reinterpret_cast<float4*>(smem);
+      if (grp > 0 && grp < kGroups) {
+        float4* to = other + (tid - kFour) * 3;
+        to[0] = make_float4(m[0], m[1], m[2], m[3]);
+        to[1] = make_float4(l[0], l[1], l[2], l[3]);
+        to[2] = make_float4(v[0], v[1], v[2], v[3]);
+      }
+      __syncthreads();
+      if (grp == 0) {
+        #pragma unroll
+        for (int g = 1; g < kGroups; ++g) {
+          const float4* at = other + (tid + (g - 1) * kFour) * 3;
+          const float4 pm = at[0], pl = at[1], pv = at[2];
+          attn_join(m[0], l[0], v[0], pm.x, pl.x, pv.x);
+          attn_join(m[1], l[1], v[1], pm.y, pl.y, pv.y);
+          attn_join(m[2], l[2], v[2], pm.z, pl.z, pv.z);
+          attn_join(m[3], l[3], v[3], pm.w, pl.w, pv.w);
+        }
+      }
+    }
+    if (grp == 0) {
+      const int col = attn_col<D, NT>(x);
+      #pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int row = it.r0 + r + j;
+        if (row >= p.rows) continue;
+        p.out[row_at(it, row, p.ldo) + col] = l[j] != 0.f ? v[j] / l[j] : 0.f;
+        if (kW && col == 0) put_lse(it, row, m[j], l[j]);
+      }
+    }
+    if (tid == 0) p.arrived[it.b * walk.hc_count + it.hc] = 0;
+    __syncthreads();
+  }
 }
 
 // The weights from the kept scores: one thread per (sequence, kv head, slot).

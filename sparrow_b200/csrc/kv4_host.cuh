@@ -90,19 +90,21 @@ int kv4_launch_attn(Ctx* ctx, Kv4Attn p, const Kv4View& v, cudaStream_t st) {
   }
   const size_t heads = static_cast<size_t>(v.n_seq) * v.n_kv;
   p.chunks = static_cast<int>(cdiv(p.rows, 4 * NT));
-  const int grid = 2 * ctx->sms;
+  const int grid = ctx->sms;
   VMLM_TRY(ensure(ctx->kv4_part, static_cast<size_t>(grid) * 2 * 4 * NT * (D + 2) * 4));
   VMLM_TRY(ensure_zeroed(ctx->kv4_arrived, heads * p.chunks * 4, st));
   p.part = static_cast<float*>(ctx->kv4_part.p);
   p.arrived = static_cast<int*>(ctx->kv4_arrived.p);
-  p.min_units = D == 64 ? 8 : D == 128 ? 4 : 2;
+  p.mul4 = 4, p.mul64 = 64;
+  if (heads * p.chunks * static_cast<size_t>(cdiv(v.cap, 4096 / D)) >= kKv4MaxDim)
+    return fail(VMLM_ERR_SHAPE, "kv4_attn_dev: n_seq * n_q * m * cap is too large");
   if (kW) {
     VMLM_TRY(ensure(ctx->kv4_lse, heads * p.rows * 4));
     VMLM_TRY(ensure(ctx->kv4_score, heads * p.rows * static_cast<size_t>(v.cap) * 4));
     p.lse = static_cast<float*>(ctx->kv4_lse.p);
     p.score = static_cast<float*>(ctx->kv4_score.p);
   }
-  VMLM_TRY(launch(kv4_attn_kernel<D, NT, kW>, dim3(grid), dim3(kAttnWarps * 32), kSmem, st, false, p, v, ctx->err));
+  VMLM_TRY(launch(kv4_attn_kernel<D, NT, kW>, dim3(grid), dim3(attn_warps(D, NT) * 32), kSmem, st, false, p, v, ctx->err));
   if (!kW || v.cap == 0) return VMLM_OK;
   if (heads >= 65536) return fail(VMLM_ERR_SHAPE, "kv4_attn_dev: n_seq * n_kv must be < 65536 with w_out");
   return launch(kv4_weights_kernel, dim3(static_cast<unsigned>(cdiv(v.cap, 256)), static_cast<unsigned>(heads)), dim3(256),
