@@ -50,7 +50,7 @@ struct Kv4Rows {
   long long tokens, n_pos, m; // m tokens of each sequence
   float eps;
   int n_q, n_kv, rot, interleaved;
-  int vec;                    // every row starts on a 16-byte boundary
+  int vec, vec_g;             // every row starts on a 16-byte boundary; so do the gains
 };
 
 __device__ __forceinline__ uint32_t kv4_pack_sb(float step, float base) {
@@ -140,100 +140,138 @@ __device__ __forceinline__ void kv4_store_row(const float (&x)[D / 32], uint8_t*
   if (lane % kLanes == 0) sb[row * (D / kKv4Group) + lane / kLanes] = kv4_pack_sb(step, base);
 }
 
-// One warp per row (token, head): heads 0 .. n_q-1 are queries, then n_kv keys,
-// then (with a cache) n_kv values.
+// The sum of a row's squares, s_i of columns V*l + i in lane l, added in halves
+// (columns c and c + d/2, then d/4, ...): the same tree, and so the same bits,
+// whatever the lanes hold. While a lane has several values, each exchange sends
+// one half of them and keeps the sums of the other, so a row of 128 takes 8
+// shuffles instead of 20: at 1 shuffle a cycle and SM, 20 of them and the
+// rotation's 4 are most of the 43 cycles that the row's bytes take.
+template <int V>
+__device__ __forceinline__ float tree_sum(float (&s)[V]) {
+  const int lane = threadIdx.x & 31;
+  int o = 16;
+  #pragma unroll
+  for (int h = V / 2; h > 0; h /= 2, o >>= 1) {
+    const bool up = lane & o;
+    #pragma unroll
+    for (int i = 0; i < h; ++i) {
+      const float mine = up ? s[i + h] : s[i], other = up ? s[i] : s[i + h];
+      s[i] = __fadd_rn(mine, __shfl_xor_sync(0xffffffffu, other, o));
+    }
+  }
+  for (; o > 0; o >>= 1) s[0] = __fadd_rn(s[0], __shfl_xor_sync(0xffffffffu, s[0], o));
+  // lane bits 16, 8, ... now say which of the lane's values s[0] is the sum of
+  #pragma unroll
+  for (int x = 16, h = V / 2; h > 0; h /= 2, x >>= 1) s[0] = __fadd_rn(s[0], __shfl_xor_sync(0xffffffffu, s[0], x));
+  return s[0];
+}
+
+// R rows (heads) of one token a warp: heads 0 .. n_q-1 are queries, then n_kv
+// keys, then (with a cache) n_kv values.
 //   y = x * (1 / sqrt(sum(x^2) / d + eps)) * gain        (gain given)
 //   (a, b) -> (a cos - b sin, b cos + a sin)             (table given)
-// on the pairs (i, i + rot/2) or (2i, 2i + 1) of the first rot columns. The sum
-// of squares adds halves (i and i + d/2, then d/4, ...), a tree whose order does
-// not depend on the lane layout. Products and sums are rounded one by one: a
-// key's code must not depend on whether a compiler fused them.
-// Bound by HBM: each value is read once and written once.
-template <int D, bool kCache>
+// on the pairs (i, i + rot/2) or (2i, 2i + 1) of the first rot columns. Products
+// and sums are rounded one by one: a key's code must not depend on whether a
+// compiler fused them.
+// Bound by HBM: each value is read once and written once. R = 4 keeps four
+// rows' loads in flight a warp and reads the token's cos and sin once for them;
+// R = 1 spreads few rows over more warps.
+template <int D, bool kCache, int R>
 __global__ void __launch_bounds__(256) kv4_rows_kernel(const Kv4Rows p, const Kv4View c, int* __restrict__ err) {
   constexpr int V = D / 32;
+  pdl_wait_prior();
+  pdl_launch_dependents();
   const int lane = threadIdx.x & 31;
   const int heads = p.n_q + p.n_kv + (kCache ? p.n_kv : 0);
-  const long long row = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const long long tok = row / heads;
+  const uint32_t sets = static_cast<uint32_t>(heads + R - 1) / R;  // of R heads
+  const uint32_t at = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const uint32_t tok = at / sets;
   if (tok >= p.tokens) return;
-  const int head = static_cast<int>(row - tok * heads);
-  const bool is_q = head < p.n_q;
-  const int kvh = is_q ? 0 : (head - p.n_q) % p.n_kv;
-  const bool is_v = head >= p.n_q + p.n_kv;
-  const float* src = is_q ? p.q + tok * p.ldq + static_cast<long long>(head) * D
-                          : (is_v ? p.v + tok * p.ldv : p.k + tok * p.ldk) + static_cast<long long>(kvh) * D;
-  float x[V];
-  load_row<V>(src + lane * V, p.vec, x);
-  if (!is_v) {
-    const float* gain = is_q ? p.gq : p.gk;
-    if (gain) {
-      float s[V];
-      #pragma unroll
-      for (int i = 0; i < V; ++i) s[i] = __fmul_rn(x[i], x[i]);
-      #pragma unroll
-      for (int o = 16; o > 0; o >>= 1)
-        #pragma unroll
-        for (int i = 0; i < V; ++i) s[i] = __fadd_rn(s[i], __shfl_xor_sync(0xffffffffu, s[i], o));
-      #pragma unroll
-      for (int h = V / 2; h > 0; h /= 2)
-        #pragma unroll
-        for (int i = 0; i < h; ++i) s[i] = __fadd_rn(s[i], s[i + h]);
-      const float inv = __frcp_rn(__fsqrt_rn(__fadd_rn(__fdiv_rn(s[0], static_cast<float>(D)), p.eps)));
-      #pragma unroll
-      for (int i = 0; i < V; ++i) x[i] = __fmul_rn(__fmul_rn(x[i], inv), __ldg(gain + lane * V + i));
-    }
-    if (p.cos_t) {
-      const long long at = __ldg(p.pos + tok);
-      if (at < 0 || at >= p.n_pos) {
-        if (lane == 0) atomicCAS(err, 0, kDevRopePos);
-        return;
-      }
-      const int half = p.rot / 2;
-      const float *ct = p.cos_t + at * half, *sn = p.sin_t + at * half;
-      const int d0 = lane * V;
-      if (p.interleaved) {
-        #pragma unroll
-        for (int i = 0; i < V; i += 2) {
-          if (d0 + i < p.rot) {
-            const float cv = __ldg(ct + (d0 + i) / 2), sv = __ldg(sn + (d0 + i) / 2);
-            const float a = x[i], b = x[i + 1];
-            x[i] = __fsub_rn(__fmul_rn(a, cv), __fmul_rn(b, sv));
-            x[i + 1] = __fadd_rn(__fmul_rn(b, cv), __fmul_rn(a, sv));
-          }
-        }
-      } else {
-        const bool first = d0 < half;  // rot is a multiple of 16, so a lane's columns lie on one side
-        const int other = first ? lane + half / V : lane - half / V;
-        #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float y = __shfl_sync(0xffffffffu, x[i], other & 31);
-          if (d0 < p.rot) {
-            const int e = first ? d0 + i : d0 + i - half;
-            const float cv = __ldg(ct + e), sv = __ldg(sn + e);
-            x[i] = first ? __fsub_rn(__fmul_rn(x[i], cv), __fmul_rn(y, sv))
-                         : __fadd_rn(__fmul_rn(x[i], cv), __fmul_rn(y, sv));
-          }
-        }
-      }
-    }
+  const int h0 = static_cast<int>(at - tok * sets) * R;
+  const bool vec = p.vec;
+  float x[R][V];
+  #pragma unroll
+  for (int j = 0; j < R; ++j) {
+    const int h = h0 + j;
+    if (h >= heads) break;
+    const float* src = h < p.n_q ? p.q + tok * p.ldq + h * D
+                     : h < p.n_q + p.n_kv ? p.k + tok * p.ldk + (h - p.n_q) * D
+                                          : p.v + tok * p.ldv + (h - p.n_q - p.n_kv) * D;
+    load_row<V>(src + lane * V, vec, x[j]);
   }
-  if (is_q) {
-    store_row<V>(p.qo + tok * p.ldqo + static_cast<long long>(head) * D + lane * V, p.vec, x);
-    return;
-  }
-  if constexpr (!kCache) {
-    store_row<V>(p.ko + tok * p.ldko + static_cast<long long>(kvh) * D + lane * V, p.vec, x);
-  } else {
-    const long long b = tok / p.m;
-    const long long had = __ldg(p.len + b);
-    if (had < 0) return;  // an idle sequence
-    const long long slot = had + (tok - b * p.m);
-    if (slot >= c.cap) {
-      if (lane == 0) atomicCAS(err, 0, kDevKv4Slot);
+  const int d0 = lane * V, half = p.rot / 2;
+  const bool turn = p.cos_t != nullptr;
+  const bool first = d0 < half;  // rot is a multiple of 16, so a lane's columns lie on one side
+  const int other = p.interleaved ? lane : (first ? lane + half / V : lane - half / V) & 31;
+  float cs[V], sn[V];  // of the lane's columns; the sine with the sign that its term has
+  #pragma unroll
+  for (int i = 0; i < V; ++i) cs[i] = 1.f, sn[i] = 0.f;
+  if (turn) {
+    const long long row = __ldg(p.pos + tok);
+    if (row < 0 || row >= p.n_pos) {
+      if (lane == 0) atomicCAS(err, 0, kDevRopePos);
       return;
     }
-    kv4_store_row<D>(x, is_v ? c.v : c.k, is_v ? c.vs : c.ks, (b * c.n_kv + kvh) * c.cap + slot);
+    if (d0 < p.rot && h0 < p.n_q + p.n_kv) {
+      #pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const long long e = row * half + (p.interleaved ? (d0 + i) / 2 : first ? d0 + i : d0 + i - half);
+        cs[i] = __ldg(p.cos_t + e);
+        const float s = __ldg(p.sin_t + e);
+        sn[i] = (p.interleaved ? (i & 1) == 0 : first) ? -s : s;
+      }
+    }
+  }
+  #pragma unroll
+  for (int j = 0; j < R; ++j) {
+    const int h = h0 + j;
+    if (h >= heads) break;
+    const bool is_q = h < p.n_q, is_v = h >= p.n_q + p.n_kv;
+    if (!is_v) {
+      const float* gain = is_q ? p.gq : p.gk;
+      if (gain) {
+        float s[V], g[V];
+        load_row<V>(gain + d0, p.vec_g, g);
+        #pragma unroll
+        for (int i = 0; i < V; ++i) s[i] = __fmul_rn(x[j][i], x[j][i]);
+        const float sum = tree_sum<V>(s);
+        const float inv = __frcp_rn(__fsqrt_rn(__fadd_rn(__fmul_rn(sum, 1.f / D), p.eps)));
+        #pragma unroll
+        for (int i = 0; i < V; ++i) x[j][i] = __fmul_rn(__fmul_rn(x[j][i], inv), g[i]);
+      }
+      if (turn) {
+        float y[V];
+        #pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float z = __shfl_sync(0xffffffffu, x[j][i], other);
+          y[i] = z;
+        }
+        if (p.interleaved) {
+          #pragma unroll
+          for (int i = 0; i < V; i += 2) y[i] = x[j][i + 1], y[i + 1] = x[j][i];
+        }
+        if (d0 < p.rot) {  // a cos - b sin, b cos + a sin: the difference is the sum with the product's sign turned
+          #pragma unroll
+          for (int i = 0; i < V; ++i) x[j][i] = __fadd_rn(__fmul_rn(x[j][i], cs[i]), __fmul_rn(y[i], sn[i]));
+        }
+      }
+    }
+    if (is_q) {
+      store_row<V>(p.qo + tok * p.ldqo + h * D + d0, vec, x[j]);
+    } else if constexpr (!kCache) {
+      store_row<V>(p.ko + tok * p.ldko + (h - p.n_q) * D + d0, vec, x[j]);
+    } else {
+      const uint32_t b = tok / static_cast<uint32_t>(p.m);
+      const int kvh = h - p.n_q - (is_v ? p.n_kv : 0);
+      const long long had = __ldg(p.len + b);
+      if (had < 0) continue;  // an idle sequence
+      const long long slot = had + (tok - b * static_cast<uint32_t>(p.m));
+      if (slot >= c.cap) {
+        if (lane == 0) atomicCAS(err, 0, kDevKv4Slot);
+        continue;
+      }
+      kv4_store_row<D>(x[j], is_v ? c.v : c.k, is_v ? c.vs : c.ks, (static_cast<long long>(b) * c.n_kv + kvh) * c.cap + slot);
+    }
   }
 }
 
@@ -248,43 +286,56 @@ __device__ __forceinline__ void kv4_unpack(uint32_t w, __half2 step, __half2 bas
   }
 }
 
-// Values as halves: one thread per code word (8 columns) of K and of V. Rows
+// Values as halves: a thread takes code words (8 columns) of K and of V. Rows
 // start[b] + i, i < count; a row at or behind end[b] reads as zeros. Bound by
-// the halves it writes (4 d bytes a slot against 1.25 d read).
+// the halves it writes (4 d bytes a slot against 1.25 d read). Grid: (words,
+// n_seq * n_kv).
+constexpr int kReadWords = 2;  // of K, and as many of V, that a thread has in flight
+
 template <int D>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4View c, const int32_t* __restrict__ start,
-                                                       const int32_t* __restrict__ end, long long count,
+                                                       const int32_t* __restrict__ end, int count,
                                                        __half* __restrict__ ko, __half* __restrict__ vo,
                                                        int* __restrict__ err) {
   constexpr int W = D / 8;
-  const long long rows = static_cast<long long>(c.n_seq) * c.n_kv * count;
-  for (long long t = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; t < rows * W * 2;
-       t += static_cast<long long>(gridDim.x) * 256) {
-    const bool is_v = t >= rows * W;
-    const long long u = is_v ? t - rows * W : t;
-    const long long r = u / W;
-    const int w = static_cast<int>(u % W);
-    const long long bh = r / count;
-    const long long b = bh / c.n_kv;
-    const long long slot = __ldg(start + b) + (r - bh * count);
-    uint4 o = make_uint4(0, 0, 0, 0);
-    if (slot < __ldg(end + b)) {
-      if (slot < 0 || slot >= c.cap) {
-        atomicCAS(err, 0, kDevKv4Slot);
-      } else {
-        const long long at = bh * c.cap + slot;
-        const uint32_t word = __ldg(reinterpret_cast<const uint32_t*>(is_v ? c.v : c.k) + at * W + w);
-        const uint32_t sb = __ldg((is_v ? c.vs : c.ks) + at * (D / kKv4Group) + w / 4);
-        const __half2 sb2 = *reinterpret_cast<const __half2*>(&sb);
+  pdl_wait_prior();
+  pdl_launch_dependents();
+  for (long long bh = blockIdx.y; bh < static_cast<long long>(c.n_seq) * c.n_kv; bh += gridDim.y) {
+    const int b = static_cast<int>(bh / c.n_kv);
+    const long long s0 = __ldg(start + b), e = __ldg(end + b);
+    uint32_t word[kReadWords][2], sb[kReadWords][2];
+    #pragma unroll
+    for (int i = 0; i < kReadWords; ++i) {
+      const long long t = static_cast<long long>(blockIdx.x) * (256 * kReadWords) + i * 256 + threadIdx.x;
+      const int r = static_cast<int>(t / W), w = threadIdx.x % W;
+      const long long slot = s0 + r, at = bh * c.cap + slot;
+      const bool on = r < count && slot < e;
+      const bool in = slot >= 0 && slot < c.cap;
+      if (on && !in) atomicCAS(err, 0, kDevKv4Slot);
+      word[i][0] = word[i][1] = sb[i][0] = sb[i][1] = 0;
+      if (on && in) {
+        word[i][0] = __ldg(reinterpret_cast<const uint32_t*>(c.k) + at * W + w);
+        word[i][1] = __ldg(reinterpret_cast<const uint32_t*>(c.v) + at * W + w);
+        sb[i][0] = __ldg(c.ks + at * (D / kKv4Group) + w / 4);
+        sb[i][1] = __ldg(c.vs + at * (D / kKv4Group) + w / 4);
+      }
+    }
+    #pragma unroll
+    for (int i = 0; i < kReadWords; ++i) {
+      const long long t = static_cast<long long>(blockIdx.x) * (256 * kReadWords) + i * 256 + threadIdx.x;
+      if (t / W >= count) break;
+      #pragma unroll
+      for (int z = 0; z < 2; ++z) {
+        const __half2 sb2 = *reinterpret_cast<const __half2*>(&sb[i][z]);
         __half2 h[4];
-        kv4_unpack(word, __low2half2(sb2), __high2half2(sb2), h);
+        kv4_unpack(word[i][z], __low2half2(sb2), __high2half2(sb2), h);
         const __half2 p01 = __lows2half2(h[0], h[1]), p23 = __lows2half2(h[2], h[3]);
         const __half2 p45 = __highs2half2(h[0], h[1]), p67 = __highs2half2(h[2], h[3]);
-        o = make_uint4(*reinterpret_cast<const uint32_t*>(&p01), *reinterpret_cast<const uint32_t*>(&p23),
+        reinterpret_cast<uint4*>(z ? vo : ko)[bh * count * W + t] =
+            make_uint4(*reinterpret_cast<const uint32_t*>(&p01), *reinterpret_cast<const uint32_t*>(&p23),
                        *reinterpret_cast<const uint32_t*>(&p45), *reinterpret_cast<const uint32_t*>(&p67));
       }
     }
-    *reinterpret_cast<uint4*>((is_v ? vo : ko) + r * D + w * 8) = o;
   }
 }
 
@@ -298,127 +349,222 @@ __device__ __forceinline__ uint32_t kv4_weight_key(float w) {
 }
 
 constexpr int kEvictThreads = 1024;
+constexpr int kEvictMaxCluster = 8;
+constexpr int kEvictBins = 2048;   // 11 bits a pass of the radix select: 11, 11, 10
+constexpr int kEvictKeys = 44 * 1024;  // keys that a CTA's shared memory holds
 
-// One CTA per (sequence, kv head) picks the slots to keep. The first `first`
-// and the last `recent` are kept; of the others the `keep - first - recent`
-// largest weights, found by a radix select of 8 bits a pass (histogram, then
-// the bin that holds the wanted rank): T, the key of the last one kept, and how
-// many keys equal to T are kept, lowest slots first. A last pass writes the kept
-// slots in order. len_out[b] = min(len, keep).
-__global__ void __launch_bounds__(kEvictThreads)
-    kv4_select_kernel(const float* __restrict__ w, const int32_t* __restrict__ len, long long cap, int n_kv, int keep,
-                      int first, int recent, int32_t* __restrict__ idx, float* __restrict__ w_out,
-                      int32_t* __restrict__ len_out, int* __restrict__ err) {
-  __shared__ uint32_t hist[256];
-  __shared__ uint32_t s_prefix, s_rank;
-  __shared__ uint32_t warp_eq[32], warp_kept[32];
-  const int bh = blockIdx.x, b = bh / n_kv, tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
-  long long n = __ldg(len + b);
-  if (n > cap) {
-    if (tid == 0) atomicCAS(err, 0, kDevKv4Slot);
-    n = cap;
+// Shared memory: a histogram, the scans' words, the CTA's keys (and later its kept slots).
+__host__ __device__ constexpr int evict_smem_bytes(int keys) { return kEvictBins * 4 + 256 + keys * 4; }
+
+struct Kv4Evict {
+  const float* w;
+  const int32_t* len;
+  int32_t* idx;
+  float* w_out;
+  int32_t* len_out;
+  int keep, first, recent;
+  int keys;  // keys of a share that lie in shared memory; the others are read again
+};
+
+// An exclusive sum over the block's threads and the total; scratch: 33 words.
+__device__ __forceinline__ int block_scan(int v, int* scratch, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = v;
+  #pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
   }
-  if (n < 0) n = 0;
-  const float* wr = w + static_cast<long long>(bh) * cap;
-  int32_t* io = idx + static_cast<long long>(bh) * keep;
-  float* wo = w_out ? w_out + static_cast<long long>(bh) * keep : nullptr;
-  if (bh % n_kv == 0 && tid == 0) len_out[b] = static_cast<int32_t>(n < keep ? n : keep);
-  if (keep == 0) return;  // w and idx may be null
-  if (n <= keep) {
-    for (int i = tid; i < keep; i += kEvictThreads) {
-      io[i] = i < n ? i : -1;
-      if (wo) wo[i] = i < n ? wr[i] : 0.f;
+  if (lane == 31) scratch[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    int s = scratch[lane];
+    #pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += y;
     }
-    return;
+    scratch[lane] = s;
   }
-  const int lo = first, hi = static_cast<int>(n) - recent;  // candidates
-  const uint32_t want = static_cast<uint32_t>(keep - first - recent);
-  uint32_t prefix = 0, rank = want;  // the rank-th largest among keys with this prefix
-  if (want > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += kEvictThreads) hist[i] = 0;
-      __syncthreads();
-      for (int i = lo + tid; i < hi; i += kEvictThreads) {
-        const uint32_t key = kv4_weight_key(wr[i]);
-        if (shift == 24 || (key >> (shift + 8)) == prefix) atomicAdd(&hist[(key >> shift) & 255], 1u);
-      }
-      __syncthreads();
-      if (tid == 0) {
-        uint32_t above = 0;
-        int bin = 255;
-        for (; bin > 0; --bin) {
-          if (above + hist[bin] >= rank) break;
-          above += hist[bin];
-        }
-        s_prefix = (prefix << 8) | static_cast<uint32_t>(bin);
-        s_rank = rank - above;
-      }
-      __syncthreads();
-      prefix = s_prefix;
-      rank = s_rank;
-      __syncthreads();
-    }
-  }
-  // prefix = T, rank = how many of the keys equal to T are kept (0 where nothing is wanted)
-  uint32_t eq_seen = 0, kept = 0;
-  for (int i0 = 0; i0 < n; i0 += kEvictThreads) {
-    const int i = i0 + tid;
-    const bool in = i < n;
-    const bool cand = in && i >= lo && i < hi;
-    const float x = in ? wr[i] : 0.f;
-    const uint32_t key = kv4_weight_key(x);
-    const bool eq = cand && want > 0 && key == prefix;
-    const uint32_t below = (1u << lane) - 1u;
-    const uint32_t eq_mask = __ballot_sync(0xffffffffu, eq);
-    if (lane == 0) warp_eq[wid] = __popc(eq_mask);
-    __syncthreads();
-    uint32_t eq_before = eq_seen, eq_total = 0;
-    for (int j = 0; j < 32; ++j) {
-      if (j < wid) eq_before += warp_eq[j];
-      eq_total += warp_eq[j];
-    }
-    const bool take = in && (!cand || (want > 0 && key > prefix) ||
-                             (eq && eq_before + __popc(eq_mask & below) < rank));
-    const uint32_t mask = __ballot_sync(0xffffffffu, take);
-    if (lane == 0) warp_kept[wid] = __popc(mask);
-    __syncthreads();
-    uint32_t at = kept, total = 0;
-    for (int j = 0; j < 32; ++j) {
-      if (j < wid) at += warp_kept[j];
-      total += warp_kept[j];
-    }
-    at += __popc(mask & below);
-    if (take && at < static_cast<uint32_t>(keep)) {
-      io[at] = i;
-      if (wo) wo[at] = x;
-    }
-    eq_seen += eq_total;
-    kept += total;
-    __syncthreads();
-  }
+  __syncthreads();
+  const int before = warp ? scratch[warp - 1] : 0;
+  *total = scratch[31];
+  __syncthreads();
+  return before + x - v;
 }
 
-// Kept rows to the other cache: one thread per 16 bytes of codes of K or V, the
-// steps and bases beside them.
+__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// One cluster per (sequence, kv head), each CTA an equal share of the slots.
+// The first `first` and the last `recent` slots are kept; of the others the
+// `keep - first - recent` largest weights, found by a radix select over order-
+// preserving keys: T, the key of the last one kept, and how many keys equal to
+// T are kept, lowest slots first. Each pass counts the keys that share the
+// digits found so far by their next digit, in the CTA, then adds the cluster's
+// counts; the keys are read from global memory once and stay in shared memory.
+// Then every CTA knows what it keeps and where its first kept slot goes, and
+// moves its rows. Bound by HBM for long caches (4 bytes a slot, 2.5 d a kept
+// one), by the passes' barriers for short ones.
 template <int D>
-__global__ void __launch_bounds__(256) kv4_move_kernel(const Kv4View src, const Kv4View dst, const int32_t* __restrict__ idx,
-                                                       int keep) {
-  constexpr int U = D / 32;  // 16-byte units of codes in a row, and words of (step, base)
-  const long long rows = static_cast<long long>(src.n_seq) * src.n_kv * keep;
-  for (long long t = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; t < rows * U * 2;
-       t += static_cast<long long>(gridDim.x) * 256) {
-    const bool is_v = t >= rows * U;
-    const long long u = is_v ? t - rows * U : t;
-    const long long r = u / U;
-    const int i = static_cast<int>(u % U);
-    const int from = __ldg(idx + r);
-    if (from < 0) continue;
-    const long long bh = r / keep;
-    const long long s = bh * src.cap + from, d = bh * dst.cap + (r - bh * keep);
-    reinterpret_cast<uint4*>(is_v ? dst.v : dst.k)[d * U + i] =
-        __ldg(reinterpret_cast<const uint4*>(is_v ? src.v : src.k) + s * U + i);
-    (is_v ? dst.vs : dst.ks)[d * U + i] = __ldg((is_v ? src.vs : src.ks) + s * U + i);
+__global__ void __launch_bounds__(kEvictThreads, 1)
+    kv4_evict_kernel(const Kv4Evict p, const Kv4View src, const Kv4View dst, int* __restrict__ err) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  uint32_t* hist = reinterpret_cast<uint32_t*>(smem);            // [kEvictBins]
+  int* scratch = reinterpret_cast<int*>(hist + kEvictBins);      // [33 + 31]
+  uint32_t* keys = reinterpret_cast<uint32_t*>(scratch + 64);    // [p.keys]
+  __shared__ int s_pick[2], s_count[2];
+  const int tid = threadIdx.x;
+  const uint32_t rank = cluster_ctarank();
+  uint32_t size;
+  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(size));
+  const int bh = blockIdx.y, b = bh / src.n_kv;
+  pdl_wait_prior();
+  pdl_launch_dependents();
+  long long n_all = __ldg(p.len + b);
+  if (n_all > src.cap) {
+    if (tid == 0 && rank == 0) atomicCAS(err, 0, kDevKv4Slot);
+    n_all = src.cap;
   }
+  const int n = n_all < 0 ? 0 : static_cast<int>(n_all), keep = p.keep;
+  if (bh - b * src.n_kv == 0 && rank == 0 && tid == 0) p.len_out[b] = min(n, keep);
+  if (keep == 0) return;  // w and idx may be null
+  const int i0 = static_cast<int>(static_cast<long long>(n) * rank / size);
+  const int i1 = static_cast<int>(static_cast<long long>(n) * (rank + 1) / size);
+  const float* w = p.w + static_cast<long long>(bh) * src.cap;
+  int32_t* io = p.idx + static_cast<long long>(bh) * keep;
+  float* wo = p.w_out ? p.w_out + static_cast<long long>(bh) * keep : nullptr;
+  const int lo = p.first, hi = n - p.recent;  // the slots that the weights decide about
+  const bool all = n <= keep;
+  uint32_t prefix = 0;
+  int want = all ? 0 : keep - p.first - p.recent;  // the want-th largest of the keys that begin with prefix
+  auto key_at = [&](int i) { return i - i0 < p.keys ? keys[i - i0] : kv4_weight_key(__ldg(w + i)); };
+  if (want > 0) {  // the same in the whole cluster
+    for (int i = i0 + tid; i < min(i1, i0 + p.keys); i += kEvictThreads) keys[i - i0] = kv4_weight_key(__ldg(w + i));
+    #pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+      for (int i = tid; i < kEvictBins; i += kEvictThreads) hist[i] = 0;
+      __syncthreads();
+      // equal neighbours in a thread's sequence are counted together: many slots may have the same weight
+      int last = -1, run = 0;
+      for (int i = max(i0, lo) + tid; i < min(i1, hi); i += kEvictThreads) {
+        const uint32_t key = key_at(i);
+        if (pass > 0 && (key >> (shift + bits)) != prefix) continue;
+        const int bin = static_cast<int>(key >> shift & ((1u << bits) - 1u));
+        if (bin != last) {
+          if (run) atomicAdd(hist + last, static_cast<uint32_t>(run));
+          last = bin, run = 0;
+        }
+        ++run;
+      }
+      if (run) atomicAdd(hist + last, static_cast<uint32_t>(run));
+      __syncthreads();
+      if (size > 1) cluster_sync();
+      // thread t has bins kEvictBins - 1 - 2 t and the one below: a sum from the top
+      uint32_t c[2] = {0, 0};
+      const int top = kEvictBins - 1 - 2 * tid;
+      #pragma unroll
+      for (int z = 0; z < 2; ++z) {
+        if (size == 1) {
+          c[z] = hist[top - z];
+        } else {
+          const uint32_t addr = smem_u32(hist + top - z);
+          for (uint32_t r = 0; r < size; ++r) c[z] += ld_cluster_u32(mapa_shared(addr, r));
+        }
+      }
+      int total;
+      const int above = block_scan(static_cast<int>(c[0] + c[1]), scratch, &total);
+      if (above < want && above + static_cast<int>(c[0]) >= want) s_pick[0] = top, s_pick[1] = want - above;
+      if (above + static_cast<int>(c[0]) < want && above + static_cast<int>(c[0] + c[1]) >= want)
+        s_pick[0] = top - 1, s_pick[1] = want - above - static_cast<int>(c[0]);
+      __syncthreads();
+      prefix = prefix << bits | static_cast<uint32_t>(s_pick[0]);
+      want = s_pick[1];
+      if (size > 1) cluster_sync();  // the counts have been read
+      else __syncthreads();
+    }
+  }
+  // prefix = T, want = how many of the keys equal to T are kept (all kept: 0, not asked). A warp takes neighbouring
+  // slots, 32 at a time; the counts of keys above T (and of what is kept anyway) and equal to T before it say where it
+  // writes.
+  const int lane = tid & 31, warp = tid >> 5;
+  const int each = (i1 - i0 + kEvictThreads - 1) / kEvictThreads * 32;
+  const int t0 = min(i1, i0 + warp * each), t1 = min(i1, t0 + each);
+  const bool pick = !all && keep - p.first - p.recent > 0;
+  auto look = [&](int i, bool& sure, bool& equal) {
+    sure = i < t1 && (all || i < lo || i >= hi), equal = false;
+    if (i < t1 && !sure && pick) {
+      const uint32_t key = key_at(i);
+      sure = key > prefix, equal = key == prefix;
+    }
+  };
+  int sure_n = 0, equal_n = 0;
+  for (int i = t0 + lane; i - lane < t1; i += 32) {
+    bool sure, equal;
+    look(i, sure, equal);
+    sure_n += __popc(__ballot_sync(0xffffffffu, sure)), equal_n += __popc(__ballot_sync(0xffffffffu, equal));
+  }
+  __syncthreads();  // scratch is free
+  if (lane == 0) scratch[warp] = sure_n, scratch[32 + warp] = equal_n;
+  __syncthreads();
+  const int sure_w = scratch[lane], equal_w = scratch[32 + lane];
+  const int all_sure = __reduce_add_sync(0xffffffffu, sure_w), all_equal = __reduce_add_sync(0xffffffffu, equal_w);
+  int s_seen = __reduce_add_sync(0xffffffffu, lane < warp ? sure_w : 0);
+  int e_seen = __reduce_add_sync(0xffffffffu, lane < warp ? equal_w : 0);
+  int cta_sure = 0, cta_equal = 0;  // of the CTAs before
+  if (size > 1) {
+    if (tid == 0) s_count[0] = all_sure, s_count[1] = all_equal;
+    cluster_sync();
+    for (uint32_t r = 0; r < rank; ++r) {
+      cta_sure += static_cast<int>(ld_cluster_u32(mapa_shared(smem_u32(s_count), r)));
+      cta_equal += static_cast<int>(ld_cluster_u32(mapa_shared(smem_u32(s_count + 1), r)));
+    }
+  }
+  // where a slot goes: behind the sure ones before it, and the equal ones before it as far as they are kept
+  const int base = cta_sure + min(want, cta_equal);  // the CTA's first
+  s_seen += cta_sure, e_seen += cta_equal;
+  const uint32_t below = (1u << lane) - 1u;
+  for (int i = t0 + lane; i - lane < t1; i += 32) {
+    bool sure, equal;
+    look(i, sure, equal);
+    const uint32_t ms = __ballot_sync(0xffffffffu, sure), me = __ballot_sync(0xffffffffu, equal);
+    const int e_before = e_seen + __popc(me & below);
+    if (sure || (equal && e_before < want)) {
+      const int at = s_seen + __popc(ms & below) + min(want, e_before);
+      io[at] = i;
+      if (wo) wo[at] = __ldg(w + i);
+    }
+    s_seen += __popc(ms), e_seen += __popc(me);
+  }
+  const int mine = all_sure + min(max(want - cta_equal, 0), all_equal);
+  if (rank + 1 == size)
+    for (int i = base + mine + tid; i < keep; i += kEvictThreads) {
+      io[i] = -1;
+      if (wo) wo[i] = 0.f;
+    }
+  __syncthreads();  // io is read below by other threads of the CTA
+  // The rows: units of 16 bytes, U of K's codes, U of V's, and their steps and bases (d = 64: 8 bytes each, by words).
+  constexpr int U = D / 32;
+  const long long from0 = static_cast<long long>(bh) * src.cap, to0 = static_cast<long long>(bh) * dst.cap;
+  const uint4 *sk = reinterpret_cast<const uint4*>(src.k), *sv = reinterpret_cast<const uint4*>(src.v);
+  uint4 *dk = reinterpret_cast<uint4*>(dst.k), *dv = reinterpret_cast<uint4*>(dst.v);
+  #pragma unroll 2
+  for (int x = tid; x < mine * U; x += kEvictThreads) {
+    const int at = base + x / U, u = x % U;
+    const long long from = (from0 + io[at]) * U + u, to = (to0 + at) * U + u;
+    const uint4 k = __ldg(sk + from), v = __ldg(sv + from);
+    const uint32_t ks = __ldg(src.ks + from), vs = __ldg(src.vs + from);
+    dk[to] = k, dv[to] = v;
+    dst.ks[to] = ks, dst.vs[to] = vs;
+  }
+  if (size > 1) cluster_sync();  // no CTA leaves while another may read its counts
 }
 
 }  // namespace vmlm

@@ -58,16 +58,43 @@ int kv4_check_rope(const char* what, const vmlm_rope* r, size_t d) {
   return VMLM_OK;
 }
 
+template <int D, bool kCache>
+int kv4_launch_rows_d(Ctx* ctx, Kv4Rows p, const Kv4View& v, cudaStream_t st) {
+  const long long heads = p.n_q + p.n_kv + (kCache ? p.n_kv : 0);
+  // Four rows a warp once that still gives every SM 16 warps; below, a row a warp.
+  const int r = p.tokens * heads >= static_cast<long long>(ctx->sms) * 16 * 4 ? 4 : 1;
+  const long long warps = p.tokens * cdiv(heads, r);
+  if (warps == 0) return VMLM_OK;
+  if (warps >= static_cast<long long>(kKv4MaxDim))
+    return fail(VMLM_ERR_SHAPE, "tokens x heads is too large (%lld rows)", p.tokens * heads);
+  p.vec_g = (!p.gq || aligned16(p.gq)) && (!p.gk || aligned16(p.gk));
+  const dim3 grid(static_cast<unsigned>(cdiv(warps, 8)));
+  if (r == 4) return launch(kv4_rows_kernel<D, kCache, 4>, grid, dim3(256), 0, st, true, p, v, ctx->err);
+  return launch(kv4_rows_kernel<D, kCache, 1>, grid, dim3(256), 0, st, true, p, v, ctx->err);
+}
+
 template <bool kCache>
 int kv4_launch_rows(Ctx* ctx, const Kv4Rows& p, const Kv4View& v, size_t d, cudaStream_t st) {
-  const long long rows = p.tokens * (p.n_q + p.n_kv + (kCache ? p.n_kv : 0));
-  if (rows == 0) return VMLM_OK;
-  if (cdiv(rows, 8) >= static_cast<long long>(kKv4MaxDim))
-    return fail(VMLM_ERR_SHAPE, "tokens x heads is too large (%lld rows)", rows);
-  const dim3 grid(static_cast<unsigned>(cdiv(rows, 8)));
-  if (d == 64) return launch(kv4_rows_kernel<64, kCache>, grid, dim3(256), 0, st, false, p, v, ctx->err);
-  if (d == 128) return launch(kv4_rows_kernel<128, kCache>, grid, dim3(256), 0, st, false, p, v, ctx->err);
-  return launch(kv4_rows_kernel<256, kCache>, grid, dim3(256), 0, st, false, p, v, ctx->err);
+  if (d == 64) return kv4_launch_rows_d<64, kCache>(ctx, p, v, st);
+  if (d == 128) return kv4_launch_rows_d<128, kCache>(ctx, p, v, st);
+  return kv4_launch_rows_d<256, kCache>(ctx, p, v, st);
+}
+
+template <int D>
+int kv4_launch_evict(Ctx* ctx, Kv4Evict p, const Kv4View& s, const Kv4View& d, cudaStream_t st) {
+  static bool set[64] = {};
+  if (ctx->dev < 64 && !set[ctx->dev]) {
+    VMLM_CUDA(cudaFuncSetAttribute(kv4_evict_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   evict_smem_bytes(kEvictKeys)));
+    set[ctx->dev] = true;
+  }
+  // CTAs a head: as many as leave no SM without one, while each still has a thousand slots.
+  const long long heads = static_cast<long long>(s.n_seq) * s.n_kv;
+  int size = 1;
+  while (size < kEvictMaxCluster && heads * size * 2 <= ctx->sms && s.cap > 1024ll * size) size *= 2;
+  p.keys = static_cast<int>(std::min<long long>(kEvictKeys, cdiv(s.cap, size)));
+  return launch_ex(kv4_evict_kernel<D>, dim3(size, static_cast<unsigned>(heads)), dim3(kEvictThreads),
+                   evict_smem_bytes(p.keys), st, true, size, p, s, d, ctx->err);
 }
 
 void kv4_set_rope(Kv4Rows* p, const vmlm_rope* r) {
@@ -203,13 +230,15 @@ int vmlm_kv4_read_dev(const vmlm_kv4* cache, const int32_t* start, const int32_t
   VMLM_TRY(current_ctx(&ctx));
   cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
   const Kv4View c = kv4_view(cache);
-  const long long work = static_cast<long long>(c.n_seq) * c.n_kv * static_cast<long long>(count) * (cache->d / 8) * 2;
-  const dim3 grid(static_cast<unsigned>(std::min<long long>(cdiv(work, 256), 1 << 30)));
-  const long long n = static_cast<long long>(count);
+  const long long words = static_cast<long long>(count) * static_cast<long long>(cache->d / 8);
+  const long long blocks = cdiv(words, 256 * kReadWords);
+  if (blocks >= static_cast<long long>(kKv4MaxDim)) return fail(VMLM_ERR_SHAPE, "%s: count is too large", what);
+  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(std::min<long long>(static_cast<long long>(c.n_seq) * c.n_kv, 65535)));
+  const int n = static_cast<int>(count);
   __half *ko = reinterpret_cast<__half*>(k), *vo = reinterpret_cast<__half*>(v);
-  if (cache->d == 64) return launch(kv4_read_kernel<64>, grid, dim3(256), 0, st, false, c, start, end, n, ko, vo, ctx->err);
-  if (cache->d == 128) return launch(kv4_read_kernel<128>, grid, dim3(256), 0, st, false, c, start, end, n, ko, vo, ctx->err);
-  return launch(kv4_read_kernel<256>, grid, dim3(256), 0, st, false, c, start, end, n, ko, vo, ctx->err);
+  if (cache->d == 64) return launch(kv4_read_kernel<64>, grid, dim3(256), 0, st, true, c, start, end, n, ko, vo, ctx->err);
+  if (cache->d == 128) return launch(kv4_read_kernel<128>, grid, dim3(256), 0, st, true, c, start, end, n, ko, vo, ctx->err);
+  return launch(kv4_read_kernel<256>, grid, dim3(256), 0, st, true, c, start, end, n, ko, vo, ctx->err);
 }
 
 int vmlm_kv4_attn_dev(const vmlm_kv4* cache, const float* q, size_t ldq, const int32_t* len, float* out, size_t ldo,
@@ -267,17 +296,14 @@ int vmlm_kv4_evict_dev(const vmlm_kv4* src, const vmlm_kv4* dst, const float* w,
   VMLM_TRY(current_ctx(&ctx));
   cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
   const Kv4View s = kv4_view(src), d = kv4_view(dst);
-  VMLM_TRY(launch(kv4_select_kernel, dim3(static_cast<unsigned>(s.n_seq) * s.n_kv), dim3(kEvictThreads), 0, st, false,
-                  w, len, s.cap, s.n_kv, static_cast<int>(keep), static_cast<int>(first), static_cast<int>(recent),
-                  idx, w_out, len_out, ctx->err));
-  const long long work = static_cast<long long>(s.n_seq) * s.n_kv * static_cast<long long>(keep) * (src->d / 32) * 2;
-  if (work == 0) return VMLM_OK;
-  const dim3 grid(static_cast<unsigned>(std::min<long long>(cdiv(work, 256), 1 << 30)));
-  const int kp = static_cast<int>(keep);
-  const int32_t* ci = idx;
-  if (src->d == 64) return launch(kv4_move_kernel<64>, grid, dim3(256), 0, st, false, s, d, ci, kp);
-  if (src->d == 128) return launch(kv4_move_kernel<128>, grid, dim3(256), 0, st, false, s, d, ci, kp);
-  return launch(kv4_move_kernel<256>, grid, dim3(256), 0, st, false, s, d, ci, kp);
+  if (static_cast<long long>(s.n_seq) * s.n_kv >= 65536)
+    return fail(VMLM_ERR_SHAPE, "%s: n_seq * n_kv must be < 65536", what);
+  Kv4Evict p = {};
+  p.w = w, p.len = len, p.idx = idx, p.w_out = w_out, p.len_out = len_out;
+  p.keep = static_cast<int>(keep), p.first = static_cast<int>(first), p.recent = static_cast<int>(recent);
+  if (src->d == 64) return kv4_launch_evict<64>(ctx, p, s, d, st);
+  if (src->d == 128) return kv4_launch_evict<128>(ctx, p, s, d, st);
+  return kv4_launch_evict<256>(ctx, p, s, d, st);
 }
 
 }  // extern "C"

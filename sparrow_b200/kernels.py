@@ -34,6 +34,16 @@ def _host_ptr(x, dtype, count, name):
     return ctypes.c_void_p(x.ctypes.data) if x.size else None
 
 
+_dtype_names = {}  # torch dtype -> its name: str(dtype) costs more than all other checks of a tensor
+
+
+def _dtype_name(dt):
+    name = _dtype_names.get(dt)
+    if name is None:
+        name = _dtype_names[dt] = str(dt).replace("torch.", "")
+    return name
+
+
 def _dev_ptr(x, dtype_name, count, name):
     if x is None:
         return None
@@ -41,7 +51,7 @@ def _dev_ptr(x, dtype_name, count, name):
         return ctypes.c_void_p(x)
     if not getattr(x, "is_cuda", False):
         raise ValueError(f"{name}: expected a CUDA tensor or a device address")
-    if str(x.dtype) != f"torch.{dtype_name}":
+    if _dtype_name(x.dtype) != dtype_name:
         raise ValueError(f"{name}: expected torch.{dtype_name}, got {x.dtype}")
     if not x.is_contiguous():
         raise ValueError(f"{name}: must be contiguous")
@@ -418,11 +428,12 @@ def emb_dev(table, idx, out, stream=None) -> None:
 
 def _rows_ptr(x, rows, width, name):
     """(address, row stride) of a [rows, >= width] float32 CUDA tensor whose rows may be slices of wider ones."""
-    if str(x.dtype) != "torch.float32" or not x.is_cuda:
+    if not x.is_cuda or _dtype_name(x.dtype) != "float32":
         raise ValueError(f"{name}: expected a float32 CUDA tensor")
-    if x.dim() != 2 or x.shape[0] < rows or x.shape[1] < width or (x.shape[1] > 1 and x.stride(1) != 1):
-        raise ValueError(f"{name}: needs {rows} rows of {width} values with unit column stride, has {tuple(x.shape)}")
-    return x.data_ptr(), x.stride(0) if x.shape[0] > 1 else max(x.stride(0), x.shape[1])
+    shape, stride = x.shape, x.stride()
+    if len(shape) != 2 or shape[0] < rows or shape[1] < width or (stride[1] != 1 and shape[1] > 1):
+        raise ValueError(f"{name}: needs {rows} rows of {width} values with unit column stride, has {tuple(shape)}")
+    return x.data_ptr(), stride[0] if shape[0] > 1 else max(stride[0], shape[1])
 
 
 class Rope:
