@@ -50,7 +50,7 @@ struct Kv4Rows {
   long long tokens, n_pos, m; // m tokens of each sequence
   float eps;
   int n_q, n_kv, rot, interleaved;
-  int vec, vec_g;             // every row starts on a 16-byte boundary; so do the gains
+  int vec, vec_g, vec_t;      // every row starts on a 16-byte boundary; so do the gains, and the table's rows
 };
 
 __device__ __forceinline__ uint32_t kv4_pack_sb(float step, float base) {
@@ -90,68 +90,68 @@ __device__ __forceinline__ void load_row(const float* __restrict__ p, bool vec, 
   }
 }
 
-template <int V>
-__device__ __forceinline__ void store_row(float* __restrict__ p, bool vec, const float (&x)[V]) {
+__device__ __forceinline__ void store4(float* p, bool vec, const float* x) {
   if (vec) {
-    if constexpr (V == 2) {
-      *reinterpret_cast<float2*>(p) = make_float2(x[0], x[1]);
-    } else {
-      #pragma unroll
-      for (int i = 0; i < V; i += 4) *reinterpret_cast<float4*>(p + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
-    }
+    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
   } else {
     #pragma unroll
-    for (int i = 0; i < V; ++i) p[i] = x[i];
+    for (int i = 0; i < 4; ++i) p[i] = x[i];
   }
 }
 
-// Quantise the row that a warp holds (lane l has columns V*l .. V*l + V - 1)
-// and store it. Every step is one IEEE operation in f32, so the codes are those
-// of the definition evaluated in f32 by any other program.
+// How a row lies in the D/8 lanes that hold it: lane l has columns 4 l .. 4 l + 3
+// (x[0..3]) and D/2 + 4 l .. (x[4..7]), so 16-byte accesses of neighbouring lanes
+// are contiguous, the pairs (i, i + d/2) of a full rotation meet in one lane, and
+// a warp does 256 / d rows with one instruction.
+
+// Quantise and store the rows that a warp holds; `on` lanes' rows are stored.
+// Every step is one IEEE operation in f32, so the codes are those of the
+// definition evaluated in f32 by any other program.
 template <int D>
-__device__ __forceinline__ void kv4_store_row(const float (&x)[D / 32], uint8_t* codes, uint32_t* sb, long long row) {
-  constexpr int V = D / 32;
-  constexpr int kLanes = kKv4Group / V;  // lanes of one group
-  const int lane = threadIdx.x & 31;
-  float c[V];
+__device__ __forceinline__ void kv4_store_rows(const float (&x)[8], bool on, uint8_t* codes, uint32_t* sb,
+                                               long long row) {
+  constexpr int L = D / 8;
+  const int l = threadIdx.x & (L - 1);
   #pragma unroll
-  for (int i = 0; i < V; ++i) c[i] = min_nan(max_nan(x[i], -kKv4Clamp), kKv4Clamp);
-  float lo = c[0], hi = c[0];
-  #pragma unroll
-  for (int i = 1; i < V; ++i) lo = min_nan(lo, c[i]), hi = max_nan(hi, c[i]);
-  #pragma unroll
-  for (int o = kLanes / 2; o > 0; o >>= 1) {
-    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+  for (int h = 0; h < 2; ++h) {  // groups of 32 columns: 8 lanes of one half
+    float c[4];
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = min_nan(max_nan(x[4 * h + i], -kKv4Clamp), kKv4Clamp);
+    float lo = min_nan(min_nan(c[0], c[1]), min_nan(c[2], c[3])), hi = max_nan(max_nan(c[0], c[1]), max_nan(c[2], c[3]));
+    #pragma unroll
+    for (int o = 4; o > 0; o >>= 1) {
+      lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+    const float step = __half2float(__float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f)));
+    const float base = __half2float(__float2half_rn(__fsub_rn(lo, __fmul_rn(16.f, step))));
+    const float inv = step > 0.f ? __frcp_rn(step) : 0.f;
+    uint32_t bits = 0;
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float t = __fsub_rn(rintf(__fmul_rn(__fsub_rn(c[i], base), inv)), 16.f);
+      bits |= static_cast<uint32_t>(fminf(fmaxf(t, 0.f), 15.f)) << (4 * i);
+    }
+    if (on) {
+      *reinterpret_cast<uint16_t*>(codes + row * (D / 2) + h * (D / 4) + l * 2) = static_cast<uint16_t>(bits);
+      if ((l & 7) == 0) sb[row * (D / kKv4Group) + h * (D / 64) + l / 8] = kv4_pack_sb(step, base);
+    }
   }
-  const float step = __half2float(__float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f)));
-  const float base = __half2float(__float2half_rn(__fsub_rn(lo, __fmul_rn(16.f, step))));
-  const float inv = step > 0.f ? __fdiv_rn(1.f, step) : 0.f;
-  uint32_t bits = 0;
-  #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const float t = __fsub_rn(rintf(__fmul_rn(__fsub_rn(c[i], base), inv)), 16.f);
-    bits |= static_cast<uint32_t>(fminf(fmaxf(t, 0.f), 15.f)) << (4 * i);
-  }
-  uint8_t* dst = codes + row * (D / 2) + lane * (V / 2);
-  if constexpr (V == 2) *dst = static_cast<uint8_t>(bits);
-  if constexpr (V == 4) *reinterpret_cast<uint16_t*>(dst) = static_cast<uint16_t>(bits);
-  if constexpr (V == 8) *reinterpret_cast<uint32_t*>(dst) = bits;
-  if (lane % kLanes == 0) sb[row * (D / kKv4Group) + lane / kLanes] = kv4_pack_sb(step, base);
 }
 
-// The sum of a row's squares, s_i of columns V*l + i in lane l, added in halves
-// (columns c and c + d/2, then d/4, ...): the same tree, and so the same bits,
-// whatever the lanes hold. While a lane has several values, each exchange sends
-// one half of them and keeps the sums of the other, so a row of 128 takes 8
-// shuffles instead of 20: at 1 shuffle a cycle and SM, 20 of them and the
-// rotation's 4 are most of the 43 cycles that the row's bytes take.
-template <int V>
-__device__ __forceinline__ float tree_sum(float (&s)[V]) {
-  const int lane = threadIdx.x & 31;
-  int o = 16;
+// The sum of a row's squares, added in halves (columns c and c + d/2, then d/4,
+// ...): the same tree, and so the same bits, whatever the lanes hold. While a
+// lane has several values, each exchange sends one half of them and keeps the
+// sums of the other: 7 shuffles for the two rows of d = 128 that a warp holds.
+template <int D>
+__device__ __forceinline__ float tree_sum(const float (&x)[8]) {
+  constexpr int L = D / 8;
+  const int lane = threadIdx.x;
+  float s[4];
   #pragma unroll
-  for (int h = V / 2; h > 0; h /= 2, o >>= 1) {
+  for (int i = 0; i < 4; ++i) s[i] = __fadd_rn(__fmul_rn(x[i], x[i]), __fmul_rn(x[i + 4], x[i + 4]));
+  #pragma unroll
+  for (int h = 2, o = L / 2; h > 0; h /= 2, o /= 2) {
     const bool up = lane & o;
     #pragma unroll
     for (int i = 0; i < h; ++i) {
@@ -159,118 +159,172 @@ __device__ __forceinline__ float tree_sum(float (&s)[V]) {
       s[i] = __fadd_rn(mine, __shfl_xor_sync(0xffffffffu, other, o));
     }
   }
-  for (; o > 0; o >>= 1) s[0] = __fadd_rn(s[0], __shfl_xor_sync(0xffffffffu, s[0], o));
-  // lane bits 16, 8, ... now say which of the lane's values s[0] is the sum of
   #pragma unroll
-  for (int x = 16, h = V / 2; h > 0; h /= 2, x >>= 1) s[0] = __fadd_rn(s[0], __shfl_xor_sync(0xffffffffu, s[0], x));
-  return s[0];
+  for (int o = L / 8; o > 0; o /= 2) s[0] = __fadd_rn(s[0], __shfl_xor_sync(0xffffffffu, s[0], o));
+  // lane bits L/2 and L/4 say which of the four values s[0] is the sum of
+  s[0] = __fadd_rn(s[0], __shfl_xor_sync(0xffffffffu, s[0], L / 2));
+  return __fadd_rn(s[0], __shfl_xor_sync(0xffffffffu, s[0], L / 4));
 }
 
-// R rows (heads) of one token a warp: heads 0 .. n_q-1 are queries, then n_kv
-// keys, then (with a cache) n_kv values.
+__device__ __forceinline__ void load4(const float* p, bool vec, float* x) {
+  if (vec) {
+    const float4 t = *reinterpret_cast<const float4*>(p);
+    x[0] = t.x, x[1] = t.y, x[2] = t.z, x[3] = t.w;
+  } else {
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = p[i];
+  }
+}
+
+// Heads 0 .. n_q-1 of a token are queries, then n_kv keys, then (with a cache)
+// n_kv values; a warp takes R * 256 / d rows of one token.
 //   y = x * (1 / sqrt(sum(x^2) / d + eps)) * gain        (gain given)
 //   (a, b) -> (a cos - b sin, b cos + a sin)             (table given)
 // on the pairs (i, i + rot/2) or (2i, 2i + 1) of the first rot columns. Products
 // and sums are rounded one by one: a key's code must not depend on whether a
-// compiler fused them.
-// Bound by HBM: each value is read once and written once. R = 4 keeps four
-// rows' loads in flight a warp and reads the token's cos and sin once for them;
-// R = 1 spreads few rows over more warps.
+// compiler fused them. Queries and keys may be written in place: a row is read
+// whole before it is written, by the same lanes.
+// Bound by HBM: each value is read once and written once; of the instructions,
+// which are the next bound, the root and the tree count for 256 / d rows. R = 2
+// keeps more loads in flight; R = 1 spreads few rows over more warps.
 template <int D, bool kCache, int R>
 __global__ void __launch_bounds__(256) kv4_rows_kernel(const Kv4Rows p, const Kv4View c, int* __restrict__ err) {
-  constexpr int V = D / 32;
+  constexpr int L = D / 8, kRows = 32 / L;
   pdl_wait_prior();
   pdl_launch_dependents();
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, l = lane & (L - 1);
   const int heads = p.n_q + p.n_kv + (kCache ? p.n_kv : 0);
-  const uint32_t sets = static_cast<uint32_t>(heads + R - 1) / R;  // of R heads
+  const uint32_t sets = static_cast<uint32_t>(heads + R * kRows - 1) / (R * kRows);
   const uint32_t at = blockIdx.x * 8 + (threadIdx.x >> 5);
   const uint32_t tok = at / sets;
   if (tok >= p.tokens) return;
-  const int h0 = static_cast<int>(at - tok * sets) * R;
+  const int h0 = static_cast<int>(at - tok * sets) * (R * kRows) + lane / L;
   const bool vec = p.vec;
-  float x[R][V];
+  const float *q = p.q + tok * p.ldq, *k = p.k + tok * p.ldk, *v = p.v + tok * p.ldv;
+  float x[R][8];
   #pragma unroll
   for (int j = 0; j < R; ++j) {
-    const int h = h0 + j;
-    if (h >= heads) break;
-    const float* src = h < p.n_q ? p.q + tok * p.ldq + h * D
-                     : h < p.n_q + p.n_kv ? p.k + tok * p.ldk + (h - p.n_q) * D
-                                          : p.v + tok * p.ldv + (h - p.n_q - p.n_kv) * D;
-    load_row<V>(src + lane * V, vec, x[j]);
+    const int h = h0 + j * kRows;
+    const float* src = h < p.n_q ? q + h * D : h < p.n_q + p.n_kv ? k + (h - p.n_q) * D : v + (h - p.n_q - p.n_kv) * D;
+    if (h < heads) {
+      load4(src + 4 * l, vec, x[j]);
+      load4(src + D / 2 + 4 * l, vec, x[j] + 4);
+    } else {
+      #pragma unroll
+      for (int i = 0; i < 8; ++i) x[j][i] = 0.f;
+    }
   }
-  const int d0 = lane * V, half = p.rot / 2;
-  const bool turn = p.cos_t != nullptr;
-  const bool first = d0 < half;  // rot is a multiple of 16, so a lane's columns lie on one side
-  const int other = p.interleaved ? lane : (first ? lane + half / V : lane - half / V) & 31;
-  float cs[V], sn[V];  // of the lane's columns; the sine with the sign that its term has
-  #pragma unroll
-  for (int i = 0; i < V; ++i) cs[i] = 1.f, sn[i] = 0.f;
-  if (turn) {
+  // The token's cosines and sines of the lane's columns; columns behind rot: 1 and 0.
+  float cs[8], sn[8];
+  const int half = p.rot / 2;
+  const bool whole = !p.interleaved && p.rot == D;
+  if (p.cos_t) {
     const long long row = __ldg(p.pos + tok);
     if (row < 0 || row >= p.n_pos) {
       if (lane == 0) atomicCAS(err, 0, kDevRopePos);
       return;
     }
-    if (d0 < p.rot && h0 < p.n_q + p.n_kv) {
-      #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const long long e = row * half + (p.interleaved ? (d0 + i) / 2 : first ? d0 + i : d0 + i - half);
-        cs[i] = __ldg(p.cos_t + e);
-        const float s = __ldg(p.sin_t + e);
-        sn[i] = (p.interleaved ? (i & 1) == 0 : first) ? -s : s;
+    const float *ct = p.cos_t + row * half, *st = p.sin_t + row * half;
+    #pragma unroll
+    for (int z = 0; z < 2; ++z) {
+      const int c0 = z * (D / 2) + 4 * l;  // the lane's first column here
+      if (whole && z == 1) {
+        #pragma unroll
+        for (int i = 4; i < 8; ++i) cs[i] = cs[i - 4], sn[i] = sn[i - 4];
+      } else if (c0 >= p.rot) {
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) cs[4 * z + i] = 1.f, sn[4 * z + i] = 0.f;
+      } else if (p.interleaved) {
+        const int e = c0 / 2;
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) cs[4 * z + i] = __ldg(ct + e + i / 2), sn[4 * z + i] = __ldg(st + e + i / 2);
+      } else {
+        const int e = c0 < half ? c0 : c0 - half;
+        load4(ct + e, p.vec_t, cs + 4 * z);
+        load4(st + e, p.vec_t, sn + 4 * z);
       }
     }
   }
   #pragma unroll
   for (int j = 0; j < R; ++j) {
-    const int h = h0 + j;
-    if (h >= heads) break;
-    const bool is_q = h < p.n_q, is_v = h >= p.n_q + p.n_kv;
-    if (!is_v) {
-      const float* gain = is_q ? p.gq : p.gk;
-      if (gain) {
-        float s[V], g[V];
-        load_row<V>(gain + d0, p.vec_g, g);
+    const int h = h0 + j * kRows;
+    const bool in = h < heads, is_q = h < p.n_q, is_v = h >= p.n_q + p.n_kv;
+    const float* gain = is_q ? p.gq : p.gk;
+    float y[8];
+    const float sum = tree_sum<D>(x[j]);  // of values too: the lanes of a warp stay together
+    if (gain) {
+      float g[8];
+      load4(gain + 4 * l, p.vec_g, g);
+      load4(gain + D / 2 + 4 * l, p.vec_g, g + 4);
+      const float inv = __frcp_rn(__fsqrt_rn(__fadd_rn(__fmul_rn(sum, 1.f / D), p.eps)));
+      #pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = __fmul_rn(__fmul_rn(x[j][i], inv), g[i]);
+    } else {
+      #pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = x[j][i];
+    }
+    if (p.cos_t) {
+      // a cos - b sin and b cos + a sin, the difference as a sum with the sine's sign turned: the same bits
+      float z[8];
+      if (whole) {
         #pragma unroll
-        for (int i = 0; i < V; ++i) s[i] = __fmul_rn(x[j][i], x[j][i]);
-        const float sum = tree_sum<V>(s);
-        const float inv = __frcp_rn(__fsqrt_rn(__fadd_rn(__fmul_rn(sum, 1.f / D), p.eps)));
-        #pragma unroll
-        for (int i = 0; i < V; ++i) x[j][i] = __fmul_rn(__fmul_rn(x[j][i], inv), g[i]);
-      }
-      if (turn) {
-        float y[V];
-        #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float z = __shfl_sync(0xffffffffu, x[j][i], other);
-          y[i] = z;
+        for (int i = 0; i < 4; ++i) {
+          z[i] = __fadd_rn(__fmul_rn(y[i], cs[i]), __fmul_rn(y[i + 4], -sn[i]));
+          z[i + 4] = __fadd_rn(__fmul_rn(y[i + 4], cs[i]), __fmul_rn(y[i], sn[i]));
         }
-        if (p.interleaved) {
+      } else if (p.interleaved) {
+        #pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+          z[i] = __fadd_rn(__fmul_rn(y[i], cs[i]), __fmul_rn(y[i + 1], -sn[i]));
+          z[i + 1] = __fadd_rn(__fmul_rn(y[i + 1], cs[i]), __fmul_rn(y[i], sn[i]));
+        }
+      } else {
+        // the partner of a lane's four columns is another lane's four, of either half of the row
+        #pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const int c0 = w * (D / 2) + 4 * l, at = c0 < half ? c0 + half : c0 - half;
+          const int from = lane - l + (at >= 0 ? at / 4 % L : l);
+          const bool upper = at >= D / 2, low = c0 < half;
           #pragma unroll
-          for (int i = 0; i < V; i += 2) y[i] = x[j][i + 1], y[i + 1] = x[j][i];
-        }
-        if (d0 < p.rot) {  // a cos - b sin, b cos + a sin: the difference is the sum with the product's sign turned
-          #pragma unroll
-          for (int i = 0; i < V; ++i) x[j][i] = __fadd_rn(__fmul_rn(x[j][i], cs[i]), __fmul_rn(y[i], sn[i]));
+          for (int i = 0; i < 4; ++i) {
+            const float a = __shfl_sync(0xffffffffu, y[i], from);
+            const float b = p.rot > D / 2 ? __shfl_sync(0xffffffffu, y[4 + i], from) : 0.f;
+            const float other = upper ? b : a, s = sn[4 * w + i];
+            z[4 * w + i] = __fadd_rn(__fmul_rn(y[4 * w + i], cs[4 * w + i]), __fmul_rn(other, low ? -s : s));
+          }
         }
       }
+      #pragma unroll
+      for (int w = 0; w < 2; ++w)
+        if (w * (D / 2) + 4 * l < p.rot) {
+          #pragma unroll
+          for (int i = 4 * w; i < 4 * w + 4; ++i) y[i] = z[i];
+        }
     }
     if (is_q) {
-      store_row<V>(p.qo + tok * p.ldqo + h * D + d0, vec, x[j]);
+      float* to = p.qo + tok * p.ldqo + h * D + 4 * l;
+      store4(to, vec, y);
+      store4(to + D / 2, vec, y + 4);
     } else if constexpr (!kCache) {
-      store_row<V>(p.ko + tok * p.ldko + (h - p.n_q) * D + d0, vec, x[j]);
-    } else {
-      const uint32_t b = tok / static_cast<uint32_t>(p.m);
-      const int kvh = h - p.n_q - (is_v ? p.n_kv : 0);
-      const long long had = __ldg(p.len + b);
-      if (had < 0) continue;  // an idle sequence
-      const long long slot = had + (tok - b * static_cast<uint32_t>(p.m));
-      if (slot >= c.cap) {
-        if (lane == 0) atomicCAS(err, 0, kDevKv4Slot);
-        continue;
+      if (in) {
+        float* to = p.ko + tok * p.ldko + (h - p.n_q) * D + 4 * l;
+        store4(to, vec, y);
+        store4(to + D / 2, vec, y + 4);
       }
-      kv4_store_row<D>(x[j], is_v ? c.v : c.k, is_v ? c.vs : c.ks, (static_cast<long long>(b) * c.n_kv + kvh) * c.cap + slot);
+    }
+    if constexpr (kCache) {
+      if (__any_sync(0xffffffffu, in && !is_q)) {
+        const uint32_t b = tok / static_cast<uint32_t>(p.m);
+        const long long had = __ldg(p.len + b), slot = had + (tok - b * static_cast<uint32_t>(p.m));
+        if (had >= 0 && slot >= c.cap && lane == 0) atomicCAS(err, 0, kDevKv4Slot);
+        const bool on = in && !is_q && had >= 0 && slot < c.cap;  // had < 0: an idle sequence
+        const int kvh = h - p.n_q - (is_v ? p.n_kv : 0);
+        float o[8];
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = is_v ? x[j][i] : y[i];
+        kv4_store_rows<D>(o, on, is_v ? c.v : c.k, is_v ? c.vs : c.ks,
+                          on ? (static_cast<long long>(b) * c.n_kv + kvh) * c.cap + slot : 0);
+      }
     }
   }
 }
