@@ -39,9 +39,10 @@ struct Kv4Attn {
   float* score;       // [n_seq][n_kv][rows][cap]: log2 of the unnormalised weights (w_out only)
   float* lse;         // [n_seq][n_kv][rows]: log2 of their sum
   float* part;        // two partial results a CTA: m, l, O of a chunk of rows
-  int* arrived;       // [n_seq][n_kv][chunks]: partial results written, zero between calls
+  int2* split;        // [n_seq][n_kv][chunks]: the first CTA of an item and how many have a part of it (one: the output is there)
   float scale2;       // scale * log2(e)
-  int m, n_q, group, rows, chunks;  // rows = m * group query rows a kv head, in chunks
+  int m, n_q, group, rows;  // rows = m * group query rows a kv head
+  int chunks, chunk_rows;   // in chunks of a multiple of 4
   int vec;            // q rows start on 16-byte boundaries
   uint32_t mul4, mul64;  // 4 and 64, as values that the compiler does not know: see kv4_pair
 };
@@ -117,6 +118,41 @@ template <bool kHigh>
 __device__ __forceinline__ uint32_t kv4_pair(uint32_t u, uint32_t mul, __half2 step, __half2 base) {
   const uint32_t t = (u & (kHigh ? 0x00F000F0u : 0x000F000Fu)) * mul + 0x4C004C00u;  // mul: 4 (high) or 64
   return h2_bits(__hfma2(bits_h2(t), step, base));
+}
+
+// A query row as B fragments of its halves, a power of two apart from the row so
+// that its largest value lies in [1, 2), with the scale's sign in it. Lane (gid,
+// tig) has columns tig * D/4 .. of row gid / 2 of four: hi for even gid, lo for
+// odd. Returns what a score has to be multiplied by to be in log2 units.
+template <int D>
+__device__ __forceinline__ float attn_query(const float* src, bool vec, float scale2, uint32_t (&qb)[D / 16][2]) {
+  const int gid = (threadIdx.x & 31) >> 2, tig = threadIdx.x & 3;
+  float x[D / 4];
+  if (src) {
+    load_row<D / 4>(src + tig * (D / 4), vec, x);
+  } else {
+    #pragma unroll
+    for (int i = 0; i < D / 4; ++i) x[i] = 0.f;
+  }
+  float top = 0.f;
+  #pragma unroll
+  for (int i = 0; i < D / 4; ++i) top = fmaxf(top, fabsf(x[i]));
+  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  const int e = min(max(static_cast<int>((__float_as_uint(top) >> 23) & 255) - 127, -120), 120);
+  const float down = copysignf(__uint_as_float(static_cast<uint32_t>(127 - e) << 23), scale2);
+  #pragma unroll
+  for (int w = 0; w < D / 32; ++w) {
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float a = x[8 * w + i] * down, b = x[8 * w + i + 4] * down;
+      const __half2 hi = __floats2half2_rn(a, b);
+      const __half2 lo = __floats2half2_rn(a - __low2float(hi), b - __high2float(hi));
+      qb[2 * w + (i >> 1)][i & 1] = (gid & 1) ? h2_bits(lo) : h2_bits(hi);
+    }
+  }
+  // not 0, or a hidden slot's -inf would become a NaN
+  return fmaxf(__uint_as_float(static_cast<uint32_t>(127 + e) << 23) * fabsf(scale2), 1e-37f);
 }
 
 // Where a slot's 16-byte chunk c of codes lies in its row in shared memory: the
@@ -239,6 +275,24 @@ __device__ __forceinline__ void attn_join(float& m, float& l, float& v, float pm
   l = fmaf(l, f, pl * fp), v = fmaf(v, f, pv * fp), m = mm;
 }
 
+// A query row's token; its place in q and in the output; where its log2 sum goes.
+__device__ __forceinline__ int attn_token(const Kv4Attn& p, int row) { return p.m == 1 ? 0 : row / p.group; }
+template <int D>
+__device__ __forceinline__ long long attn_row_at(const Kv4Attn& p, const AttnRun& s, int row, long long ld) {
+  const int t = attn_token(p, row);
+  return (static_cast<long long>(s.b) * p.m + t) * ld + static_cast<long long>(s.head * p.group + row - t * p.group) * D;
+}
+__device__ __forceinline__ void attn_put_lse(const Kv4Attn& p, const Kv4View& c, const AttnRun& s, int row, float m, float l) {
+  p.lse[(static_cast<long long>(s.b) * c.n_kv + s.head) * p.rows + row] = m - kAttnShift + log2f(l);
+}
+
+// An item's first run says which CTAs have parts of it: shares of `each` tiles, one more for the first `extra` CTAs.
+__device__ __forceinline__ void attn_put_split(const Kv4Attn& p, const AttnRun& s, int hc_count, int cta, int each, int extra) {
+  const int last = s.first + s.units - 1, big = (each + 1) * extra;
+  const int end = last < big ? last / (each + 1) : extra + (last - big) / each;
+  p.split[s.b * hc_count + s.hc] = make_int2(cta, end - cta + 1);
+}
+
 // D: head size. NT: chunks hold 4 * NT rows. kW: scores are kept for w_out.
 template <int D, int NT, bool kW>
 __global__ void __launch_bounds__(attn_warps(D, NT) * 32, 1) kv4_attn_kernel(const Kv4Attn p, const Kv4View c,
@@ -259,18 +313,20 @@ __global__ void __launch_bounds__(attn_warps(D, NT) * 32, 1) kv4_attn_kernel(con
   // that other warps began, 2 w + 1 the beginning of one that others end.
   __shared__ int s_state[2 * kWarps];  // 0: none, 1: the item ends here, 2: it goes on
   __shared__ int s_from[2 * kWarps];   // the output part: bytes into smem
-  __shared__ AttnRun s_run[2 * kWarps], s_part[2];
-  __shared__ int s_last[2], s_c0[2], s_parts;
+  __shared__ AttnRun s_run[2 * kWarps];
+  __shared__ int s_parts;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int gid = lane >> 2, tig = lane & 3;
   unsigned char* ring = smem + warp * 2 * kAttnStageBytes;
   float* heads = reinterpret_cast<float*>(smem + kWarps * 2 * kAttnStageBytes);  // [warp][RC * D]
   float* ml = heads + kWarps * RC * D;                                           // [warp][head, tail][row][m, l]
 
+  pdl_wait_prior();
+  pdl_launch_dependents();
   // All tiles, this CTA's share of them, and this warp's share of those.
   AttnWalk<TS> walk;
   walk.len = p.len, walk.n_seq = c.n_seq, walk.hc_count = c.n_kv * p.chunks, walk.cap = c.cap;
-  walk.chunks = p.chunks, walk.chunk_rows = RC;
+  walk.chunks = p.chunks, walk.chunk_rows = p.chunk_rows;
   int units = 0, longest = 0, used = 0;
   #pragma unroll 1
   for (int i = lane; i < c.n_seq; i += 32) {
@@ -369,15 +425,9 @@ __global__ void __launch_bounds__(attn_warps(D, NT) * 32, 1) kv4_attn_kernel(con
     }
   };
   auto first_row = [&](const AttnRun& s) { return (static_cast<long long>(s.b) * c.n_kv + s.head) * c.cap; };
-  // A query row's token; its place in q and in the output; where its log2 sum goes.
-  auto token = [&](int row) { return p.m == 1 ? 0 : row / p.group; };
-  auto row_at = [&](const AttnRun& s, int row, long long ld) {
-    const int t = token(row);
-    return (static_cast<long long>(s.b) * p.m + t) * ld + static_cast<long long>(s.head * p.group + row - t * p.group) * D;
-  };
-  auto put_lse = [&](const AttnRun& s, int row, float m, float l) {
-    p.lse[(static_cast<long long>(s.b) * c.n_kv + s.head) * p.rows + row] = m - kAttnShift + log2f(l);
-  };
+  auto token = [&](int row) { return attn_token(p, row); };
+  auto row_at = [&](const AttnRun& s, int row, long long ld) { return attn_row_at<D>(p, s, row, ld); };
+  auto put_lse = [&](const AttnRun& s, int row, float m, float l) { attn_put_lse(p, c, s, row, m, l); };
 
   if (lane < 2) s_state[2 * warp + lane] = 0;
   __syncwarp();
@@ -398,45 +448,18 @@ __global__ void __launch_bounds__(attn_warps(D, NT) * 32, 1) kv4_attn_kernel(con
     if (more) row1 = first_row(nxt) + nxt.s0, left1 = nxt.s1 - nxt.s0;
     const int r0 = run.r0;
 
-    // The chunk's rows: B fragments of their halves, a power of two apart from
-    // the row so that its largest value lies in [1, 2). Lane (gid, tig) has row
-    // gid / 2 of each four, hi for even gid and lo for odd.
+    // The chunk's rows.
     uint32_t qb[NT][2 * KW][2];
     float sc[NT];  // what a score has to be multiplied by to be in log2 units, of row tig; not negative
     int vis[NT];   // slots that row tig sees
-    int all_see = 0x7fffffff;  // slots that every row sees
     #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int r = r0 + nt * 4 + (gid >> 1);
-      float x[D / 4];
-      if (r < p.rows) {
-        load_row<D / 4>(p.q + row_at(run, r, p.ldq) + tig * (D / 4), p.vec, x);
-      } else {
-        #pragma unroll
-        for (int i = 0; i < D / 4; ++i) x[i] = 0.f;
-      }
-      float top = 0.f;
-      #pragma unroll
-      for (int i = 0; i < D / 4; ++i) top = fmaxf(top, fabsf(x[i]));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int e = min(max(static_cast<int>((__float_as_uint(top) >> 23) & 255) - 127, -120), 120);
-      const float down = copysignf(__uint_as_float(static_cast<uint32_t>(127 - e) << 23), p.scale2);
-      sc[nt] = __shfl_sync(0xffffffffu, __uint_as_float(static_cast<uint32_t>(127 + e) << 23), 8 * tig) * fabsf(p.scale2);
-      #pragma unroll
-      for (int w = 0; w < KW; ++w) {
-        #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float a = x[8 * w + i] * down, b = x[8 * w + i + 4] * down;
-          const __half2 top2 = __floats2half2_rn(a, b);
-          const __half2 low2 = __floats2half2_rn(a - __low2float(top2), b - __high2float(top2));
-          qb[nt][2 * w + (i >> 1)][i & 1] = (gid & 1) ? h2_bits(low2) : h2_bits(top2);
-        }
-      }
-      const int rt = r0 + nt * 4 + tig;
+      const int r = r0 + nt * 4 + (gid >> 1), rt = r0 + nt * 4 + tig;
+      const float up = attn_query<D>(r < p.rows ? p.q + row_at(run, r, p.ldq) : nullptr, p.vec, p.scale2, qb[nt]);
+      sc[nt] = __shfl_sync(0xffffffffu, up, 8 * tig);
       vis[nt] = rt < p.rows ? run.n - (p.m - 1 - token(rt)) : 0;
     }
-    all_see = r0 + RC > p.rows ? 0 : run.n - (p.m - 1 - token(r0));
+    const int all_see = r0 + RC > p.rows ? 0 : run.n - (p.m - 1 - token(r0));  // slots that every row sees
 
     float top[NT], sum[NT], o[OT][2][NT];
     #pragma unroll
@@ -665,6 +688,7 @@ __global__ void __launch_bounds__(attn_warps(D, NT) * 32, 1) kv4_attn_kernel(con
           if (kW && lane == 0) put_lse(run, r0 + r, tp, sm);
         }
       }
+      if (lane == 0) p.split[run.b * walk.hc_count + run.hc] = make_int2(cta, 1);
       __syncwarp();
     } else if (lane == 0) {
       s_state[which] = run.leave ? 2 : 1;
@@ -680,7 +704,6 @@ __global__ void __launch_bounds__(attn_warps(D, NT) * 32, 1) kv4_attn_kernel(con
 
   // Parts of one item left by neighbouring warps become one result: all of the item, or this CTA's part of it, of which
   // there are at most two (kind 0: it began in an earlier CTA; kind 1: it began here and goes on).
-  uint32_t part_on = 0;  // bit: kind
   int next = 0;
   while (true) {
     while (next < 2 * kWarps && !s_state[next]) ++next;
@@ -739,115 +762,112 @@ __global__ void __launch_bounds__(attn_warps(D, NT) * 32, 1) kv4_attn_kernel(con
       else if (it.r0 + r < p.rows)
         p.out[row_at(it, it.r0 + r, p.ldo) + attn_col<D, NT>(x)] = v;
     }
+    if (kind == 1 && tid == 0) {
+      if (final_here)
+        p.split[it.b * walk.hc_count + it.hc] = make_int2(cta, 1);
+      else
+        attn_put_split(p, it, walk.hc_count, cta, each, extra);
+    }
     if (next < 2 * kWarps) __syncthreads();  // s_mul is used again
-    if (!final_here) {
-      part_on |= 1u << kind;
-      if (tid == 0) s_part[kind] = it;
-    }
-  }
-  if (!part_on) return;
-
-  // The CTA that finds every other part of an item written joins them. The barrier orders the CTA's stores before the
-  // counting thread's release, and its acquire before the other threads' loads.
-  __syncthreads();
-  auto cta_of = [&](int u) {
-    const int big = (each + 1) * extra;
-    return u < big ? u / (each + 1) : extra + (u - big) / each;
-  };
-  if (tid < 2 && (part_on >> tid & 1)) {
-    const AttnRun& it = s_part[tid];
-    const int c0 = cta_of(it.first), c1 = cta_of(it.first + it.units - 1);
-    const int item = it.b * walk.hc_count + it.hc;
-    s_c0[tid] = c0;
-    s_last[tid] = atom_add_acq_rel_gpu(p.arrived + item, 1) == c1 - c0 ? c1 - c0 + 1 : 0;
-  }
-  __syncthreads();
-  #pragma unroll 1
-  for (int kind = 0; kind < 2; ++kind) {
-    if (!(part_on >> kind & 1) || s_last[kind] == 0) continue;
-    const AttnRun it = s_part[kind];
-    const int parts = s_last[kind], c0 = s_c0[kind];
-    // Thread groups that cover the chunk once take turns with the parts, four values a thread (the four rows of a
-    // column), each with its own running maximum and sum: one round of loads.
-    const float* from = p.part + static_cast<long long>(c0) * 2 * kPart;
-    constexpr int kFour = RC * D / 4, kGroups = kThreads / kFour;
-    const int x = tid % kFour * 4, grp = tid / kFour, r = attn_row<NT>(x);
-    float m[4] = {-1e30f, -1e30f, -1e30f, -1e30f}, l[4] = {}, v[4] = {};
-    if (grp < kGroups) {
-      constexpr int kAhead = 5;
-      #pragma unroll 1
-      for (int k0 = grp; k0 < parts; k0 += kAhead * kGroups) {
-        float4 pm[kAhead], pl[kAhead], pv[kAhead];
-        #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-          const int k = k0 + i * kGroups;
-          if (k >= parts) continue;
-          const float* at = from + static_cast<long long>(k) * 2 * kPart + (k == 0 ? kPart : 0);
-          pm[i] = __ldcg(reinterpret_cast<const float4*>(at + r));
-          pl[i] = __ldcg(reinterpret_cast<const float4*>(at + RC + r));
-          pv[i] = __ldcg(reinterpret_cast<const float4*>(at + 2 * RC + x));
-        }
-        #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-          if (k0 + i * kGroups >= parts) continue;
-          const float am[4] = {pm[i].x, pm[i].y, pm[i].z, pm[i].w}, al[4] = {pl[i].x, pl[i].y, pl[i].z, pl[i].w},
-                      av[4] = {pv[i].x, pv[i].y, pv[i].z, pv[i].w};
-          #pragma unroll
-          for (int j = 0; j < 4; ++j) attn_join(m[j], l[j], v[j], am[j], al[j], av[j]);
-        }
-      }
-    }
-    if constexpr (kGroups > 1) {
-      static_assert((kGroups - 1) * kFour * 48 <= kWarps * 2 * kAttnStageBytes, "the joins' values lie in the rings");
-      float4* other = reinterpret_cast<float4*>(smem);
-      if (grp > 0 && grp < kGroups) {
-        float4* to = other + (tid - kFour) * 3;
-        to[0] = make_float4(m[0], m[1], m[2], m[3]);
-        to[1] = make_float4(l[0], l[1], l[2], l[3]);
-        to[2] = make_float4(v[0], v[1], v[2], v[3]);
-      }
-      __syncthreads();
-      if (grp == 0) {
-        #pragma unroll
-        for (int g = 1; g < kGroups; ++g) {
-          const float4* at = other + (tid + (g - 1) * kFour) * 3;
-          const float4 pm = at[0], pl = at[1], pv = at[2];
-          attn_join(m[0], l[0], v[0], pm.x, pl.x, pv.x);
-          attn_join(m[1], l[1], v[1], pm.y, pl.y, pv.y);
-          attn_join(m[2], l[2], v[2], pm.z, pl.z, pv.z);
-          attn_join(m[3], l[3], v[3], pm.w, pl.w, pv.w);
-        }
-      }
-    }
-    if (grp == 0) {
-      const int col = attn_col<D, NT>(x);
-      #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int row = it.r0 + r + j;
-        if (row >= p.rows) continue;
-        p.out[row_at(it, row, p.ldo) + col] = l[j] != 0.f ? v[j] / l[j] : 0.f;
-        if (kW && col == 0) put_lse(it, row, m[j], l[j]);
-      }
-    }
-    if (tid == 0) p.arrived[it.b * walk.hc_count + it.hc] = 0;
-    __syncthreads();
   }
 }
 
-// The weights from the kept scores: one thread per (sequence, kv head, slot).
-__global__ void __launch_bounds__(256) kv4_weights_kernel(const Kv4Attn p, const Kv4View c) {
-  const long long j = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-  const long long bh = blockIdx.y;
-  const long long b = bh / c.n_kv;
+// The parts of split items, once every CTA's are written: a block has 32 times four values of an item's chunk (the four
+// rows of a column), its warps take turns with the parts, and their maxima, sums and values are joined in shared memory.
+constexpr int kJoinWarps = 4;
+
+template <int D, int NT, bool kW>
+__global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(const Kv4Attn p, const Kv4View c) {
+  constexpr int RC = 4 * NT, kPart = RC * (D + 2), kSlices = RC * D / 128;
+  __shared__ float4 s_join[kJoinWarps - 1][3][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  pdl_wait_prior();
+  pdl_launch_dependents();
+  const int item = blockIdx.x / kSlices, slice = blockIdx.x - item * kSlices;
+  const int hc = item % (c.n_kv * p.chunks), b = item / (c.n_kv * p.chunks);
+  if (__ldg(p.len + b) <= 0) return;
+  const int2 s = p.split[item];
+  if (s.y <= 1) return;
+  const int x = (slice * 32 + lane) * 4, r = attn_row<NT>(x);
+  AttnRun it;
+  it.b = b, it.head = hc / p.chunks, it.r0 = (hc - it.head * p.chunks) * p.chunk_rows;
+  const int rows = min(p.chunk_rows, p.rows - it.r0);
+  float m[4] = {-1e30f, -1e30f, -1e30f, -1e30f}, l[4] = {}, v[4] = {};
+  constexpr int kAhead = 5;
+  #pragma unroll 1
+  for (int k0 = warp; k0 < s.y; k0 += kAhead * kJoinWarps) {
+    float4 pm[kAhead], pl[kAhead], pv[kAhead];
+    #pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int k = k0 + i * kJoinWarps;
+      if (k >= s.y || r >= rows) continue;
+      const float* at = p.part + (static_cast<long long>(s.x + k) * 2 + (k == 0 ? 1 : 0)) * kPart;
+      pm[i] = *reinterpret_cast<const float4*>(at + r);
+      pl[i] = *reinterpret_cast<const float4*>(at + RC + r);
+      pv[i] = *reinterpret_cast<const float4*>(at + 2 * RC + x);
+    }
+    #pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (k0 + i * kJoinWarps >= s.y || r >= rows) continue;
+      attn_join(m[0], l[0], v[0], pm[i].x, pl[i].x, pv[i].x);
+      attn_join(m[1], l[1], v[1], pm[i].y, pl[i].y, pv[i].y);
+      attn_join(m[2], l[2], v[2], pm[i].z, pl[i].z, pv[i].z);
+      attn_join(m[3], l[3], v[3], pm[i].w, pl[i].w, pv[i].w);
+    }
+  }
+  if (warp > 0) {
+    s_join[warp - 1][0][lane] = make_float4(m[0], m[1], m[2], m[3]);
+    s_join[warp - 1][1][lane] = make_float4(l[0], l[1], l[2], l[3]);
+    s_join[warp - 1][2][lane] = make_float4(v[0], v[1], v[2], v[3]);
+  }
+  __syncthreads();
+  if (warp > 0) return;
+  #pragma unroll
+  for (int g = 0; g < kJoinWarps - 1; ++g) {
+    const float4 pm = s_join[g][0][lane], pl = s_join[g][1][lane], pv = s_join[g][2][lane];
+    attn_join(m[0], l[0], v[0], pm.x, pl.x, pv.x);
+    attn_join(m[1], l[1], v[1], pm.y, pl.y, pv.y);
+    attn_join(m[2], l[2], v[2], pm.z, pl.z, pv.z);
+    attn_join(m[3], l[3], v[3], pm.w, pl.w, pv.w);
+  }
+  const int col = attn_col<D, NT>(x);
+  #pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (r + j >= rows) continue;
+    p.out[attn_row_at<D>(p, it, it.r0 + r + j, p.ldo) + col] = l[j] != 0.f ? v[j] / l[j] : 0.f;
+    if (kW && col == 0) attn_put_lse(p, c, it, it.r0 + r + j, m[j], l[j]);
+  }
+}
+
+// The weights that slots received, from the kept scores and the rows' sums: a thread a slot, 256 slots of a kv head a block.
+// Bound by the scores' reads (4 bytes a row and slot).
+constexpr int kWeightThreads = 256;
+
+__global__ void __launch_bounds__(kWeightThreads) kv4_weights_kernel(const Kv4Attn p, const Kv4View c, int blocks) {
+  __shared__ float s_lse[kWeightThreads];
+  pdl_wait_prior();
+  pdl_launch_dependents();
+  const int tid = threadIdx.x, bh = blockIdx.x / blocks, b = bh / c.n_kv;
+  const long long j0 = static_cast<long long>(blockIdx.x - bh * blocks) * kWeightThreads, j = j0 + tid;
   long long n = __ldg(p.len + b);
   if (n > c.cap) n = c.cap;
-  if (j >= n) return;
-  float w = 0.f;
-  const float* s = p.score + bh * p.rows * c.cap + j;
-  for (int r = 0; r < p.rows; ++r)
-    if (j < n - (p.m - 1 - r / p.group)) w += ex2(__ldg(s + r * c.cap) - __ldg(p.lse + bh * p.rows + r));
-  const long long at = bh * c.cap + j;
-  p.w_out[at] = (p.w_in && j < n - p.m ? p.w_in[at] : 0.f) + w;
+  if (j0 >= n) return;
+  const long long at = static_cast<long long>(bh) * c.cap + j;
+  float w = j < n - p.m && p.w_in ? p.w_in[at] : 0.f;
+  // rows of tokens that do not see the slot come first
+  const long long late = j - (n - p.m);
+  const int skip = late > 0 ? static_cast<int>(late) * p.group : 0;
+  for (int r0 = 0; r0 < p.rows; r0 += kWeightThreads) {
+    const int rows = min(kWeightThreads, p.rows - r0);
+    __syncthreads();
+    if (tid < rows) s_lse[tid] = p.lse[static_cast<long long>(bh) * p.rows + r0 + tid];
+    __syncthreads();
+    if (j >= n) continue;
+    const float* s = p.score + (static_cast<long long>(bh) * p.rows + r0) * c.cap + j;
+    #pragma unroll 8
+    for (int r = max(0, skip - r0); r < rows; ++r) w += ex2(__ldg(s + r * c.cap) - s_lse[r]);
+  }
+  if (j < n) p.w_out[at] = w;
 }
 
 }  // namespace vmlm

@@ -1,0 +1,369 @@
+// kv4_attn_rows.cuh -- attention over a 4-bit cache for many query rows a kv head
+// (several new tokens, or many heads that share keys and values).
+//
+// The products and their layouts are those of kv4_attn.cuh. There every warp
+// unpacks its own slots and multiplies them with all rows, whose output it holds;
+// with many rows that does not fit, and a chunk of few rows unpacks the cache
+// again for every chunk. Here a CTA of 8 warps shares a tile of 64 slots:
+//   scores   warp (slots 16 s .., half g of the rows): K unpacked twice
+//   weights  to shared memory as B fragments, with a maximum shared by the tile
+//   output   warp w: its columns of V (16 or 32; d = 64: and half of the rows),
+//            V unpacked once (d = 64: twice), all 64 slots, all rows
+// Three barriers a tile; two CTAs on an SM fill each other's. What bounds it is
+// mma.sync (one m16n8k16 in two cycles an SM: d rows of 64 slots take d * rows / 8
+// MMAs) and, nearly, the B fragments' reads from shared memory (256 bytes each).
+#pragma once
+#include "kv4_attn.cuh"
+
+namespace vmlm {
+
+constexpr int kRowsWarps = 8, kRowsThreads = kRowsWarps * 32, kRowsSlots = 64;
+
+// Fours of rows that a chunk holds at most: what the registers of two CTAs an SM hold.
+__host__ __device__ constexpr int rows_most(int D) { return D == 64 ? 12 : 8; }
+__host__ __device__ constexpr int rows_stage_bytes(int D) { return kRowsSlots * D / 4 * 5; }
+// Shared memory: two tiles, the queries' and the weights' fragments, per row 4 maxima, factor, 4 sums, scale and sight.
+__host__ __device__ constexpr int rows_smem_bytes(int D, int NT) {
+  return 2 * rows_stage_bytes(D) + NT * (D / 32) * 512 + 4 * NT * 256 + NT * 4 * 11 * 4;
+}
+
+// NT: fours of rows of a chunk, an even number; rows that are not there are zeros that see nothing.
+template <int D, int NT, bool kW>
+__global__ void __launch_bounds__(kRowsThreads, 2) kv4_attn_rows_kernel(const Kv4Attn p, const Kv4View c,
+                                                                        int* __restrict__ err) {
+  constexpr int NG = NT / 2;  // fours of rows of a half
+  constexpr int RC = 4 * NT, kPart = RC * (D + 2);
+  constexpr int TS = kRowsSlots;
+  constexpr int KW = D / 32, VW = D / 64, kCh = D / 32;
+  constexpr int kStage = rows_stage_bytes(D);
+  constexpr int kVAt = TS * D / 2, kKsAt = TS * D, kVsAt = TS * D + TS * D / 8;  // in a stage: K, V, K's and V's scales
+  constexpr int TP = D == 256 ? 2 : 1;   // output tiles of a warp
+  constexpr int OG = D == 64 ? 2 : 1;    // parts of the rows that the warps of an output tile share
+  constexpr int ON = NT / OG;            // fours of rows of such a part
+  extern __shared__ __align__(128) unsigned char smem[];
+  uint4* qs = reinterpret_cast<uint4*>(smem + 2 * kStage);                          // [NT][KW][lane]
+  uint2* ps = reinterpret_cast<uint2*>(smem + 2 * kStage + NT * KW * 512);          // [4][NT][lane]
+  float* s_max = reinterpret_cast<float*>(ps + 4 * NT * 32);                        // [4][RC]
+  float* s_fac = s_max + 4 * RC;                                                    // [RC]
+  float* s_sum = s_fac + RC;                                                        // [4][RC]
+  float* s_scale = s_sum + 4 * RC;                                                  // [RC]
+  int* s_see = reinterpret_cast<int*>(s_scale + RC);                                // [RC]: slots that a row sees
+  __shared__ int s_grown[2][2];  // a half's maxima grew in a tile: by the tile's parity
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int gid = lane >> 2, tig = lane & 3;
+  const int st = warp & 3, half = warp >> 2;            // scores: slots 16 st .., fours half * NG ..
+  const int ot = D == 64 ? warp & 3 : warp * TP;        // output: first tile
+
+  pdl_wait_prior();
+  pdl_launch_dependents();
+  AttnWalk<TS> walk;
+  walk.len = p.len, walk.n_seq = c.n_seq, walk.hc_count = c.n_kv * p.chunks, walk.cap = c.cap;
+  walk.chunks = p.chunks, walk.chunk_rows = p.chunk_rows;
+  int units = 0;
+  #pragma unroll 1
+  for (int i = lane; i < c.n_seq; i += 32) {
+    if (__ldg(p.len + i) > c.cap && tid == lane) atomicCAS(err, 0, kDevKv4Slot);
+    units += walk.tiles(i);
+  }
+  units = __reduce_add_sync(0xffffffffu, units) * walk.hc_count;
+  const int cta = blockIdx.x, grid = gridDim.x;
+  #pragma unroll 1
+  for (int i = cta; i < c.n_seq; i += grid) {  // sequences without a slot: zeros
+    if (walk.length(i) > 0) continue;
+    #pragma unroll 1
+    for (long long x = tid; x < static_cast<long long>(p.m) * p.n_q * D; x += kRowsThreads) {
+      const long long t = x / (p.n_q * D);
+      p.out[(static_cast<long long>(i) * p.m + t) * p.ldo + (x - t * p.n_q * D)] = 0.f;
+    }
+  }
+  const int ctas = min(grid, units);
+  if (cta >= ctas) return;
+  const int each = units / ctas, extra = units - each * ctas;
+  walk.pos = cta * each + min(cta, extra), walk.end = walk.pos + each + (cta < extra);
+  walk.template seek<false>(walk.pos);
+
+  auto fetch = [&](long long row, int left, int stage) {
+    unsigned char* to = smem + stage * kStage;
+    const uint8_t *k = c.k + row * (D / 2), *v = c.v + row * (D / 2);
+    const uint8_t* ks = reinterpret_cast<const uint8_t*>(c.ks) + row * (D / 8);
+    const uint8_t* vs = reinterpret_cast<const uint8_t*>(c.vs) + row * (D / 8);
+    #pragma unroll
+    for (int x = tid; x < TS * kCh; x += kRowsThreads) {
+      const int slot = x / kCh, at = slot * (D / 2) + attn_swizzle<D>(slot, x % kCh) * 16;
+      const bool on = slot < left;  // rows that do not exist become zeros
+      cp_async16(smem_u32(to + at), on ? k + x * 16 : c.k, on);
+      cp_async16(smem_u32(to + kVAt + at), on ? v + x * 16 : c.v, on);
+    }
+    constexpr int kSb = D == 64 ? 8 : 16;
+    for (int x = tid; x < TS * D / 8 / kSb; x += kRowsThreads) {
+      const bool on = x * kSb / (D / 8) < left;
+      const void *a = on ? static_cast<const void*>(ks + x * kSb) : c.ks, *b = on ? static_cast<const void*>(vs + x * kSb) : c.vs;
+      if constexpr (D == 64) {
+        cp_async8(smem_u32(to + kKsAt + x * 8), a, on);
+        cp_async8(smem_u32(to + kVsAt + x * 8), b, on);
+      } else {
+        cp_async16(smem_u32(to + kKsAt + x * 16), a, on);
+        cp_async16(smem_u32(to + kVsAt + x * 16), b, on);
+      }
+    }
+  };
+  auto first_row = [&](const AttnRun& s) { return (static_cast<long long>(s.b) * c.n_kv + s.head) * c.cap; };
+
+  const int k_at = (st * 16 + gid) * (D / 2) + (D == 64 ? tig * 8 : D == 128 ? attn_swizzle<D>(gid, tig) * 16 : 0);
+  const int ks_at = kKsAt + (st * 16 + gid) * (D / 8) + (D == 64 ? (tig >> 1) * 4 : tig * (D / 32));
+  const int v_in = gid * VW * 4;
+  const int va_at = kVAt + 2 * tig * (D / 2) + attn_swizzle<D>(2 * tig, v_in / 16) * 16 + v_in % 16;
+  const int vb_at = kVAt + (2 * tig + 1) * (D / 2) + attn_swizzle<D>(2 * tig + 1, v_in / 16) * 16 + v_in % 16;
+  const int vs_at = kVsAt + 2 * tig * (D / 8) + gid * VW / 4 * 4;
+
+  AttnRun run, nxt;
+  walk.next(run);  // a CTA's share is not empty
+  long long row0 = first_row(run);
+  fetch(row0 + run.s0, run.s1 - run.s0, 0);
+  cp_async_commit();
+  int stage = 0, parity = 0;
+  if (tid < 4) s_grown[tid >> 1][tid & 1] = 0;
+
+  while (true) {
+    const bool more = walk.next(nxt);
+    long long row1 = 0;
+    int left1 = 0;
+    if (more) row1 = first_row(nxt) + nxt.s0, left1 = nxt.s1 - nxt.s0;
+    const int rows = min(p.chunk_rows, p.rows - run.r0);  // of this chunk
+    __syncthreads();  // the last run's fragments have been read
+    for (int nt = warp; nt < NT; nt += kRowsWarps) {
+      const int r = nt * 4 + (gid >> 1);
+      uint32_t qb[2 * KW][2];
+      const float up = attn_query<D>(r < rows ? p.q + attn_row_at<D>(p, run, run.r0 + r, p.ldq) : nullptr, p.vec, p.scale2, qb);
+      #pragma unroll
+      for (int w = 0; w < KW; ++w)
+        qs[(nt * KW + w) * 32 + lane] = make_uint4(qb[2 * w][0], qb[2 * w][1], qb[2 * w + 1][0], qb[2 * w + 1][1]);
+      if (tig == 0 && !(gid & 1)) {
+        s_scale[r] = up;
+        s_see[r] = r < rows ? run.n - (p.m - 1 - attn_token(p, run.r0 + r)) : 0;
+      }
+    }
+    // the first four of rows of this warp's scores, and of its output
+    const int n0 = half * NG, o0 = OG == 1 ? 0 : half * NG;
+    float top[NG], sum[NG];
+    #pragma unroll
+    for (int i = 0; i < NG; ++i) top[i] = -1e30f, sum[i] = 0.f;
+    const int all_see = rows < RC ? 0 : run.n - (p.m - 1 - attn_token(p, run.r0));
+    float o[TP][2][ON];
+    #pragma unroll
+    for (int i = 0; i < ON; ++i)
+      #pragma unroll
+      for (int z = 0; z < TP; ++z) o[z][0][i] = o[z][1][i] = 0.f;
+
+    #pragma unroll 1
+    for (int at = run.s0; at < run.s1; at += TS) {
+      cp_async_wait<0>();
+      __syncthreads();  // the tile is there; the other stage and the weights of the last tile have been read
+      const bool same = at + TS < run.s1;
+      if (same || more) fetch(same ? row0 + at + TS : row1, same ? run.s1 - at - TS : left1, stage ^ 1);
+      cp_async_commit();
+      const unsigned char* tile = smem + stage * kStage;
+      const int left = run.s1 - at;
+
+      // scores of 16 slots and half of the rows
+      float acc[NG][4];
+      {
+        const unsigned char *pk = tile + k_at, *pc = tile + ks_at;
+        #pragma unroll
+        for (int w = 0; w < KW; ++w) {
+          int off = w * 4;
+          if constexpr (D == 256) off = attn_swizzle<D>(gid, tig * 2 + w / 4) * 16 + w % 4 * 4;
+          const uint32_t wa = *reinterpret_cast<const uint32_t*>(pk + off);
+          const uint32_t wb = *reinterpret_cast<const uint32_t*>(pk + 8 * (D / 2) + off);
+          const __half2 sa = *reinterpret_cast<const __half2*>(pc + w / 4 * 4);
+          const __half2 sb = *reinterpret_cast<const __half2*>(pc + 8 * (D / 8) + w / 4 * 4);
+          const __half2 sta = __low2half2(sa), bsa = __high2half2(sa), stb = __low2half2(sb), bsb = __high2half2(sb);
+          const uint32_t a0 = kv4_pair<false>(wa, p.mul64, sta, bsa), b0 = kv4_pair<false>(wb, p.mul64, stb, bsb);
+          const uint32_t a1 = kv4_pair<true>(wa, p.mul4, sta, bsa), b1 = kv4_pair<true>(wb, p.mul4, stb, bsb);
+          const uint32_t xa = wa >> 8, xb = wb >> 8;
+          const uint32_t a2 = kv4_pair<false>(xa, p.mul64, sta, bsa), b2 = kv4_pair<false>(xb, p.mul64, stb, bsb);
+          const uint32_t a3 = kv4_pair<true>(xa, p.mul4, sta, bsa), b3 = kv4_pair<true>(xb, p.mul4, stb, bsb);
+          #pragma unroll
+          for (int i = 0; i < NG; ++i) {
+              const uint4 q = qs[((n0 + i) * KW + w) * 32 + lane];
+            if (w == 0)
+              mma_f16_first(acc[i], a0, b0, a1, b1, q.x, q.y);
+            else
+              mma_f16(acc[i], a0, b0, a1, b1, q.x, q.y);
+            mma_f16(acc[i], a2, b2, a3, b3, q.z, q.w);
+          }
+        }
+      }
+      // hidden slots, and whether a maximum has grown
+      const bool some_hidden = left < TS || at + TS > all_see;
+      bool grown = false;
+      float* kept = nullptr;
+      if (kW)
+        kept = p.score + ((static_cast<long long>(run.b) * c.n_kv + run.head) * p.rows + run.r0 + n0 * 4 + tig) * c.cap + at +
+               st * 16 + gid;
+      #pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        const int r = (n0 + i) * 4 + tig;
+        float s0 = acc[i][0] + acc[i][1], s1 = acc[i][2] + acc[i][3];
+        const float sc = s_scale[r];
+        if (kW) {
+          if (r < rows && st * 16 + gid < left) kept[0] = s0 * sc;
+          if (r < rows && st * 16 + gid + 8 < left) kept[8] = s1 * sc;
+          kept += 4 * c.cap;
+        }
+        if (some_hidden) {
+          const int see = min(left, s_see[r] - at) - st * 16;
+          if (gid >= see) s0 = -INFINITY;
+          if (gid + 8 >= see) s1 = -INFINITY;
+        }
+        acc[i][0] = s0 * sc, acc[i][1] = s1 * sc;
+        grown |= fmaxf(acc[i][0], acc[i][1]) > top[i] + kAttnSlack;
+      }
+      if (named_bar_or(1 + half, 128, grown)) {  // the four warps that share these rows
+        #pragma unroll
+        for (int i = 0; i < NG; ++i) {
+          float best = fmaxf(acc[i][0], acc[i][1]);
+          best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 4));
+          best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 8));
+          best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 16));
+          if (gid == 0) s_max[st * RC + (n0 + i) * 4 + tig] = best;
+        }
+        named_bar_sync(1 + half, 128);
+        #pragma unroll
+        for (int i = 0; i < NG; ++i) {
+          const int r = (n0 + i) * 4 + tig;
+          const float best = fmaxf(fmaxf(fmaxf(s_max[r], s_max[RC + r]), fmaxf(s_max[2 * RC + r], s_max[3 * RC + r])), top[i]);
+          const float f = ex2(top[i] - best);
+          top[i] = best, sum[i] *= f;
+          if (st == 0 && gid == 0) s_fac[r] = f;
+        }
+        if (st == 0 && lane == 0) s_grown[parity][half] = 1;
+      }
+      #pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        const float off = kAttnShift - top[i];
+        uint32_t pb[2];
+        #pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float e = ex2(acc[i][h] + off);
+          sum[i] += e;
+          const float big = __uint_as_float(__float_as_uint(e) & 0xFFFFE000u);
+          pb[h] = transpose8x8(h2_bits(__floats2half2_rn(big, e - big)));
+        }
+        ps[(st * NT + n0 + i) * 32 + lane] = make_uint2(pb[0], pb[1]);
+      }
+      __syncthreads();  // the weights are there
+
+      // output: this warp's columns, all slots
+      const bool g0 = s_grown[parity][0], g1 = s_grown[parity][1];
+      if (g0 || g1) {
+        #pragma unroll
+        for (int i = 0; i < ON; ++i) {
+          if (!(o0 + i < NG ? g0 : g1)) continue;
+          const float f = s_fac[(o0 + i) * 4 + tig];
+          #pragma unroll
+          for (int z = 0; z < TP; ++z) o[z][0][i] *= f, o[z][1][i] *= f;
+        }
+      }
+      if (tid < 2) s_grown[parity ^ 1][tid] = 0;  // read last before this tile's first barrier
+      // d = 64: tile n is columns n and 4 + n of the lane's word; else tile 8 w + n is columns n of words 2 w, 2 w + 1.
+      // Even tiles are low nibbles, odd ones high nibbles.
+      uint32_t a[4][TP][4];
+      #pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        #pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const unsigned char* pc = tile + vs_at + (u * 16 + h * 8) * (D / 8);
+          const uint32_t s = *reinterpret_cast<const uint32_t*>(pc), t = *reinterpret_cast<const uint32_t*>(pc + D / 8);
+          const __half2 step = bits_h2(__byte_perm(s, t, 0x5410)), base = bits_h2(__byte_perm(s, t, 0x7632));
+          #pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            const int word = VW == 1 ? 0 : ot / 8 * 2 + z, byte = VW == 1 ? ot / 2 + 2 * z : ot % 8 / 2;
+            const int off = (u * 16 + h * 8) * (D / 2) + word * 4;
+            const uint32_t wa = *reinterpret_cast<const uint32_t*>(tile + va_at + off);
+            const uint32_t wb = *reinterpret_cast<const uint32_t*>(tile + vb_at + off);
+            const uint32_t both = __byte_perm(wa, wb, byte | (byte + 4) << 8);
+            if constexpr (TP == 2) {
+              a[u][0][2 * h + z] = kv4_pair<false>(both, p.mul64, step, base);
+              a[u][1][2 * h + z] = kv4_pair<true>(both, p.mul4, step, base);
+            } else {
+              // the nibbles that the warp's tile has, moved to the low ones
+              a[u][0][2 * h + z] = kv4_pair<false>(both >> (ot & 1) * 4, p.mul64, step, base);
+            }
+          }
+        }
+      }
+      #pragma unroll
+      for (int i = 0; i < ON; ++i) {
+        float d[TP][4];
+        #pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const uint2 b = ps[(u * NT + o0 + i) * 32 + lane];
+          #pragma unroll
+          for (int z = 0; z < TP; ++z) {
+            if (u == 0)
+              mma_f16_first(d[z], a[u][z][0], a[u][z][1], a[u][z][2], a[u][z][3], b.x, b.y);
+            else
+              mma_f16(d[z], a[u][z][0], a[u][z][1], a[u][z][2], a[u][z][3], b.x, b.y);
+          }
+        }
+        #pragma unroll
+        for (int z = 0; z < TP; ++z) o[z][0][i] += d[z][0] + d[z][1], o[z][1][i] += d[z][2] + d[z][3];
+      }
+      stage ^= 1, parity ^= 1;
+    }
+
+    // the rows' sums and maxima, then the output or this CTA's part of it
+    __syncthreads();
+    #pragma unroll
+    for (int i = 0; i < NG; ++i) {
+      #pragma unroll
+      for (int x = 4; x < 32; x <<= 1) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], x);
+      const int r = (n0 + i) * 4 + tig;
+      if (gid == 0) {
+        s_sum[st * RC + r] = sum[i];
+        if (st == 0) s_max[r] = top[i];
+      }
+    }
+    __syncthreads();
+    const bool whole = !run.enter && !run.leave;
+    const int kind = run.enter ? 0 : 1;
+    float* part = p.part + (static_cast<long long>(cta) * 2 + kind) * kPart;
+    for (int r = tid; r < RC; r += kRowsThreads) {
+      const float l = s_sum[r] + s_sum[RC + r] + s_sum[2 * RC + r] + s_sum[3 * RC + r];
+      if (!whole)
+        part[r] = s_max[r], part[RC + r] = l;
+      else if (kW && r < rows)
+        attn_put_lse(p, c, run, run.r0 + r, s_max[r], l);
+    }
+    #pragma unroll
+    for (int i = 0; i < ON; ++i) {
+      const int r = (o0 + i) * 4 + tig;
+      #pragma unroll
+      for (int z = 0; z < TP; ++z) {
+        #pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int x = (((ot + z) * 2 + h) * NT + o0 + i) * 32 + lane;
+          if (!whole) {
+            part[2 * RC + x] = o[z][h][i];
+          } else if (r < rows) {
+            const float l = s_sum[r] + s_sum[RC + r] + s_sum[2 * RC + r] + s_sum[3 * RC + r];
+            p.out[attn_row_at<D>(p, run, run.r0 + r, p.ldo) + attn_col<D, NT>(x)] = l != 0.f ? o[z][h][i] / l : 0.f;
+          }
+        }
+      }
+    }
+    if (tid == 0 && !run.enter) {
+      if (whole)
+        p.split[run.b * walk.hc_count + run.hc] = make_int2(cta, 1);
+      else
+        attn_put_split(p, run, walk.hc_count, cta, each, extra);
+    }
+    if (!more) break;
+    row0 = row1 - nxt.s0;
+    run = nxt;
+  }
+  cp_async_wait<0>();
+}
+
+}  // namespace vmlm

@@ -108,6 +108,41 @@ void kv4_set_rope(Kv4Rows* p, const vmlm_rope* r) {
   p->interleaved = r->interleaved;
 }
 
+// The launches behind the attention kernel: the join of items that several CTAs had parts of (`whole`: there can be none,
+// whatever the lengths are), and the weights of a call with w_out.
+template <int D, int NT, bool kW>
+int kv4_launch_finish(const Kv4Attn& p, const Kv4View& v, bool whole, cudaStream_t st) {
+  const long long heads = static_cast<long long>(v.n_seq) * v.n_kv;
+  const long long joins = heads * p.chunks * (4 * NT * D / 128), blocks = cdiv(v.cap, kWeightThreads);
+  if (joins >= static_cast<long long>(kKv4MaxDim) || heads * blocks >= static_cast<long long>(kKv4MaxDim))
+    return fail(VMLM_ERR_SHAPE, "kv4_attn_dev: n_seq * n_q * m * cap is too large");
+  if (!whole && joins > 0)
+    VMLM_TRY(launch(kv4_join_kernel<D, NT, kW>, dim3(static_cast<unsigned>(joins)), dim3(kJoinWarps * 32), 0, st, true, p, v));
+  if (!kW || heads * blocks == 0) return VMLM_OK;
+  return launch(kv4_weights_kernel, dim3(static_cast<unsigned>(heads * blocks)), dim3(kWeightThreads), 0, st, true, p, v,
+                static_cast<int>(blocks));
+}
+
+// Workspace and limits that both kernels share: nt fours of rows a chunk, `grid` CTAs, tiles of `tile` slots.
+int kv4_prepare_attn(Ctx* ctx, Kv4Attn* p, const Kv4View& v, int nt, int d, int grid, int tile) {
+  const size_t heads = static_cast<size_t>(v.n_seq) * v.n_kv;
+  p->chunks = static_cast<int>(cdiv(p->rows, 4 * nt));
+  p->mul4 = 4, p->mul64 = 64;
+  if (heads * p->chunks * static_cast<size_t>(cdiv(v.cap, tile)) >= kKv4MaxDim)
+    return fail(VMLM_ERR_SHAPE, "kv4_attn_dev: n_seq * n_q * m * cap is too large");
+  VMLM_TRY(ensure(ctx->kv4_part, static_cast<size_t>(grid) * 2 * 4 * nt * (d + 2) * 4));
+  VMLM_TRY(ensure(ctx->kv4_split, heads * p->chunks * sizeof(int2)));
+  p->part = static_cast<float*>(ctx->kv4_part.p);
+  p->split = static_cast<int2*>(ctx->kv4_split.p);
+  if (p->w_out) {
+    VMLM_TRY(ensure(ctx->kv4_lse, heads * p->rows * 4));
+    VMLM_TRY(ensure(ctx->kv4_score, heads * p->rows * static_cast<size_t>(v.cap) * 4));
+    p->lse = static_cast<float*>(ctx->kv4_lse.p);
+    p->score = static_cast<float*>(ctx->kv4_score.p);
+  }
+  return VMLM_OK;
+}
+
 template <int D, int NT, bool kW>
 int kv4_launch_attn(Ctx* ctx, Kv4Attn p, const Kv4View& v, cudaStream_t st) {
   constexpr int kSmem = attn_smem_bytes(D, NT);
@@ -116,37 +151,49 @@ int kv4_launch_attn(Ctx* ctx, Kv4Attn p, const Kv4View& v, cudaStream_t st) {
     VMLM_CUDA(cudaFuncSetAttribute(kv4_attn_kernel<D, NT, kW>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
     set[ctx->dev] = true;
   }
-  const size_t heads = static_cast<size_t>(v.n_seq) * v.n_kv;
-  p.chunks = static_cast<int>(cdiv(p.rows, 4 * NT));
   const int grid = ctx->sms;
-  VMLM_TRY(ensure(ctx->kv4_part, static_cast<size_t>(grid) * 2 * 4 * NT * (D + 2) * 4));
-  VMLM_TRY(ensure_zeroed(ctx->kv4_arrived, heads * p.chunks * 4, st));
-  p.part = static_cast<float*>(ctx->kv4_part.p);
-  p.arrived = static_cast<int*>(ctx->kv4_arrived.p);
-  p.mul4 = 4, p.mul64 = 64;
-  if (heads * p.chunks * static_cast<size_t>(cdiv(v.cap, 4096 / D)) >= kKv4MaxDim)
-    return fail(VMLM_ERR_SHAPE, "kv4_attn_dev: n_seq * n_q * m * cap is too large");
-  if (kW) {
-    VMLM_TRY(ensure(ctx->kv4_lse, heads * p.rows * 4));
-    VMLM_TRY(ensure(ctx->kv4_score, heads * p.rows * static_cast<size_t>(v.cap) * 4));
-    p.lse = static_cast<float*>(ctx->kv4_lse.p);
-    p.score = static_cast<float*>(ctx->kv4_score.p);
-  }
-  VMLM_TRY(launch(kv4_attn_kernel<D, NT, kW>, dim3(grid), dim3(attn_warps(D, NT) * 32), kSmem, st, false, p, v, ctx->err));
-  if (!kW || v.cap == 0) return VMLM_OK;
-  if (heads >= 65536) return fail(VMLM_ERR_SHAPE, "kv4_attn_dev: n_seq * n_kv must be < 65536 with w_out");
-  return launch(kv4_weights_kernel, dim3(static_cast<unsigned>(cdiv(v.cap, 256)), static_cast<unsigned>(heads)), dim3(256),
-                0, st, false, p, v);
+  VMLM_TRY(kv4_prepare_attn(ctx, &p, v, NT, D, grid, 4096 / D));
+  p.chunk_rows = 4 * NT;
+  VMLM_TRY(launch(kv4_attn_kernel<D, NT, kW>, dim3(grid), dim3(attn_warps(D, NT) * 32), kSmem, st, true, p, v, ctx->err));
+  const bool whole = static_cast<long long>(v.n_seq) * v.n_kv * p.chunks <= grid &&
+                     v.cap <= static_cast<long long>(attn_warps(D, NT)) * kAttnAlone * (4096 / D);
+  return kv4_launch_finish<D, NT, kW>(p, v, whole, st);
 }
 
-// Rows of a chunk: 4 where that holds them all, else 8, or (d = 64) 16. A chunk's
-// rows share the unpacked values; more than 256 / d * 4 do not fit the registers.
+template <int D, int NT, bool kW>
+int kv4_launch_attn_rows(Ctx* ctx, Kv4Attn p, const Kv4View& v, cudaStream_t st) {
+  constexpr int kSmem = rows_smem_bytes(D, NT);
+  static bool set[64] = {};
+  if (ctx->dev < 64 && !set[ctx->dev]) {
+    VMLM_CUDA(cudaFuncSetAttribute(kv4_attn_rows_kernel<D, NT, kW>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    set[ctx->dev] = true;
+  }
+  const int grid = 2 * ctx->sms;
+  VMLM_TRY(kv4_prepare_attn(ctx, &p, v, NT, D, grid, kRowsSlots));
+  p.chunk_rows = static_cast<int>(cdiv(cdiv(p.rows, p.chunks), 4)) * 4;  // even chunks
+  VMLM_TRY(launch(kv4_attn_rows_kernel<D, NT, kW>, dim3(grid), dim3(kRowsThreads), kSmem, st, true, p, v, ctx->err));
+  return kv4_launch_finish<D, NT, kW>(p, v, v.cap <= kRowsSlots, st);
+}
+
+// Few rows a kv head: a warp unpacks for all of them, 4 or 8 at a time. More: a CTA shares what it unpacks, in as few
+// chunks as hold the rows, and with the smallest count of fours that holds a chunk.
 template <int D, bool kW>
 int kv4_pick_attn(Ctx* ctx, const Kv4Attn& p, const Kv4View& v, cudaStream_t st) {
-  if (p.rows <= 4 || D == 256) return kv4_launch_attn<D, 1, kW>(ctx, p, v, st);
+  if (p.rows <= 4) return kv4_launch_attn<D, 1, kW>(ctx, p, v, st);
   if constexpr (D != 256) {
-    if (p.rows <= 8 || D == 128) return kv4_launch_attn<D, 2, kW>(ctx, p, v, st);
-    if constexpr (D == 64) return kv4_launch_attn<D, 4, kW>(ctx, p, v, st);
+    if (p.rows <= 8) return kv4_launch_attn<D, 2, kW>(ctx, p, v, st);
+  }
+  const long long chunks = cdiv(p.rows, 4 * rows_most(D)), fours = cdiv(cdiv(p.rows, chunks), 4);
+  if constexpr (D == 256) {
+    if (fours <= 2) return kv4_launch_attn_rows<D, 2, kW>(ctx, p, v, st);
+  }
+  if (fours <= 4) return kv4_launch_attn_rows<D, 4, kW>(ctx, p, v, st);
+  if (fours <= 6) return kv4_launch_attn_rows<D, 6, kW>(ctx, p, v, st);
+  if constexpr (D != 64) return kv4_launch_attn_rows<D, 8, kW>(ctx, p, v, st);
+  if constexpr (D == 64) {
+    if (fours <= 8) return kv4_launch_attn_rows<D, 8, kW>(ctx, p, v, st);
+    if (fours <= 10) return kv4_launch_attn_rows<D, 10, kW>(ctx, p, v, st);
+    return kv4_launch_attn_rows<D, 12, kW>(ctx, p, v, st);
   }
   return VMLM_OK;
 }
