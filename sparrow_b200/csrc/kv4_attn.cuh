@@ -175,31 +175,36 @@ struct AttnRun {
   int b, hc;          // sequence, kv head * chunks + chunk
   int head, r0;       // kv head, the chunk's first row
   int s0, s1, n;      // slots [s0, s1) of the n of the sequence
-  int first, units;   // the item's first tile among all, and its number of tiles
+  int first, units;   // where the item's tiles begin among all units, and how many they are
   bool enter, leave;  // the item has tiles before, behind this run
 };
+
+// The shares are counted in units: an item is its tiles, and before them kAttnRunCost units for what a run costs besides
+// (its queries and its result), so that short items do not gather in one share.
+constexpr int kAttnRunCost = 1;
 
 template <int TS>
 struct AttnWalk {
   const int32_t* len;
   int n_seq, hc_count, chunks, chunk_rows;
   long long cap;
-  int pos, end, base;  // tiles [pos, end); base: the first tile of sequence b
+  int pos, end, base;  // units [pos, end); base: the first unit of sequence b
   int b;
 
   __device__ __forceinline__ int length(int i) const {
     const long long n = __ldg(len + i);
     return static_cast<int>(n > cap ? cap : n < 0 ? 0 : n);
   }
-  __device__ __forceinline__ int tiles(int i) const { return (length(i) + TS - 1) / TS; }
-  // Moves (b, base) to the sequence that holds tile `at`; with kItems, to the one that holds the at-th item.
+  __device__ __forceinline__ int units_of(int n) const { return n > 0 ? (n + TS - 1) / TS + kAttnRunCost : 0; }
+  // Moves (b, base) to the sequence that holds unit `at`; with kItems, to the one that holds the at-th item. Returns how
+  // many come before that sequence.
   template <bool kItems>
   __device__ __forceinline__ int seek(int at) {
     const int lane = threadIdx.x & 31;
-    int before = 0, tile = 0;
+    int before = 0, unit = 0;
     #pragma unroll 1
     for (int i0 = 0; i0 < n_seq; i0 += 32) {
-      const int t = i0 + lane < n_seq ? tiles(i0 + lane) * hc_count : 0;
+      const int t = i0 + lane < n_seq ? units_of(length(i0 + lane)) * hc_count : 0;
       const int w = kItems ? (t > 0 ? hc_count : 0) : t;
       int sum = w, sum_t = t;
       #pragma unroll
@@ -211,39 +216,41 @@ struct AttnWalk {
       if (past) {
         const int l = __ffs(past) - 1;
         b = i0 + l;
-        base = tile + __shfl_sync(0xffffffffu, sum_t - t, l);
+        base = unit + __shfl_sync(0xffffffffu, sum_t - t, l);
         return before + __shfl_sync(0xffffffffu, sum - w, l);
       }
       before += __shfl_sync(0xffffffffu, sum, 31);
-      tile += __shfl_sync(0xffffffffu, sum_t, 31);
+      unit += __shfl_sync(0xffffffffu, sum_t, 31);
     }
     return before;
   }
   __device__ __forceinline__ bool next(AttnRun& s) {
-    if (pos >= end) return false;
-    int n, u;
-    while (true) {
-      n = length(b);
-      u = (n + TS - 1) / TS;
-      if (pos < base + u * hc_count) break;
-      base += u * hc_count;
-      ++b;
+    while (pos < end) {
+      const int n = length(b), u = units_of(n);
+      if (pos >= base + u * hc_count) {
+        base += u * hc_count;
+        ++b;
+        continue;
+      }
+      const int at = pos - base;
+      s.hc = hc_count == 1 ? 0 : at / u;
+      const int off = at - s.hc * u, take = min(end - pos, u - off);
+      const int t0 = max(0, off - kAttnRunCost), t1 = off + take - kAttnRunCost;  // its tiles
+      s.first = pos - off + kAttnRunCost;
+      pos += take;
+      if (t1 <= t0) continue;
+      s.b = b;
+      s.head = chunks == 1 ? s.hc : s.hc / chunks;
+      s.r0 = (s.hc - s.head * chunks) * chunk_rows;
+      s.n = n;
+      s.s0 = t0 * TS;
+      s.s1 = min(n, t1 * TS);
+      s.units = u - kAttnRunCost;
+      s.enter = t0 > 0;
+      s.leave = t1 < s.units;
+      return true;
     }
-    const int at = pos - base;
-    s.b = b;
-    s.hc = hc_count == 1 ? 0 : at / u;
-    s.head = chunks == 1 ? s.hc : s.hc / chunks;
-    s.r0 = (s.hc - s.head * chunks) * chunk_rows;
-    const int off = at - s.hc * u, take = min(end - pos, u - off);
-    s.n = n;
-    s.s0 = off * TS;
-    s.s1 = min(n, (off + take) * TS);
-    s.first = pos - off;
-    s.units = u;
-    s.enter = off > 0;
-    s.leave = off + take < u;
-    pos += take;
-    return true;
+    return false;
   }
 };
 
@@ -331,16 +338,16 @@ __global__ void __launch_bounds__(attn_warps(D, NT) * 32, 1) kv4_attn_kernel(con
   #pragma unroll 1
   for (int i = lane; i < c.n_seq; i += 32) {
     if (__ldg(p.len + i) > c.cap && tid == lane) atomicCAS(err, 0, kDevKv4Slot);
-    const int u = walk.tiles(i);
+    const int u = walk.units_of(walk.length(i));
     units += u, longest = max(longest, u), used += u > 0;
   }
   units = __reduce_add_sync(0xffffffffu, units) * walk.hc_count;
   longest = __reduce_max_sync(0xffffffffu, longest);
   used = __reduce_add_sync(0xffffffffu, used) * walk.hc_count;
   const int cta = blockIdx.x, grid = gridDim.x;
-  const bool alone = used <= grid && longest <= kWarps * kAttnAlone;
+  const bool alone = used <= grid && longest <= kWarps * kAttnAlone + kAttnRunCost;
   const int ctas = alone ? used : max(1, min(grid, units / kWarps));
-  const int each = units / max(1, ctas), extra = units - each * ctas;  // the first `extra` CTAs have one tile more
+  const int each = units / max(1, ctas), extra = units - each * ctas;  // the first `extra` CTAs have one unit more
 
   // Sequences without a slot: zeros.
   #pragma unroll 1
@@ -356,7 +363,7 @@ __global__ void __launch_bounds__(attn_warps(D, NT) * 32, 1) kv4_attn_kernel(con
   int lo, hi;
   if (alone) {
     const int before = walk.template seek<true>(cta);
-    const int u = walk.tiles(walk.b);
+    const int u = walk.units_of(walk.length(walk.b));
     lo = walk.base + (cta - before) * u, hi = lo + u;
   } else {
     lo = cta * each + min(cta, extra), hi = lo + each + (cta < extra);

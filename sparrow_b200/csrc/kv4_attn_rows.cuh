@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) kv4_attn_rows_kernel(const Kv
   #pragma unroll 1
   for (int i = lane; i < c.n_seq; i += 32) {
     if (__ldg(p.len + i) > c.cap && tid == lane) atomicCAS(err, 0, kDevKv4Slot);
-    units += walk.tiles(i);
+    units += walk.units_of(walk.length(i));
   }
   units = __reduce_add_sync(0xffffffffu, units) * walk.hc_count;
   const int cta = blockIdx.x, grid = gridDim.x;
@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) kv4_attn_rows_kernel(const Kv
   const int vs_at = kVsAt + 2 * tig * (D / 8) + gid * VW / 4 * 4;
 
   AttnRun run, nxt;
-  walk.next(run);  // a CTA's share is not empty
+  if (!walk.next(run)) return;  // a share may be an item's run cost alone
   long long row0 = first_row(run);
   fetch(row0 + run.s0, run.s1 - run.s0, 0);
   cp_async_commit();
@@ -339,18 +339,18 @@ __global__ void __launch_bounds__(kRowsThreads, 2) kv4_attn_rows_kernel(const Kv
     #pragma unroll
     for (int i = 0; i < ON; ++i) {
       const int r = (o0 + i) * 4 + tig;
-      #pragma unroll
-      for (int z = 0; z < TP; ++z) {
+      if (!whole) {
         #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int x = (((ot + z) * 2 + h) * NT + o0 + i) * 32 + lane;
-          if (!whole) {
-            part[2 * RC + x] = o[z][h][i];
-          } else if (r < rows) {
-            const float l = s_sum[r] + s_sum[RC + r] + s_sum[2 * RC + r] + s_sum[3 * RC + r];
-            p.out[attn_row_at<D>(p, run, run.r0 + r, p.ldo) + attn_col<D, NT>(x)] = l != 0.f ? o[z][h][i] / l : 0.f;
-          }
-        }
+        for (int z = 0; z < TP; ++z)
+          #pragma unroll
+          for (int h = 0; h < 2; ++h) part[2 * RC + (((ot + z) * 2 + h) * NT + o0 + i) * 32 + lane] = o[z][h][i];
+      } else if (r < rows) {
+        const float l = s_sum[r] + s_sum[RC + r] + s_sum[2 * RC + r] + s_sum[3 * RC + r], inv = l != 0.f ? 1.f / l : 0.f;
+        float* to = p.out + attn_row_at<D>(p, run, run.r0 + r, p.ldo);
+        #pragma unroll
+        for (int z = 0; z < TP; ++z)
+          #pragma unroll
+          for (int h = 0; h < 2; ++h) to[attn_col<D, NT>((((ot + z) * 2 + h) * NT + o0 + i) * 32 + lane)] = o[z][h][i] * inv;
       }
     }
     if (tid == 0 && !run.enter) {
