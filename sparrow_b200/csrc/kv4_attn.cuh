@@ -314,14 +314,13 @@ __global__ void __launch_bounds__(attn_warps(D, NT) * 32, 1) kv4_attn_kernel(con
   constexpr int kCh = D / 32;       // 16-byte chunks of a row of codes
   constexpr int kPart = RC * (D + 2);
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ float s_mul[RC][2 * kWarps];  // the factors of the parts that are joined, and where they lie
-  __shared__ int s_at[2 * kWarps];
+  __shared__ __align__(16) float s_mul[kWarps * 32 * RC];  // a warp's factors for the parts that it joins, and where they lie
+  __shared__ int s_at[kWarps * 32];
   // Parts of items that the warps leave for each other, in the order of the work: 2 w of warp w is the end of an item
   // that other warps began, 2 w + 1 the beginning of one that others end.
   __shared__ int s_state[2 * kWarps];  // 0: none, 1: the item ends here, 2: it goes on
   __shared__ int s_from[2 * kWarps];   // the output part: bytes into smem
   __shared__ AttnRun s_run[2 * kWarps];
-  __shared__ int s_parts;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int gid = lane >> 2, tig = lane & 3;
   unsigned char* ring = smem + warp * 2 * kAttnStageBytes;
@@ -438,10 +437,23 @@ __global__ void __launch_bounds__(attn_warps(D, NT) * 32, 1) kv4_attn_kernel(con
 
   if (lane < 2) s_state[2 * warp + lane] = 0;
   __syncwarp();
+  // A run's queries on their way to L1, before they are needed.
+  auto touch = [&](const AttnRun& s) {
+    #pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = s.r0 + nt * 4 + (gid >> 1);
+      if (r < p.rows) {
+        const float* at = p.q + row_at(s, r, p.ldq) + tig * (D / 4);
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(at));
+        if constexpr (D == 256) asm volatile("prefetch.global.L1 [%0];" ::"l"(at + 32));
+      }
+    }
+  };
   AttnRun run, nxt;
   bool have = walk.next(run);
   long long row0 = 0;
   if (have) {
+    touch(run);
     row0 = first_row(run);
     fetch(row0 + run.s0, run.s1 - run.s0, 0);
   }
@@ -710,72 +722,77 @@ __global__ void __launch_bounds__(attn_warps(D, NT) * 32, 1) kv4_attn_kernel(con
   __syncthreads();
 
   // Parts of one item left by neighbouring warps become one result: all of the item, or this CTA's part of it, of which
-  // there are at most two (kind 0: it began in an earlier CTA; kind 1: it began here and goes on).
-  int next = 0;
-  while (true) {
-    while (next < 2 * kWarps && !s_state[next]) ++next;
-    if (next >= 2 * kWarps) break;
-    const int first = next, kind = first & 1;  // a list that begins with a head: the item entered this CTA
-    int last = first;
-    bool open = s_state[first] == 2;
-    while (open) {
-      int k = last + 1;
-      while (k < 2 * kWarps && !s_state[k]) ++k;
-      if (k >= 2 * kWarps) break;
-      last = k, open = s_state[k] == 2;
-    }
-    next = last + 1;
-    const AttnRun it = s_run[first];
-    const bool final_here = kind == 1 && !open;
+  // there are at most two (kind 0: it began in an earlier CTA; kind 1: it began here and goes on). Lane k knows part k. A
+  // list begins with every beginning of an item (odd parts), and with the first part if that is the end of one; each warp
+  // takes a slice of a list.
+  const uint32_t valid = __ballot_sync(0xffffffffu, lane < 2 * kWarps && s_state[lane] != 0);
+  if (!valid) return;
+  const uint32_t begins = (valid & 0xAAAAAAAAu) | (valid & -valid);
+  const int lists = __popc(begins);
+  for (int mine = warp; mine < max(lists, kWarps / lists * lists); mine += kWarps) {
+    const int list = mine % lists, slice = mine / lists, slices = lists < kWarps ? kWarps / lists : 1;
+    uint32_t left = begins;
+    for (int i = 0; i < list; ++i) left &= left - 1;
+    const int first = __ffs(left) - 1;
+    left &= left - 1;
+    const uint32_t parts = valid & ~((1u << first) - 1u) & (left ? (1u << (__ffs(left) - 1)) - 1u : 0xffffffffu);
+    const int kind = first & 1, last = 31 - __clz(parts);
+    const bool final_here = kind == 1 && s_state[last] == 1;
+    const AttnRun& it = s_run[first];
     float* part = p.part + (static_cast<long long>(cta) * 2 + kind) * kPart;
-    // A warp a row: lane k has part k, and its factor.
-    #pragma unroll 1
-    for (int r = warp; r < RC; r += kWarps) {
-      const int k = first + lane;
-      const bool on = k <= last && s_state[k];
-      const float mk = on ? ml[(k * RC + r) * 2] : -1e30f, lk = on ? ml[(k * RC + r) * 2 + 1] : 0.f;
-      float m = mk;
-      #pragma unroll
-      for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-      const float f = ex2(mk - m);
-      float l = f * lk;
-      #pragma unroll
-      for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-      const uint32_t parts = __ballot_sync(0xffffffffu, on);
-      const int at = __popc(parts & ((1u << lane) - 1u));
-      if (on) {
-        s_mul[r][at] = final_here ? (l != 0.f ? f / l : 0.f) : f;
-        if (r == 0) s_at[at] = s_from[k];
-      }
-      if (lane == 0) {
-        if (r == 0) s_parts = __popc(parts);
-        if (!final_here)
-          part[r] = m, part[RC + r] = l;
-        else if (kW && it.r0 + r < p.rows)
-          put_lse(it, it.r0 + r, m, l);
-      }
-    }
-    __syncthreads();
+    // Lane (row, group): the row's maximum and sum over the parts, which the groups take in turn; then the factors.
+    const int count = __popc(parts), row = lane % RC, group = lane / RC;
+    constexpr int kGroups = 32 / RC;
+    float* mul = s_mul + warp * 32 * RC;  // [part][row]
+    int* from = s_at + warp * 32;         // [part]
+    if (parts >> lane & 1) from[__popc(parts & ((1u << lane) - 1u))] = lane;
+    __syncwarp();
+    float m = -1e30f, l = 0.f;
+    for (int i = group; i < count; i += kGroups) m = fmaxf(m, ml[(from[i] * RC + row) * 2]);
     #pragma unroll
-    for (int x0 = 0; x0 < RC * D; x0 += kThreads) {
-      const int x = x0 + tid, r = attn_row<NT>(x);
-      if (x >= RC * D) break;
-      float v = 0.f;
-      const int parts = s_parts;
-      #pragma unroll 4
-      for (int k = 0; k < parts; ++k) v = fmaf(s_mul[r][k], reinterpret_cast<const float*>(smem + s_at[k])[x], v);
-      if (!final_here)
-        part[2 * RC + x] = v;
-      else if (it.r0 + r < p.rows)
-        p.out[row_at(it, it.r0 + r, p.ldo) + attn_col<D, NT>(x)] = v;
+    for (int x = RC; x < 32; x *= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+    for (int i = group; i < count; i += kGroups) {
+      const float f = ex2(ml[(from[i] * RC + row) * 2] - m);
+      l = fmaf(f, ml[(from[i] * RC + row) * 2 + 1], l);
+      mul[i * RC + row] = f;
     }
-    if (kind == 1 && tid == 0) {
+    #pragma unroll
+    for (int x = RC; x < 32; x *= 2) l += __shfl_xor_sync(0xffffffffu, l, x);
+    const float inv = final_here ? (l != 0.f ? 1.f / l : 0.f) : 1.f;
+    if (slice == 0 && group == 0) {
+      if (!final_here)
+        part[row] = m, part[RC + row] = l;
+      else if (kW && it.r0 + row < p.rows)
+        put_lse(it, it.r0 + row, m, l);
+    }
+    __syncwarp();
+    if ((parts >> lane & 1) != 0) from[__popc(parts & ((1u << lane) - 1u))] = s_from[lane];
+    __syncwarp();
+    for (int x = (slice * 32 + lane) * 4; x < RC * D; x += slices * 128) {  // the four rows of a column
+      const int r = attn_row<NT>(x);
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      #pragma unroll 4
+      for (int i = 0; i < count; ++i) {
+        const float4 f = *reinterpret_cast<const float4*>(mul + i * RC + r);
+        const float4 y = *reinterpret_cast<const float4*>(smem + from[i] + x * 4);
+        v.x = fmaf(f.x, y.x, v.x), v.y = fmaf(f.y, y.y, v.y), v.z = fmaf(f.z, y.z, v.z), v.w = fmaf(f.w, y.w, v.w);
+      }
+      if (!final_here) *reinterpret_cast<float4*>(part + 2 * RC + x) = v;
+      const float w[4] = {v.x, v.y, v.z, v.w};
+      #pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float scale = __shfl_sync(0xffffffffu, inv, r + j);  // lane r + j has row r + j
+        if (final_here && it.r0 + r + j < p.rows)
+          p.out[row_at(it, it.r0 + r + j, p.ldo) + attn_col<D, NT>(x)] = w[j] * scale;
+      }
+    }
+    if (kind == 1 && slice == 0 && lane == 0) {
       if (final_here)
         p.split[it.b * walk.hc_count + it.hc] = make_int2(cta, 1);
       else
         attn_put_split(p, it, walk.hc_count, cta, each, extra);
     }
-    if (next < 2 * kWarps) __syncthreads();  // s_mul is used again
+    __syncwarp();
   }
 }
 
@@ -792,9 +809,9 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(const Kv4Attn
   pdl_launch_dependents();
   const int item = blockIdx.x / kSlices, slice = blockIdx.x - item * kSlices;
   const int hc = item % (c.n_kv * p.chunks), b = item / (c.n_kv * p.chunks);
-  if (__ldg(p.len + b) <= 0) return;
-  const int2 s = p.split[item];
-  if (s.y <= 1) return;
+  const int n = __ldg(p.len + b);
+  const int2 s = p.split[item];  // of a sequence without slots: left over
+  if (n <= 0 || s.y <= 1) return;
   const int x = (slice * 32 + lane) * 4, r = attn_row<NT>(x);
   AttnRun it;
   it.b = b, it.head = hc / p.chunks, it.r0 = (hc - it.head * p.chunks) * p.chunk_rows;

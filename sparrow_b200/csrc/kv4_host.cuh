@@ -128,7 +128,7 @@ int kv4_prepare_attn(Ctx* ctx, Kv4Attn* p, const Kv4View& v, int nt, int d, int 
   const size_t heads = static_cast<size_t>(v.n_seq) * v.n_kv;
   p->chunks = static_cast<int>(cdiv(p->rows, 4 * nt));
   p->mul4 = 4, p->mul64 = 64;
-  if (heads * p->chunks * static_cast<size_t>(cdiv(v.cap, tile)) >= kKv4MaxDim)
+  if (heads * p->chunks * static_cast<size_t>(cdiv(v.cap, tile) + kAttnRunCost) >= kKv4MaxDim)
     return fail(VMLM_ERR_SHAPE, "kv4_attn_dev: n_seq * n_q * m * cap is too large");
   VMLM_TRY(ensure(ctx->kv4_part, static_cast<size_t>(grid) * 2 * 4 * nt * (d + 2) * 4));
   VMLM_TRY(ensure(ctx->kv4_split, heads * p->chunks * sizeof(int2)));
