@@ -129,8 +129,9 @@ __device__ __forceinline__ void kv4_store_rows(const float (&x)[8], bool on, uin
     uint32_t bits = 0;
     #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float t = __fsub_rn(rintf(__fmul_rn(__fsub_rn(c[i], base), inv)), 16.f);
-      bits |= static_cast<uint32_t>(fminf(fmaxf(t, 0.f), 15.f)) << (4 * i);
+      // rint by adding 1.5 * 2^23 (|x| is far below 2^22): the integer lies in the low bits, and no conversion is needed
+      const int n = __float_as_int(__fadd_rn(__fmul_rn(__fsub_rn(c[i], base), inv), 12582912.f)) - 0x4B400000 - 16;
+      bits |= static_cast<uint32_t>(min(max(n, 0), 15)) << (4 * i);
     }
     if (on) {
       *reinterpret_cast<uint16_t*>(codes + row * (D / 2) + h * (D / 4) + l * 2) = static_cast<uint16_t>(bits);
@@ -186,9 +187,11 @@ __device__ __forceinline__ void load4(const float* p, bool vec, float* x) {
 // whole before it is written, by the same lanes.
 // Bound by HBM: each value is read once and written once; of the instructions,
 // which are the next bound, the root and the tree count for 256 / d rows. R = 2
-// keeps more loads in flight; R = 1 spreads few rows over more warps.
+// keeps more loads in flight and shares a token's table rows; R = 1 spreads few
+// rows over more warps. Five blocks an SM: 8191 tokens of 32 + 2 x 8 heads of 128
+// take 80 us, with the registers of two 90, and R = 4 is slower at any count.
 template <int D, bool kCache, int R>
-__global__ void __launch_bounds__(256) kv4_rows_kernel(const Kv4Rows p, const Kv4View c, int* __restrict__ err) {
+__global__ void __launch_bounds__(256, 5) kv4_rows_kernel(const Kv4Rows p, const Kv4View c, int* __restrict__ err) {
   constexpr int L = D / 8, kRows = 32 / L;
   pdl_wait_prior();
   pdl_launch_dependents();
@@ -251,8 +254,9 @@ __global__ void __launch_bounds__(256) kv4_rows_kernel(const Kv4Rows p, const Kv
     const bool in = h < heads, is_q = h < p.n_q, is_v = h >= p.n_q + p.n_kv;
     const float* gain = is_q ? p.gq : p.gk;
     float y[8];
-    const float sum = tree_sum<D>(x[j]);  // of values too: the lanes of a warp stay together
-    if (gain) {
+    const bool turns = __any_sync(0xffffffffu, !is_v);  // a warp of values has nothing to do before they are stored
+    const float sum = turns ? tree_sum<D>(x[j]) : 0.f;
+    if (turns && gain) {
       float g[8];
       load4(gain + 4 * l, p.vec_g, g);
       load4(gain + D / 2 + 4 * l, p.vec_g, g + 4);
@@ -263,14 +267,15 @@ __global__ void __launch_bounds__(256) kv4_rows_kernel(const Kv4Rows p, const Kv
       #pragma unroll
       for (int i = 0; i < 8; ++i) y[i] = x[j][i];
     }
-    if (p.cos_t) {
+    if (turns && p.cos_t) {
       // a cos - b sin and b cos + a sin, the difference as a sum with the sine's sign turned: the same bits
       float z[8];
       if (whole) {
         #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          z[i] = __fadd_rn(__fmul_rn(y[i], cs[i]), __fmul_rn(y[i + 4], -sn[i]));
-          z[i + 4] = __fadd_rn(__fmul_rn(y[i + 4], cs[i]), __fmul_rn(y[i], sn[i]));
+          const float a = y[i], b = y[i + 4];
+          y[i] = __fadd_rn(__fmul_rn(a, cs[i]), __fmul_rn(b, -sn[i]));
+          y[i + 4] = __fadd_rn(__fmul_rn(b, cs[i]), __fmul_rn(a, sn[i]));
         }
       } else if (p.interleaved) {
         #pragma unroll
@@ -296,7 +301,7 @@ __global__ void __launch_bounds__(256) kv4_rows_kernel(const Kv4Rows p, const Kv
       }
       #pragma unroll
       for (int w = 0; w < 2; ++w)
-        if (w * (D / 2) + 4 * l < p.rot) {
+        if (!whole && w * (D / 2) + 4 * l < p.rot) {
           #pragma unroll
           for (int i = 4 * w; i < 4 * w + 4; ++i) y[i] = z[i];
         }
@@ -405,7 +410,8 @@ __device__ __forceinline__ uint32_t kv4_weight_key(float w) {
 constexpr int kEvictThreads = 1024;
 constexpr int kEvictMaxCluster = 8;
 constexpr int kEvictBins = 2048;   // 11 bits a pass of the radix select: 11, 11, 10
-constexpr int kEvictKeys = 44 * 1024;  // keys that a CTA's shared memory holds
+constexpr int kEvictKeys = 24 * 1024;  // keys that a CTA's shared memory holds, two CTAs on an SM
+constexpr int kEvictShare = 4096;      // slots a CTA from which a cluster is made larger
 
 // Shared memory: a histogram, the scans' words, the CTA's keys (and later its kept slots).
 __host__ __device__ constexpr int evict_smem_bytes(int keys) { return kEvictBins * 4 + 256 + keys * 4; }
@@ -467,13 +473,13 @@ __device__ __forceinline__ void cluster_sync() {
 // moves its rows. Bound by HBM for long caches (4 bytes a slot, 2.5 d a kept
 // one), by the passes' barriers for short ones.
 template <int D>
-__global__ void __launch_bounds__(kEvictThreads, 1)
+__global__ void __launch_bounds__(kEvictThreads, 2)
     kv4_evict_kernel(const Kv4Evict p, const Kv4View src, const Kv4View dst, int* __restrict__ err) {
   extern __shared__ __align__(128) unsigned char smem[];
   uint32_t* hist = reinterpret_cast<uint32_t*>(smem);            // [kEvictBins]
   int* scratch = reinterpret_cast<int*>(hist + kEvictBins);      // [33 + 31]
   uint32_t* keys = reinterpret_cast<uint32_t*>(scratch + 64);    // [p.keys]
-  __shared__ int s_pick[2], s_count[2];
+  __shared__ int s_pick[3], s_count[2];
   const int tid = threadIdx.x;
   const uint32_t rank = cluster_ctarank();
   uint32_t size;
@@ -497,13 +503,15 @@ __global__ void __launch_bounds__(kEvictThreads, 1)
   const int lo = p.first, hi = n - p.recent;  // the slots that the weights decide about
   const bool all = n <= keep;
   uint32_t prefix = 0;
+  int shift = 0;  // of a key's digits to prefix
   int want = all ? 0 : keep - p.first - p.recent;  // the want-th largest of the keys that begin with prefix
   auto key_at = [&](int i) { return i - i0 < p.keys ? keys[i - i0] : kv4_weight_key(__ldg(w + i)); };
   if (want > 0) {  // the same in the whole cluster
     for (int i = i0 + tid; i < min(i1, i0 + p.keys); i += kEvictThreads) keys[i - i0] = kv4_weight_key(__ldg(w + i));
     #pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
-      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+      const int bits = pass == 2 ? 10 : 11;
+      shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
       for (int i = tid; i < kEvictBins; i += kEvictThreads) hist[i] = 0;
       __syncthreads();
       // equal neighbours in a thread's sequence are counted together: many slots may have the same weight
@@ -535,19 +543,22 @@ __global__ void __launch_bounds__(kEvictThreads, 1)
       }
       int total;
       const int above = block_scan(static_cast<int>(c[0] + c[1]), scratch, &total);
-      if (above < want && above + static_cast<int>(c[0]) >= want) s_pick[0] = top, s_pick[1] = want - above;
+      if (above < want && above + static_cast<int>(c[0]) >= want)
+        s_pick[0] = top, s_pick[1] = want - above, s_pick[2] = c[0];
       if (above + static_cast<int>(c[0]) < want && above + static_cast<int>(c[0] + c[1]) >= want)
-        s_pick[0] = top - 1, s_pick[1] = want - above - static_cast<int>(c[0]);
+        s_pick[0] = top - 1, s_pick[1] = want - above - static_cast<int>(c[0]), s_pick[2] = c[1];
       __syncthreads();
       prefix = prefix << bits | static_cast<uint32_t>(s_pick[0]);
       want = s_pick[1];
+      const bool done = want == s_pick[2];  // all keys with these digits are kept: the others do not matter
       if (size > 1) cluster_sync();  // the counts have been read
       else __syncthreads();
+      if (done) break;
     }
   }
-  // prefix = T, want = how many of the keys equal to T are kept (all kept: 0, not asked). A warp takes neighbouring
-  // slots, 32 at a time; the counts of keys above T (and of what is kept anyway) and equal to T before it say where it
-  // writes.
+  // prefix = T (or the digits of T that decide), want = how many of the keys equal to it are kept (all kept: 0, not
+  // asked). A warp takes neighbouring slots, 32 at a time; the counts of keys above T (and of what is kept anyway) and
+  // equal to T before it say where it writes.
   const int lane = tid & 31, warp = tid >> 5;
   const int each = (i1 - i0 + kEvictThreads - 1) / kEvictThreads * 32;
   const int t0 = min(i1, i0 + warp * each), t1 = min(i1, t0 + each);
@@ -555,7 +566,7 @@ __global__ void __launch_bounds__(kEvictThreads, 1)
   auto look = [&](int i, bool& sure, bool& equal) {
     sure = i < t1 && (all || i < lo || i >= hi), equal = false;
     if (i < t1 && !sure && pick) {
-      const uint32_t key = key_at(i);
+      const uint32_t key = key_at(i) >> shift;
       sure = key > prefix, equal = key == prefix;
     }
   };
@@ -609,14 +620,31 @@ __global__ void __launch_bounds__(kEvictThreads, 1)
   const long long from0 = static_cast<long long>(bh) * src.cap, to0 = static_cast<long long>(bh) * dst.cap;
   const uint4 *sk = reinterpret_cast<const uint4*>(src.k), *sv = reinterpret_cast<const uint4*>(src.v);
   uint4 *dk = reinterpret_cast<uint4*>(dst.k), *dv = reinterpret_cast<uint4*>(dst.v);
-  #pragma unroll 2
-  for (int x = tid; x < mine * U; x += kEvictThreads) {
-    const int at = base + x / U, u = x % U;
-    const long long from = (from0 + io[at]) * U + u, to = (to0 + at) * U + u;
-    const uint4 k = __ldg(sk + from), v = __ldg(sv + from);
-    const uint32_t ks = __ldg(src.ks + from), vs = __ldg(src.vs + from);
-    dk[to] = k, dv[to] = v;
-    dst.ks[to] = ks, dst.vs[to] = vs;
+  constexpr int kBatch = 2;  // units in flight a thread; of its registers, 32, they take 20
+  #pragma unroll 1
+  for (int x0 = tid; x0 < mine * U; x0 += kBatch * kEvictThreads) {
+    long long from[kBatch];
+    #pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int x = x0 + i * kEvictThreads;
+      from[i] = x < mine * U ? (from0 + io[base + x / U]) * U + x % U : 0;
+    }
+    uint4 k[kBatch], v[kBatch];
+    uint32_t ks[kBatch], vs[kBatch];
+    #pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (x0 + i * kEvictThreads >= mine * U) continue;
+      k[i] = __ldg(sk + from[i]), v[i] = __ldg(sv + from[i]);
+      ks[i] = __ldg(src.ks + from[i]), vs[i] = __ldg(src.vs + from[i]);
+    }
+    #pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int x = x0 + i * kEvictThreads;
+      if (x >= mine * U) continue;
+      const long long to = (to0 + base) * U + x;
+      dk[to] = k[i], dv[to] = v[i];
+      dst.ks[to] = ks[i], dst.vs[to] = vs[i];
+    }
   }
   if (size > 1) cluster_sync();  // no CTA leaves while another may read its counts
 }

@@ -53,9 +53,9 @@ constexpr float kAttnSlack = 1.f;        // a running maximum may lag by this (l
 constexpr int kAttnAlone = 4;            // tiles a warp up to which a CTA takes an item alone
 
 // Warps of the one CTA on an SM. A chunk of rows takes D/8 registers a four rows
-// for its queries and as many for its output; 256 values of d x fours fit 168
-// registers (12 warps), 128 fit 128 (16 warps).
-__host__ __device__ constexpr int attn_warps(int D, int NT) { return NT * D > 128 ? 12 : 16; }
+// for its queries and as many for its output; 8 rows, or d = 256, fit 168
+// registers (12 warps), 4 rows fit 128 (16 warps).
+__host__ __device__ constexpr int attn_warps(int D, int NT) { return NT > 1 || D == 256 ? 12 : 16; }
 // Dynamic shared memory: the warps' rings, a partial result and two (m, l) lists a warp.
 __host__ __device__ constexpr int attn_smem_bytes(int D, int NT) {
   return attn_warps(D, NT) * (2 * kAttnStageBytes + 4 * NT * D * 4 + 2 * 4 * NT * 8);
@@ -863,35 +863,51 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(const Kv4Attn
   }
 }
 
-// The weights that slots received, from the kept scores and the rows' sums: a thread a slot, 256 slots of a kv head a block.
-// Bound by the scores' reads (4 bytes a row and slot).
-constexpr int kWeightThreads = 256;
+// The weights that slots received, from the kept scores and the rows' sums: a thread has kWeightSlots slots, 256 apart, of
+// a kv head. Bound by the scores' reads (4 bytes a row and slot): four slots keep enough of them in flight for few rows (8 x
+// 8 heads of 4 rows, up to 16384 slots: the call takes 33.9 us, with one slot 37), one slot makes enough blocks where many
+// rows do that (72 heads of 33 rows, 4097 slots: 67 us, with four 74.6).
+constexpr int kWeightThreads = 256, kWeightFewRows = 8;
 
+template <int kWeightSlots>
 __global__ void __launch_bounds__(kWeightThreads) kv4_weights_kernel(const Kv4Attn p, const Kv4View c, int blocks) {
   __shared__ float s_lse[kWeightThreads];
   pdl_wait_prior();
   pdl_launch_dependents();
   const int tid = threadIdx.x, bh = blockIdx.x / blocks, b = bh / c.n_kv;
-  const long long j0 = static_cast<long long>(blockIdx.x - bh * blocks) * kWeightThreads, j = j0 + tid;
+  const long long j0 = static_cast<long long>(blockIdx.x - bh * blocks) * (kWeightThreads * kWeightSlots);
   long long n = __ldg(p.len + b);
   if (n > c.cap) n = c.cap;
   if (j0 >= n) return;
-  const long long at = static_cast<long long>(bh) * c.cap + j;
-  float w = j < n - p.m && p.w_in ? p.w_in[at] : 0.f;
-  // rows of tokens that do not see the slot come first
-  const long long late = j - (n - p.m);
-  const int skip = late > 0 ? static_cast<int>(late) * p.group : 0;
+  const long long at = static_cast<long long>(bh) * c.cap + j0 + tid;
+  // slots of this thread, and rows that come too early to see each of them
+  const int have = static_cast<int>(n - j0 - tid), old = static_cast<int>(n - p.m - j0 - tid);
+  float w[kWeightSlots];
+  int skip[kWeightSlots];
+  #pragma unroll
+  for (int i = 0; i < kWeightSlots; ++i) {
+    const int late = i * kWeightThreads - old;
+    w[i] = late < 0 && p.w_in ? p.w_in[at + i * kWeightThreads] : 0.f;
+    skip[i] = i * kWeightThreads >= have ? p.rows : late > 0 ? late * p.group : 0;
+  }
   for (int r0 = 0; r0 < p.rows; r0 += kWeightThreads) {
     const int rows = min(kWeightThreads, p.rows - r0);
     __syncthreads();
     if (tid < rows) s_lse[tid] = p.lse[static_cast<long long>(bh) * p.rows + r0 + tid];
     __syncthreads();
-    if (j >= n) continue;
-    const float* s = p.score + (static_cast<long long>(bh) * p.rows + r0) * c.cap + j;
-    #pragma unroll 8
-    for (int r = max(0, skip - r0); r < rows; ++r) w += ex2(__ldg(s + r * c.cap) - s_lse[r]);
+    const float* s = p.score + (static_cast<long long>(bh) * p.rows + r0) * c.cap + j0 + tid;
+    #pragma unroll 4
+    for (int r = 0; r < rows; ++r) {
+      const float lse = s_lse[r];
+      #pragma unroll
+      for (int i = 0; i < kWeightSlots; ++i)
+        if (r0 + r >= skip[i]) w[i] += ex2(__ldg(s + i * kWeightThreads) - lse);
+      s += c.cap;
+    }
   }
-  if (j < n) p.w_out[at] = w;
+  #pragma unroll
+  for (int i = 0; i < kWeightSlots; ++i)
+    if (i * kWeightThreads < have) p.w_out[at + i * kWeightThreads] = w[i];
 }
 
 }  // namespace vmlm

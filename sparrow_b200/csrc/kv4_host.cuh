@@ -89,10 +89,11 @@ int kv4_launch_evict(Ctx* ctx, Kv4Evict p, const Kv4View& s, const Kv4View& d, c
                                    evict_smem_bytes(kEvictKeys)));
     set[ctx->dev] = true;
   }
-  // CTAs a head: as many as leave no SM without one, while each still has a thousand slots.
+  // CTAs a head: as many as two an SM have room for, while each still has kEvictShare slots: below, the barriers of a
+  // cluster cost more than the work that it divides.
   const long long heads = static_cast<long long>(s.n_seq) * s.n_kv;
   int size = 1;
-  while (size < kEvictMaxCluster && heads * size * 2 <= ctx->sms && s.cap > 1024ll * size) size *= 2;
+  while (size < kEvictMaxCluster && heads * size <= ctx->sms && s.cap > kEvictShare * size) size *= 2;
   p.keys = static_cast<int>(std::min<long long>(kEvictKeys, cdiv(s.cap, size)));
   return launch_ex(kv4_evict_kernel<D>, dim3(size, static_cast<unsigned>(heads)), dim3(kEvictThreads),
                    evict_smem_bytes(p.keys), st, true, size, p, s, d, ctx->err);
@@ -113,14 +114,14 @@ void kv4_set_rope(Kv4Rows* p, const vmlm_rope* r) {
 template <int D, int NT, bool kW>
 int kv4_launch_finish(const Kv4Attn& p, const Kv4View& v, bool whole, cudaStream_t st) {
   const long long heads = static_cast<long long>(v.n_seq) * v.n_kv;
-  const long long joins = heads * p.chunks * (4 * NT * D / 128), blocks = cdiv(v.cap, kWeightThreads);
+  const long long joins = heads * p.chunks * (4 * NT * D / 128), blocks = cdiv(v.cap, kWeightThreads * (p.rows <= kWeightFewRows ? 4 : 1));
   if (joins >= static_cast<long long>(kKv4MaxDim) || heads * blocks >= static_cast<long long>(kKv4MaxDim))
     return fail(VMLM_ERR_SHAPE, "kv4_attn_dev: n_seq * n_q * m * cap is too large");
   if (!whole && joins > 0)
     VMLM_TRY(launch(kv4_join_kernel<D, NT, kW>, dim3(static_cast<unsigned>(joins)), dim3(kJoinWarps * 32), 0, st, true, p, v));
   if (!kW || heads * blocks == 0) return VMLM_OK;
-  return launch(kv4_weights_kernel, dim3(static_cast<unsigned>(heads * blocks)), dim3(kWeightThreads), 0, st, true, p, v,
-                static_cast<int>(blocks));
+  return launch(p.rows <= kWeightFewRows ? kv4_weights_kernel<4> : kv4_weights_kernel<1>,
+                dim3(static_cast<unsigned>(heads * blocks)), dim3(kWeightThreads), 0, st, true, p, v, static_cast<int>(blocks));
 }
 
 // Workspace and limits that both kernels share: nt fours of rows a chunk, `grid` CTAs, tiles of `tile` slots.

@@ -426,14 +426,31 @@ def emb_dev(table, idx, out, stream=None) -> None:
 
 # ------------------------------------- a 4-bit key/value cache for decode
 
+_F32 = None  # torch.float32, once a tensor of it has been seen
+
+
 def _rows_ptr(x, rows, width, name):
     """(address, row stride) of a [rows, >= width] float32 CUDA tensor whose rows may be slices of wider ones."""
-    if not x.is_cuda or _dtype_name(x.dtype) != "float32":
-        raise ValueError(f"{name}: expected a float32 CUDA tensor")
-    shape, stride = x.shape, x.stride()
-    if len(shape) != 2 or shape[0] < rows or shape[1] < width or (stride[1] != 1 and shape[1] > 1):
-        raise ValueError(f"{name}: needs {rows} rows of {width} values with unit column stride, has {tuple(shape)}")
-    return x.data_ptr(), stride[0] if shape[0] > 1 else max(stride[0], shape[1])
+    global _F32
+    if x.dtype is not _F32:
+        if _dtype_name(x.dtype) != "float32":
+            raise ValueError(f"{name}: expected a float32 CUDA tensor")
+        _F32 = x.dtype
+    if x.dim() != 2 or not x.is_cuda:
+        raise ValueError(f"{name}: expected a CUDA tensor of rows")
+    (n, w), (ld, step) = x.shape, x.stride()
+    if n < rows or w < width or (step != 1 and w > 1):
+        raise ValueError(f"{name}: needs {rows} rows of {width} values with unit column stride, has {tuple(x.shape)}")
+    return x.data_ptr(), ld if n > 1 else max(ld, w)
+
+
+def _ptr(x, dtype_name, count, name):
+    """_dev_ptr for the calls of a decode step, whose host time counts: a plain address."""
+    if x is None or isinstance(x, int):
+        return x
+    if not x.is_cuda or _dtype_name(x.dtype) != dtype_name or x.numel() < count or not x.is_contiguous():
+        return _dev_ptr(x, dtype_name, count, name)  # says what is wrong
+    return x.data_ptr()
 
 
 class Rope:
@@ -477,10 +494,6 @@ class Kv4Cache:
         return cls(*codes, *sb)
 
 
-def _gain_ptr(g, d, name):
-    return None if g is None else _dev_ptr(g, "float32", d, name)
-
-
 def _rope_ref(rope, tokens):
     if rope is None:
         return None
@@ -496,7 +509,7 @@ def qk_norm_rope_dev(q, k, gq, gk, eps, rope, qo, ko, tokens, n_q, n_kv, d, stre
     pqo, ldqo = _rows_ptr(qo, tokens, n_q * d, "qo") if n_q else (None, 0)
     pk, ldk = _rows_ptr(k, tokens, n_kv * d, "k") if n_kv else (None, 0)
     pko, ldko = _rows_ptr(ko, tokens, n_kv * d, "ko") if n_kv else (None, 0)
-    check(lib().vmlm_qk_norm_rope_dev(pq, ldq, pk, ldk, _gain_ptr(gq, d, "gq"), _gain_ptr(gk, d, "gk"), eps,
+    check(lib().vmlm_qk_norm_rope_dev(pq, ldq, pk, ldk, _ptr(gq, "float32", d, "gq"), _ptr(gk, "float32", d, "gk"), eps,
                                       _rope_ref(rope, tokens), pqo, ldqo, pko, ldko, tokens, n_q, n_kv, d,
                                       _stream_ptr(stream)))
 
@@ -510,18 +523,18 @@ def kv4_append_dev(cache, k, v, length, m, q=None, qo=None, n_q=0, gq=None, gk=N
     pv, ldv = _rows_ptr(v, tokens, cache.n_kv * d, "v")
     pq, ldq = _rows_ptr(q, tokens, n_q * d, "q") if n_q else (None, 0)
     pqo, ldqo = _rows_ptr(qo, tokens, n_q * d, "qo") if n_q else (None, 0)
-    check(lib().vmlm_kv4_append_dev(cache.ref, pq, ldq, pqo, ldqo, n_q, pk, ldk, pv, ldv, _gain_ptr(gq, d, "gq"),
-                                    _gain_ptr(gk, d, "gk"), eps, _rope_ref(rope, tokens),
-                                    _dev_ptr(length, "int32", cache.n_seq, "length"), m, _stream_ptr(stream)))
+    check(lib().vmlm_kv4_append_dev(cache.ref, pq, ldq, pqo, ldqo, n_q, pk, ldk, pv, ldv, _ptr(gq, "float32", d, "gq"),
+                                    _ptr(gk, "float32", d, "gk"), eps, _rope_ref(rope, tokens),
+                                    _ptr(length, "int32", cache.n_seq, "length"), m, _stream_ptr(stream)))
 
 
 def kv4_read_dev(cache, start, end, count, k, v, stream=None) -> None:
     """Rows start[b] .. start[b] + count - 1 of each sequence and kv head as the values they stand for: k, v float16
     [n_seq, n_kv, count, d]; rows at or behind end[b] are zeros."""
     n = cache.n_seq * cache.n_kv * count * cache.d
-    check(lib().vmlm_kv4_read_dev(cache.ref, _dev_ptr(start, "int32", cache.n_seq, "start"),
-                                  _dev_ptr(end, "int32", cache.n_seq, "end"), count, _dev_ptr(k, "float16", n, "k"),
-                                  _dev_ptr(v, "float16", n, "v"), _stream_ptr(stream)))
+    check(lib().vmlm_kv4_read_dev(cache.ref, _ptr(start, "int32", cache.n_seq, "start"),
+                                  _ptr(end, "int32", cache.n_seq, "end"), count, _ptr(k, "float16", n, "k"),
+                                  _ptr(v, "float16", n, "v"), _stream_ptr(stream)))
 
 
 def kv4_attn_dev(cache, q, length, out, m, n_q, scale, w_in=None, w_out=None, stream=None) -> None:
@@ -531,9 +544,9 @@ def kv4_attn_dev(cache, q, length, out, m, n_q, scale, w_in=None, w_out=None, st
     pq, ldq = _rows_ptr(q, tokens, width, "q")
     po, ldo = _rows_ptr(out, tokens, width, "out")
     slots = cache.n_seq * cache.n_kv * cache.cap
-    check(lib().vmlm_kv4_attn_dev(cache.ref, pq, ldq, _dev_ptr(length, "int32", cache.n_seq, "length"), po, ldo, m, n_q,
-                                  scale, _dev_ptr(w_in, "float32", slots, "w_in"),
-                                  _dev_ptr(w_out, "float32", slots, "w_out"), _stream_ptr(stream)))
+    check(lib().vmlm_kv4_attn_dev(cache.ref, pq, ldq, _ptr(length, "int32", cache.n_seq, "length"), po, ldo, m, n_q, scale,
+                                  _ptr(w_in, "float32", slots, "w_in"), _ptr(w_out, "float32", slots, "w_out"),
+                                  _stream_ptr(stream)))
 
 
 def kv4_evict_dev(src, dst, w, length, keep, first, recent, idx, w_out, len_out, stream=None) -> None:
@@ -541,10 +554,10 @@ def kv4_evict_dev(src, dst, w, length, keep, first, recent, idx, w_out, len_out,
     and the last `recent` always among them) from src to dst, in slot order; idx, w_out [n_seq, n_kv, keep] and len_out
     [n_seq] say which they are. w_out may be None."""
     out = src.n_seq * src.n_kv * keep
-    check(lib().vmlm_kv4_evict_dev(src.ref, dst.ref, _dev_ptr(w, "float32", src.n_seq * src.n_kv * src.cap, "w"),
-                                   _dev_ptr(length, "int32", src.n_seq, "length"), keep, first, recent,
-                                   _dev_ptr(idx, "int32", out, "idx"), _dev_ptr(w_out, "float32", out, "w_out"),
-                                   _dev_ptr(len_out, "int32", src.n_seq, "len_out"), _stream_ptr(stream)))
+    check(lib().vmlm_kv4_evict_dev(src.ref, dst.ref, _ptr(w, "float32", src.n_seq * src.n_kv * src.cap, "w"),
+                                   _ptr(length, "int32", src.n_seq, "length"), keep, first, recent,
+                                   _ptr(idx, "int32", out, "idx"), _ptr(w_out, "float32", out, "w_out"),
+                                   _ptr(len_out, "int32", src.n_seq, "len_out"), _stream_ptr(stream)))
 
 
 # ------------------------------------------------------ the OP_GEMM operator
