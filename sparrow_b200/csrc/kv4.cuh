@@ -50,6 +50,8 @@ struct Kv4Rows {
   long long tokens, n_pos, m; // m tokens of each sequence
   float eps;
   int n_q, n_kv, rot, interleaved;
+  int steps;                  // times 256 / d rows that a warp takes
+  uint32_t sets;              // warps of a token
   int vec, vec_g, vec_t;      // every row starts on a 16-byte boundary; so do the gains, and the table's rows
 };
 
@@ -99,6 +101,23 @@ __device__ __forceinline__ void store4(float* p, bool vec, const float* x) {
   }
 }
 
+// Two f32 operations in one instruction, each rounded as its own: the rows
+// kernel is bound by how many instructions it issues.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(r)
+      : "l"(*reinterpret_cast<const unsigned long long*>(&a)), "l"(*reinterpret_cast<const unsigned long long*>(&b)));
+  return *reinterpret_cast<const float2*>(&r);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(r)
+      : "l"(*reinterpret_cast<const unsigned long long*>(&a)), "l"(*reinterpret_cast<const unsigned long long*>(&b)));
+  return *reinterpret_cast<const float2*>(&r);
+}
+
 // How a row lies in the D/8 lanes that hold it: lane l has columns 4 l .. 4 l + 3
 // (x[0..3]) and D/2 + 4 l .. (x[4..7]), so 16-byte accesses of neighbouring lanes
 // are contiguous, the pairs (i, i + d/2) of a full rotation meet in one lane, and
@@ -127,10 +146,14 @@ __device__ __forceinline__ void kv4_store_rows(const float (&x)[8], bool on, uin
     const float base = __half2float(__float2half_rn(__fsub_rn(lo, __fmul_rn(16.f, step))));
     const float inv = step > 0.f ? __frcp_rn(step) : 0.f;
     uint32_t bits = 0;
+    const float2 less = make_float2(-base, -base), by = make_float2(inv, inv), magic = make_float2(12582912.f, 12582912.f);
+    const float2 r0 = add2(mul2(add2(make_float2(c[0], c[1]), less), by), magic);
+    const float2 r1 = add2(mul2(add2(make_float2(c[2], c[3]), less), by), magic);
+    const float r[4] = {r0.x, r0.y, r1.x, r1.y};
     #pragma unroll
     for (int i = 0; i < 4; ++i) {
       // rint by adding 1.5 * 2^23 (|x| is far below 2^22): the integer lies in the low bits, and no conversion is needed
-      const int n = __float_as_int(__fadd_rn(__fmul_rn(__fsub_rn(c[i], base), inv), 12582912.f)) - 0x4B400000 - 16;
+      const int n = __float_as_int(r[i]) - 0x4B400000 - 16;
       bits |= static_cast<uint32_t>(min(max(n, 0), 15)) << (4 * i);
     }
     if (on) {
@@ -150,7 +173,11 @@ __device__ __forceinline__ float tree_sum(const float (&x)[8]) {
   const int lane = threadIdx.x;
   float s[4];
   #pragma unroll
-  for (int i = 0; i < 4; ++i) s[i] = __fadd_rn(__fmul_rn(x[i], x[i]), __fmul_rn(x[i + 4], x[i + 4]));
+  for (int i = 0; i < 4; i += 2) {
+    const float2 a = make_float2(x[i], x[i + 1]), b = make_float2(x[i + 4], x[i + 5]);
+    const float2 y = add2(mul2(a, a), mul2(b, b));
+    s[i] = y.x, s[i + 1] = y.y;
+  }
   #pragma unroll
   for (int h = 2, o = L / 2; h > 0; h /= 2, o /= 2) {
     const bool up = lane & o;
@@ -178,45 +205,44 @@ __device__ __forceinline__ void load4(const float* p, bool vec, float* x) {
 }
 
 // Heads 0 .. n_q-1 of a token are queries, then n_kv keys, then (with a cache)
-// n_kv values; a warp takes R * 256 / d rows of one token.
+// n_kv values; a warp takes 256 / d rows of one token at a time, p.steps times.
 //   y = x * (1 / sqrt(sum(x^2) / d + eps)) * gain        (gain given)
 //   (a, b) -> (a cos - b sin, b cos + a sin)             (table given)
 // on the pairs (i, i + rot/2) or (2i, 2i + 1) of the first rot columns. Products
 // and sums are rounded one by one: a key's code must not depend on whether a
 // compiler fused them. Queries and keys may be written in place: a row is read
 // whole before it is written, by the same lanes.
-// Bound by HBM: each value is read once and written once; of the instructions,
-// which are the next bound, the root and the tree count for 256 / d rows. R = 2
-// keeps more loads in flight and shares a token's table rows; R = 1 spreads few
-// rows over more warps. Five blocks an SM: 8191 tokens of 32 + 2 x 8 heads of 128
-// take 80 us, with the registers of two 90, and R = 4 is slower at any count.
-template <int D, bool kCache, int R>
-__global__ void __launch_bounds__(256, 5) kv4_rows_kernel(const Kv4Rows p, const Kv4View c, int* __restrict__ err) {
+// Bound by HBM (each value is read once and written once) and nearly as much by
+// instructions: the root and the tree count for 256 / d rows, the token's table
+// rows and addresses for all steps. While a step is computed the next one's rows
+// are on their way.
+template <int D, bool kCache>
+__global__ void __launch_bounds__(256, 4) kv4_rows_kernel(const Kv4Rows p, const Kv4View c,
+                                                                       int* __restrict__ err) {
   constexpr int L = D / 8, kRows = 32 / L;
   pdl_wait_prior();
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, l = lane & (L - 1);
   const int heads = p.n_q + p.n_kv + (kCache ? p.n_kv : 0);
-  const uint32_t sets = static_cast<uint32_t>(heads + R * kRows - 1) / (R * kRows);
-  const uint32_t at = blockIdx.x * 8 + (threadIdx.x >> 5);
-  const uint32_t tok = at / sets;
+  const uint32_t at = blockIdx.x * 8 + (threadIdx.x >> 5), tok = at / p.sets;
   if (tok >= p.tokens) return;
-  const int h0 = static_cast<int>(at - tok * sets) * (R * kRows) + lane / L;
+  int h = static_cast<int>(at - tok * p.sets) * (p.steps * kRows) + lane / L;
+  const int h1 = min(heads, h - lane / L + p.steps * kRows);
   const bool vec = p.vec;
-  const float *q = p.q + tok * p.ldq, *k = p.k + tok * p.ldk, *v = p.v + tok * p.ldv;
-  float x[R][8];
-  #pragma unroll
-  for (int j = 0; j < R; ++j) {
-    const int h = h0 + j * kRows;
-    const float* src = h < p.n_q ? q + h * D : h < p.n_q + p.n_kv ? k + (h - p.n_q) * D : v + (h - p.n_q - p.n_kv) * D;
-    if (h < heads) {
-      load4(src + 4 * l, vec, x[j]);
-      load4(src + D / 2 + 4 * l, vec, x[j] + 4);
+  const float *q = p.q + tok * p.ldq + 4 * l, *k = p.k + tok * p.ldk + 4 * l - p.n_q * D,
+              *v = p.v + tok * p.ldv + 4 * l - (p.n_q + p.n_kv) * D;  // of head 0: a row is h * D further
+  auto fetch = [&](int at, float (&x)[8]) {
+    if (at < heads) {
+      const float* src = (at < p.n_q ? q : at < p.n_q + p.n_kv ? k : v) + at * D;
+      load4(src, vec, x);
+      load4(src + D / 2, vec, x + 4);
     } else {
       #pragma unroll
-      for (int i = 0; i < 8; ++i) x[j][i] = 0.f;
+      for (int i = 0; i < 8; ++i) x[i] = 0.f;
     }
-  }
+  };
+  float x[8], ahead[8];
+  fetch(h, x);
   // The token's cosines and sines of the lane's columns; columns behind rot: 1 and 0.
   float cs[8], sn[8];
   const int half = p.rot / 2;
@@ -238,99 +264,101 @@ __global__ void __launch_bounds__(256, 5) kv4_rows_kernel(const Kv4Rows p, const
         #pragma unroll
         for (int i = 0; i < 4; ++i) cs[4 * z + i] = 1.f, sn[4 * z + i] = 0.f;
       } else if (p.interleaved) {
-        const int e = c0 / 2;
         #pragma unroll
-        for (int i = 0; i < 4; ++i) cs[4 * z + i] = __ldg(ct + e + i / 2), sn[4 * z + i] = __ldg(st + e + i / 2);
+        for (int i = 0; i < 4; i += 2) {
+          const float co = __ldg(ct + (c0 + i) / 2), si = __ldg(st + (c0 + i) / 2);
+          cs[4 * z + i] = cs[4 * z + i + 1] = co, sn[4 * z + i] = sn[4 * z + i + 1] = si;
+        }
       } else {
         const int e = c0 < half ? c0 : c0 - half;
         load4(ct + e, p.vec_t, cs + 4 * z);
         load4(st + e, p.vec_t, sn + 4 * z);
       }
     }
-  }
-  #pragma unroll
-  for (int j = 0; j < R; ++j) {
-    const int h = h0 + j * kRows;
-    const bool in = h < heads, is_q = h < p.n_q, is_v = h >= p.n_q + p.n_kv;
-    const float* gain = is_q ? p.gq : p.gk;
-    float y[8];
-    const bool turns = __any_sync(0xffffffffu, !is_v);  // a warp of values has nothing to do before they are stored
-    const float sum = turns ? tree_sum<D>(x[j]) : 0.f;
-    if (turns && gain) {
-      float g[8];
-      load4(gain + 4 * l, p.vec_g, g);
-      load4(gain + D / 2 + 4 * l, p.vec_g, g + 4);
-      const float inv = __frcp_rn(__fsqrt_rn(__fadd_rn(__fmul_rn(sum, 1.f / D), p.eps)));
-      #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = __fmul_rn(__fmul_rn(x[j][i], inv), g[i]);
-    } else {
-      #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = x[j][i];
+    // The sine with the sign that it has where it is added: a cos - b sin as a sum, the same bits.
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const bool first = p.interleaved ? (i & 1) == 0 : (i / 4) * (D / 2) + 4 * l < half;
+      if (first) sn[i] = -sn[i];
     }
-    if (turns && p.cos_t) {
-      // a cos - b sin and b cos + a sin, the difference as a sum with the sine's sign turned: the same bits
-      float z[8];
-      if (whole) {
-        #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float a = y[i], b = y[i + 4];
-          y[i] = __fadd_rn(__fmul_rn(a, cs[i]), __fmul_rn(b, -sn[i]));
-          y[i + 4] = __fadd_rn(__fmul_rn(b, cs[i]), __fmul_rn(a, sn[i]));
-        }
-      } else if (p.interleaved) {
-        #pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-          z[i] = __fadd_rn(__fmul_rn(y[i], cs[i]), __fmul_rn(y[i + 1], -sn[i]));
-          z[i + 1] = __fadd_rn(__fmul_rn(y[i + 1], cs[i]), __fmul_rn(y[i], sn[i]));
-        }
-      } else {
-        // the partner of a lane's four columns is another lane's four, of either half of the row
-        #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const int c0 = w * (D / 2) + 4 * l, at = c0 < half ? c0 + half : c0 - half;
-          const int from = lane - l + (at >= 0 ? at / 4 % L : l);
-          const bool upper = at >= D / 2, low = c0 < half;
+  }
+  const uint32_t b = kCache ? tok / static_cast<uint32_t>(p.m) : 0;
+  long long cache_row = -1;  // of kv head 0; negative: not written
+  if constexpr (kCache) {
+    const long long had = __ldg(p.len + b), slot = had + (tok - b * static_cast<uint32_t>(p.m));
+    if (had >= 0 && slot >= c.cap && lane == 0) atomicCAS(err, 0, kDevKv4Slot);
+    if (had >= 0 && slot < c.cap) cache_row = static_cast<long long>(b) * c.n_kv * c.cap + slot;  // had < 0: an idle sequence
+  }
+
+  #pragma unroll 1
+  for (; h - lane / L < h1; h += kRows) {
+    if (h - lane / L + kRows < h1) fetch(h + kRows, ahead);
+    const bool in = h < heads, is_q = h < p.n_q, is_v = h >= p.n_q + p.n_kv;
+    if (__any_sync(0xffffffffu, !is_v)) {  // a warp of values has nothing to do before they are stored
+      const float* gain = is_q ? p.gq : p.gk;
+      const float sum = tree_sum<D>(x);
+      if (gain) {
+        float g[8];
+        load4(gain + 4 * l, p.vec_g, g);
+        load4(gain + D / 2 + 4 * l, p.vec_g, g + 4);
+        const float inv = __frcp_rn(__fsqrt_rn(__fadd_rn(__fmul_rn(sum, 1.f / D), p.eps)));
+        if (!is_v) {
           #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float a = __shfl_sync(0xffffffffu, y[i], from);
-            const float b = p.rot > D / 2 ? __shfl_sync(0xffffffffu, y[4 + i], from) : 0.f;
-            const float other = upper ? b : a, s = sn[4 * w + i];
-            z[4 * w + i] = __fadd_rn(__fmul_rn(y[4 * w + i], cs[4 * w + i]), __fmul_rn(other, low ? -s : s));
+          for (int i = 0; i < 8; i += 2) {
+            const float2 z = mul2(mul2(make_float2(x[i], x[i + 1]), make_float2(inv, inv)), make_float2(g[i], g[i + 1]));
+            x[i] = z.x, x[i + 1] = z.y;
           }
         }
       }
-      #pragma unroll
-      for (int w = 0; w < 2; ++w)
-        if (!whole && w * (D / 2) + 4 * l < p.rot) {
+      if (p.cos_t) {
+        float y[8];  // each column's partner
+        if (whole) {
           #pragma unroll
-          for (int i = 4 * w; i < 4 * w + 4; ++i) y[i] = z[i];
+          for (int i = 0; i < 8; ++i) y[i] = x[i ^ 4];
+        } else if (p.interleaved) {
+          #pragma unroll
+          for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
+        } else {
+          // the partner of a lane's four columns is another lane's four, of either half of the row
+          #pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const int c0 = w * (D / 2) + 4 * l, to = c0 < half ? c0 + half : c0 - half;
+            const int from = lane - l + (to >= 0 ? to / 4 % L : l);
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float lower = __shfl_sync(0xffffffffu, x[i], from);
+              const float upper = p.rot > D / 2 ? __shfl_sync(0xffffffffu, x[4 + i], from) : 0.f;
+              y[4 * w + i] = to >= D / 2 ? upper : lower;
+            }
+          }
         }
-    }
-    if (is_q) {
-      float* to = p.qo + tok * p.ldqo + h * D + 4 * l;
-      store4(to, vec, y);
-      store4(to + D / 2, vec, y + 4);
-    } else if constexpr (!kCache) {
-      if (in) {
-        float* to = p.ko + tok * p.ldko + (h - p.n_q) * D + 4 * l;
-        store4(to, vec, y);
-        store4(to + D / 2, vec, y + 4);
+        #pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          if (!is_v && (whole || w * (D / 2) + 4 * l < p.rot)) {
+            #pragma unroll
+            for (int i = 4 * w; i < 4 * w + 4; i += 2) {
+              const float2 z = add2(mul2(make_float2(x[i], x[i + 1]), make_float2(cs[i], cs[i + 1])),
+                                    mul2(make_float2(y[i], y[i + 1]), make_float2(sn[i], sn[i + 1])));
+              x[i] = z.x, x[i + 1] = z.y;
+            }
+          }
+        }
       }
+    }
+    if (is_q || (!kCache && in)) {
+      float* to = is_q ? p.qo + tok * p.ldqo + h * D + 4 * l : p.ko + tok * p.ldko + (h - p.n_q) * D + 4 * l;
+      store4(to, vec, x);
+      store4(to + D / 2, vec, x + 4);
     }
     if constexpr (kCache) {
       if (__any_sync(0xffffffffu, in && !is_q)) {
-        const uint32_t b = tok / static_cast<uint32_t>(p.m);
-        const long long had = __ldg(p.len + b), slot = had + (tok - b * static_cast<uint32_t>(p.m));
-        if (had >= 0 && slot >= c.cap && lane == 0) atomicCAS(err, 0, kDevKv4Slot);
-        const bool on = in && !is_q && had >= 0 && slot < c.cap;  // had < 0: an idle sequence
+        const bool on = in && !is_q && cache_row >= 0;
         const int kvh = h - p.n_q - (is_v ? p.n_kv : 0);
-        float o[8];
-        #pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = is_v ? x[j][i] : y[i];
-        kv4_store_rows<D>(o, on, is_v ? c.v : c.k, is_v ? c.vs : c.ks,
-                          on ? (static_cast<long long>(b) * c.n_kv + kvh) * c.cap + slot : 0);
+        kv4_store_rows<D>(x, on, is_v ? c.v : c.k, is_v ? c.vs : c.ks, on ? cache_row + kvh * c.cap : 0);
       }
     }
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = ahead[i];
   }
 }
 

@@ -61,17 +61,20 @@ int kv4_check_rope(const char* what, const vmlm_rope* r, size_t d) {
 template <int D, bool kCache>
 int kv4_launch_rows_d(Ctx* ctx, Kv4Rows p, const Kv4View& v, cudaStream_t st) {
   const long long heads = p.n_q + p.n_kv + (kCache ? p.n_kv : 0);
-  // Two sets of 256 / d rows a warp once that still gives every SM 16 warps; below, one.
-  const int r = p.tokens * heads >= static_cast<long long>(ctx->sms) * 16 * 2 * (256 / D) ? 2 : 1;
-  const long long warps = p.tokens * cdiv(heads, r * (256 / D));
+  // Steps of 256 / d rows a warp: as many as leave every SM 64 warps, so that a token's table rows and addresses are
+  // shared by more rows; one where there are few rows.
+  const long long all = cdiv(heads, 256 / D);
+  p.steps = static_cast<int>(std::max<long long>(1, std::min<long long>(all, p.tokens * all / (ctx->sms * 64ll))));
+  p.sets = static_cast<uint32_t>(cdiv(all, p.steps));
+  p.steps = static_cast<int>(cdiv(all, p.sets));  // evenly
+  const long long warps = p.tokens * p.sets;
   if (warps == 0) return VMLM_OK;
   if (warps >= static_cast<long long>(kKv4MaxDim))
     return fail(VMLM_ERR_SHAPE, "tokens x heads is too large (%lld rows)", p.tokens * heads);
   p.vec_g = (!p.gq || aligned16(p.gq)) && (!p.gk || aligned16(p.gk));
   p.vec_t = aligned16(p.cos_t) && aligned16(p.sin_t);  // rot is a multiple of 16, so rows of the table are too
-  const dim3 grid(static_cast<unsigned>(cdiv(warps, 8)));
-  if (r == 2) return launch(kv4_rows_kernel<D, kCache, 2>, grid, dim3(256), 0, st, true, p, v, ctx->err);
-  return launch(kv4_rows_kernel<D, kCache, 1>, grid, dim3(256), 0, st, true, p, v, ctx->err);
+  return launch(kv4_rows_kernel<D, kCache>, dim3(static_cast<unsigned>(cdiv(warps, 8))), dim3(256), 0, st, true, p, v,
+                ctx->err);
 }
 
 template <bool kCache>
