@@ -102,7 +102,9 @@ __device__ __forceinline__ void store4(float* p, bool vec, const float* x) {
 }
 
 // Two f32 operations in one instruction, each rounded as its own: the rows
-// kernel is bound by how many instructions it issues.
+// kernel is bound by how many instructions it issues. A sum of products is added
+// by scalar operations: a paired product and a paired sum would be contracted to
+// a fused multiply-add in spite of their .rn.
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   unsigned long long r;
   asm("mul.rn.f32x2 %0, %1, %2;"
@@ -146,14 +148,13 @@ __device__ __forceinline__ void kv4_store_rows(const float (&x)[8], bool on, uin
     const float base = __half2float(__float2half_rn(__fsub_rn(lo, __fmul_rn(16.f, step))));
     const float inv = step > 0.f ? __frcp_rn(step) : 0.f;
     uint32_t bits = 0;
-    const float2 less = make_float2(-base, -base), by = make_float2(inv, inv), magic = make_float2(12582912.f, 12582912.f);
-    const float2 r0 = add2(mul2(add2(make_float2(c[0], c[1]), less), by), magic);
-    const float2 r1 = add2(mul2(add2(make_float2(c[2], c[3]), less), by), magic);
+    const float2 less = make_float2(-base, -base), by = make_float2(inv, inv);
+    const float2 r0 = mul2(add2(make_float2(c[0], c[1]), less), by), r1 = mul2(add2(make_float2(c[2], c[3]), less), by);
     const float r[4] = {r0.x, r0.y, r1.x, r1.y};
     #pragma unroll
     for (int i = 0; i < 4; ++i) {
       // rint by adding 1.5 * 2^23 (|x| is far below 2^22): the integer lies in the low bits, and no conversion is needed
-      const int n = __float_as_int(r[i]) - 0x4B400000 - 16;
+      const int n = __float_as_int(__fadd_rn(r[i], 12582912.f)) - 0x4B400000 - 16;
       bits |= static_cast<uint32_t>(min(max(n, 0), 15)) << (4 * i);
     }
     if (on) {
@@ -175,8 +176,8 @@ __device__ __forceinline__ float tree_sum(const float (&x)[8]) {
   #pragma unroll
   for (int i = 0; i < 4; i += 2) {
     const float2 a = make_float2(x[i], x[i + 1]), b = make_float2(x[i + 4], x[i + 5]);
-    const float2 y = add2(mul2(a, a), mul2(b, b));
-    s[i] = y.x, s[i + 1] = y.y;
+    const float2 y = mul2(a, a), z = mul2(b, b);
+    s[i] = __fadd_rn(y.x, z.x), s[i + 1] = __fadd_rn(y.y, z.y);
   }
   #pragma unroll
   for (int h = 2, o = L / 2; h > 0; h /= 2, o /= 2) {
@@ -337,9 +338,9 @@ __global__ void __launch_bounds__(256, 4) kv4_rows_kernel(const Kv4Rows p, const
           if (!is_v && (whole || w * (D / 2) + 4 * l < p.rot)) {
             #pragma unroll
             for (int i = 4 * w; i < 4 * w + 4; i += 2) {
-              const float2 z = add2(mul2(make_float2(x[i], x[i + 1]), make_float2(cs[i], cs[i + 1])),
-                                    mul2(make_float2(y[i], y[i + 1]), make_float2(sn[i], sn[i + 1])));
-              x[i] = z.x, x[i + 1] = z.y;
+              const float2 z = mul2(make_float2(x[i], x[i + 1]), make_float2(cs[i], cs[i + 1]));
+              const float2 w2 = mul2(make_float2(y[i], y[i + 1]), make_float2(sn[i], sn[i + 1]));
+              x[i] = __fadd_rn(z.x, w2.x), x[i + 1] = __fadd_rn(z.y, w2.y);
             }
           }
         }

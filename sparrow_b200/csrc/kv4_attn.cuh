@@ -36,13 +36,14 @@ struct Kv4Attn {
   const int32_t* len;
   const float* w_in;
   float* w_out;
-  float* score;       // [n_seq][n_kv][rows][cap]: log2 of the unnormalised weights (w_out only)
+  float* score;       // [n_seq][n_kv][kept_rows][cap]: log2 of the unnormalised weights (w_out only)
   float* lse;         // [n_seq][n_kv][rows]: log2 of their sum
   float* part;        // two partial results a CTA: m, l, O of a chunk of rows
   int2* split;        // [n_seq][n_kv][chunks]: the first CTA of an item and how many have a part of it (one: the output is there)
   float scale2;       // scale * log2(e)
   int m, n_q, group, rows;  // rows = m * group query rows a kv head
   int chunks, chunk_rows;   // in chunks of a multiple of 4
+  int kept_rows;            // chunks * chunk_rows: rows that are not there have a place among the kept scores
   int vec;            // q rows start on 16-byte boundaries
   uint32_t mul4, mul64;  // 4 and 64, as values that the compiler does not know: see kv4_pair
 };
@@ -179,11 +180,11 @@ struct AttnRun {
   bool enter, leave;  // the item has tiles before, behind this run
 };
 
-// The shares are counted in units: an item is its tiles, and before them kAttnRunCost units for what a run costs besides
+// The shares are counted in units: an item is its tiles, and before them `cost` units for what a run costs besides
 // (its queries and its result), so that short items do not gather in one share.
-constexpr int kAttnRunCost = 1;
+constexpr int kAttnRunCost = 2;  // of a warp here: 48 ragged sequences take 55.8 us, with 1 56.6
 
-template <int TS>
+template <int TS, int kCost>
 struct AttnWalk {
   const int32_t* len;
   int n_seq, hc_count, chunks, chunk_rows;
@@ -195,7 +196,7 @@ struct AttnWalk {
     const long long n = __ldg(len + i);
     return static_cast<int>(n > cap ? cap : n < 0 ? 0 : n);
   }
-  __device__ __forceinline__ int units_of(int n) const { return n > 0 ? (n + TS - 1) / TS + kAttnRunCost : 0; }
+  __device__ __forceinline__ int units_of(int n) const { return n > 0 ? (n + TS - 1) / TS + kCost : 0; }
   // Moves (b, base) to the sequence that holds unit `at`; with kItems, to the one that holds the at-th item. Returns how
   // many come before that sequence.
   template <bool kItems>
@@ -235,8 +236,8 @@ struct AttnWalk {
       const int at = pos - base;
       s.hc = hc_count == 1 ? 0 : at / u;
       const int off = at - s.hc * u, take = min(end - pos, u - off);
-      const int t0 = max(0, off - kAttnRunCost), t1 = off + take - kAttnRunCost;  // its tiles
-      s.first = pos - off + kAttnRunCost;
+      const int t0 = max(0, off - kCost), t1 = off + take - kCost;  // its tiles
+      s.first = pos - off + kCost;
       pos += take;
       if (t1 <= t0) continue;
       s.b = b;
@@ -245,7 +246,7 @@ struct AttnWalk {
       s.n = n;
       s.s0 = t0 * TS;
       s.s1 = min(n, t1 * TS);
-      s.units = u - kAttnRunCost;
+      s.units = u - kCost;
       s.enter = t0 > 0;
       s.leave = t1 < s.units;
       return true;
@@ -330,7 +331,7 @@ __global__ void __launch_bounds__(attn_warps(D, NT) * 32, 1) kv4_attn_kernel(con
   pdl_wait_prior();
   pdl_launch_dependents();
   // All tiles, this CTA's share of them, and this warp's share of those.
-  AttnWalk<TS> walk;
+  AttnWalk<TS, kAttnRunCost> walk;
   walk.len = p.len, walk.n_seq = c.n_seq, walk.hc_count = c.n_kv * p.chunks, walk.cap = c.cap;
   walk.chunks = p.chunks, walk.chunk_rows = p.chunk_rows;
   int units = 0, longest = 0, used = 0;
@@ -545,17 +546,16 @@ __global__ void __launch_bounds__(attn_warps(D, NT) * 32, 1) kv4_attn_kernel(con
         }
       }
       if (kW) {
+        float* to = p.score + ((static_cast<long long>(run.b) * c.n_kv + run.head) * p.kept_rows + r0 + tig) * c.cap + at + gid;
         #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          const int r = r0 + nt * 4 + tig;
-          if (r < p.rows) {
-            float* to = p.score + ((static_cast<long long>(run.b) * c.n_kv + run.head) * p.rows + r) * c.cap + at;
-            #pragma unroll
-            for (int u = 0; u < ST; ++u) {
-              if (u * 16 + gid < left) to[u * 16 + gid] = s[u][0][nt] * sc[nt];
-              if (u * 16 + gid + 8 < left) to[u * 16 + gid + 8] = s[u][1][nt] * sc[nt];
-            }
+          const int have = r0 + nt * 4 + tig < p.rows ? left : 0;
+          #pragma unroll
+          for (int u = 0; u < ST; ++u) {
+            if (u * 16 + gid < have) to[u * 16] = s[u][0][nt] * sc[nt];
+            if (u * 16 + gid + 8 < have) to[u * 16 + 8] = s[u][1][nt] * sc[nt];
           }
+          to += 4 * c.cap;
         }
       }
       // slots that a row does not see; then the running maximum, and the weights as split halves
@@ -895,7 +895,7 @@ __global__ void __launch_bounds__(kWeightThreads) kv4_weights_kernel(const Kv4At
     __syncthreads();
     if (tid < rows) s_lse[tid] = p.lse[static_cast<long long>(bh) * p.rows + r0 + tid];
     __syncthreads();
-    const float* s = p.score + (static_cast<long long>(bh) * p.rows + r0) * c.cap + j0 + tid;
+    const float* s = p.score + (static_cast<long long>(bh) * p.kept_rows + r0) * c.cap + j0 + tid;
     #pragma unroll 4
     for (int r = 0; r < rows; ++r) {
       const float lse = s_lse[r];

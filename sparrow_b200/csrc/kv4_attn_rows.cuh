@@ -4,40 +4,48 @@
 // The products and their layouts are those of kv4_attn.cuh. There every warp
 // unpacks its own slots and multiplies them with all rows, whose output it holds;
 // with many rows that does not fit, and a chunk of few rows unpacks the cache
-// again for every chunk. Here a CTA of 8 warps shares a tile of 64 slots:
-//   scores   warp (slots 16 s .., half g of the rows): K unpacked twice
+// again for every chunk. Here a CTA shares a tile of 64 slots:
+//   scores   warp (slots 16 s .., part g of the rows): K unpacked once a part
 //   weights  to shared memory as B fragments, with a maximum shared by the tile
-//   output   warp w: its columns of V (16 or 32; d = 64: and half of the rows),
-//            V unpacked once (d = 64: twice), all 64 slots, all rows
-// Three barriers a tile; two CTAs on an SM fill each other's. What bounds it is
-// mma.sync (one m16n8k16 in two cycles an SM: d rows of 64 slots take d * rows / 8
-// MMAs) and, nearly, the B fragments' reads from shared memory (256 bytes each).
+//   output   each warp its 16 columns of V (d = 64: and half of the rows), V
+//            unpacked once (d = 64: twice), all 64 slots, all rows
+// Three barriers a tile. d = 64 and 128: 8 warps, two parts, and two CTAs on an SM
+// that fill each other's waits; d = 256: 16 warps and four parts, so that 80 rows
+// (16 heads of 5 tokens) are one chunk. What bounds it is mma.sync (one m16n8k16
+// in two cycles an SM: 64 slots take d * rows / 8 of them), the B fragments' reads
+// from shared memory (256 bytes for one or two), and, for d = 64, the instructions
+// of the softmax: about 25 for two scores a lane.
 #pragma once
 #include "kv4_attn.cuh"
 
 namespace vmlm {
 
-constexpr int kRowsWarps = 8, kRowsThreads = kRowsWarps * 32, kRowsSlots = 64;
+constexpr int kRowsSlots = 64;
 
-// Fours of rows that a chunk holds at most: what the registers of two CTAs an SM hold.
-__host__ __device__ constexpr int rows_most(int D) { return D == 64 ? 12 : 8; }
+__host__ __device__ constexpr int rows_warps(int D) { return D == 256 ? 16 : 8; }
+__host__ __device__ constexpr int rows_ctas(int D) { return D == 256 ? 1 : 2; }  // on an SM
+// Fours of rows that a chunk holds at most: what 128 registers a thread hold.
+__host__ __device__ constexpr int rows_most(int D) { return D == 64 ? 12 : D == 128 ? 8 : 20; }
+// What a run costs besides its tiles, in tiles (its queries' fragments and its result).
+__host__ __device__ constexpr int rows_run_cost(int D) { return D == 256 ? 3 : 1; }
 __host__ __device__ constexpr int rows_stage_bytes(int D) { return kRowsSlots * D / 4 * 5; }
 // Shared memory: two tiles, the queries' and the weights' fragments, per row 4 maxima, factor, 4 sums, scale and sight.
 __host__ __device__ constexpr int rows_smem_bytes(int D, int NT) {
   return 2 * rows_stage_bytes(D) + NT * (D / 32) * 512 + 4 * NT * 256 + NT * 4 * 11 * 4;
 }
 
-// NT: fours of rows of a chunk, an even number; rows that are not there are zeros that see nothing.
+// NT: fours of rows of a chunk, a multiple of the parts (2 or 4); rows that are not there are zeros that see nothing.
 template <int D, int NT, bool kW>
-__global__ void __launch_bounds__(kRowsThreads, 2) kv4_attn_rows_kernel(const Kv4Attn p, const Kv4View c,
-                                                                        int* __restrict__ err) {
-  constexpr int NG = NT / 2;  // fours of rows of a half
+__global__ void __launch_bounds__(rows_warps(D) * 32, rows_ctas(D)) kv4_attn_rows_kernel(const Kv4Attn p, const Kv4View c,
+                                                                                          int* __restrict__ err) {
+  constexpr int kRowsWarps = rows_warps(D), kRowsThreads = kRowsWarps * 32;
+  constexpr int PARTS = kRowsWarps / 4, NG = NT / PARTS;  // parts of the rows, fours of rows of each
+  static_assert(NT % PARTS == 0, "");
   constexpr int RC = 4 * NT, kPart = RC * (D + 2);
   constexpr int TS = kRowsSlots;
   constexpr int KW = D / 32, VW = D / 64, kCh = D / 32;
   constexpr int kStage = rows_stage_bytes(D);
   constexpr int kVAt = TS * D / 2, kKsAt = TS * D, kVsAt = TS * D + TS * D / 8;  // in a stage: K, V, K's and V's scales
-  constexpr int TP = D == 256 ? 2 : 1;   // output tiles of a warp
   constexpr int OG = D == 64 ? 2 : 1;    // parts of the rows that the warps of an output tile share
   constexpr int ON = NT / OG;            // fours of rows of such a part
   extern __shared__ __align__(128) unsigned char smem[];
@@ -48,15 +56,15 @@ __global__ void __launch_bounds__(kRowsThreads, 2) kv4_attn_rows_kernel(const Kv
   float* s_sum = s_fac + RC;                                                        // [4][RC]
   float* s_scale = s_sum + 4 * RC;                                                  // [RC]
   int* s_see = reinterpret_cast<int*>(s_scale + RC);                                // [RC]: slots that a row sees
-  __shared__ int s_grown[2][2];  // a half's maxima grew in a tile: by the tile's parity
+  __shared__ int s_grown[2][4];  // a part's maxima grew in a tile: by the tile's parity
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int gid = lane >> 2, tig = lane & 3;
-  const int st = warp & 3, half = warp >> 2;            // scores: slots 16 st .., fours half * NG ..
-  const int ot = D == 64 ? warp & 3 : warp * TP;        // output: first tile
+  const int st = warp & 3, share = warp >> 2;           // scores: slots 16 st .., fours share * NG ..
+  const int ot = D == 64 ? warp & 3 : warp;             // output: its tile
 
   pdl_wait_prior();
   pdl_launch_dependents();
-  AttnWalk<TS> walk;
+  AttnWalk<TS, rows_run_cost(D)> walk;
   walk.len = p.len, walk.n_seq = c.n_seq, walk.hc_count = c.n_kv * p.chunks, walk.cap = c.cap;
   walk.chunks = p.chunks, walk.chunk_rows = p.chunk_rows;
   int units = 0;
@@ -118,11 +126,20 @@ __global__ void __launch_bounds__(kRowsThreads, 2) kv4_attn_rows_kernel(const Kv
 
   AttnRun run, nxt;
   if (!walk.next(run)) return;  // a share may be an item's run cost alone
+  // the first run's queries on their way to L1
+  for (int nt = warp; nt < NT; nt += kRowsWarps) {
+    const int r = nt * 4 + (gid >> 1);
+    if (r < min(p.chunk_rows, p.rows - run.r0)) {
+      const float* at = p.q + attn_row_at<D>(p, run, run.r0 + r, p.ldq) + tig * (D / 4);
+      asm volatile("prefetch.global.L1 [%0];" ::"l"(at));
+      if constexpr (D == 256) asm volatile("prefetch.global.L1 [%0];" ::"l"(at + 32));
+    }
+  }
   long long row0 = first_row(run);
   fetch(row0 + run.s0, run.s1 - run.s0, 0);
   cp_async_commit();
   int stage = 0, parity = 0;
-  if (tid < 4) s_grown[tid >> 1][tid & 1] = 0;
+  if (tid < 8) s_grown[tid >> 2][tid & 3] = 0;
 
   while (true) {
     const bool more = walk.next(nxt);
@@ -144,16 +161,17 @@ __global__ void __launch_bounds__(kRowsThreads, 2) kv4_attn_rows_kernel(const Kv
       }
     }
     // the first four of rows of this warp's scores, and of its output
-    const int n0 = half * NG, o0 = OG == 1 ? 0 : half * NG;
-    float top[NG], sum[NG];
-    #pragma unroll
-    for (int i = 0; i < NG; ++i) top[i] = -1e30f, sum[i] = 0.f;
+    const int n0 = share * NG, o0 = OG == 1 ? 0 : share * NG;
+    // of a row: what a score is multiplied by, kAttnShift - its maximum so far, the score from which that has grown
+    float sc[NG], off[NG], grow[NG], sum[NG];
     const int all_see = rows < RC ? 0 : run.n - (p.m - 1 - attn_token(p, run.r0));
-    float o[TP][2][ON];
+    __syncthreads();
     #pragma unroll
-    for (int i = 0; i < ON; ++i)
-      #pragma unroll
-      for (int z = 0; z < TP; ++z) o[z][0][i] = o[z][1][i] = 0.f;
+    for (int i = 0; i < NG; ++i)
+      sc[i] = s_scale[(n0 + i) * 4 + tig], off[i] = kAttnShift + 1e30f, grow[i] = -3e38f, sum[i] = 0.f;
+    float o[2][ON];
+    #pragma unroll
+    for (int i = 0; i < ON; ++i) o[0][i] = o[1][i] = 0.f;
 
     #pragma unroll 1
     for (int at = run.s0; at < run.s1; at += TS) {
@@ -165,7 +183,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) kv4_attn_rows_kernel(const Kv
       const unsigned char* tile = smem + stage * kStage;
       const int left = run.s1 - at;
 
-      // scores of 16 slots and half of the rows
+      // scores of 16 slots and a part of the rows
       float acc[NG][4];
       {
         const unsigned char *pk = tile + k_at, *pc = tile + ks_at;
@@ -194,58 +212,62 @@ __global__ void __launch_bounds__(kRowsThreads, 2) kv4_attn_rows_kernel(const Kv
           }
         }
       }
-      // hidden slots, and whether a maximum has grown
+      // scores kept for w_out: rows of the chunk that are not there have their own place, so only slots are checked
       const bool some_hidden = left < TS || at + TS > all_see;
+      if (kW) {
+        float* kept = p.score + ((static_cast<long long>(run.b) * c.n_kv + run.head) * p.kept_rows + run.r0 + n0 * 4 + tig) * c.cap +
+                      at + st * 16 + gid;
+        const long long next = 4 * c.cap;
+        const bool on0 = st * 16 + gid < left, on1 = st * 16 + gid + 8 < left;
+        #pragma unroll
+        for (int i = 0; i < NG; ++i) {
+          if ((n0 + i) * 4 < p.chunk_rows) {
+            if (on0) kept[0] = (acc[i][0] + acc[i][1]) * sc[i];
+            if (on1) kept[8] = (acc[i][2] + acc[i][3]) * sc[i];
+          }
+          kept += next;
+        }
+      }
+      // hidden slots, and whether a maximum has grown
       bool grown = false;
-      float* kept = nullptr;
-      if (kW)
-        kept = p.score + ((static_cast<long long>(run.b) * c.n_kv + run.head) * p.rows + run.r0 + n0 * 4 + tig) * c.cap + at +
-               st * 16 + gid;
       #pragma unroll
       for (int i = 0; i < NG; ++i) {
-        const int r = (n0 + i) * 4 + tig;
         float s0 = acc[i][0] + acc[i][1], s1 = acc[i][2] + acc[i][3];
-        const float sc = s_scale[r];
-        if (kW) {
-          if (r < rows && st * 16 + gid < left) kept[0] = s0 * sc;
-          if (r < rows && st * 16 + gid + 8 < left) kept[8] = s1 * sc;
-          kept += 4 * c.cap;
-        }
         if (some_hidden) {
-          const int see = min(left, s_see[r] - at) - st * 16;
+          const int see = min(left, s_see[(n0 + i) * 4 + tig] - at) - st * 16;
           if (gid >= see) s0 = -INFINITY;
           if (gid + 8 >= see) s1 = -INFINITY;
         }
-        acc[i][0] = s0 * sc, acc[i][1] = s1 * sc;
-        grown |= fmaxf(acc[i][0], acc[i][1]) > top[i] + kAttnSlack;
+        acc[i][0] = s0, acc[i][1] = s1;
+        grown |= fmaxf(s0, s1) > grow[i];
       }
-      if (named_bar_or(1 + half, 128, grown)) {  // the four warps that share these rows
+      if (named_bar_or(1 + share, 128, grown)) {  // the four warps that share these rows
         #pragma unroll
         for (int i = 0; i < NG; ++i) {
-          float best = fmaxf(acc[i][0], acc[i][1]);
+          float best = fmaxf(acc[i][0], acc[i][1]) * sc[i];
           best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 4));
           best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 8));
           best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 16));
           if (gid == 0) s_max[st * RC + (n0 + i) * 4 + tig] = best;
         }
-        named_bar_sync(1 + half, 128);
+        named_bar_sync(1 + share, 128);
         #pragma unroll
         for (int i = 0; i < NG; ++i) {
           const int r = (n0 + i) * 4 + tig;
-          const float best = fmaxf(fmaxf(fmaxf(s_max[r], s_max[RC + r]), fmaxf(s_max[2 * RC + r], s_max[3 * RC + r])), top[i]);
-          const float f = ex2(top[i] - best);
-          top[i] = best, sum[i] *= f;
+          const float best = fmaxf(fmaxf(fmaxf(s_max[r], s_max[RC + r]), fmaxf(s_max[2 * RC + r], s_max[3 * RC + r])),
+                                   kAttnShift - off[i]);
+          const float now = kAttnShift - best, f = ex2(now - off[i]);
+          off[i] = now, grow[i] = best > -1e30f ? (best + kAttnSlack) / sc[i] : -3e38f, sum[i] *= f;
           if (st == 0 && gid == 0) s_fac[r] = f;
         }
-        if (st == 0 && lane == 0) s_grown[parity][half] = 1;
+        if (st == 0 && lane == 0) s_grown[parity][share] = 1;
       }
       #pragma unroll
       for (int i = 0; i < NG; ++i) {
-        const float off = kAttnShift - top[i];
         uint32_t pb[2];
         #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float e = ex2(acc[i][h] + off);
+          const float e = ex2(fmaf(acc[i][h], sc[i], off[i]));
           sum[i] += e;
           const float big = __uint_as_float(__float_as_uint(e) & 0xFFFFE000u);
           pb[h] = transpose8x8(h2_bits(__floats2half2_rn(big, e - big)));
@@ -255,20 +277,22 @@ __global__ void __launch_bounds__(kRowsThreads, 2) kv4_attn_rows_kernel(const Kv
       __syncthreads();  // the weights are there
 
       // output: this warp's columns, all slots
-      const bool g0 = s_grown[parity][0], g1 = s_grown[parity][1];
-      if (g0 || g1) {
-        #pragma unroll
-        for (int i = 0; i < ON; ++i) {
-          if (!(o0 + i < NG ? g0 : g1)) continue;
-          const float f = s_fac[(o0 + i) * 4 + tig];
+      #pragma unroll
+      for (int g = 0; g < NT / NG; ++g) {
+        if (OG > 1 && g != share) continue;
+        if (s_grown[parity][g]) {
           #pragma unroll
-          for (int z = 0; z < TP; ++z) o[z][0][i] *= f, o[z][1][i] *= f;
+          for (int i = 0; i < NG; ++i) {
+            const float f = s_fac[(g * NG + i) * 4 + tig];
+            const int at = OG > 1 ? i : g * NG + i;
+            o[0][at] *= f, o[1][at] *= f;
+          }
         }
       }
-      if (tid < 2) s_grown[parity ^ 1][tid] = 0;  // read last before this tile's first barrier
+      if (tid < 4) s_grown[parity ^ 1][tid] = 0;  // read last before this tile's first barrier
       // d = 64: tile n is columns n and 4 + n of the lane's word; else tile 8 w + n is columns n of words 2 w, 2 w + 1.
-      // Even tiles are low nibbles, odd ones high nibbles.
-      uint32_t a[4][TP][4];
+      // Odd tiles are high nibbles: moved to the low ones.
+      uint32_t a[4][4];
       #pragma unroll
       for (int u = 0; u < 4; ++u) {
         #pragma unroll
@@ -283,32 +307,22 @@ __global__ void __launch_bounds__(kRowsThreads, 2) kv4_attn_rows_kernel(const Kv
             const uint32_t wa = *reinterpret_cast<const uint32_t*>(tile + va_at + off);
             const uint32_t wb = *reinterpret_cast<const uint32_t*>(tile + vb_at + off);
             const uint32_t both = __byte_perm(wa, wb, byte | (byte + 4) << 8);
-            if constexpr (TP == 2) {
-              a[u][0][2 * h + z] = kv4_pair<false>(both, p.mul64, step, base);
-              a[u][1][2 * h + z] = kv4_pair<true>(both, p.mul4, step, base);
-            } else {
-              // the nibbles that the warp's tile has, moved to the low ones
-              a[u][0][2 * h + z] = kv4_pair<false>(both >> (ot & 1) * 4, p.mul64, step, base);
-            }
+            a[u][2 * h + z] = kv4_pair<false>(both >> (ot & 1) * 4, p.mul64, step, base);
           }
         }
       }
       #pragma unroll
       for (int i = 0; i < ON; ++i) {
-        float d[TP][4];
+        float d[4];
         #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const uint2 b = ps[(u * NT + o0 + i) * 32 + lane];
-          #pragma unroll
-          for (int z = 0; z < TP; ++z) {
-            if (u == 0)
-              mma_f16_first(d[z], a[u][z][0], a[u][z][1], a[u][z][2], a[u][z][3], b.x, b.y);
-            else
-              mma_f16(d[z], a[u][z][0], a[u][z][1], a[u][z][2], a[u][z][3], b.x, b.y);
-          }
+          if (u == 0)
+            mma_f16_first(d, a[u][0], a[u][1], a[u][2], a[u][3], b.x, b.y);
+          else
+            mma_f16(d, a[u][0], a[u][1], a[u][2], a[u][3], b.x, b.y);
         }
-        #pragma unroll
-        for (int z = 0; z < TP; ++z) o[z][0][i] += d[z][0] + d[z][1], o[z][1][i] += d[z][2] + d[z][3];
+        o[0][i] += d[0] + d[1], o[1][i] += d[2] + d[3];
       }
       stage ^= 1, parity ^= 1;
     }
@@ -322,7 +336,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) kv4_attn_rows_kernel(const Kv
       const int r = (n0 + i) * 4 + tig;
       if (gid == 0) {
         s_sum[st * RC + r] = sum[i];
-        if (st == 0) s_max[r] = top[i];
+        if (st == 0) s_max[r] = kAttnShift - off[i];
       }
     }
     __syncthreads();
@@ -331,26 +345,34 @@ __global__ void __launch_bounds__(kRowsThreads, 2) kv4_attn_rows_kernel(const Kv
     float* part = p.part + (static_cast<long long>(cta) * 2 + kind) * kPart;
     for (int r = tid; r < RC; r += kRowsThreads) {
       const float l = s_sum[r] + s_sum[RC + r] + s_sum[2 * RC + r] + s_sum[3 * RC + r];
-      if (!whole)
-        part[r] = s_max[r], part[RC + r] = l;
-      else if (kW && r < rows)
-        attn_put_lse(p, c, run, run.r0 + r, s_max[r], l);
-    }
-    #pragma unroll
-    for (int i = 0; i < ON; ++i) {
-      const int r = (o0 + i) * 4 + tig;
       if (!whole) {
+        part[r] = s_max[r], part[RC + r] = l;
+      } else {
+        s_fac[r] = l != 0.f ? 1.f / l : 0.f;
+        if (kW && r < rows) attn_put_lse(p, c, run, run.r0 + r, s_max[r], l);
+      }
+    }
+    if (!whole) {
+      #pragma unroll
+      for (int i = 0; i < ON; ++i)
         #pragma unroll
-        for (int z = 0; z < TP; ++z)
-          #pragma unroll
-          for (int h = 0; h < 2; ++h) part[2 * RC + (((ot + z) * 2 + h) * NT + o0 + i) * 32 + lane] = o[z][h][i];
-      } else if (r < rows) {
-        const float l = s_sum[r] + s_sum[RC + r] + s_sum[2 * RC + r] + s_sum[3 * RC + r], inv = l != 0.f ? 1.f / l : 0.f;
+        for (int h = 0; h < 2; ++h) part[2 * RC + ((ot * 2 + h) * NT + o0 + i) * 32 + lane] = o[h][i];
+    } else {
+      // Through shared memory, where the queries were, as rows: a lane's columns lie 16 or 32 apart, and 32 stores to 32
+      // sectors each took 18 us for 80 rows of 256. Columns are moved so that few lanes share a bank.
+      float* out = reinterpret_cast<float*>(qs);  // [RC][D], the queries' size
+      auto place = [&](int r, int col) { return r * D + (col ^ ((col >> 5) | (r & 3) << 3)); };
+      #pragma unroll
+      for (int i = 0; i < ON; ++i)
+        #pragma unroll
+        for (int h = 0; h < 2; ++h)
+          out[place((o0 + i) * 4 + tig, attn_col<D, NT>(((ot * 2 + h) * NT + o0 + i) * 32 + lane))] = o[h][i];
+      __syncthreads();
+      for (int r = warp; r < rows; r += kRowsWarps) {
         float* to = p.out + attn_row_at<D>(p, run, run.r0 + r, p.ldo);
+        const float inv = s_fac[r];
         #pragma unroll
-        for (int z = 0; z < TP; ++z)
-          #pragma unroll
-          for (int h = 0; h < 2; ++h) to[attn_col<D, NT>((((ot + z) * 2 + h) * NT + o0 + i) * 32 + lane)] = o[z][h][i] * inv;
+        for (int x = 0; x < D; x += 32) to[x + lane] = out[place(r, x + lane)] * inv;
       }
     }
     if (tid == 0 && !run.enter) {

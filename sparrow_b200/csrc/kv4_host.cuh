@@ -127,12 +127,14 @@ int kv4_launch_finish(const Kv4Attn& p, const Kv4View& v, bool whole, cudaStream
                 dim3(static_cast<unsigned>(heads * blocks)), dim3(kWeightThreads), 0, st, true, p, v, static_cast<int>(blocks));
 }
 
-// Workspace and limits that both kernels share: nt fours of rows a chunk, `grid` CTAs, tiles of `tile` slots.
+// Workspace and limits that both kernels share: nt fours of rows a chunk at most, `grid` CTAs, tiles of `tile` slots.
 int kv4_prepare_attn(Ctx* ctx, Kv4Attn* p, const Kv4View& v, int nt, int d, int grid, int tile) {
   const size_t heads = static_cast<size_t>(v.n_seq) * v.n_kv;
   p->chunks = static_cast<int>(cdiv(p->rows, 4 * nt));
+  p->chunk_rows = static_cast<int>(cdiv(cdiv(p->rows, p->chunks), 4)) * 4;  // even chunks
+  p->kept_rows = p->chunks * p->chunk_rows;
   p->mul4 = 4, p->mul64 = 64;
-  if (heads * p->chunks * static_cast<size_t>(cdiv(v.cap, tile) + kAttnRunCost) >= kKv4MaxDim)
+  if (heads * p->chunks * static_cast<size_t>(cdiv(v.cap, tile) + 4) >= kKv4MaxDim)  // units, with a run's cost
     return fail(VMLM_ERR_SHAPE, "kv4_attn_dev: n_seq * n_q * m * cap is too large");
   VMLM_TRY(ensure(ctx->kv4_part, static_cast<size_t>(grid) * 2 * 4 * nt * (d + 2) * 4));
   VMLM_TRY(ensure(ctx->kv4_split, heads * p->chunks * sizeof(int2)));
@@ -140,7 +142,7 @@ int kv4_prepare_attn(Ctx* ctx, Kv4Attn* p, const Kv4View& v, int nt, int d, int 
   p->split = static_cast<int2*>(ctx->kv4_split.p);
   if (p->w_out) {
     VMLM_TRY(ensure(ctx->kv4_lse, heads * p->rows * 4));
-    VMLM_TRY(ensure(ctx->kv4_score, heads * p->rows * static_cast<size_t>(v.cap) * 4));
+    VMLM_TRY(ensure(ctx->kv4_score, heads * p->kept_rows * static_cast<size_t>(v.cap) * 4));
     p->lse = static_cast<float*>(ctx->kv4_lse.p);
     p->score = static_cast<float*>(ctx->kv4_score.p);
   }
@@ -157,7 +159,6 @@ int kv4_launch_attn(Ctx* ctx, Kv4Attn p, const Kv4View& v, cudaStream_t st) {
   }
   const int grid = ctx->sms;
   VMLM_TRY(kv4_prepare_attn(ctx, &p, v, NT, D, grid, 4096 / D));
-  p.chunk_rows = 4 * NT;
   VMLM_TRY(launch(kv4_attn_kernel<D, NT, kW>, dim3(grid), dim3(attn_warps(D, NT) * 32), kSmem, st, true, p, v, ctx->err));
   const bool whole = static_cast<long long>(v.n_seq) * v.n_kv * p.chunks <= grid &&
                      v.cap <= static_cast<long long>(attn_warps(D, NT)) * kAttnAlone * (4096 / D);
@@ -172,10 +173,9 @@ int kv4_launch_attn_rows(Ctx* ctx, Kv4Attn p, const Kv4View& v, cudaStream_t st)
     VMLM_CUDA(cudaFuncSetAttribute(kv4_attn_rows_kernel<D, NT, kW>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
     set[ctx->dev] = true;
   }
-  const int grid = 2 * ctx->sms;
+  const int grid = rows_ctas(D) * ctx->sms;
   VMLM_TRY(kv4_prepare_attn(ctx, &p, v, NT, D, grid, kRowsSlots));
-  p.chunk_rows = static_cast<int>(cdiv(cdiv(p.rows, p.chunks), 4)) * 4;  // even chunks
-  VMLM_TRY(launch(kv4_attn_rows_kernel<D, NT, kW>, dim3(grid), dim3(kRowsThreads), kSmem, st, true, p, v, ctx->err));
+  VMLM_TRY(launch(kv4_attn_rows_kernel<D, NT, kW>, dim3(grid), dim3(rows_warps(D) * 32), kSmem, st, true, p, v, ctx->err));
   return kv4_launch_finish<D, NT, kW>(p, v, v.cap <= kRowsSlots, st);
 }
 
@@ -188,16 +188,19 @@ int kv4_pick_attn(Ctx* ctx, const Kv4Attn& p, const Kv4View& v, cudaStream_t st)
     if (p.rows <= 8) return kv4_launch_attn<D, 2, kW>(ctx, p, v, st);
   }
   const long long chunks = cdiv(p.rows, 4 * rows_most(D)), fours = cdiv(cdiv(p.rows, chunks), 4);
-  if constexpr (D == 256) {
-    if (fours <= 2) return kv4_launch_attn_rows<D, 2, kW>(ctx, p, v, st);
-  }
   if (fours <= 4) return kv4_launch_attn_rows<D, 4, kW>(ctx, p, v, st);
-  if (fours <= 6) return kv4_launch_attn_rows<D, 6, kW>(ctx, p, v, st);
-  if constexpr (D != 64) return kv4_launch_attn_rows<D, 8, kW>(ctx, p, v, st);
+  if constexpr (D != 256) {
+    if (fours <= 6) return kv4_launch_attn_rows<D, 6, kW>(ctx, p, v, st);
+  }
+  if (fours <= 8 || D == 128) return kv4_launch_attn_rows<D, 8, kW>(ctx, p, v, st);
   if constexpr (D == 64) {
-    if (fours <= 8) return kv4_launch_attn_rows<D, 8, kW>(ctx, p, v, st);
     if (fours <= 10) return kv4_launch_attn_rows<D, 10, kW>(ctx, p, v, st);
     return kv4_launch_attn_rows<D, 12, kW>(ctx, p, v, st);
+  }
+  if constexpr (D == 256) {
+    if (fours <= 12) return kv4_launch_attn_rows<D, 12, kW>(ctx, p, v, st);
+    if (fours <= 16) return kv4_launch_attn_rows<D, 16, kW>(ctx, p, v, st);
+    return kv4_launch_attn_rows<D, 20, kW>(ctx, p, v, st);
   }
   return VMLM_OK;
 }

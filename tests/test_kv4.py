@@ -293,6 +293,54 @@ def test_norm_and_rotation(kernels, d, n_q, n_kv, rot, inter, norm, tokens, slic
     assert (qo[tokens] == 7).all() and (ko[tokens] == 7).all()
 
 
+def np_norm_rope_f32(x, gain, cos, sin, inter):
+    """The definition step by step in f32: squares added in halves, every operation rounded on its own."""
+    f = np.float32
+    sq = x * x
+    while sq.shape[-1] > 1:
+        h = sq.shape[-1] // 2
+        sq = sq[..., :h] + sq[..., h:]
+    y = x * (f(1) / np.sqrt(sq / f(x.shape[-1]) + f(EPS))) * gain
+    rot = 2 * cos.shape[-1]
+    i, j = (slice(0, rot, 2), slice(1, rot, 2)) if inter else (slice(0, rot // 2), slice(rot // 2, rot))
+    a, b, c, s = y[..., i].copy(), y[..., j].copy(), cos[:, None], sin[:, None]
+    y[..., i], y[..., j] = a * c - b * s, b * c + a * s
+    return y
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,rot,inter,tokens", [(64, 64, False, 300), (64, 32, True, 300), (128, 128, False, 300),
+                                                (128, 64, False, 1000), (128, 96, False, 50), (256, 256, True, 200),
+                                                (256, 48, False, 9), (128, 128, True, 3)])
+def test_norm_rotation_and_append_bit_for_bit(kernels, d, rot, inter, tokens):
+    # a code must not depend on fused or reordered operations: queries, and the codes of keys and values, are numpy's
+    torch = _torch()
+    rng = np.random.default_rng(d + rot)
+    n_q, n_kv, cap = 4, 3, tokens + 5
+    x = (rng.standard_normal((tokens, (n_q + 2 * n_kv) * d)) * np.exp(rng.standard_normal((n_q + 2 * n_kv) * d))).astype(np.float32)
+    gq, gk = (rng.uniform(0.5, 1.5, d).astype(np.float32) for _ in range(2))
+    pos = rng.integers(0, 2000, tokens).astype(np.int32)
+    tc, ts = _tables(2000, rot)
+    _, cache = _random_cache(rng, 1, n_kv, cap, d, [0])
+    xd = _up(x)
+    qo = torch.empty((tokens, n_q * d), device="cuda")
+    st = torch.cuda.current_stream()
+    K.kv4_append_dev(cache, xd[:, n_q * d:(n_q + n_kv) * d], xd[:, (n_q + n_kv) * d:], _up(np.array([2], np.int32)), tokens,
+                     q=xd[:, :n_q * d], qo=qo, n_q=n_q, gq=_up(gq), gk=_up(gk), eps=EPS,
+                     rope=K.Rope(_up(tc), _up(ts), _up(pos), interleaved=inter), stream=st)
+    K.sync(st)
+    q = np_norm_rope_f32(x[:, :n_q * d].reshape(tokens, n_q, d), gq, tc[pos], ts[pos], inter)
+    assert np.array_equal(qo.cpu().numpy().reshape(q.shape), q)
+    k = np_norm_rope_f32(x[:, n_q * d:(n_q + n_kv) * d].reshape(tokens, n_kv, d), gk, tc[pos], ts[pos], inter)
+    v = x[:, (n_q + n_kv) * d:].reshape(tokens, n_kv, d)
+    for ref, codes, sb in ((k, cache.k, cache.ks), (v, cache.v, cache.vs)):
+        c, s, b = np_quantise(ref.transpose(1, 0, 2))
+        got = codes[0, :, 2:2 + tokens].cpu().numpy()
+        assert np.array_equal(got & 15, c[..., 0::2]) and np.array_equal(got >> 4, c[..., 1::2])
+        sbg = sb[0, :, 2:2 + tokens].cpu().numpy()
+        assert np.array_equal(sbg[..., 0], s) and np.array_equal(sbg[..., 1], b)
+
+
 @pytest.mark.gpu
 def test_norm_and_rotation_in_place_and_bad_position(kernels):
     torch = _torch()
