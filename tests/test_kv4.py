@@ -750,3 +750,21 @@ def test_calls_in_a_graph(kernels):
             assert torch.equal(t.view(torch.uint8), r.view(torch.uint8))
     K.sync(st)
     del graph
+
+
+@pytest.mark.gpu
+def test_decode_example(kernels):
+    """The block of examples/kv4_decode.py: prompt, decode and evictions together. Keys and values are off by at most half a
+    code step of their 32 columns (a step is about 4.1 / 15 of their deviation, so 0.08 of it in the mean square), which
+    averages out over the slots of a row: 0.2 leaves room for rows that see few slots."""
+    import importlib.util
+    import os
+
+    from conftest import ROOT
+    spec = importlib.util.spec_from_file_location("kv4_decode", os.path.join(ROOT, "examples", "kv4_decode.py"))
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    got = example.run(prompt=90, tokens=40, n_seq=3, cap=100, keep=60, recent=16, check=True)
+    assert got["evictions"] == 1 and 0 < got["error"] < 0.2
+    got = example.run(prompt=33, tokens=50, n_seq=1, cap=48, keep=40, recent=8, check=True)
+    assert got["evictions"] == 5 and 0 < got["error"] < 0.2
