@@ -38,6 +38,30 @@ pub mod ffi {
         pub k: usize,
     }
 
+    /// A 4-bit key/value cache (device pointers).
+    #[repr(C)]
+    pub struct vmlm_kv4 {
+        pub k: *mut c_void,
+        pub v: *mut c_void,
+        pub ks: *mut c_void,
+        pub vs: *mut c_void,
+        pub n_seq: usize,
+        pub n_kv: usize,
+        pub cap: usize,
+        pub d: usize,
+    }
+
+    /// The rotation of queries and keys: tables and the tokens' positions (device pointers).
+    #[repr(C)]
+    pub struct vmlm_rope {
+        pub cos_t: *const f32,
+        pub sin_t: *const f32,
+        pub pos: *const i32,
+        pub n_pos: usize,
+        pub rot: usize,
+        pub interleaved: c_int,
+    }
+
     /// Opaque device constant pool of a .vmb program.
     #[repr(C)]
     pub struct vmlm_pool {
@@ -75,6 +99,22 @@ pub mod ffi {
         pub fn vmlm_op_gemm(fl: c_uint, d: *const vmlm_slot, a: *const vmlm_slot, b: *const vmlm_slot,
                             scale: *const vmlm_slot) -> c_int;
         pub fn vmlm_gemm_nt_int8_batch_dev(calls: *const vmlm_q8_call, count: usize, stream: *mut c_void) -> c_int;
+        pub fn vmlm_qk_norm_rope_dev(q: *const f32, ldq: usize, k: *const f32, ldk: usize, gq: *const f32,
+                                     gk: *const f32, eps: f32, rope: *const vmlm_rope, qo: *mut f32, ldqo: usize,
+                                     ko: *mut f32, ldko: usize, tokens: usize, n_q: usize, n_kv: usize, d: usize,
+                                     stream: *mut c_void) -> c_int;
+        pub fn vmlm_kv4_append_dev(cache: *const vmlm_kv4, q: *const f32, ldq: usize, qo: *mut f32, ldqo: usize,
+                                   n_q: usize, k: *const f32, ldk: usize, v: *const f32, ldv: usize,
+                                   gq: *const f32, gk: *const f32, eps: f32, rope: *const vmlm_rope,
+                                   len: *const i32, m: usize, stream: *mut c_void) -> c_int;
+        pub fn vmlm_kv4_read_dev(cache: *const vmlm_kv4, start: *const i32, end: *const i32, count: usize,
+                                 k: *mut u16, v: *mut u16, stream: *mut c_void) -> c_int;
+        pub fn vmlm_kv4_attn_dev(cache: *const vmlm_kv4, q: *const f32, ldq: usize, len: *const i32,
+                                 out: *mut f32, ldo: usize, m: usize, n_q: usize, scale: f32, w_in: *const f32,
+                                 w_out: *mut f32, stream: *mut c_void) -> c_int;
+        pub fn vmlm_kv4_evict_dev(src: *const vmlm_kv4, dst: *const vmlm_kv4, w: *const f32, len: *const i32,
+                                  keep: usize, first: usize, recent: usize, idx: *mut i32, w_out: *mut f32,
+                                  len_out: *mut i32, stream: *mut c_void) -> c_int;
         pub fn vmlm_pool_load(vmb: *const c_void, len: usize, weights: *const c_void, weights_len: usize,
                               out: *mut *mut vmlm_pool) -> c_int;
         pub fn vmlm_pool_free(pool: *mut vmlm_pool) -> c_int;
