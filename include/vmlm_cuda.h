@@ -360,7 +360,10 @@ VMLM_API int vmlm_kv4_read_dev(const vmlm_kv4 *cache, const int32_t *start, cons
  * head's query heads for j < len[b] (w_in counts as 0 for the m newest slots
  * and where it is NULL; w_in and w_out may be the same). Other slots of w_out
  * are not written. A len above cap is taken as cap and reported by vmlm_sync.
- * Sums are f32; products with cached values are exact. */
+ * Sums are f32; products with cached values are exact. With w_out the call
+ * holds n_seq * n_kv * cap scores a query row of a kv head in workspace
+ * (f32; rows rounded up to a multiple of 4): a prompt's last tokens are a
+ * cheaper source of weights than all of them. */
 VMLM_API int vmlm_kv4_attn_dev(const vmlm_kv4 *cache, const float *q, size_t ldq, const int32_t *len, float *out,
                                size_t ldo, size_t m, size_t n_q, float scale, const float *w_in, float *w_out,
                                void *stream);

@@ -36,14 +36,14 @@ struct Kv4Attn {
   const int32_t* len;
   const float* w_in;
   float* w_out;
-  float* score;       // [n_seq][n_kv][kept_rows][cap]: log2 of the unnormalised weights (w_out only)
+  float* score;       // [n_seq][n_kv][chunks][kept_rows][cap]: log2 of the unnormalised weights (w_out only)
   float* lse;         // [n_seq][n_kv][rows]: log2 of their sum
   float* part;        // two partial results a CTA: m, l, O of a chunk of rows
   int2* split;        // [n_seq][n_kv][chunks]: the first CTA of an item and how many have a part of it (one: the output is there)
   float scale2;       // scale * log2(e)
   int m, n_q, group, rows;  // rows = m * group query rows a kv head
   int chunks, chunk_rows;   // in chunks of a multiple of 4
-  int kept_rows;            // chunks * chunk_rows: rows that are not there have a place among the kept scores
+  int kept_rows;            // of a chunk among the kept scores: chunk_rows and what a kernel rounds them up to
   int vec;            // q rows start on 16-byte boundaries
   uint32_t mul4, mul64;  // 4 and 64, as values that the compiler does not know: see kv4_pair
 };
@@ -546,7 +546,7 @@ __global__ void __launch_bounds__(attn_warps(D, NT) * 32, 1) kv4_attn_kernel(con
         }
       }
       if (kW) {
-        float* to = p.score + ((static_cast<long long>(run.b) * c.n_kv + run.head) * p.kept_rows + r0 + tig) * c.cap + at + gid;
+        float* to = p.score + ((static_cast<long long>(run.b) * walk.hc_count + run.hc) * RC + tig) * c.cap + at + gid;
         #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const int have = r0 + nt * 4 + tig < p.rows ? left : 0;
@@ -890,12 +890,12 @@ __global__ void __launch_bounds__(kWeightThreads) kv4_weights_kernel(const Kv4At
     w[i] = late < 0 && p.w_in ? p.w_in[at + i * kWeightThreads] : 0.f;
     skip[i] = i * kWeightThreads >= have ? p.rows : late > 0 ? late * p.group : 0;
   }
-  for (int r0 = 0; r0 < p.rows; r0 += kWeightThreads) {
-    const int rows = min(kWeightThreads, p.rows - r0);
+  for (int chunk = 0, r0 = 0; chunk < p.chunks; ++chunk, r0 += p.chunk_rows) {  // at most 80 rows
+    const int rows = min(p.chunk_rows, p.rows - r0);
     __syncthreads();
     if (tid < rows) s_lse[tid] = p.lse[static_cast<long long>(bh) * p.rows + r0 + tid];
     __syncthreads();
-    const float* s = p.score + (static_cast<long long>(bh) * p.kept_rows + r0) * c.cap + j0 + tid;
+    const float* s = p.score + (static_cast<long long>(bh) * p.chunks + chunk) * p.kept_rows * c.cap + j0 + tid;
     #pragma unroll 4
     for (int r = 0; r < rows; ++r) {
       const float lse = s_lse[r];

@@ -40,7 +40,7 @@ __global__ void __launch_bounds__(rows_warps(D) * 32, rows_ctas(D)) kv4_attn_row
                                                                                           int* __restrict__ err) {
   constexpr int kRowsWarps = rows_warps(D), kRowsThreads = kRowsWarps * 32;
   constexpr int PARTS = kRowsWarps / 4, NG = NT / PARTS;  // parts of the rows, fours of rows of each
-  static_assert(NT % PARTS == 0, "");
+  static_assert(NT % PARTS == 0 && kRowsSlots * D / 32 <= kRowsThreads, "");
   constexpr int RC = 4 * NT, kPart = RC * (D + 2);
   constexpr int TS = kRowsSlots;
   constexpr int KW = D / 32, VW = D / 64, kCh = D / 32;
@@ -90,28 +90,33 @@ __global__ void __launch_bounds__(rows_warps(D) * 32, rows_ctas(D)) kv4_attn_row
   walk.pos = cta * each + min(cta, extra), walk.end = walk.pos + each + (cta < extra);
   walk.template seek<false>(walk.pos);
 
-  auto fetch = [&](long long row, int left, int stage) {
-    unsigned char* to = smem + stage * kStage;
-    const uint8_t *k = c.k + row * (D / 2), *v = c.v + row * (D / 2);
-    const uint8_t* ks = reinterpret_cast<const uint8_t*>(c.ks) + row * (D / 8);
-    const uint8_t* vs = reinterpret_cast<const uint8_t*>(c.vs) + row * (D / 8);
-    #pragma unroll
-    for (int x = tid; x < TS * kCh; x += kRowsThreads) {
-      const int slot = x / kCh, at = slot * (D / 2) + attn_swizzle<D>(slot, x % kCh) * 16;
-      const bool on = slot < left;  // rows that do not exist become zeros
-      cp_async16(smem_u32(to + at), on ? k + x * 16 : c.k, on);
-      cp_async16(smem_u32(to + kVAt + at), on ? v + x * 16 : c.v, on);
+  // A thread's part of a tile: one 16-byte chunk of K's codes and of V's (d = 64: half of the threads), and the first
+  // threads one chunk of the steps and bases of each (d = 64: 8 bytes, a row's).
+  constexpr int kSb = D == 64 ? 8 : 16;
+  const bool has_codes = tid < TS * kCh, has_sb = tid < TS * D / 8 / kSb;
+  const int code_slot = tid / kCh, sb_slot = tid * kSb / (D / 8);
+  const uint32_t code_to = smem_u32(smem) + code_slot * (D / 2) + attn_swizzle<D>(code_slot, tid % kCh) * 16;
+  const uint32_t sb_to = smem_u32(smem) + kKsAt + tid * kSb;
+  const uint8_t *k_from = c.k + tid * 16, *v_from = c.v + tid * 16;
+  const uint8_t* ks_from = reinterpret_cast<const uint8_t*>(c.ks) + tid * kSb;
+  const uint8_t* vs_from = reinterpret_cast<const uint8_t*>(c.vs) + tid * kSb;
+  auto fetch = [&](long long row, int left, int stage) {  // rows that do not exist become zeros
+    const uint32_t to = stage * kStage;
+    if (has_codes) {
+      const bool on = code_slot < left;
+      const long long at = on ? row * (D / 2) : -tid * 16ll;
+      cp_async16(code_to + to, k_from + at, on);
+      cp_async16(code_to + to + kVAt, v_from + at, on);
     }
-    constexpr int kSb = D == 64 ? 8 : 16;
-    for (int x = tid; x < TS * D / 8 / kSb; x += kRowsThreads) {
-      const bool on = x * kSb / (D / 8) < left;
-      const void *a = on ? static_cast<const void*>(ks + x * kSb) : c.ks, *b = on ? static_cast<const void*>(vs + x * kSb) : c.vs;
+    if (has_sb) {
+      const bool on = sb_slot < left;
+      const long long at = on ? row * (D / 8) : static_cast<long long>(-tid) * kSb;
       if constexpr (D == 64) {
-        cp_async8(smem_u32(to + kKsAt + x * 8), a, on);
-        cp_async8(smem_u32(to + kVsAt + x * 8), b, on);
+        cp_async8(sb_to + to, ks_from + at, on);
+        cp_async8(sb_to + to + kVsAt - kKsAt, vs_from + at, on);
       } else {
-        cp_async16(smem_u32(to + kKsAt + x * 16), a, on);
-        cp_async16(smem_u32(to + kVsAt + x * 16), b, on);
+        cp_async16(sb_to + to, ks_from + at, on);
+        cp_async16(sb_to + to + kVsAt - kKsAt, vs_from + at, on);
       }
     }
   };
@@ -123,6 +128,7 @@ __global__ void __launch_bounds__(rows_warps(D) * 32, rows_ctas(D)) kv4_attn_row
   const int va_at = kVAt + 2 * tig * (D / 2) + attn_swizzle<D>(2 * tig, v_in / 16) * 16 + v_in % 16;
   const int vb_at = kVAt + (2 * tig + 1) * (D / 2) + attn_swizzle<D>(2 * tig + 1, v_in / 16) * 16 + v_in % 16;
   const int vs_at = kVsAt + 2 * tig * (D / 8) + gid * VW / 4 * 4;
+  const uint32_t nibbles = ot & 1 ? 0x00F000F0u : 0x000F000Fu, to_top = ot & 1 ? p.mul4 : p.mul64;
 
   AttnRun run, nxt;
   if (!walk.next(run)) return;  // a share may be an item's run cost alone
@@ -212,20 +218,23 @@ __global__ void __launch_bounds__(rows_warps(D) * 32, rows_ctas(D)) kv4_attn_row
           }
         }
       }
-      // scores kept for w_out: rows of the chunk that are not there have their own place, so only slots are checked
       const bool some_hidden = left < TS || at + TS > all_see;
-      if (kW) {
-        float* kept = p.score + ((static_cast<long long>(run.b) * c.n_kv + run.head) * p.kept_rows + run.r0 + n0 * 4 + tig) * c.cap +
-                      at + st * 16 + gid;
+      if (kW) {  // rows of the chunk that are not there have a place too: only slots are checked, in a tile that is not whole
+        float* kept = p.score + ((static_cast<long long>(run.b) * walk.hc_count + run.hc) * RC + n0 * 4 + tig) * c.cap + at + st * 16 + gid;
         const long long next = 4 * c.cap;
         const bool on0 = st * 16 + gid < left, on1 = st * 16 + gid + 8 < left;
-        #pragma unroll
-        for (int i = 0; i < NG; ++i) {
-          if ((n0 + i) * 4 < p.chunk_rows) {
+        if (left >= TS) {
+          #pragma unroll
+          for (int i = 0; i < NG; ++i, kept += next) {
+            kept[0] = (acc[i][0] + acc[i][1]) * sc[i];
+            kept[8] = (acc[i][2] + acc[i][3]) * sc[i];
+          }
+        } else {
+          #pragma unroll
+          for (int i = 0; i < NG; ++i, kept += next) {
             if (on0) kept[0] = (acc[i][0] + acc[i][1]) * sc[i];
             if (on1) kept[8] = (acc[i][2] + acc[i][3]) * sc[i];
           }
-          kept += next;
         }
       }
       // hidden slots, and whether a maximum has grown
@@ -291,7 +300,7 @@ __global__ void __launch_bounds__(rows_warps(D) * 32, rows_ctas(D)) kv4_attn_row
       }
       if (tid < 4) s_grown[parity ^ 1][tid] = 0;  // read last before this tile's first barrier
       // d = 64: tile n is columns n and 4 + n of the lane's word; else tile 8 w + n is columns n of words 2 w, 2 w + 1.
-      // Odd tiles are high nibbles: moved to the low ones.
+      // Odd tiles are high nibbles.
       uint32_t a[4][4];
       #pragma unroll
       for (int u = 0; u < 4; ++u) {
@@ -307,7 +316,7 @@ __global__ void __launch_bounds__(rows_warps(D) * 32, rows_ctas(D)) kv4_attn_row
             const uint32_t wa = *reinterpret_cast<const uint32_t*>(tile + va_at + off);
             const uint32_t wb = *reinterpret_cast<const uint32_t*>(tile + vb_at + off);
             const uint32_t both = __byte_perm(wa, wb, byte | (byte + 4) << 8);
-            a[u][2 * h + z] = kv4_pair<false>(both >> (ot & 1) * 4, p.mul64, step, base);
+            a[u][2 * h + z] = h2_bits(__hfma2(bits_h2((both & nibbles) * to_top + 0x4C004C00u), step, base));  // kv4_pair
           }
         }
       }

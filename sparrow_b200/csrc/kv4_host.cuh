@@ -132,7 +132,7 @@ int kv4_prepare_attn(Ctx* ctx, Kv4Attn* p, const Kv4View& v, int nt, int d, int 
   const size_t heads = static_cast<size_t>(v.n_seq) * v.n_kv;
   p->chunks = static_cast<int>(cdiv(p->rows, 4 * nt));
   p->chunk_rows = static_cast<int>(cdiv(cdiv(p->rows, p->chunks), 4)) * 4;  // even chunks
-  p->kept_rows = p->chunks * p->chunk_rows;
+  p->kept_rows = 4 * nt;
   p->mul4 = 4, p->mul64 = 64;
   if (heads * p->chunks * static_cast<size_t>(cdiv(v.cap, tile) + 4) >= kKv4MaxDim)  // units, with a run's cost
     return fail(VMLM_ERR_SHAPE, "kv4_attn_dev: n_seq * n_q * m * cap is too large");
@@ -141,8 +141,11 @@ int kv4_prepare_attn(Ctx* ctx, Kv4Attn* p, const Kv4View& v, int nt, int d, int 
   p->part = static_cast<float*>(ctx->kv4_part.p);
   p->split = static_cast<int2*>(ctx->kv4_split.p);
   if (p->w_out) {
+    if (static_cast<double>(heads) * p->chunks * p->kept_rows * static_cast<double>(v.cap) > 2.5e11)
+      return fail(VMLM_ERR_SHAPE, "kv4_attn_dev: the scores of a call with w_out take %.3g bytes",
+                  4.0 * static_cast<double>(heads) * p->chunks * p->kept_rows * static_cast<double>(v.cap));
     VMLM_TRY(ensure(ctx->kv4_lse, heads * p->rows * 4));
-    VMLM_TRY(ensure(ctx->kv4_score, heads * p->kept_rows * static_cast<size_t>(v.cap) * 4));
+    VMLM_TRY(ensure(ctx->kv4_score, heads * p->chunks * p->kept_rows * static_cast<size_t>(v.cap) * 4));
     p->lse = static_cast<float*>(ctx->kv4_lse.p);
     p->score = static_cast<float*>(ctx->kv4_score.p);
   }
