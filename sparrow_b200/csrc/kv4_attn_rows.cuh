@@ -20,7 +20,10 @@
 
 namespace vmlm {
 
-constexpr int kRowsSlots = 64;
+// Slots of a tile: 64 a step; two steps a tile halve the barriers and double what a warp has to overlap (d = 64, 33 rows:
+// XX us against YY), d = 256 has no registers for that.
+__host__ __device__ constexpr int rows_steps(int D) { return D == 256 ? 1 : 2; }
+__host__ __device__ constexpr int rows_slots(int D) { return 64 * rows_steps(D); }
 
 __host__ __device__ constexpr int rows_warps(int D) { return D == 256 ? 16 : 8; }
 __host__ __device__ constexpr int rows_ctas(int D) { return D == 256 ? 1 : 2; }  // on an SM
@@ -28,10 +31,10 @@ __host__ __device__ constexpr int rows_ctas(int D) { return D == 256 ? 1 : 2; } 
 __host__ __device__ constexpr int rows_most(int D) { return D == 64 ? 12 : D == 128 ? 8 : 20; }
 // What a run costs besides its tiles, in tiles (its queries' fragments and its result).
 __host__ __device__ constexpr int rows_run_cost(int D) { return D == 256 ? 3 : 1; }
-__host__ __device__ constexpr int rows_stage_bytes(int D) { return kRowsSlots * D / 4 * 5; }
+__host__ __device__ constexpr int rows_stage_bytes(int D) { return rows_slots(D) * D / 4 * 5; }
 // Shared memory: two tiles, the queries' and the weights' fragments, per row 4 maxima, factor, 4 sums, scale and sight.
 __host__ __device__ constexpr int rows_smem_bytes(int D, int NT) {
-  return 2 * rows_stage_bytes(D) + NT * (D / 32) * 512 + 4 * NT * 256 + NT * 4 * 11 * 4;
+  return 2 * rows_stage_bytes(D) + NT * (D / 32) * 512 + 4 * rows_steps(D) * NT * 256 + NT * 4 * 11 * 4;
 }
 
 // NT: fours of rows of a chunk, a multiple of the parts (2 or 4); rows that are not there are zeros that see nothing.
@@ -40,9 +43,9 @@ __global__ void __launch_bounds__(rows_warps(D) * 32, rows_ctas(D)) kv4_attn_row
                                                                                           int* __restrict__ err) {
   constexpr int kRowsWarps = rows_warps(D), kRowsThreads = kRowsWarps * 32;
   constexpr int PARTS = kRowsWarps / 4, NG = NT / PARTS;  // parts of the rows, fours of rows of each
-  static_assert(NT % PARTS == 0 && kRowsSlots * D / 32 <= kRowsThreads, "");
+  static_assert(NT % PARTS == 0 && 64 * D / 32 <= kRowsThreads, "");
   constexpr int RC = 4 * NT, kPart = RC * (D + 2);
-  constexpr int TS = kRowsSlots;
+  constexpr int SUB = rows_steps(D), TS = rows_slots(D);
   constexpr int KW = D / 32, VW = D / 64, kCh = D / 32;
   constexpr int kStage = rows_stage_bytes(D);
   constexpr int kVAt = TS * D / 2, kKsAt = TS * D, kVsAt = TS * D + TS * D / 8;  // in a stage: K, V, K's and V's scales
@@ -50,8 +53,8 @@ __global__ void __launch_bounds__(rows_warps(D) * 32, rows_ctas(D)) kv4_attn_row
   constexpr int ON = NT / OG;            // fours of rows of such a part
   extern __shared__ __align__(128) unsigned char smem[];
   uint4* qs = reinterpret_cast<uint4*>(smem + 2 * kStage);                          // [NT][KW][lane]
-  uint2* ps = reinterpret_cast<uint2*>(smem + 2 * kStage + NT * KW * 512);          // [4][NT][lane]
-  float* s_max = reinterpret_cast<float*>(ps + 4 * NT * 32);                        // [4][RC]
+  uint2* ps = reinterpret_cast<uint2*>(smem + 2 * kStage + NT * KW * 512);          // [SUB][4][NT][lane]
+  float* s_max = reinterpret_cast<float*>(ps + SUB * 4 * NT * 32);                        // [4][RC]
   float* s_fac = s_max + 4 * RC;                                                    // [RC]
   float* s_sum = s_fac + RC;                                                        // [4][RC]
   float* s_scale = s_sum + 4 * RC;                                                  // [RC]
@@ -90,10 +93,10 @@ __global__ void __launch_bounds__(rows_warps(D) * 32, rows_ctas(D)) kv4_attn_row
   walk.pos = cta * each + min(cta, extra), walk.end = walk.pos + each + (cta < extra);
   walk.template seek<false>(walk.pos);
 
-  // A thread's part of a tile: one 16-byte chunk of K's codes and of V's (d = 64: half of the threads), and the first
+  // A thread's part of a step: one 16-byte chunk of K's codes and of V's (d = 64: half of the threads), and the first
   // threads one chunk of the steps and bases of each (d = 64: 8 bytes, a row's).
   constexpr int kSb = D == 64 ? 8 : 16;
-  const bool has_codes = tid < TS * kCh, has_sb = tid < TS * D / 8 / kSb;
+  const bool has_codes = tid < 64 * kCh, has_sb = tid < 64 * D / 8 / kSb;
   const int code_slot = tid / kCh, sb_slot = tid * kSb / (D / 8);
   const uint32_t code_to = smem_u32(smem) + code_slot * (D / 2) + attn_swizzle<D>(code_slot, tid % kCh) * 16;
   const uint32_t sb_to = smem_u32(smem) + kKsAt + tid * kSb;
@@ -101,22 +104,25 @@ __global__ void __launch_bounds__(rows_warps(D) * 32, rows_ctas(D)) kv4_attn_row
   const uint8_t* ks_from = reinterpret_cast<const uint8_t*>(c.ks) + tid * kSb;
   const uint8_t* vs_from = reinterpret_cast<const uint8_t*>(c.vs) + tid * kSb;
   auto fetch = [&](long long row, int left, int stage) {  // rows that do not exist become zeros
-    const uint32_t to = stage * kStage;
-    if (has_codes) {
-      const bool on = code_slot < left;
-      const long long at = on ? row * (D / 2) : -tid * 16ll;
-      cp_async16(code_to + to, k_from + at, on);
-      cp_async16(code_to + to + kVAt, v_from + at, on);
-    }
-    if (has_sb) {
-      const bool on = sb_slot < left;
-      const long long at = on ? row * (D / 8) : static_cast<long long>(-tid) * kSb;
-      if constexpr (D == 64) {
-        cp_async8(sb_to + to, ks_from + at, on);
-        cp_async8(sb_to + to + kVsAt - kKsAt, vs_from + at, on);
-      } else {
-        cp_async16(sb_to + to, ks_from + at, on);
-        cp_async16(sb_to + to + kVsAt - kKsAt, vs_from + at, on);
+    #pragma unroll
+    for (int s = 0; s < SUB; ++s) {
+      const uint32_t to = stage * kStage;
+      if (has_codes) {
+        const bool on = code_slot + 64 * s < left;
+        const long long at = on ? (row + 64 * s) * (D / 2) : -tid * 16ll;
+        cp_async16(code_to + to + s * 32 * D, k_from + at, on);
+        cp_async16(code_to + to + s * 32 * D + kVAt, v_from + at, on);
+      }
+      if (has_sb) {
+        const bool on = sb_slot + 64 * s < left;
+        const long long at = on ? (row + 64 * s) * (D / 8) : static_cast<long long>(-tid) * kSb;
+        if constexpr (D == 64) {
+          cp_async8(sb_to + to + s * 8 * D, ks_from + at, on);
+          cp_async8(sb_to + to + s * 8 * D + kVsAt - kKsAt, vs_from + at, on);
+        } else {
+          cp_async16(sb_to + to + s * 8 * D, ks_from + at, on);
+          cp_async16(sb_to + to + s * 8 * D + kVsAt - kKsAt, vs_from + at, on);
+        }
       }
     }
   };
@@ -190,9 +196,10 @@ __global__ void __launch_bounds__(rows_warps(D) * 32, rows_ctas(D)) kv4_attn_row
       const int left = run.s1 - at;
 
       // scores of 16 slots and a part of the rows
-      float acc[NG][4];
-      {
-        const unsigned char *pk = tile + k_at, *pc = tile + ks_at;
+      float acc[SUB][NG][4];
+      #pragma unroll
+      for (int s = 0; s < SUB; ++s) {
+        const unsigned char *pk = tile + k_at + s * 32 * D, *pc = tile + ks_at + s * 8 * D;
         #pragma unroll
         for (int w = 0; w < KW; ++w) {
           int off = w * 4;
@@ -211,10 +218,10 @@ __global__ void __launch_bounds__(rows_warps(D) * 32, rows_ctas(D)) kv4_attn_row
           for (int i = 0; i < NG; ++i) {
               const uint4 q = qs[((n0 + i) * KW + w) * 32 + lane];
             if (w == 0)
-              mma_f16_first(acc[i], a0, b0, a1, b1, q.x, q.y);
+              mma_f16_first(acc[s][i], a0, b0, a1, b1, q.x, q.y);
             else
-              mma_f16(acc[i], a0, b0, a1, b1, q.x, q.y);
-            mma_f16(acc[i], a2, b2, a3, b3, q.z, q.w);
+              mma_f16(acc[s][i], a0, b0, a1, b1, q.x, q.y);
+            mma_f16(acc[s][i], a2, b2, a3, b3, q.z, q.w);
           }
         }
       }
@@ -222,38 +229,50 @@ __global__ void __launch_bounds__(rows_warps(D) * 32, rows_ctas(D)) kv4_attn_row
       if (kW) {  // rows of the chunk that are not there have a place too: only slots are checked, in a tile that is not whole
         float* kept = p.score + ((static_cast<long long>(run.b) * walk.hc_count + run.hc) * RC + n0 * 4 + tig) * c.cap + at + st * 16 + gid;
         const long long next = 4 * c.cap;
-        const bool on0 = st * 16 + gid < left, on1 = st * 16 + gid + 8 < left;
-        if (left >= TS) {
-          #pragma unroll
-          for (int i = 0; i < NG; ++i, kept += next) {
-            kept[0] = (acc[i][0] + acc[i][1]) * sc[i];
-            kept[8] = (acc[i][2] + acc[i][3]) * sc[i];
-          }
-        } else {
-          #pragma unroll
-          for (int i = 0; i < NG; ++i, kept += next) {
-            if (on0) kept[0] = (acc[i][0] + acc[i][1]) * sc[i];
-            if (on1) kept[8] = (acc[i][2] + acc[i][3]) * sc[i];
+        #pragma unroll
+        for (int s = 0; s < SUB; ++s) {
+          float* to = kept + 64 * s;
+          const int have = left - 64 * s - st * 16 - gid;
+          if (left >= TS) {
+            #pragma unroll
+            for (int i = 0; i < NG; ++i, to += next) {
+              to[0] = (acc[s][i][0] + acc[s][i][1]) * sc[i];
+              to[8] = (acc[s][i][2] + acc[s][i][3]) * sc[i];
+            }
+          } else {
+            #pragma unroll
+            for (int i = 0; i < NG; ++i, to += next) {
+              if (have > 0) to[0] = (acc[s][i][0] + acc[s][i][1]) * sc[i];
+              if (have > 8) to[8] = (acc[s][i][2] + acc[s][i][3]) * sc[i];
+            }
           }
         }
       }
       // hidden slots, and whether a maximum has grown
       bool grown = false;
+      float s[SUB][2][NG];
       #pragma unroll
       for (int i = 0; i < NG; ++i) {
-        float s0 = acc[i][0] + acc[i][1], s1 = acc[i][2] + acc[i][3];
-        if (some_hidden) {
-          const int see = min(left, s_see[(n0 + i) * 4 + tig] - at) - st * 16;
-          if (gid >= see) s0 = -INFINITY;
-          if (gid + 8 >= see) s1 = -INFINITY;
+        float best = -INFINITY;
+        #pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+          float s0 = acc[u][i][0] + acc[u][i][1], s1 = acc[u][i][2] + acc[u][i][3];
+          if (some_hidden) {
+            const int see = min(left, s_see[(n0 + i) * 4 + tig] - at) - st * 16 - u * 64;
+            if (gid >= see) s0 = -INFINITY;
+            if (gid + 8 >= see) s1 = -INFINITY;
+          }
+          s[u][0][i] = s0, s[u][1][i] = s1;
+          best = fmaxf(best, fmaxf(s0, s1));
         }
-        acc[i][0] = s0, acc[i][1] = s1;
-        grown |= fmaxf(s0, s1) > grow[i];
+        grown |= best > grow[i];
       }
       if (named_bar_or(1 + share, 128, grown)) {  // the four warps that share these rows
         #pragma unroll
         for (int i = 0; i < NG; ++i) {
-          float best = fmaxf(acc[i][0], acc[i][1]) * sc[i];
+          float best = fmaxf(s[0][0][i], s[0][1][i]);
+          if constexpr (SUB == 2) best = fmaxf(best, fmaxf(s[1][0][i], s[1][1][i]));
+          best *= sc[i];
           best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 4));
           best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 8));
           best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 16));
@@ -273,15 +292,18 @@ __global__ void __launch_bounds__(rows_warps(D) * 32, rows_ctas(D)) kv4_attn_row
       }
       #pragma unroll
       for (int i = 0; i < NG; ++i) {
-        uint32_t pb[2];
         #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float e = ex2(fmaf(acc[i][h], sc[i], off[i]));
-          sum[i] += e;
-          const float big = __uint_as_float(__float_as_uint(e) & 0xFFFFE000u);
-          pb[h] = transpose8x8(h2_bits(__floats2half2_rn(big, e - big)));
+        for (int u = 0; u < SUB; ++u) {
+          uint32_t pb[2];
+          #pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float e = ex2(fmaf(s[u][h][i], sc[i], off[i]));
+            sum[i] += e;
+            const float big = __uint_as_float(__float_as_uint(e) & 0xFFFFE000u);
+            pb[h] = transpose8x8(h2_bits(__floats2half2_rn(big, e - big)));
+          }
+          ps[((u * 4 + st) * NT + n0 + i) * 32 + lane] = make_uint2(pb[0], pb[1]);
         }
-        ps[(st * NT + n0 + i) * 32 + lane] = make_uint2(pb[0], pb[1]);
       }
       __syncthreads();  // the weights are there
 
@@ -301,37 +323,40 @@ __global__ void __launch_bounds__(rows_warps(D) * 32, rows_ctas(D)) kv4_attn_row
       if (tid < 4) s_grown[parity ^ 1][tid] = 0;  // read last before this tile's first barrier
       // d = 64: tile n is columns n and 4 + n of the lane's word; else tile 8 w + n is columns n of words 2 w, 2 w + 1.
       // Odd tiles are high nibbles.
-      uint32_t a[4][4];
       #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const unsigned char* pc = tile + vs_at + (u * 16 + h * 8) * (D / 8);
-          const uint32_t s = *reinterpret_cast<const uint32_t*>(pc), t = *reinterpret_cast<const uint32_t*>(pc + D / 8);
-          const __half2 step = bits_h2(__byte_perm(s, t, 0x5410)), base = bits_h2(__byte_perm(s, t, 0x7632));
-          #pragma unroll
-          for (int z = 0; z < 2; ++z) {
-            const int word = VW == 1 ? 0 : ot / 8 * 2 + z, byte = VW == 1 ? ot / 2 + 2 * z : ot % 8 / 2;
-            const int off = (u * 16 + h * 8) * (D / 2) + word * 4;
-            const uint32_t wa = *reinterpret_cast<const uint32_t*>(tile + va_at + off);
-            const uint32_t wb = *reinterpret_cast<const uint32_t*>(tile + vb_at + off);
-            const uint32_t both = __byte_perm(wa, wb, byte | (byte + 4) << 8);
-            a[u][2 * h + z] = h2_bits(__hfma2(bits_h2((both & nibbles) * to_top + 0x4C004C00u), step, base));  // kv4_pair
-          }
-        }
-      }
-      #pragma unroll
-      for (int i = 0; i < ON; ++i) {
-        float d[4];
+      for (int s = 0; s < SUB; ++s) {
+        uint32_t a[4][4];
         #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          const uint2 b = ps[(u * NT + o0 + i) * 32 + lane];
-          if (u == 0)
-            mma_f16_first(d, a[u][0], a[u][1], a[u][2], a[u][3], b.x, b.y);
-          else
-            mma_f16(d, a[u][0], a[u][1], a[u][2], a[u][3], b.x, b.y);
+          #pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const unsigned char* pc = tile + vs_at + (s * 64 + u * 16 + h * 8) * (D / 8);
+            const uint32_t x = *reinterpret_cast<const uint32_t*>(pc), y = *reinterpret_cast<const uint32_t*>(pc + D / 8);
+            const __half2 step = bits_h2(__byte_perm(x, y, 0x5410)), base = bits_h2(__byte_perm(x, y, 0x7632));
+            #pragma unroll
+            for (int z = 0; z < 2; ++z) {
+              const int word = VW == 1 ? 0 : ot / 8 * 2 + z, byte = VW == 1 ? ot / 2 + 2 * z : ot % 8 / 2;
+              const int off = (s * 64 + u * 16 + h * 8) * (D / 2) + word * 4;
+              const uint32_t wa = *reinterpret_cast<const uint32_t*>(tile + va_at + off);
+              const uint32_t wb = *reinterpret_cast<const uint32_t*>(tile + vb_at + off);
+              const uint32_t both = __byte_perm(wa, wb, byte | (byte + 4) << 8);
+              a[u][2 * h + z] = h2_bits(__hfma2(bits_h2((both & nibbles) * to_top + 0x4C004C00u), step, base));  // kv4_pair
+            }
+          }
         }
-        o[0][i] += d[0] + d[1], o[1][i] += d[2] + d[3];
+        #pragma unroll
+        for (int i = 0; i < ON; ++i) {
+          float d[4];
+          #pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const uint2 b = ps[((s * 4 + u) * NT + o0 + i) * 32 + lane];
+            if (u == 0)
+              mma_f16_first(d, a[u][0], a[u][1], a[u][2], a[u][3], b.x, b.y);
+            else
+              mma_f16(d, a[u][0], a[u][1], a[u][2], a[u][3], b.x, b.y);
+          }
+          o[0][i] += d[0] + d[1], o[1][i] += d[2] + d[3];
+        }
       }
       stage ^= 1, parity ^= 1;
     }

@@ -177,9 +177,9 @@ int kv4_launch_attn_rows(Ctx* ctx, Kv4Attn p, const Kv4View& v, cudaStream_t st)
     set[ctx->dev] = true;
   }
   const int grid = rows_ctas(D) * ctx->sms;
-  VMLM_TRY(kv4_prepare_attn(ctx, &p, v, NT, D, grid, kRowsSlots));
+  VMLM_TRY(kv4_prepare_attn(ctx, &p, v, NT, D, grid, rows_slots(D)));
   VMLM_TRY(launch(kv4_attn_rows_kernel<D, NT, kW>, dim3(grid), dim3(rows_warps(D) * 32), kSmem, st, true, p, v, ctx->err));
-  return kv4_launch_finish<D, NT, kW>(p, v, v.cap <= kRowsSlots, st);
+  return kv4_launch_finish<D, NT, kW>(p, v, v.cap <= rows_slots(D), st);
 }
 
 // Few rows a kv head: a warp unpacks for all of them, 4 or 8 at a time. More: a CTA shares what it unpacks, in as few
