@@ -21,7 +21,7 @@
 namespace vmlm {
 
 // Slots of a tile: 64 a step; two steps a tile halve the barriers and double what a warp has to overlap (d = 64, 33 rows:
-// XX us against YY), d = 256 has no registers for that.
+// weights kept: 67 us a call against 69.5), d = 256 has no registers for that.
 __host__ __device__ constexpr int rows_steps(int D) { return D == 256 ? 1 : 2; }
 __host__ __device__ constexpr int rows_slots(int D) { return 64 * rows_steps(D); }
 
@@ -198,10 +198,11 @@ __global__ void __launch_bounds__(rows_warps(D) * 32, rows_ctas(D)) kv4_attn_row
       // scores of 16 slots and a part of the rows
       float acc[SUB][NG][4];
       #pragma unroll
-      for (int s = 0; s < SUB; ++s) {
-        const unsigned char *pk = tile + k_at + s * 32 * D, *pc = tile + ks_at + s * 8 * D;
+      for (int w = 0; w < KW; ++w) {
+        uint32_t a[SUB][2][4];  // of both steps, so that a query fragment is read once
         #pragma unroll
-        for (int w = 0; w < KW; ++w) {
+        for (int s = 0; s < SUB; ++s) {
+          const unsigned char *pk = tile + k_at + s * 32 * D, *pc = tile + ks_at + s * 8 * D;
           int off = w * 4;
           if constexpr (D == 256) off = attn_swizzle<D>(gid, tig * 2 + w / 4) * 16 + w % 4 * 4;
           const uint32_t wa = *reinterpret_cast<const uint32_t*>(pk + off);
@@ -209,19 +210,23 @@ __global__ void __launch_bounds__(rows_warps(D) * 32, rows_ctas(D)) kv4_attn_row
           const __half2 sa = *reinterpret_cast<const __half2*>(pc + w / 4 * 4);
           const __half2 sb = *reinterpret_cast<const __half2*>(pc + 8 * (D / 8) + w / 4 * 4);
           const __half2 sta = __low2half2(sa), bsa = __high2half2(sa), stb = __low2half2(sb), bsb = __high2half2(sb);
-          const uint32_t a0 = kv4_pair<false>(wa, p.mul64, sta, bsa), b0 = kv4_pair<false>(wb, p.mul64, stb, bsb);
-          const uint32_t a1 = kv4_pair<true>(wa, p.mul4, sta, bsa), b1 = kv4_pair<true>(wb, p.mul4, stb, bsb);
-          const uint32_t xa = wa >> 8, xb = wb >> 8;
-          const uint32_t a2 = kv4_pair<false>(xa, p.mul64, sta, bsa), b2 = kv4_pair<false>(xb, p.mul64, stb, bsb);
-          const uint32_t a3 = kv4_pair<true>(xa, p.mul4, sta, bsa), b3 = kv4_pair<true>(xb, p.mul4, stb, bsb);
           #pragma unroll
-          for (int i = 0; i < NG; ++i) {
-              const uint4 q = qs[((n0 + i) * KW + w) * 32 + lane];
+          for (int y = 0; y < 2; ++y) {
+            const uint32_t xa = wa >> 8 * y, xb = wb >> 8 * y;
+            a[s][y][0] = kv4_pair<false>(xa, p.mul64, sta, bsa), a[s][y][1] = kv4_pair<false>(xb, p.mul64, stb, bsb);
+            a[s][y][2] = kv4_pair<true>(xa, p.mul4, sta, bsa), a[s][y][3] = kv4_pair<true>(xb, p.mul4, stb, bsb);
+          }
+        }
+        #pragma unroll
+        for (int i = 0; i < NG; ++i) {
+          const uint4 q = qs[((n0 + i) * KW + w) * 32 + lane];
+          #pragma unroll
+          for (int s = 0; s < SUB; ++s) {
             if (w == 0)
-              mma_f16_first(acc[s][i], a0, b0, a1, b1, q.x, q.y);
+              mma_f16_first(acc[s][i], a[s][0][0], a[s][0][1], a[s][0][2], a[s][0][3], q.x, q.y);
             else
-              mma_f16(acc[s][i], a0, b0, a1, b1, q.x, q.y);
-            mma_f16(acc[s][i], a2, b2, a3, b3, q.z, q.w);
+              mma_f16(acc[s][i], a[s][0][0], a[s][0][1], a[s][0][2], a[s][0][3], q.x, q.y);
+            mma_f16(acc[s][i], a[s][1][0], a[s][1][1], a[s][1][2], a[s][1][3], q.z, q.w);
           }
         }
       }
