@@ -44,6 +44,7 @@ struct Kv4Attn {
   int m, n_q, group, rows;  // rows = m * group query rows a kv head
   int chunks, chunk_rows;   // in chunks of a multiple of 4
   int kept_rows;            // of a chunk among the kept scores: chunk_rows and what a kernel rounds them up to
+  int alone;          // few and short items get a CTA each: up to how many tiles
   int vec;            // q rows start on 16-byte boundaries
   uint32_t mul4, mul64;  // 4 and 64, as values that the compiler does not know: see kv4_pair
 };
@@ -51,12 +52,18 @@ struct Kv4Attn {
 constexpr int kAttnStageBytes = 5120;    // 4096 values of K and of V with their steps and bases
 constexpr float kAttnShift = 14.f;       // weights are held as 2^14 times their value: their halves keep 2^-39 of the largest
 constexpr float kAttnSlack = 1.f;        // a running maximum may lag by this (log2): 2^15 is still a half
-constexpr int kAttnAlone = 4;            // tiles a warp up to which a CTA takes an item alone
+constexpr int kAttnAlone = 4;            // tiles a warp up to which a CTA may take an item alone
 
 // Warps of the one CTA on an SM. A chunk of rows takes D/8 registers a four rows
-// for its queries and as many for its output; 8 rows, or d = 256, fit 168
-// registers (12 warps), 4 rows fit 128 (16 warps).
-__host__ __device__ constexpr int attn_warps(int D, int NT) { return NT > 1 || D == 256 ? 12 : 16; }
+// for its queries and as many for its output: 4 rows of d = 64 or 128 fit 128
+// registers (16 warps), of d = 256 168 (12 warps; 8: 139 us against 134 for 8 rows
+// over 16 x 8 heads of 8192 slots). More rows run best with 8 warps of 255
+// registers, whose instructions overlap instead of the warps (d = 64, 33 rows, weights
+// kept: 56 us against 60 with 12 warps).
+__host__ __device__ constexpr int attn_warps(int D, int NT) { return NT > 1 ? 8 : D == 256 ? 12 : 16; }
+// Fours of rows that a chunk holds at most.
+__host__ __device__ constexpr int attn_most(int D) { return D == 64 ? 4 : D == 128 ? 2 : 1; }
+constexpr int kAttnManyRows = 25;  // d = 256: rows from which a CTA shares what it unpacks
 // Dynamic shared memory: the warps' rings, a partial result and two (m, l) lists a warp.
 __host__ __device__ constexpr int attn_smem_bytes(int D, int NT) {
   return attn_warps(D, NT) * (2 * kAttnStageBytes + 4 * NT * D * 4 + 2 * 4 * NT * 8);
@@ -169,9 +176,11 @@ __device__ __forceinline__ int attn_swizzle(int slot, int c) {
 // The work is the tiles of TS = 4096 / d slots of every item (sequence, kv head,
 // chunk of rows), in that order, in equal contiguous shares for the CTAs and,
 // within a CTA, for its warps, whatever the lengths are: a warp's share is a few
-// runs, each a part of an item or all of it. Few and short items (one a CTA, at
-// most kAttnAlone tiles a warp) get a CTA each instead: joining the parts of an
-// item across CTAs costs about 4 us, which such a call does not otherwise last.
+// runs, each a part of an item or all of it. Few and short items (at most one a
+// CTA, of at most p.alone tiles) get a CTA each instead, where sharing would save
+// no more than a tile a warp: the join of parts across CTAs costs as much. d = 64,
+// one row: 144 items of 4096 slots take 18.0 us alone and 19.3 shared, 36 items of
+// 4096 slots 16.3 alone and 11.5 shared.
 struct AttnRun {
   int b, hc;          // sequence, kv head * chunks + chunk
   int head, r0;       // kv head, the chunk's first row
@@ -345,7 +354,7 @@ __global__ void __launch_bounds__(attn_warps(D, NT) * 32, 1) kv4_attn_kernel(con
   longest = __reduce_max_sync(0xffffffffu, longest);
   used = __reduce_add_sync(0xffffffffu, used) * walk.hc_count;
   const int cta = blockIdx.x, grid = gridDim.x;
-  const bool alone = used <= grid && longest <= kWarps * kAttnAlone + kAttnRunCost;
+  const bool alone = used <= grid && longest <= p.alone + kAttnRunCost;
   const int ctas = alone ? used : max(1, min(grid, units / kWarps));
   const int each = units / max(1, ctas), extra = units - each * ctas;  // the first `extra` CTAs have one unit more
 
@@ -546,16 +555,24 @@ __global__ void __launch_bounds__(attn_warps(D, NT) * 32, 1) kv4_attn_kernel(con
         }
       }
       if (kW) {
+        // rows of the chunk that are not there have a place too: only slots are checked, in a tile that is not whole
         float* to = p.score + ((static_cast<long long>(run.b) * walk.hc_count + run.hc) * RC + tig) * c.cap + at + gid;
-        #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const int have = r0 + nt * 4 + tig < p.rows ? left : 0;
+        const long long next = 4 * c.cap;
+        if (left >= TS) {
           #pragma unroll
-          for (int u = 0; u < ST; ++u) {
-            if (u * 16 + gid < have) to[u * 16] = s[u][0][nt] * sc[nt];
-            if (u * 16 + gid + 8 < have) to[u * 16 + 8] = s[u][1][nt] * sc[nt];
+          for (int nt = 0; nt < NT; ++nt, to += next) {
+            #pragma unroll
+            for (int u = 0; u < ST; ++u) to[u * 16] = s[u][0][nt] * sc[nt], to[u * 16 + 8] = s[u][1][nt] * sc[nt];
           }
-          to += 4 * c.cap;
+        } else {
+          #pragma unroll
+          for (int nt = 0; nt < NT; ++nt, to += next) {
+            #pragma unroll
+            for (int u = 0; u < ST; ++u) {
+              if (u * 16 + gid < left) to[u * 16] = s[u][0][nt] * sc[nt];
+              if (u * 16 + gid + 8 < left) to[u * 16 + 8] = s[u][1][nt] * sc[nt];
+            }
+          }
         }
       }
       // slots that a row does not see; then the running maximum, and the weights as split halves
@@ -741,8 +758,10 @@ __global__ void __launch_bounds__(attn_warps(D, NT) * 32, 1) kv4_attn_kernel(con
     const AttnRun& it = s_run[first];
     float* part = p.part + (static_cast<long long>(cta) * 2 + kind) * kPart;
     // Lane (row, group): the row's maximum and sum over the parts, which the groups take in turn; then the factors.
-    const int count = __popc(parts), row = lane % RC, group = lane / RC;
-    constexpr int kGroups = 32 / RC;
+    constexpr int kRowLanes = RC > 8 ? 16 : RC, kGroups = 32 / kRowLanes;  // a power of two; lanes of rows that are not there repeat row 0
+    const int count = __popc(parts), lane_row = lane % kRowLanes, group = lane / kRowLanes;
+    const bool has_row = lane_row < RC;
+    const int row = has_row ? lane_row : 0;
     float* mul = s_mul + warp * 32 * RC;  // [part][row]
     int* from = s_at + warp * 32;         // [part]
     if (parts >> lane & 1) from[__popc(parts & ((1u << lane) - 1u))] = lane;
@@ -750,16 +769,16 @@ __global__ void __launch_bounds__(attn_warps(D, NT) * 32, 1) kv4_attn_kernel(con
     float m = -1e30f, l = 0.f;
     for (int i = group; i < count; i += kGroups) m = fmaxf(m, ml[(from[i] * RC + row) * 2]);
     #pragma unroll
-    for (int x = RC; x < 32; x *= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+    for (int x = kRowLanes; x < 32; x *= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
     for (int i = group; i < count; i += kGroups) {
       const float f = ex2(ml[(from[i] * RC + row) * 2] - m);
       l = fmaf(f, ml[(from[i] * RC + row) * 2 + 1], l);
-      mul[i * RC + row] = f;
+      if (has_row) mul[i * RC + row] = f;
     }
     #pragma unroll
-    for (int x = RC; x < 32; x *= 2) l += __shfl_xor_sync(0xffffffffu, l, x);
+    for (int x = kRowLanes; x < 32; x *= 2) l += __shfl_xor_sync(0xffffffffu, l, x);
     const float inv = final_here ? (l != 0.f ? 1.f / l : 0.f) : 1.f;
-    if (slice == 0 && group == 0) {
+    if (slice == 0 && group == 0 && has_row) {
       if (!final_here)
         part[row] = m, part[RC + row] = l;
       else if (kW && it.r0 + row < p.rows)
@@ -882,12 +901,12 @@ __global__ void __launch_bounds__(kWeightThreads) kv4_weights_kernel(const Kv4At
   const long long at = static_cast<long long>(bh) * c.cap + j0 + tid;
   // slots of this thread, and rows that come too early to see each of them
   const int have = static_cast<int>(n - j0 - tid), old = static_cast<int>(n - p.m - j0 - tid);
-  float w[kWeightSlots];
+  float w[kWeightSlots], got[kWeightSlots];  // what was received is added up by itself, then to the old weight: one rounding of that
   int skip[kWeightSlots];
   #pragma unroll
   for (int i = 0; i < kWeightSlots; ++i) {
     const int late = i * kWeightThreads - old;
-    w[i] = late < 0 && p.w_in ? p.w_in[at + i * kWeightThreads] : 0.f;
+    w[i] = late < 0 && p.w_in ? p.w_in[at + i * kWeightThreads] : 0.f, got[i] = 0.f;
     skip[i] = i * kWeightThreads >= have ? p.rows : late > 0 ? late * p.group : 0;
   }
   for (int chunk = 0, r0 = 0; chunk < p.chunks; ++chunk, r0 += p.chunk_rows) {  // at most 80 rows
@@ -901,13 +920,13 @@ __global__ void __launch_bounds__(kWeightThreads) kv4_weights_kernel(const Kv4At
       const float lse = s_lse[r];
       #pragma unroll
       for (int i = 0; i < kWeightSlots; ++i)
-        if (r0 + r >= skip[i]) w[i] += ex2(__ldg(s + i * kWeightThreads) - lse);
+        if (r0 + r >= skip[i]) got[i] += ex2(__ldg(s + i * kWeightThreads) - lse);
       s += c.cap;
     }
   }
   #pragma unroll
   for (int i = 0; i < kWeightSlots; ++i)
-    if (i * kWeightThreads < have) p.w_out[at + i * kWeightThreads] = w[i];
+    if (i * kWeightThreads < have) p.w_out[at + i * kWeightThreads] = w[i] + got[i];
 }
 
 }  // namespace vmlm

@@ -1,60 +1,49 @@
-// kv4_attn_rows.cuh -- attention over a 4-bit cache for many query rows a kv head
-// (several new tokens, or many heads that share keys and values).
+// kv4_attn_rows.cuh -- attention over a 4-bit cache for many query rows a kv head of
+// d = 256 (several new tokens, or many heads that share keys and values).
 //
 // The products and their layouts are those of kv4_attn.cuh. There every warp
-// unpacks its own slots and multiplies them with all rows, whose output it holds;
-// with many rows that does not fit, and a chunk of few rows unpacks the cache
-// again for every chunk. Here a CTA shares a tile of 64 slots:
+// unpacks its own slots and multiplies them with all rows, whose output it holds:
+// 4 rows at d = 256, and the cache is unpacked again for every 4. Here a CTA of 16
+// warps shares a tile of 64 slots, and up to 80 rows (16 heads of 5 tokens) are one
+// chunk:
 //   scores   warp (slots 16 s .., part g of the rows): K unpacked once a part
 //   weights  to shared memory as B fragments, with a maximum shared by the tile
-//   output   each warp its 16 columns of V (d = 64: and half of the rows), V
-//            unpacked once (d = 64: twice), all 64 slots, all rows
-// Three barriers a tile. d = 64 and 128: 8 warps, two parts, and two CTAs on an SM
-// that fill each other's waits; d = 256: 16 warps and four parts, so that 80 rows
-// (16 heads of 5 tokens) are one chunk. What bounds it is mma.sync (one m16n8k16
-// in two cycles an SM: 64 slots take d * rows / 8 of them), the B fragments' reads
-// from shared memory (256 bytes for one or two), and, for d = 64, the instructions
-// of the softmax: about 25 for two scores a lane.
+//   output   each warp its 16 columns of V, V unpacked once, all slots, all rows
+// Three barriers a tile. What bounds it is the latency between them, with four
+// warps a scheduler (38% of issue slots, mma.sync 21% active; 80 rows over 16 ragged
+// caches of up to 3001 slots take 46 us), then mma.sync (one m16n8k16 in two cycles an SM: 64 slots take
+// d * rows / 8 of them) and the B fragments' reads from shared memory (256 bytes
+// for one).
 #pragma once
 #include "kv4_attn.cuh"
 
 namespace vmlm {
 
-// Slots of a tile: 64 a step; two steps a tile halve the barriers and double what a warp has to overlap (d = 64, 33 rows:
-// weights kept: 67 us a call against 69.5), d = 256 has no registers for that.
-__host__ __device__ constexpr int rows_steps(int D) { return D == 256 ? 1 : 2; }
-__host__ __device__ constexpr int rows_slots(int D) { return 64 * rows_steps(D); }
-
-__host__ __device__ constexpr int rows_warps(int D) { return D == 256 ? 16 : 8; }
-__host__ __device__ constexpr int rows_ctas(int D) { return D == 256 ? 1 : 2; }  // on an SM
-// Fours of rows that a chunk holds at most: what 128 registers a thread hold.
-__host__ __device__ constexpr int rows_most(int D) { return D == 64 ? 12 : D == 128 ? 8 : 20; }
-// What a run costs besides its tiles, in tiles (its queries' fragments and its result).
-__host__ __device__ constexpr int rows_run_cost(int D) { return D == 256 ? 3 : 1; }
-__host__ __device__ constexpr int rows_stage_bytes(int D) { return rows_slots(D) * D / 4 * 5; }
+constexpr int kRowsHead = 256;
+constexpr int kRowsSlots = 64;        // of a tile
+constexpr int kRowsWarps = 16;
+constexpr int kRowsMost = 20;         // fours of rows that a chunk holds at most: what 128 registers a thread hold
+constexpr int kRowsRunCost = 3;       // what a run costs besides its tiles, in tiles (its queries' fragments and its result)
+constexpr int kRowsStageBytes = kRowsSlots * kRowsHead / 4 * 5;
 // Shared memory: two tiles, the queries' and the weights' fragments, per row 4 maxima, factor, 4 sums, scale and sight.
-__host__ __device__ constexpr int rows_smem_bytes(int D, int NT) {
-  return 2 * rows_stage_bytes(D) + NT * (D / 32) * 512 + 4 * rows_steps(D) * NT * 256 + NT * 4 * 11 * 4;
+__host__ __device__ constexpr int rows_smem_bytes(int NT) {
+  return 2 * kRowsStageBytes + NT * (kRowsHead / 32) * 512 + 4 * NT * 256 + NT * 4 * 11 * 4;
 }
 
-// NT: fours of rows of a chunk, a multiple of the parts (2 or 4); rows that are not there are zeros that see nothing.
-template <int D, int NT, bool kW>
-__global__ void __launch_bounds__(rows_warps(D) * 32, rows_ctas(D)) kv4_attn_rows_kernel(const Kv4Attn p, const Kv4View c,
-                                                                                          int* __restrict__ err) {
-  constexpr int kRowsWarps = rows_warps(D), kRowsThreads = kRowsWarps * 32;
+// NT: fours of rows of a chunk, a multiple of the 4 parts; rows that are not there are zeros that see nothing.
+template <int NT, bool kW>
+__global__ void __launch_bounds__(kRowsWarps * 32, 1) kv4_attn_rows_kernel(const Kv4Attn p, const Kv4View c, int* __restrict__ err) {
+  constexpr int D = kRowsHead, TS = kRowsSlots, kRowsThreads = kRowsWarps * 32;
   constexpr int PARTS = kRowsWarps / 4, NG = NT / PARTS;  // parts of the rows, fours of rows of each
-  static_assert(NT % PARTS == 0 && 64 * D / 32 <= kRowsThreads, "");
+  static_assert(NT % PARTS == 0 && TS * D / 32 == kRowsThreads, "");
   constexpr int RC = 4 * NT, kPart = RC * (D + 2);
-  constexpr int SUB = rows_steps(D), TS = rows_slots(D);
   constexpr int KW = D / 32, VW = D / 64, kCh = D / 32;
-  constexpr int kStage = rows_stage_bytes(D);
+  constexpr int kStage = kRowsStageBytes;
   constexpr int kVAt = TS * D / 2, kKsAt = TS * D, kVsAt = TS * D + TS * D / 8;  // in a stage: K, V, K's and V's scales
-  constexpr int OG = D == 64 ? 2 : 1;    // parts of the rows that the warps of an output tile share
-  constexpr int ON = NT / OG;            // fours of rows of such a part
   extern __shared__ __align__(128) unsigned char smem[];
   uint4* qs = reinterpret_cast<uint4*>(smem + 2 * kStage);                          // [NT][KW][lane]
-  uint2* ps = reinterpret_cast<uint2*>(smem + 2 * kStage + NT * KW * 512);          // [SUB][4][NT][lane]
-  float* s_max = reinterpret_cast<float*>(ps + SUB * 4 * NT * 32);                        // [4][RC]
+  uint2* ps = reinterpret_cast<uint2*>(smem + 2 * kStage + NT * KW * 512);          // [4][NT][lane]
+  float* s_max = reinterpret_cast<float*>(ps + 4 * NT * 32);                              // [4][RC]
   float* s_fac = s_max + 4 * RC;                                                    // [RC]
   float* s_sum = s_fac + RC;                                                        // [4][RC]
   float* s_scale = s_sum + 4 * RC;                                                  // [RC]
@@ -63,11 +52,11 @@ __global__ void __launch_bounds__(rows_warps(D) * 32, rows_ctas(D)) kv4_attn_row
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int gid = lane >> 2, tig = lane & 3;
   const int st = warp & 3, share = warp >> 2;           // scores: slots 16 st .., fours share * NG ..
-  const int ot = D == 64 ? warp & 3 : warp;             // output: its tile
+  const int ot = warp;                                  // output: its tile
 
   pdl_wait_prior();
   pdl_launch_dependents();
-  AttnWalk<TS, rows_run_cost(D)> walk;
+  AttnWalk<TS, kRowsRunCost> walk;
   walk.len = p.len, walk.n_seq = c.n_seq, walk.hc_count = c.n_kv * p.chunks, walk.cap = c.cap;
   walk.chunks = p.chunks, walk.chunk_rows = p.chunk_rows;
   int units = 0;
@@ -93,43 +82,32 @@ __global__ void __launch_bounds__(rows_warps(D) * 32, rows_ctas(D)) kv4_attn_row
   walk.pos = cta * each + min(cta, extra), walk.end = walk.pos + each + (cta < extra);
   walk.template seek<false>(walk.pos);
 
-  // A thread's part of a step: one 16-byte chunk of K's codes and of V's (d = 64: half of the threads), and the first
-  // threads one chunk of the steps and bases of each (d = 64: 8 bytes, a row's).
-  constexpr int kSb = D == 64 ? 8 : 16;
-  const bool has_codes = tid < 64 * kCh, has_sb = tid < 64 * D / 8 / kSb;
-  const int code_slot = tid / kCh, sb_slot = tid * kSb / (D / 8);
+  // A thread's part of a tile: one 16-byte chunk of K's codes and of V's, and the first threads one chunk of the steps
+  // and bases of each.
+  const bool has_sb = tid < TS * D / 8 / 16;
+  const int code_slot = tid / kCh, sb_slot = tid * 16 / (D / 8);
   const uint32_t code_to = smem_u32(smem) + code_slot * (D / 2) + attn_swizzle<D>(code_slot, tid % kCh) * 16;
-  const uint32_t sb_to = smem_u32(smem) + kKsAt + tid * kSb;
+  const uint32_t sb_to = smem_u32(smem) + kKsAt + tid * 16;
   const uint8_t *k_from = c.k + tid * 16, *v_from = c.v + tid * 16;
-  const uint8_t* ks_from = reinterpret_cast<const uint8_t*>(c.ks) + tid * kSb;
-  const uint8_t* vs_from = reinterpret_cast<const uint8_t*>(c.vs) + tid * kSb;
+  const uint8_t* ks_from = reinterpret_cast<const uint8_t*>(c.ks) + tid * 16;
+  const uint8_t* vs_from = reinterpret_cast<const uint8_t*>(c.vs) + tid * 16;
   auto fetch = [&](long long row, int left, int stage) {  // rows that do not exist become zeros
-    #pragma unroll
-    for (int s = 0; s < SUB; ++s) {
-      const uint32_t to = stage * kStage;
-      if (has_codes) {
-        const bool on = code_slot + 64 * s < left;
-        const long long at = on ? (row + 64 * s) * (D / 2) : -tid * 16ll;
-        cp_async16(code_to + to + s * 32 * D, k_from + at, on);
-        cp_async16(code_to + to + s * 32 * D + kVAt, v_from + at, on);
-      }
-      if (has_sb) {
-        const bool on = sb_slot + 64 * s < left;
-        const long long at = on ? (row + 64 * s) * (D / 8) : static_cast<long long>(-tid) * kSb;
-        if constexpr (D == 64) {
-          cp_async8(sb_to + to + s * 8 * D, ks_from + at, on);
-          cp_async8(sb_to + to + s * 8 * D + kVsAt - kKsAt, vs_from + at, on);
-        } else {
-          cp_async16(sb_to + to + s * 8 * D, ks_from + at, on);
-          cp_async16(sb_to + to + s * 8 * D + kVsAt - kKsAt, vs_from + at, on);
-        }
-      }
+    const uint32_t to = stage * kStage;
+    bool on = code_slot < left;
+    long long at = on ? row * (D / 2) : -tid * 16ll;
+    cp_async16(code_to + to, k_from + at, on);
+    cp_async16(code_to + to + kVAt, v_from + at, on);
+    if (has_sb) {
+      on = sb_slot < left;
+      at = on ? row * (D / 8) : -tid * 16ll;
+      cp_async16(sb_to + to, ks_from + at, on);
+      cp_async16(sb_to + to + kVsAt - kKsAt, vs_from + at, on);
     }
   };
   auto first_row = [&](const AttnRun& s) { return (static_cast<long long>(s.b) * c.n_kv + s.head) * c.cap; };
 
-  const int k_at = (st * 16 + gid) * (D / 2) + (D == 64 ? tig * 8 : D == 128 ? attn_swizzle<D>(gid, tig) * 16 : 0);
-  const int ks_at = kKsAt + (st * 16 + gid) * (D / 8) + (D == 64 ? (tig >> 1) * 4 : tig * (D / 32));
+  const int k_at = (st * 16 + gid) * (D / 2);
+  const int ks_at = kKsAt + (st * 16 + gid) * (D / 8) + tig * (D / 32);
   const int v_in = gid * VW * 4;
   const int va_at = kVAt + 2 * tig * (D / 2) + attn_swizzle<D>(2 * tig, v_in / 16) * 16 + v_in % 16;
   const int vb_at = kVAt + (2 * tig + 1) * (D / 2) + attn_swizzle<D>(2 * tig + 1, v_in / 16) * 16 + v_in % 16;
@@ -144,7 +122,7 @@ __global__ void __launch_bounds__(rows_warps(D) * 32, rows_ctas(D)) kv4_attn_row
     if (r < min(p.chunk_rows, p.rows - run.r0)) {
       const float* at = p.q + attn_row_at<D>(p, run, run.r0 + r, p.ldq) + tig * (D / 4);
       asm volatile("prefetch.global.L1 [%0];" ::"l"(at));
-      if constexpr (D == 256) asm volatile("prefetch.global.L1 [%0];" ::"l"(at + 32));
+      asm volatile("prefetch.global.L1 [%0];" ::"l"(at + 32));
     }
   }
   long long row0 = first_row(run);
@@ -172,8 +150,7 @@ __global__ void __launch_bounds__(rows_warps(D) * 32, rows_ctas(D)) kv4_attn_row
         s_see[r] = r < rows ? run.n - (p.m - 1 - attn_token(p, run.r0 + r)) : 0;
       }
     }
-    // the first four of rows of this warp's scores, and of its output
-    const int n0 = share * NG, o0 = OG == 1 ? 0 : share * NG;
+    const int n0 = share * NG;  // the first four of rows of this warp's scores
     // of a row: what a score is multiplied by, kAttnShift - its maximum so far, the score from which that has grown
     float sc[NG], off[NG], grow[NG], sum[NG];
     const int all_see = rows < RC ? 0 : run.n - (p.m - 1 - attn_token(p, run.r0));
@@ -181,9 +158,9 @@ __global__ void __launch_bounds__(rows_warps(D) * 32, rows_ctas(D)) kv4_attn_row
     #pragma unroll
     for (int i = 0; i < NG; ++i)
       sc[i] = s_scale[(n0 + i) * 4 + tig], off[i] = kAttnShift + 1e30f, grow[i] = -3e38f, sum[i] = 0.f;
-    float o[2][ON];
+    float o[2][NT];
     #pragma unroll
-    for (int i = 0; i < ON; ++i) o[0][i] = o[1][i] = 0.f;
+    for (int i = 0; i < NT; ++i) o[0][i] = o[1][i] = 0.f;
 
     #pragma unroll 1
     for (int at = run.s0; at < run.s1; at += TS) {
@@ -196,88 +173,69 @@ __global__ void __launch_bounds__(rows_warps(D) * 32, rows_ctas(D)) kv4_attn_row
       const int left = run.s1 - at;
 
       // scores of 16 slots and a part of the rows
-      float acc[SUB][NG][4];
+      float acc[NG][4];
       #pragma unroll
       for (int w = 0; w < KW; ++w) {
-        uint32_t a[SUB][2][4];  // of both steps, so that a query fragment is read once
+        const unsigned char *pk = tile + k_at + attn_swizzle<D>(gid, tig * 2 + w / 4) * 16 + w % 4 * 4, *pc = tile + ks_at;
+        const uint32_t wa = *reinterpret_cast<const uint32_t*>(pk), wb = *reinterpret_cast<const uint32_t*>(pk + 8 * (D / 2));
+        const __half2 sa = *reinterpret_cast<const __half2*>(pc + w / 4 * 4);
+        const __half2 sb = *reinterpret_cast<const __half2*>(pc + 8 * (D / 8) + w / 4 * 4);
+        const __half2 sta = __low2half2(sa), bsa = __high2half2(sa), stb = __low2half2(sb), bsb = __high2half2(sb);
+        uint32_t a[2][4];
         #pragma unroll
-        for (int s = 0; s < SUB; ++s) {
-          const unsigned char *pk = tile + k_at + s * 32 * D, *pc = tile + ks_at + s * 8 * D;
-          int off = w * 4;
-          if constexpr (D == 256) off = attn_swizzle<D>(gid, tig * 2 + w / 4) * 16 + w % 4 * 4;
-          const uint32_t wa = *reinterpret_cast<const uint32_t*>(pk + off);
-          const uint32_t wb = *reinterpret_cast<const uint32_t*>(pk + 8 * (D / 2) + off);
-          const __half2 sa = *reinterpret_cast<const __half2*>(pc + w / 4 * 4);
-          const __half2 sb = *reinterpret_cast<const __half2*>(pc + 8 * (D / 8) + w / 4 * 4);
-          const __half2 sta = __low2half2(sa), bsa = __high2half2(sa), stb = __low2half2(sb), bsb = __high2half2(sb);
-          #pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            const uint32_t xa = wa >> 8 * y, xb = wb >> 8 * y;
-            a[s][y][0] = kv4_pair<false>(xa, p.mul64, sta, bsa), a[s][y][1] = kv4_pair<false>(xb, p.mul64, stb, bsb);
-            a[s][y][2] = kv4_pair<true>(xa, p.mul4, sta, bsa), a[s][y][3] = kv4_pair<true>(xb, p.mul4, stb, bsb);
-          }
+        for (int y = 0; y < 2; ++y) {
+          const uint32_t xa = wa >> 8 * y, xb = wb >> 8 * y;
+          a[y][0] = kv4_pair<false>(xa, p.mul64, sta, bsa), a[y][1] = kv4_pair<false>(xb, p.mul64, stb, bsb);
+          a[y][2] = kv4_pair<true>(xa, p.mul4, sta, bsa), a[y][3] = kv4_pair<true>(xb, p.mul4, stb, bsb);
         }
         #pragma unroll
         for (int i = 0; i < NG; ++i) {
           const uint4 q = qs[((n0 + i) * KW + w) * 32 + lane];
-          #pragma unroll
-          for (int s = 0; s < SUB; ++s) {
-            if (w == 0)
-              mma_f16_first(acc[s][i], a[s][0][0], a[s][0][1], a[s][0][2], a[s][0][3], q.x, q.y);
-            else
-              mma_f16(acc[s][i], a[s][0][0], a[s][0][1], a[s][0][2], a[s][0][3], q.x, q.y);
-            mma_f16(acc[s][i], a[s][1][0], a[s][1][1], a[s][1][2], a[s][1][3], q.z, q.w);
-          }
+          if (w == 0)
+            mma_f16_first(acc[i], a[0][0], a[0][1], a[0][2], a[0][3], q.x, q.y);
+          else
+            mma_f16(acc[i], a[0][0], a[0][1], a[0][2], a[0][3], q.x, q.y);
+          mma_f16(acc[i], a[1][0], a[1][1], a[1][2], a[1][3], q.z, q.w);
         }
       }
       const bool some_hidden = left < TS || at + TS > all_see;
       if (kW) {  // rows of the chunk that are not there have a place too: only slots are checked, in a tile that is not whole
-        float* kept = p.score + ((static_cast<long long>(run.b) * walk.hc_count + run.hc) * RC + n0 * 4 + tig) * c.cap + at + st * 16 + gid;
+        float* to = p.score + ((static_cast<long long>(run.b) * walk.hc_count + run.hc) * RC + n0 * 4 + tig) * c.cap + at + st * 16 + gid;
         const long long next = 4 * c.cap;
-        #pragma unroll
-        for (int s = 0; s < SUB; ++s) {
-          float* to = kept + 64 * s;
-          const int have = left - 64 * s - st * 16 - gid;
-          if (left >= TS) {
-            #pragma unroll
-            for (int i = 0; i < NG; ++i, to += next) {
-              to[0] = (acc[s][i][0] + acc[s][i][1]) * sc[i];
-              to[8] = (acc[s][i][2] + acc[s][i][3]) * sc[i];
-            }
-          } else {
-            #pragma unroll
-            for (int i = 0; i < NG; ++i, to += next) {
-              if (have > 0) to[0] = (acc[s][i][0] + acc[s][i][1]) * sc[i];
-              if (have > 8) to[8] = (acc[s][i][2] + acc[s][i][3]) * sc[i];
-            }
+        const int have = left - st * 16 - gid;
+        if (left >= TS) {
+          #pragma unroll
+          for (int i = 0; i < NG; ++i, to += next) {
+            to[0] = (acc[i][0] + acc[i][1]) * sc[i];
+            to[8] = (acc[i][2] + acc[i][3]) * sc[i];
+          }
+        } else {
+          #pragma unroll
+          for (int i = 0; i < NG; ++i, to += next) {
+            if (have > 0) to[0] = (acc[i][0] + acc[i][1]) * sc[i];
+            if (have > 8) to[8] = (acc[i][2] + acc[i][3]) * sc[i];
           }
         }
       }
       // hidden slots, and whether a maximum has grown
       bool grown = false;
-      float s[SUB][2][NG];
+      float s[2][NG];
       #pragma unroll
       for (int i = 0; i < NG; ++i) {
-        float best = -INFINITY;
-        #pragma unroll
-        for (int u = 0; u < SUB; ++u) {
-          float s0 = acc[u][i][0] + acc[u][i][1], s1 = acc[u][i][2] + acc[u][i][3];
-          if (some_hidden) {
-            const int see = min(left, s_see[(n0 + i) * 4 + tig] - at) - st * 16 - u * 64;
-            if (gid >= see) s0 = -INFINITY;
-            if (gid + 8 >= see) s1 = -INFINITY;
-          }
-          s[u][0][i] = s0, s[u][1][i] = s1;
-          best = fmaxf(best, fmaxf(s0, s1));
+        float s0 = acc[i][0] + acc[i][1], s1 = acc[i][2] + acc[i][3];
+        if (some_hidden) {
+          const int see = min(left, s_see[(n0 + i) * 4 + tig] - at) - st * 16;
+          if (gid >= see) s0 = -INFINITY;
+          if (gid + 8 >= see) s1 = -INFINITY;
         }
+        s[0][i] = s0, s[1][i] = s1;
+        const float best = fmaxf(s0, s1);
         grown |= best > grow[i];
       }
       if (named_bar_or(1 + share, 128, grown)) {  // the four warps that share these rows
         #pragma unroll
         for (int i = 0; i < NG; ++i) {
-          float best = fmaxf(s[0][0][i], s[0][1][i]);
-          if constexpr (SUB == 2) best = fmaxf(best, fmaxf(s[1][0][i], s[1][1][i]));
-          best *= sc[i];
+          float best = fmaxf(s[0][i], s[1][i]) * sc[i];
           best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 4));
           best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 8));
           best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 16));
@@ -297,71 +255,61 @@ __global__ void __launch_bounds__(rows_warps(D) * 32, rows_ctas(D)) kv4_attn_row
       }
       #pragma unroll
       for (int i = 0; i < NG; ++i) {
+        uint32_t pb[2];
         #pragma unroll
-        for (int u = 0; u < SUB; ++u) {
-          uint32_t pb[2];
-          #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float e = ex2(fmaf(s[u][h][i], sc[i], off[i]));
-            sum[i] += e;
-            const float big = __uint_as_float(__float_as_uint(e) & 0xFFFFE000u);
-            pb[h] = transpose8x8(h2_bits(__floats2half2_rn(big, e - big)));
-          }
-          ps[((u * 4 + st) * NT + n0 + i) * 32 + lane] = make_uint2(pb[0], pb[1]);
+        for (int h = 0; h < 2; ++h) {
+          const float e = ex2(fmaf(s[h][i], sc[i], off[i]));
+          sum[i] += e;
+          const float big = __uint_as_float(__float_as_uint(e) & 0xFFFFE000u);
+          pb[h] = transpose8x8(h2_bits(__floats2half2_rn(big, e - big)));
         }
+        ps[(st * NT + n0 + i) * 32 + lane] = make_uint2(pb[0], pb[1]);
       }
       __syncthreads();  // the weights are there
 
       // output: this warp's columns, all slots
       #pragma unroll
       for (int g = 0; g < NT / NG; ++g) {
-        if (OG > 1 && g != share) continue;
         if (s_grown[parity][g]) {
           #pragma unroll
           for (int i = 0; i < NG; ++i) {
             const float f = s_fac[(g * NG + i) * 4 + tig];
-            const int at = OG > 1 ? i : g * NG + i;
-            o[0][at] *= f, o[1][at] *= f;
+            o[0][g * NG + i] *= f, o[1][g * NG + i] *= f;
           }
         }
       }
       if (tid < 4) s_grown[parity ^ 1][tid] = 0;  // read last before this tile's first barrier
-      // d = 64: tile n is columns n and 4 + n of the lane's word; else tile 8 w + n is columns n of words 2 w, 2 w + 1.
-      // Odd tiles are high nibbles.
+      // Tile 8 w + n is columns n of words 2 w and 2 w + 1 of the lane's; odd tiles are high nibbles.
+      uint32_t a[4][4];
       #pragma unroll
-      for (int s = 0; s < SUB; ++s) {
-        uint32_t a[4][4];
+      for (int u = 0; u < 4; ++u) {
+        #pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const unsigned char* pc = tile + vs_at + (u * 16 + h * 8) * (D / 8);
+          const uint32_t x = *reinterpret_cast<const uint32_t*>(pc), y = *reinterpret_cast<const uint32_t*>(pc + D / 8);
+          const __half2 step = bits_h2(__byte_perm(x, y, 0x5410)), base = bits_h2(__byte_perm(x, y, 0x7632));
+          #pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            const int byte = ot % 8 / 2, off = (u * 16 + h * 8) * (D / 2) + (ot / 8 * 2 + z) * 4;
+            const uint32_t wa = *reinterpret_cast<const uint32_t*>(tile + va_at + off);
+            const uint32_t wb = *reinterpret_cast<const uint32_t*>(tile + vb_at + off);
+            const uint32_t both = __byte_perm(wa, wb, byte | (byte + 4) << 8);
+            a[u][2 * h + z] = h2_bits(__hfma2(bits_h2((both & nibbles) * to_top + 0x4C004C00u), step, base));  // kv4_pair
+          }
+        }
+      }
+      #pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        float d[4];
         #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const unsigned char* pc = tile + vs_at + (s * 64 + u * 16 + h * 8) * (D / 8);
-            const uint32_t x = *reinterpret_cast<const uint32_t*>(pc), y = *reinterpret_cast<const uint32_t*>(pc + D / 8);
-            const __half2 step = bits_h2(__byte_perm(x, y, 0x5410)), base = bits_h2(__byte_perm(x, y, 0x7632));
-            #pragma unroll
-            for (int z = 0; z < 2; ++z) {
-              const int word = VW == 1 ? 0 : ot / 8 * 2 + z, byte = VW == 1 ? ot / 2 + 2 * z : ot % 8 / 2;
-              const int off = (s * 64 + u * 16 + h * 8) * (D / 2) + word * 4;
-              const uint32_t wa = *reinterpret_cast<const uint32_t*>(tile + va_at + off);
-              const uint32_t wb = *reinterpret_cast<const uint32_t*>(tile + vb_at + off);
-              const uint32_t both = __byte_perm(wa, wb, byte | (byte + 4) << 8);
-              a[u][2 * h + z] = h2_bits(__hfma2(bits_h2((both & nibbles) * to_top + 0x4C004C00u), step, base));  // kv4_pair
-            }
-          }
+          const uint2 b = ps[(u * NT + i) * 32 + lane];
+          if (u == 0)
+            mma_f16_first(d, a[u][0], a[u][1], a[u][2], a[u][3], b.x, b.y);
+          else
+            mma_f16(d, a[u][0], a[u][1], a[u][2], a[u][3], b.x, b.y);
         }
-        #pragma unroll
-        for (int i = 0; i < ON; ++i) {
-          float d[4];
-          #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const uint2 b = ps[((s * 4 + u) * NT + o0 + i) * 32 + lane];
-            if (u == 0)
-              mma_f16_first(d, a[u][0], a[u][1], a[u][2], a[u][3], b.x, b.y);
-            else
-              mma_f16(d, a[u][0], a[u][1], a[u][2], a[u][3], b.x, b.y);
-          }
-          o[0][i] += d[0] + d[1], o[1][i] += d[2] + d[3];
-        }
+        o[0][i] += d[0] + d[1], o[1][i] += d[2] + d[3];
       }
       stage ^= 1, parity ^= 1;
     }
@@ -393,19 +341,19 @@ __global__ void __launch_bounds__(rows_warps(D) * 32, rows_ctas(D)) kv4_attn_row
     }
     if (!whole) {
       #pragma unroll
-      for (int i = 0; i < ON; ++i)
+      for (int i = 0; i < NT; ++i)
         #pragma unroll
-        for (int h = 0; h < 2; ++h) part[2 * RC + ((ot * 2 + h) * NT + o0 + i) * 32 + lane] = o[h][i];
+        for (int h = 0; h < 2; ++h) part[2 * RC + ((ot * 2 + h) * NT + i) * 32 + lane] = o[h][i];
     } else {
       // Through shared memory, where the queries were, as rows: a lane's columns lie 16 or 32 apart, and 32 stores to 32
       // sectors each took 18 us for 80 rows of 256. Columns are moved so that few lanes share a bank.
       float* out = reinterpret_cast<float*>(qs);  // [RC][D], the queries' size
       auto place = [&](int r, int col) { return r * D + (col ^ ((col >> 5) | (r & 3) << 3)); };
       #pragma unroll
-      for (int i = 0; i < ON; ++i)
+      for (int i = 0; i < NT; ++i)
         #pragma unroll
         for (int h = 0; h < 2; ++h)
-          out[place((o0 + i) * 4 + tig, attn_col<D, NT>(((ot * 2 + h) * NT + o0 + i) * 32 + lane))] = o[h][i];
+          out[place(i * 4 + tig, attn_col<D, NT>(((ot * 2 + h) * NT + i) * 32 + lane))] = o[h][i];
       __syncthreads();
       for (int r = warp; r < rows; r += kRowsWarps) {
         float* to = p.out + attn_row_at<D>(p, run, run.r0 + r, p.ldo);

@@ -162,52 +162,65 @@ int kv4_launch_attn(Ctx* ctx, Kv4Attn p, const Kv4View& v, cudaStream_t st) {
   }
   const int grid = ctx->sms;
   VMLM_TRY(kv4_prepare_attn(ctx, &p, v, NT, D, grid, 4096 / D));
-  VMLM_TRY(launch(kv4_attn_kernel<D, NT, kW>, dim3(grid), dim3(attn_warps(D, NT) * 32), kSmem, st, true, p, v, ctx->err));
-  const bool whole = static_cast<long long>(v.n_seq) * v.n_kv * p.chunks <= grid &&
-                     v.cap <= static_cast<long long>(attn_warps(D, NT)) * kAttnAlone * (4096 / D);
+  // An item of t tiles takes a CTA t / kWarps alone and items / grid times that shared: alone while that saves no tile.
+  const long long items = static_cast<long long>(v.n_seq) * v.n_kv * p.chunks, spare = grid - items;
+  constexpr int kWarps = attn_warps(D, NT);
+  p.alone = static_cast<int>(spare < 0 ? 0 : spare * kAttnAlone <= grid ? kWarps * kAttnAlone : kWarps * grid / spare);
+  VMLM_TRY(launch(kv4_attn_kernel<D, NT, kW>, dim3(grid), dim3(kWarps * 32), kSmem, st, true, p, v, ctx->err));
+  const bool whole = spare >= 0 && v.cap <= static_cast<long long>(p.alone) * (4096 / D);
   return kv4_launch_finish<D, NT, kW>(p, v, whole, st);
 }
 
-template <int D, int NT, bool kW>
+template <int NT, bool kW>
 int kv4_launch_attn_rows(Ctx* ctx, Kv4Attn p, const Kv4View& v, cudaStream_t st) {
-  constexpr int kSmem = rows_smem_bytes(D, NT);
+  constexpr int D = kRowsHead, kSmem = rows_smem_bytes(NT);
   static bool set[64] = {};
   if (ctx->dev < 64 && !set[ctx->dev]) {
-    VMLM_CUDA(cudaFuncSetAttribute(kv4_attn_rows_kernel<D, NT, kW>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    VMLM_CUDA(cudaFuncSetAttribute(kv4_attn_rows_kernel<NT, kW>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
     set[ctx->dev] = true;
   }
-  const int grid = rows_ctas(D) * ctx->sms;
-  VMLM_TRY(kv4_prepare_attn(ctx, &p, v, NT, D, grid, rows_slots(D)));
-  VMLM_TRY(launch(kv4_attn_rows_kernel<D, NT, kW>, dim3(grid), dim3(rows_warps(D) * 32), kSmem, st, true, p, v, ctx->err));
-  return kv4_launch_finish<D, NT, kW>(p, v, v.cap <= rows_slots(D), st);
+  const int grid = ctx->sms;
+  VMLM_TRY(kv4_prepare_attn(ctx, &p, v, NT, D, grid, kRowsSlots));
+  VMLM_TRY(launch(kv4_attn_rows_kernel<NT, kW>, dim3(grid), dim3(kRowsWarps * 32), kSmem, st, true, p, v, ctx->err));
+  return kv4_launch_finish<D, NT, kW>(p, v, v.cap <= kRowsSlots, st);
 }
 
-// Few rows a kv head: a warp unpacks for all of them, 4 or 8 at a time. More: a CTA shares what it unpacks, in as few
-// chunks as hold the rows, and with the smallest count of fours that holds a chunk.
+// A warp takes 4 to 4 * attn_most rows at a time: as few as leave no warp more than a tile, so that short caches spread
+// their rows over the SMs (d = 64, 4 x 8 heads of 512 slots, 12 rows: 7.6 us as 4 + 4 + 4, 11.3 as 12), else as many as
+// its registers hold, in even chunks (16 x 8 heads of 8192 slots, 12 rows: 42 us as 12, 53 as 8 + 4). d = 256 holds 4
+// rows; there a CTA shares what it unpacks if rows and tiles a CTA are many: with 8 heads of 8192 slots and 16 sequences,
+// 28 rows take 412 us so and 435 by fours, 80 rows 743 and 1333, 20 rows 405 and 313; 80 rows over 16 ragged caches of
+// up to 3001 slots take 46 us and 53, over 32 of 1024 (3.5 tiles a CTA) 67 and 58. Its chunks of 80 rows leave too few
+// CTAs work below twice as many tiles (the ragged caches: 47.6 us as one chunk).
 template <int D, bool kW>
 int kv4_pick_attn(Ctx* ctx, const Kv4Attn& p, const Kv4View& v, cudaStream_t st) {
-  if (p.rows <= 4) return kv4_launch_attn<D, 1, kW>(ctx, p, v, st);
-  if constexpr (D != 256) {
-    if (p.rows <= 8) return kv4_launch_attn<D, 2, kW>(ctx, p, v, st);
-  }
-  const long long chunks = cdiv(p.rows, 4 * rows_most(D)), fours = cdiv(cdiv(p.rows, chunks), 4);
-  if (fours <= 4) return kv4_launch_attn_rows<D, 4, kW>(ctx, p, v, st);
-  if constexpr (D != 256) {
-    if (fours <= 6) return kv4_launch_attn_rows<D, 6, kW>(ctx, p, v, st);
-  }
-  if (fours <= 8 || D == 128) return kv4_launch_attn_rows<D, 8, kW>(ctx, p, v, st);
-  if constexpr (D == 64) {
-    if (fours <= 10) return kv4_launch_attn_rows<D, 10, kW>(ctx, p, v, st);
-    return kv4_launch_attn_rows<D, 12, kW>(ctx, p, v, st);
-  }
   if constexpr (D == 256) {
-    if (fours <= 12) return kv4_launch_attn_rows<D, 12, kW>(ctx, p, v, st);
-    if (fours <= 16) return kv4_launch_attn_rows<D, 16, kW>(ctx, p, v, st);
-    return kv4_launch_attn_rows<D, 20, kW>(ctx, p, v, st);
+    const long long tiles = static_cast<long long>(v.n_seq) * v.n_kv * cdiv(v.cap, kRowsSlots);
+    if (p.rows >= kAttnManyRows && tiles >= 5ll * ctx->sms) {
+      const long long chunks = cdiv(p.rows, 4 * (tiles >= 10ll * ctx->sms ? kRowsMost : 16)), fours = cdiv(cdiv(p.rows, chunks), 4);
+      if (fours <= 8) return kv4_launch_attn_rows<8, kW>(ctx, p, v, st);
+      if (fours <= 12) return kv4_launch_attn_rows<12, kW>(ctx, p, v, st);
+      if (fours <= 16) return kv4_launch_attn_rows<16, kW>(ctx, p, v, st);
+      return kv4_launch_attn_rows<20, kW>(ctx, p, v, st);
+    }
+    return kv4_launch_attn<D, 1, kW>(ctx, p, v, st);
+  } else {
+    const long long heads = static_cast<long long>(v.n_seq) * v.n_kv, tiles = cdiv(v.cap, 4096 / D);
+    const long long chunks = cdiv(p.rows, 4 * attn_most(D));
+    int nt = static_cast<int>(cdiv(cdiv(p.rows, chunks), 4));
+    for (int n = 1; n < nt; ++n) {
+      const long long items = heads * cdiv(p.rows, 4 * n);
+      if (items <= ctx->sms && items * tiles <= static_cast<long long>(ctx->sms) * attn_warps(D, n)) nt = n;
+    }
+    if (nt <= 1) return kv4_launch_attn<D, 1, kW>(ctx, p, v, st);
+    if (nt == 2 || D == 128) return kv4_launch_attn<D, 2, kW>(ctx, p, v, st);
+    if constexpr (D == 64) {
+      if (nt == 3) return kv4_launch_attn<D, 3, kW>(ctx, p, v, st);
+      return kv4_launch_attn<D, 4, kW>(ctx, p, v, st);
+    }
+    return VMLM_OK;
   }
-  return VMLM_OK;
 }
-
 }  // namespace
 
 extern "C" {

@@ -539,6 +539,26 @@ def test_attention_long(kernels, d, n_kv, group, n, weights):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("d,group,m", [(64, 5, 1), (64, 9, 1), (64, 12, 1), (64, 1, 15), (64, 3, 9), (64, 33, 1), (128, 5, 1),
+                                       (128, 3, 4), (128, 33, 1), (256, 2, 3), (256, 1, 24)])
+@pytest.mark.parametrize("weights", [False, True])
+def test_attention_rows_over_long_caches(kernels, d, group, m, weights):
+    """Every count of rows that a warp takes at a time, where items are shared by warps and by CTAs."""
+    rng = np.random.default_rng(d + group + m)
+    _check_attention(rng, d, 5, 4, group, 5001, [5001, 4990, 0, 2177, 63], m, weights)
+    _check_attention(rng, d, 1, 1, group, 20011, [20009], m, weights)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n_seq,group,m,weights", [(4, 7, 4, True), (4, 1, 45, False), (4, 64, 1, True), (4, 16, 5, True),
+                                                  (8, 16, 5, False), (8, 27, 3, True)])
+def test_attention_many_rows_of_256(kernels, n_seq, group, m, weights):
+    rng = np.random.default_rng(group + m)
+    lens = [3001, 3000, 1723, 2944, 0, m - 1, 65, 2999][:n_seq]
+    _check_attention(rng, 256, n_seq, 4, group, 3001, lens, m, weights)
+
+
+@pytest.mark.gpu
 def test_attention_many_ragged(kernels):
     rng = np.random.default_rng(11)
     lens = rng.integers(0, 700, 70)
