@@ -27,6 +27,12 @@
  * calls share one workspace per device, so calls on different streams of the
  * same device must not overlap on the GPU.
  *
+ * Stream capture: a _dev call can be captured into a CUDA graph once an eager
+ * call of at least its size has sized the workspace; a call that would have to
+ * allocate cannot be captured. A workspace that captured calls use is kept until
+ * vmlm_shutdown when a later, larger call replaces it, so their graphs can still be
+ * replayed (and must not be replayed after vmlm_shutdown).
+ *
  * Aliasing: C must not overlap A (some calls clear C before they read A).
  *
  * Programmatic dependent launch: the library's GEMM kernels let the next
