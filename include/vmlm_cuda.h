@@ -334,7 +334,8 @@ typedef struct vmlm_rope {
 /* Queries and keys after their projections: for each head
  * y = x * (1 / sqrt(sum(x^2) / d + eps)) * g (g = gq or gk, [d]; NULL: no
  * norm), then the rotation (rope NULL: none). qo and ko may be q and k (same
- * stride). n_q = 0 or n_kv = 0 leaves that part out. */
+ * stride) and may share no other memory with them. n_q = 0 or n_kv = 0 leaves
+ * that part out. */
 VMLM_API int vmlm_qk_norm_rope_dev(const float *q, size_t ldq, const float *k, size_t ldk, const float *gq,
                                    const float *gk, float eps, const vmlm_rope *rope, float *qo, size_t ldqo,
                                    float *ko, size_t ldko, size_t tokens, size_t n_q, size_t n_kv, size_t d,
@@ -344,7 +345,8 @@ VMLM_API int vmlm_qk_norm_rope_dev(const float *q, size_t ldq, const float *k, s
  * (rows b * m + t) written to slots len[b] + t in 4 bits, v as it is. len is
  * not changed; len[b] < 0 marks an idle sequence, for which nothing is
  * written to the cache. A slot behind cap is not written and is reported by
- * vmlm_sync. */
+ * vmlm_sync. qo may be q (same stride) and may share no other memory with q, k
+ * or v. */
 VMLM_API int vmlm_kv4_append_dev(const vmlm_kv4 *cache, const float *q, size_t ldq, float *qo, size_t ldqo,
                                  size_t n_q, const float *k, size_t ldk, const float *v, size_t ldv, const float *gq,
                                  const float *gk, float eps, const vmlm_rope *rope, const int32_t *len, size_t m,
@@ -365,7 +367,7 @@ VMLM_API int vmlm_kv4_read_dev(const vmlm_kv4 *cache, const int32_t *start, cons
  * accumulated: w_out[j] = w_in[j] + the sum of p_j over the tokens and the kv
  * head's query heads for j < len[b] (w_in counts as 0 for the m newest slots
  * and where it is NULL; w_in and w_out may be the same). Other slots of w_out
- * are not written. A len above cap is taken as cap and reported by vmlm_sync.
+ * are not written. out may not overlap q. A len above cap is taken as cap and reported by vmlm_sync.
  * Sums are f32; products with cached values are exact. With w_out the call
  * holds n_seq * n_kv * cap scores a query row of a kv head in workspace
  * (f32; rows rounded up to a multiple of 4): a prompt's last tokens are a
@@ -381,7 +383,8 @@ VMLM_API int vmlm_kv4_attn_dev(const vmlm_kv4 *cache, const float *q, size_t ldq
  * sequence with len[b] <= keep keeps all. idx [n_seq][n_kv][keep] receives the
  * kept slots (-1 behind them), w_out (may be NULL) their weights (0 behind
  * them), len_out[b] = min(len[b], keep) (0 for a negative len). src is not
- * changed. */
+ * changed. No output may overlap an input (len_out is not len) or another
+ * output. */
 VMLM_API int vmlm_kv4_evict_dev(const vmlm_kv4 *src, const vmlm_kv4 *dst, const float *w, const int32_t *len,
                                 size_t keep, size_t first, size_t recent, int32_t *idx, float *w_out,
                                 int32_t *len_out, void *stream);

@@ -49,6 +49,26 @@ bool kv4_overlap(const void* a, size_t na, const void* b, size_t nb) {
   return na > 0 && nb > 0 && x < y + nb && y < x + na;
 }
 
+// Whether `rows` rows of wa values at a (lda apart) and of wb values at b share a byte. Slices of one wider matrix may lie
+// between each other's rows; with different strides, spans that meet count as shared.
+bool kv4_rows_overlap(const float* a, size_t lda, size_t wa, const float* b, size_t ldb, size_t wb, size_t rows) {
+  if (rows == 0 || wa == 0 || wb == 0) return false;
+  if (rows == 1 || lda != ldb) return kv4_overlap(a, ((rows - 1) * lda + wa) * 4, b, ((rows - 1) * ldb + wb) * 4);
+  if (b < a) std::swap(a, b), std::swap(wa, wb);
+  const size_t off = reinterpret_cast<uintptr_t>(b) - reinterpret_cast<uintptr_t>(a), ld = lda * 4;
+  const size_t down = off / ld, in = off % ld;  // b's first row begins `in` bytes into a's row `down`
+  return (down < rows && in < wa * 4) || (down + 1 < rows && in + wb * 4 > ld);
+}
+
+// The written rows `to` of heads that are read from `from`: in place, or apart.
+int kv4_check_out(const char* what, const char* name, const float* to, size_t ldt, const float* from, size_t ldf, size_t width,
+                  size_t rows) {
+  if (to == from && (ldt == ldf || rows == 1)) return VMLM_OK;
+  if (kv4_rows_overlap(to, ldt, width, from, ldf, width, rows))
+    return fail(VMLM_ERR_ARG, "%s: %so and %s overlap and are not the same rows", what, name, name);
+  return VMLM_OK;
+}
+
 int kv4_check_rope(const char* what, const vmlm_rope* r, size_t d) {
   if (!r) return VMLM_OK;
   if (!r->cos_t || !r->sin_t || !r->pos) return fail(VMLM_ERR_ARG, "%s: null pointer in the rotation", what);
@@ -244,6 +264,12 @@ int vmlm_qk_norm_rope_dev(const float* q, size_t ldq, const float* k, size_t ldk
     VMLM_TRY(kv4_check_rows(what, "k", k, ldk, n_kv, d));
     VMLM_TRY(kv4_check_rows(what, "ko", ko, ldko, n_kv, d));
   }
+  if (n_q > 0) VMLM_TRY(kv4_check_out(what, "q", qo, ldqo, q, ldq, n_q * d, tokens));
+  if (n_kv > 0) VMLM_TRY(kv4_check_out(what, "k", ko, ldko, k, ldk, n_kv * d, tokens));
+  if (n_q > 0 && n_kv > 0 &&
+      (kv4_rows_overlap(qo, ldqo, n_q * d, k, ldk, n_kv * d, tokens) || kv4_rows_overlap(ko, ldko, n_kv * d, q, ldq, n_q * d, tokens) ||
+       kv4_rows_overlap(qo, ldqo, n_q * d, ko, ldko, n_kv * d, tokens)))
+    return fail(VMLM_ERR_ARG, "%s: queries and keys overlap", what);
   Ctx* ctx = nullptr;
   VMLM_TRY(current_ctx(&ctx));
   cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
@@ -274,6 +300,10 @@ int vmlm_kv4_append_dev(const vmlm_kv4* cache, const float* q, size_t ldq, float
   if (n_q > 0) {
     VMLM_TRY(kv4_check_rows(what, "q", q, ldq, n_q, cache->d));
     VMLM_TRY(kv4_check_rows(what, "qo", qo, ldqo, n_q, cache->d));
+    const size_t tokens = cache->n_seq * m, wq = n_q * cache->d, wk = cache->n_kv * cache->d;
+    VMLM_TRY(kv4_check_out(what, "q", qo, ldqo, q, ldq, wq, tokens));
+    if (kv4_rows_overlap(qo, ldqo, wq, k, ldk, wk, tokens) || kv4_rows_overlap(qo, ldqo, wq, v, ldv, wk, tokens))
+      return fail(VMLM_ERR_ARG, "%s: qo overlaps k or v", what);
   }
   Ctx* ctx = nullptr;
   VMLM_TRY(current_ctx(&ctx));
@@ -326,6 +356,12 @@ int vmlm_kv4_attn_dev(const vmlm_kv4* cache, const float* q, size_t ldq, const i
   if (w_in && !w_out) return fail(VMLM_ERR_ARG, "%s: w_in without w_out", what);
   VMLM_TRY(kv4_check_rows(what, "q", q, ldq, n_q, cache->d));
   VMLM_TRY(kv4_check_rows(what, "out", out, ldo, n_q, cache->d));
+  // A part of an item may read its queries when another part's result is written, and weights before they are replaced.
+  if (kv4_rows_overlap(out, ldo, n_q * cache->d, q, ldq, n_q * cache->d, cache->n_seq * m))
+    return fail(VMLM_ERR_ARG, "%s: out overlaps q", what);
+  const size_t w_bytes = cache->n_seq * cache->n_kv * cache->cap * 4;
+  if (w_in && w_in != w_out && kv4_overlap(w_in, w_bytes, w_out, w_bytes))
+    return fail(VMLM_ERR_ARG, "%s: w_in and w_out overlap and are not the same", what);
   Ctx* ctx = nullptr;
   VMLM_TRY(current_ctx(&ctx));
   cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
@@ -355,14 +391,24 @@ int vmlm_kv4_evict_dev(const vmlm_kv4* src, const vmlm_kv4* dst, const float* w,
     return fail(VMLM_ERR_ARG, "%s: first + recent is above keep (%zu + %zu, %zu)", what, first, recent, keep);
   if (src->n_seq == 0) return VMLM_OK;
   if (!len || !len_out || (keep > 0 && (!w || !idx))) return fail(VMLM_ERR_ARG, "%s: null pointer", what);
-  const size_t rows[2] = {src->n_seq * src->n_kv * src->cap, dst->n_seq * dst->n_kv * dst->cap};
-  const void* from[4] = {src->k, src->v, src->ks, src->vs};
-  const void* to[4] = {dst->k, dst->v, dst->ks, dst->vs};
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j)
-      if (kv4_overlap(from[i], rows[0] * (i < 2 ? src->d / 2 : src->d / 8), to[j],
-                      rows[1] * (j < 2 ? src->d / 2 : src->d / 8)))
-        return fail(VMLM_ERR_ARG, "%s: src and dst overlap", what);
+  // CTAs of other heads read lengths, weights and rows while one writes: nothing is done in place.
+  struct Span {
+    const void* at;
+    size_t bytes;
+  };
+  const size_t heads = src->n_seq * src->n_kv, rs = heads * src->cap, rd = heads * dst->cap, codes = src->d / 2, sb = src->d / 8;
+  const Span read[6] = {{src->k, rs * codes}, {src->v, rs * codes}, {src->ks, rs * sb}, {src->vs, rs * sb}, {w, keep ? rs * 4 : 0},
+                        {len, src->n_seq * 4}};
+  const Span written[7] = {{dst->k, rd * codes}, {dst->v, rd * codes}, {dst->ks, rd * sb}, {dst->vs, rd * sb},
+                           {idx, heads * keep * 4}, {w_out, w_out ? heads * keep * 4 : 0}, {len_out, src->n_seq * 4}};
+  for (int i = 0; i < 7; ++i) {
+    for (int j = 0; j < 6; ++j)
+      if (kv4_overlap(written[i].at, written[i].bytes, read[j].at, read[j].bytes))
+        return fail(VMLM_ERR_ARG, i < 4 && j < 4 ? "%s: src and dst overlap" : "%s: an output overlaps an input", what);
+    for (int j = 0; j < i; ++j)
+      if (kv4_overlap(written[i].at, written[i].bytes, written[j].at, written[j].bytes))
+        return fail(VMLM_ERR_ARG, "%s: two outputs overlap", what);
+  }
   Ctx* ctx = nullptr;
   VMLM_TRY(current_ctx(&ctx));
   cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;

@@ -504,7 +504,7 @@ def _rope_ref(rope, tokens):
 
 def qk_norm_rope_dev(q, k, gq, gk, eps, rope, qo, ko, tokens, n_q, n_kv, d, stream=None) -> None:
     """RMSNorm of each query and key head (gains gq, gk [d] or None) and the rotation (rope or None), in one pass: q, qo
-    [tokens, n_q * d], k, ko [tokens, n_kv * d], rows may be slices of wider ones."""
+    [tokens, n_q * d], k, ko [tokens, n_kv * d], rows may be slices of wider ones; qo may be q, ko may be k."""
     pq, ldq = _rows_ptr(q, tokens, n_q * d, "q") if n_q else (None, 0)
     pqo, ldqo = _rows_ptr(qo, tokens, n_q * d, "qo") if n_q else (None, 0)
     pk, ldk = _rows_ptr(k, tokens, n_kv * d, "k") if n_kv else (None, 0)
@@ -539,7 +539,8 @@ def kv4_read_dev(cache, start, end, count, k, v, stream=None) -> None:
 
 def kv4_attn_dev(cache, q, length, out, m, n_q, scale, w_in=None, w_out=None, stream=None) -> None:
     """Attention of the m newest tokens of each sequence (rows b * m + t of q and out) over the cache; length[b] counts
-    them. w_out [n_seq, n_kv, cap] receives w_in plus the weight that each slot got."""
+    them. w_out [n_seq, n_kv, cap] (which may be w_in) receives w_in plus the weight that each slot got. out may not overlap
+    q."""
     tokens, width = cache.n_seq * m, n_q * cache.d
     pq, ldq = _rows_ptr(q, tokens, width, "q")
     po, ldo = _rows_ptr(out, tokens, width, "out")
@@ -552,7 +553,7 @@ def kv4_attn_dev(cache, q, length, out, m, n_q, scale, w_in=None, w_out=None, st
 def kv4_evict_dev(src, dst, w, length, keep, first, recent, idx, w_out, len_out, stream=None) -> None:
     """Copy the `keep` slots of each sequence and kv head with the most weight w [n_seq, n_kv, src.cap] (the first `first`
     and the last `recent` always among them) from src to dst, in slot order; idx, w_out [n_seq, n_kv, keep] and len_out
-    [n_seq] say which they are. w_out may be None."""
+    [n_seq] say which they are. w_out may be None. No output may overlap an input: len_out is not length."""
     out = src.n_seq * src.n_kv * keep
     check(lib().vmlm_kv4_evict_dev(src.ref, dst.ref, _ptr(w, "float32", src.n_seq * src.n_kv * src.cap, "w"),
                                    _ptr(length, "int32", src.n_seq, "length"), keep, first, recent,

@@ -4,11 +4,14 @@ not see, scores at the end of the f32 range, aliased buffers, sizes at the end o
 The definitions and the bound on a score's error (ds) are those of test_kv4.py. A slot that a token does not see has no
 part in its output, whatever its bits: the definition here sums over the visible slots alone.
 """
+import ctypes
+
 import numpy as np
 import pytest
 
 import sparrow_b200.kernels as K
-from test_kv4 import _random_cache, _torch, _up
+from sparrow_b200._lib import VmlmError
+from test_kv4 import EPS, _cache, _random_cache, _rc, _torch, _up
 
 
 # ------------------------------------------------- captured steps
@@ -89,3 +92,101 @@ def test_captured_gemm_beside_a_larger_call(kernels):
 
     outs, step = make(200)
     _replay_beside_a_larger_call(step, outs, make(4000)[1])
+
+
+# ------------------------------------------------- aliased buffers
+
+def test_eviction_refuses_outputs_that_overlap():
+    """One CTA a sequence writes its new length, perhaps before another head's has read the old one; no output may lie on an
+    input or on another output."""
+    n, M = 1 << 12, 1 << 20  # every buffer below has at most 4096 bytes: n_seq 2, n_kv 2, 8 slots of 64, 4 kept
+
+    def evict(**at):
+        p = dict(k=1, v=2, ks=3, vs=4, dk=5, dv=6, dks=7, dvs=8, w=9, length=10, idx=11, w_out=12, len_out=13)
+        p = {x: M + n * y for x, y in p.items()}
+        for x, y in at.items():
+            p[x] = p[y] if isinstance(y, str) else p[y[0]] + y[1]
+        s = _cache(k=p["k"], v=p["v"], ks=p["ks"], vs=p["vs"], n_seq=2)
+        t = _cache(k=p["dk"], v=p["dv"], ks=p["dks"], vs=p["dvs"], n_seq=2)
+        return _rc("vmlm_kv4_evict_dev", ctypes.byref(s), ctypes.byref(t), p["w"], p["length"], 4, 1, 2, p["idx"], p["w_out"],
+                   p["len_out"], None)
+
+    rc, msg = evict(len_out="length")
+    assert rc == 1 and "an output overlaps an input" in msg
+    assert evict(len_out=("length", 4))[0] == 1 and evict(w_out="w")[0] == 1 and evict(w_out=("w", 120))[0] == 1
+    assert evict(idx="w")[0] == 1 and evict(idx="length")[0] == 1 and evict(dks="vs")[0] == 1 and evict(dv="w")[0] == 1
+    rc, msg = evict(idx="w_out")
+    assert rc == 1 and "two outputs overlap" in msg
+    assert evict(len_out=("idx", 60))[0] == 1 and evict(dk="dv")[0] == 1
+
+
+def test_attention_refuses_an_output_over_its_queries():
+    P = 1 << 20
+
+    def attn(q, ldq, out, ldo, m=1, w_in=None, w_out=None):
+        c = _cache(k=1 << 24, v=2 << 24, ks=3 << 24, vs=4 << 24, n_seq=3)
+        return _rc("vmlm_kv4_attn_dev", ctypes.byref(c), q, ldq, 1 << 28, out, ldo, m, 4, 0.125, w_in, w_out, None)
+
+    rc, msg = attn(P, 256, P, 256)
+    assert rc == 1 and "out overlaps q" in msg
+    assert attn(P, 256, P + 2 * 256 * 4 + 255 * 4, 256)[0] == 1      # its last value
+    assert attn(P + 255 * 4, 256, P, 256)[0] == 1
+    assert attn(P, 600, P + 255 * 4, 600)[0] == 1 and attn(P, 600, P + 345 * 4, 600)[0] == 1  # rows between rows, one too far
+    assert attn(P, 300, P + 256 * 4, 400)[0] == 1                    # other strides over the same span
+    rc, msg = attn(P, 256, 2 * P, 256, w_in=3 * P, w_out=3 * P + 64)
+    assert rc == 1 and "w_in and w_out overlap" in msg
+
+
+def test_norm_and_append_refuse_partly_shared_rows():
+    P = 1 << 20
+
+    def norm(q=P, ldq=128, k=2 * P, ldk=128, qo=3 * P, ldqo=128, ko=4 * P, ldko=128):
+        return _rc("vmlm_qk_norm_rope_dev", q, ldq, k, ldk, None, None, 1e-5, None, qo, ldqo, ko, ldko, 5, 2, 2, 64, None)
+
+    rc, msg = norm(qo=P, ldqo=256)
+    assert rc == 1 and "qo and q overlap" in msg
+    assert norm(qo=P + 4)[0] == 1 and norm(ko=2 * P - 4)[0] == 1 and norm(ko=2 * P + 512)[0] == 1
+    rc, msg = norm(qo=2 * P)
+    assert rc == 1 and "queries and keys overlap" in msg
+    assert norm(ko=P)[0] == 1 and norm(qo=4 * P + 4 * 512)[0] == 1
+
+    def app(qo, ldqo):
+        c = _cache(k=1 << 24, v=2 << 24, ks=3 << 24, vs=4 << 24, n_seq=3)
+        return _rc("vmlm_kv4_append_dev", ctypes.byref(c), P, 512, qo, ldqo, 2, P + 512, 512, P + 1024, 512, None, None, 1e-5,
+                   None, 1 << 28, 1, None)
+
+    assert app(P, 300)[0] == 1 and app(P + 4, 512)[0] == 1 and app(P + 512, 512)[0] == 1 and app(P + 1024 + 508, 512)[0] == 1
+
+
+@pytest.mark.gpu
+def test_buffers_between_each_other(kernels):
+    """What may share memory: queries and outputs as slices of one matrix, rows in place, histories in place, one row with any
+    stride."""
+    torch = _torch()
+    rng = np.random.default_rng(1)
+    n_seq, n_kv, group, cap, d, m = 2, 2, 2, 300, 64, 3
+    width = n_kv * group * d
+    _, cache = _random_cache(rng, n_seq, n_kv, cap, d, [cap] * n_seq, bad=False)
+    lens = _up(np.array([cap, 40], np.int32))
+    both = _up(rng.standard_normal((n_seq * m, 2 * width)).astype(np.float32))
+    q = both[:, :width].clone()
+    st = torch.cuda.current_stream()
+    ref = torch.empty_like(q)
+    K.kv4_attn_dev(cache, q, lens, ref, m, n_kv * group, 0.1, stream=st)
+    K.kv4_attn_dev(cache, both[:, :width], lens, both[:, width:], m, n_kv * group, 0.1, stream=st)
+    assert torch.equal(both[:, width:], ref) and torch.equal(both[:, :width], q)
+    x = both.clone()
+    y, g = torch.empty_like(x), _up(rng.uniform(0.5, 1.5, d).astype(np.float32))
+    K.qk_norm_rope_dev(x[:, :width], x[:, width:], g, g, EPS, None, y[:, :width], y[:, width:], n_seq * m, n_kv * group,
+                       n_kv * group, d, stream=st)
+    K.qk_norm_rope_dev(x[:, :width], x[:, width:], g, g, EPS, None, x[:, :width], x[:, width:], n_seq * m, n_kv * group,
+                       n_kv * group, d, stream=st)
+    K.qk_norm_rope_dev(x[:1, :d], None, None, None, EPS, None, x[:1, :d], None, 1, 1, 0, d, stream=st)
+    assert torch.equal(x, y)
+    K.sync(st)
+    idx, w = torch.empty((n_seq, n_kv, 8), dtype=torch.int32, device="cuda"), torch.ones((n_seq, n_kv, cap), device="cuda")
+    _, small = _random_cache(rng, n_seq, n_kv, 8, d, [8] * n_seq, bad=False)
+    with pytest.raises(VmlmError):
+        K.kv4_evict_dev(cache, small, w, lens, 8, 0, 0, idx, None, lens, stream=st)
+    K.kv4_evict_dev(cache, small, w, lens, 8, 0, 0, idx, None, torch.empty_like(lens), stream=st)
+    K.sync(st)
