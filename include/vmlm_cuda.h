@@ -362,6 +362,8 @@ VMLM_API int vmlm_kv4_read_dev(const vmlm_kv4 *cache, const int32_t *start, cons
 /* Attention of the m newest tokens of each sequence (rows b * m + t of q and
  * out, n_q heads, n_q / n_kv of them to a kv head): token t sees the slots
  * j < len[b] - (m - 1 - t), len[b] counting the m tokens themselves.
+ * A slot that a token does not see has no part in its output, whatever bits it
+ * holds (a NaN among the newest values reaches the tokens that see it).
  *   out = sum_j p_j v_j, p = softmax(scale * q . k_j); no visible slot: zeros.
  * With w_out ([n_seq][n_kv][cap]), the weight that each slot received is
  * accumulated: w_out[j] = w_in[j] + the sum of p_j over the tokens and the kv

@@ -133,6 +133,34 @@ __device__ __forceinline__ uint32_t kv4_pair(uint32_t u, uint32_t mul, __half2 s
   return h2_bits(__hfma2(bits_h2(t), step, base));
 }
 
+// Values of slots that some rows of a chunk see and others do not. A hidden slot's weight is 0, but 0 times a NaN or an
+// infinity is NaN, and a product takes a slot's values for all rows: slots whose values are not finite (of one group of 32
+// columns; judged by the smallest and the largest code's value) leave the product, and the rows that see them get them
+// by scalar operations. This is looked for only in tiles that a row of the chunk sees in part.
+__device__ __forceinline__ bool kv4_infinite(__half2 step, __half2 base) {  // of the low half
+  const uint32_t lo = h2_bits(__hfma2(__float2half2_rn(16.f), step, base)), hi = h2_bits(__hfma2(__float2half2_rn(31.f), step, base));
+  return (lo & 0x7C00u) == 0x7C00u || (hi & 0x7C00u) == 0x7C00u;
+}
+// Bits 15 and 31: whether any of the pairs seen so far may be so: a step of 1024 or a base of 32768 and more.
+__device__ __forceinline__ uint32_t kv4_large(uint32_t seen, __half2 steps, __half2 bases) {
+  return seen | ((h2_bits(steps) & 0x7FFF7FFFu) + 0x1C001C00u) | ((h2_bits(bases) & 0x7FFF7FFFu) + 0x08000800u);
+}
+// Two slots' steps and bases (halves of a register each), made zero where they are not finite and `from` (0 for both, 1 for
+// the second, 2 for none) allows it: the values become zeros. Returns which, as bits 0 and 1.
+__device__ __forceinline__ uint32_t kv4_take_out(__half2& step, __half2& base, int from) {
+  const bool a = from <= 0 && kv4_infinite(step, base), b = from <= 1 && kv4_infinite(__lowhigh2highlow(step), __lowhigh2highlow(base));
+  const uint32_t keep = (a ? 0u : 0xFFFFu) | (b ? 0u : 0xFFFF0000u);
+  step = bits_h2(h2_bits(step) & keep), base = bits_h2(h2_bits(base) & keep);
+  return (a ? 1u : 0u) | (b ? 2u : 0u);
+}
+__device__ __forceinline__ float kv4_value(uint32_t word, int nibble, __half2 sb) {
+  return __half2float(__hfma(__float2half_rn(16.f + static_cast<float>(word >> 4 * nibble & 15u)), __low2half(sb), __high2half(sb)));
+}
+// A weight from its halves: slot `odd` of two in the fragments of a row's hi and lo.
+__device__ __forceinline__ float kv4_weight(uint32_t hi, uint32_t lo, int odd) {
+  return odd ? __high2float(bits_h2(hi)) + __high2float(bits_h2(lo)) : __low2float(bits_h2(hi)) + __low2float(bits_h2(lo));
+}
+
 // A query row as B fragments of its halves, a power of two apart from the row so
 // that its largest value lies in [1, 2), with the scale's sign in it. Lane (gid,
 // tig) has columns tig * D/4 .. of row gid / 2 of four: hi for even gid, lo for
@@ -315,8 +343,9 @@ __device__ __forceinline__ void attn_put_split(const Kv4Attn& p, const AttnRun& 
   p.split[s.b * hc_count + s.hc] = make_int2(cta, end - cta + 1);
 }
 
-// D: head size. NT: chunks hold 4 * NT rows. kW: scores are kept for w_out.
-template <int D, int NT, bool kW>
+// D: head size. NT: chunks hold 4 * NT rows. kW: scores are kept for w_out. kSeveral: m may be above 1, so that rows of a
+// chunk may see different slots (one token needs no look at the values: 60.7 against 59.8 us for the 48 ragged sequences).
+template <int D, int NT, bool kW, bool kSeveral>
 __global__ void __launch_bounds__(attn_warps(D, NT) * 32, 1) kv4_attn_kernel(const Kv4Attn p, const Kv4View c,
                                                                              int* __restrict__ err) {
   constexpr int kWarps = attn_warps(D, NT), kThreads = kWarps * 32;
@@ -493,7 +522,7 @@ __global__ void __launch_bounds__(attn_warps(D, NT) * 32, 1) kv4_attn_kernel(con
       sc[nt] = __shfl_sync(0xffffffffu, up, 8 * tig);
       vis[nt] = rt < p.rows ? run.n - (p.m - 1 - token(rt)) : 0;
     }
-    const int all_see = r0 + RC > p.rows ? 0 : run.n - (p.m - 1 - token(r0));  // slots that every row sees
+    const int all_see = run.n - (p.m - 1 - token(r0));  // slots that every row sees (rows that are not there: any)
 
     float top[NT], sum[NT], o[OT][2][NT];
     #pragma unroll
@@ -643,6 +672,48 @@ __global__ void __launch_bounds__(attn_warps(D, NT) * 32, 1) kv4_attn_kernel(con
           const uint32_t x = *reinterpret_cast<const uint32_t*>(ps), y = *reinterpret_cast<const uint32_t*>(ps + D / 8);
           stp[u][h] = bits_h2(__byte_perm(x, y, 0x5410));
           bas[u][h] = bits_h2(__byte_perm(x, y, 0x7632));
+        }
+      }
+      bool unsafe = false;
+      if (kSeveral && all_see < run.n && at + TS > all_see) {  // a row may not see slots that others do
+        uint32_t large = 0;
+        #pragma unroll
+        for (int u = 0; u < ST; ++u) large = kv4_large(kv4_large(large, stp[u][0], bas[u][0]), stp[u][1], bas[u][1]);
+        unsafe = __any_sync(0xffffffffu, large & 0x80008000u);
+      }
+      if (__builtin_expect(unsafe, 0)) {
+        uint32_t out_of[(TS + 31) / 32] = {};
+        #pragma unroll
+        for (int u = 0; u < ST; ++u)
+          #pragma unroll
+          for (int h = 0; h < 2; ++h)
+            out_of[u / 2] |= kv4_take_out(stp[u][h], bas[u][h], all_see - at - (u * 16 + h * 8 + 2 * tig)) << (u % 2 * 16 + h * 8 + 2 * tig);
+        #pragma unroll
+        for (int i = 0; i < (TS + 31) / 32; ++i) {
+          #pragma unroll 1
+          for (uint32_t bad = __reduce_or_sync(0xffffffffu, out_of[i]); bad; bad &= bad - 1) {
+            const int in = __ffs(bad) - 1, slot = 32 * i + in;
+            const __half2 sb = *reinterpret_cast<const __half2*>(st + 4608 + slot * (D / 8) + gid * VW / 4 * 4);
+            const bool mine = kv4_infinite(__low2half2(sb), __high2half2(sb));
+            const uint32_t* words = reinterpret_cast<const uint32_t*>(
+                st + 2048 + slot * (D / 2) + attn_swizzle<D>(slot, v_in / 16) * 16 + v_in % 16);
+            #pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              uint32_t both = 0;
+              #pragma unroll
+              for (int x = 0; x < 4 && 2 * i + x / 2 < ST; ++x)  // eights of a word of slots (an index would put pb into memory)
+                both |= pb[2 * i + x / 2][nt][x % 2] & -static_cast<uint32_t>(in / 8 == x);
+              const int from = 8 * tig + in % 8 / 2;
+              const uint32_t hi = __shfl_sync(0xffffffffu, both, from), lo = __shfl_sync(0xffffffffu, both, from + 4);
+              if (!mine || at + slot >= vis[nt]) continue;
+              const float w = kv4_weight(hi, lo, in & 1);
+              #pragma unroll
+              for (int t = 0; t < OT; ++t)
+                #pragma unroll
+                for (int h = 0; h < 2; ++h)
+                  o[t][h][nt] += w * kv4_value(words[VW == 1 ? 0 : t / 8 * 2 + h], VW == 1 ? 4 * h + t : t % 8, sb);
+            }
+          }
         }
       }
       // Tiles 2 y and 2 y + 1 are the low and the high nibbles of one byte of the words: d = 64, columns 8 gid + n and

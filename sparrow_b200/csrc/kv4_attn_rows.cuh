@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, 1) kv4_attn_rows_kernel(const
     const int n0 = share * NG;  // the first four of rows of this warp's scores
     // of a row: what a score is multiplied by, kAttnShift - its maximum so far, the score from which that has grown
     float sc[NG], off[NG], grow[NG], sum[NG];
-    const int all_see = rows < RC ? 0 : run.n - (p.m - 1 - attn_token(p, run.r0));
+    const int all_see = run.n - (p.m - 1 - attn_token(p, run.r0));  // slots that every row sees (rows that are not there: any)
     __syncthreads();
     #pragma unroll
     for (int i = 0; i < NG; ++i)
@@ -280,14 +280,17 @@ __global__ void __launch_bounds__(kRowsWarps * 32, 1) kv4_attn_rows_kernel(const
       }
       if (tid < 4) s_grown[parity ^ 1][tid] = 0;  // read last before this tile's first barrier
       // Tile 8 w + n is columns n of words 2 w and 2 w + 1 of the lane's; odd tiles are high nibbles.
-      uint32_t a[4][4];
+      uint32_t a[4][4], out_of[2] = {};
+      const bool partly = all_see < run.n && at + TS > all_see;  // a row may not see slots that others do
       #pragma unroll
       for (int u = 0; u < 4; ++u) {
         #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const unsigned char* pc = tile + vs_at + (u * 16 + h * 8) * (D / 8);
           const uint32_t x = *reinterpret_cast<const uint32_t*>(pc), y = *reinterpret_cast<const uint32_t*>(pc + D / 8);
-          const __half2 step = bits_h2(__byte_perm(x, y, 0x5410)), base = bits_h2(__byte_perm(x, y, 0x7632));
+          __half2 step = bits_h2(__byte_perm(x, y, 0x5410)), base = bits_h2(__byte_perm(x, y, 0x7632));
+          if (partly)
+            out_of[u / 2] |= kv4_take_out(step, base, all_see - at - (u * 16 + h * 8 + 2 * tig)) << (u % 2 * 16 + h * 8 + 2 * tig);
           #pragma unroll
           for (int z = 0; z < 2; ++z) {
             const int byte = ot % 8 / 2, off = (u * 16 + h * 8) * (D / 2) + (ot / 8 * 2 + z) * 4;
@@ -310,6 +313,27 @@ __global__ void __launch_bounds__(kRowsWarps * 32, 1) kv4_attn_rows_kernel(const
             mma_f16(d, a[u][0], a[u][1], a[u][2], a[u][3], b.x, b.y);
         }
         o[0][i] += d[0] + d[1], o[1][i] += d[2] + d[3];
+      }
+      if (partly) {
+        #pragma unroll 1
+        for (int k = 0; k < 2; ++k) {
+          #pragma unroll 1
+          for (uint32_t bad = __reduce_or_sync(0xffffffffu, k ? out_of[1] : out_of[0]); bad; bad &= bad - 1) {
+            const int slot = 32 * k + __ffs(bad) - 1;
+            const __half2 sb = *reinterpret_cast<const __half2*>(tile + kVsAt + slot * (D / 8) + gid * VW / 4 * 4);
+            if (!kv4_infinite(__low2half2(sb), __high2half2(sb))) continue;
+            const uint32_t* words = reinterpret_cast<const uint32_t*>(
+                tile + kVAt + slot * (D / 2) + attn_swizzle<D>(slot, v_in / 16) * 16 + v_in % 16) + ot / 8 * 2;
+            const float v0 = kv4_value(words[0], ot % 8, sb), v1 = kv4_value(words[1], ot % 8, sb);
+            const uint32_t* from = reinterpret_cast<const uint32_t*>(ps + slot / 16 * NT * 32 + 8 * tig + slot % 8 / 2) + slot / 8 % 2;
+            #pragma unroll
+            for (int i = 0; i < NT; ++i) {
+              if (at + slot >= s_see[i * 4 + tig]) continue;
+              const float w = kv4_weight(from[i * 64], from[i * 64 + 8], slot & 1);
+              o[0][i] += w * v0, o[1][i] += w * v1;
+            }
+          }
+        }
       }
       stage ^= 1, parity ^= 1;
     }

@@ -172,12 +172,14 @@ int kv4_prepare_attn(Ctx* ctx, Kv4Attn* p, const Kv4View& v, int nt, int d, int 
   return VMLM_OK;
 }
 
-template <int D, int NT, bool kW>
+template <int D, int NT, bool kW, bool kSeveral = true>
 int kv4_launch_attn(Ctx* ctx, Kv4Attn p, const Kv4View& v, cudaStream_t st) {
+  if constexpr (NT == 1 && kSeveral)
+    if (p.m == 1) return kv4_launch_attn<D, NT, kW, false>(ctx, p, v, st);
   constexpr int kSmem = attn_smem_bytes(D, NT);
   static bool set[64] = {};
   if (ctx->dev < 64 && !set[ctx->dev]) {
-    VMLM_CUDA(cudaFuncSetAttribute(kv4_attn_kernel<D, NT, kW>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    VMLM_CUDA(cudaFuncSetAttribute(kv4_attn_kernel<D, NT, kW, kSeveral>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
     set[ctx->dev] = true;
   }
   const int grid = ctx->sms;
@@ -186,7 +188,7 @@ int kv4_launch_attn(Ctx* ctx, Kv4Attn p, const Kv4View& v, cudaStream_t st) {
   const long long items = static_cast<long long>(v.n_seq) * v.n_kv * p.chunks, spare = grid - items;
   constexpr int kWarps = attn_warps(D, NT);
   p.alone = static_cast<int>(spare < 0 ? 0 : spare * kAttnAlone <= grid ? kWarps * kAttnAlone : kWarps * grid / spare);
-  VMLM_TRY(launch(kv4_attn_kernel<D, NT, kW>, dim3(grid), dim3(kWarps * 32), kSmem, st, true, p, v, ctx->err));
+  VMLM_TRY(launch(kv4_attn_kernel<D, NT, kW, kSeveral>, dim3(grid), dim3(kWarps * 32), kSmem, st, true, p, v, ctx->err));
   const bool whole = spare >= 0 && v.cap <= static_cast<long long>(p.alone) * (4096 / D);
   return kv4_launch_finish<D, NT, kW>(p, v, whole, st);
 }

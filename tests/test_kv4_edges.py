@@ -11,7 +11,7 @@ import pytest
 
 import sparrow_b200.kernels as K
 from sparrow_b200._lib import VmlmError
-from test_kv4 import EPS, _cache, _random_cache, _rc, _torch, _up
+from test_kv4 import EPS, _cache, _random_cache, _rc, _torch, _up, np_attention, np_values
 
 
 # ------------------------------------------------- captured steps
@@ -190,3 +190,72 @@ def test_buffers_between_each_other(kernels):
         K.kv4_evict_dev(cache, small, w, lens, 8, 0, 0, idx, None, lens, stream=st)
     K.kv4_evict_dev(cache, small, w, lens, 8, 0, 0, idx, None, torch.empty_like(lens), stream=st)
     K.sync(st)
+
+
+# ------------------------------------------------- what a token does not see
+
+def _visible_attention(q, k, v, seen, scale):
+    """q [rows, d], k, v [n, d] f64, seen [rows]: output and weights [rows, n], each row from its visible slots alone."""
+    out, p = np.zeros((len(q), v.shape[1])), np.zeros((len(q), len(k)))
+    for r, n in enumerate(seen):
+        if n <= 0:
+            continue
+        z = scale * (k[:n] @ q[r])
+        e = np.exp(z - z.max())
+        p[r, :n] = e / e.sum()
+        with np.errstate(invalid="ignore"):
+            out[r] = p[r, :n] @ v[:n]
+    return out, p
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,group,m,n_seq,n_kv,cap", [
+    (64, 1, 2, 2, 2, 100), (64, 1, 33, 2, 3, 400), (64, 3, 5, 3, 2, 900), (64, 1, 130, 1, 2, 300), (64, 5, 2, 2, 1, 4000),
+    (128, 1, 3, 2, 2, 70), (128, 4, 5, 3, 2, 700), (128, 2, 40, 1, 2, 3000), (256, 1, 4, 2, 2, 65), (256, 2, 9, 2, 1, 500),
+    (256, 16, 5, 8, 2, 3000), (256, 4, 8, 8, 2, 3000), (256, 1, 45, 8, 2, 3000)])
+@pytest.mark.parametrize("weights", [False, True])
+def test_attention_hidden_values_that_are_not_finite(kernels, d, group, m, n_seq, n_kv, cap, weights):
+    """NaN and infinite values, and codes whose value overflows a half, in the newest tokens: a token that does not see
+    them has a finite output; one that does has them in their columns and nowhere else."""
+    torch = _torch()
+    rng = np.random.default_rng(d + m + cap)
+    lens = np.array([max(m, cap - 13 * b) for b in range(n_seq)], np.int32)
+    host, _ = _random_cache(rng, n_seq, n_kv, cap, d, lens)
+    (kc, ks, kb), (vc, vs, vb) = host
+    for b, n in enumerate(lens):
+        vs[b, 0, n - 1, 0] = np.nan                 # the last token, its first 32 columns
+        vb[b, :, n - 1, d // 32 - 1] = -np.inf      # and its last 32
+        vs[b, n_kv - 1, n - m + 1, 1] = 4000        # the second token: codes from 1 on are infinite
+        vb[b, n_kv - 1, n - m + 1, 1] = 0
+        if n > m + 3:
+            vs[b, 0, 1, 1] = np.nan                 # a slot that every token sees
+    cache = K.Kv4Cache(_up(kc[..., 0::2] | (kc[..., 1::2] << 4)), _up(vc[..., 0::2] | (vc[..., 1::2] << 4)),
+                       _up(np.stack((ks, kb), -1)), _up(np.stack((vs, vb), -1)))
+    n_q, scale = n_kv * group, 1 / np.sqrt(d)
+    q = rng.standard_normal((n_seq * m, n_q * d)).astype(np.float32)
+    out = torch.full((n_seq * m, n_q * d), 7.0, device="cuda")
+    w_out = torch.full((n_seq, n_kv, cap), 7.0, device="cuda") if weights else None
+    st = torch.cuda.current_stream()
+    K.kv4_attn_dev(cache, _up(q), _up(lens), out, m, n_q, scale, w_out=w_out, stream=st)
+    K.sync(st)
+    got = out.cpu().numpy().reshape(n_seq, m, n_q, d)
+    q = q.reshape(n_seq, m, n_q, d).astype(np.float64)
+    for b, n in enumerate(lens):
+        seen = np.repeat(n - (m - 1 - np.arange(m)), group)
+        for h in range(n_kv):
+            k = np_values(kc[b, h, :n], ks[b, h, :n], kb[b, h, :n])
+            with np.errstate(over="ignore", invalid="ignore"):
+                v = np_values(vc[b, h, :n], vs[b, h, :n], vb[b, h, :n])
+            rows = q[b, :, h * group:(h + 1) * group].reshape(m * group, d)
+            ref, p = _visible_attention(rows, k, v, seen, scale)
+            _, _, ds = np_attention(rows, k, np.zeros_like(v), seen, scale)
+            y = got[b, :, h * group:(h + 1) * group].reshape(m * group, d)
+            assert np.array_equal(np.isfinite(y), np.isfinite(ref)), (b, h)
+            for r in range(m * group):
+                x = v[:seen[r]]
+                vmax = np.abs(x[np.isfinite(x)]).max()
+                ok = np.isfinite(ref[r])
+                assert (np.abs(y[r, ok] - ref[r, ok]) <= (2 * ds[r] + 2.0 ** -18) * vmax).all(), (b, h, r)
+            if weights:
+                tol = ((2 * ds + 2.0 ** -18)[:, None] * p).sum(0) + 2.0 ** -22 * p.sum(0) + 1e-12
+                assert (np.abs(w_out[b, h].cpu().numpy()[:n] - p.sum(0)) <= tol).all(), (b, h)
