@@ -351,7 +351,8 @@ int vmlm_kv4_attn_dev(const vmlm_kv4* cache, const float* q, size_t ldq, const i
   VMLM_TRY(kv4_check(what, cache));
   if (n_q % cache->n_kv != 0)
     return fail(VMLM_ERR_SHAPE, "%s: %zu query heads do not share %zu kv heads evenly", what, n_q, cache->n_kv);
-  if (n_q >= 65536 || m >= kKv4MaxDim || cache->n_seq * m * n_q >= kKv4MaxDim)
+  if (n_q >= 65536 || m >= kKv4MaxDim || cache->n_seq * m >= kKv4MaxDim ||  // in steps: three factors can wrap
+      cache->n_seq * m * n_q >= kKv4MaxDim)
     return fail(VMLM_ERR_SHAPE, "%s: n_seq * m * n_q must be < 2^31 and n_q < 65536", what);
   if (m == 0 || n_q == 0 || cache->n_seq == 0) return VMLM_OK;
   if (!len) return fail(VMLM_ERR_ARG, "%s: len is null", what);

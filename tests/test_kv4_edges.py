@@ -94,6 +94,16 @@ def test_captured_gemm_beside_a_larger_call(kernels):
     _replay_beside_a_larger_call(step, outs, make(4000)[1])
 
 
+# ------------------------------------------------- the end of the index range
+
+def test_attention_refuses_sizes_whose_product_wraps():
+    """n_seq * m * n_q is 2^65: below 2^31 in 64 bits."""
+    c = _cache(n_seq=1 << 25, n_kv=1)
+    rc, msg = _rc("vmlm_kv4_attn_dev", ctypes.byref(c), 4096, 64 << 15, 4096, 1 << 28, 64 << 15, 1 << 25, 1 << 15, 0.125, None,
+                  None, None)
+    assert rc == 2 and "n_seq * m * n_q" in msg
+
+
 # ------------------------------------------------- aliased buffers
 
 def test_eviction_refuses_outputs_that_overlap():
