@@ -311,8 +311,8 @@ VMLM_API int vmlm_pool_gemm(vmlm_pool *pool, const void *ins, void *stream);
  *   c = clamp(rint((x - base) * (1 / step)) - 16, 0, 15), or 0 where step = 0.
  * A NaN makes its whole group NaN. Buffers belong to the caller (16-byte
  * aligned): k and v n_seq * n_kv * cap * d/2 bytes, ks and vs
- * n_seq * n_kv * cap * d/32 * 4 bytes. Slots at or behind a sequence's length
- * are never read: they may hold anything. */
+ * n_seq * n_kv * cap * d/32 * 4 bytes; cap is at most 2^31 - 8192. Slots at or
+ * behind a sequence's length are never read: they may hold anything. */
 typedef struct vmlm_kv4 {
   void *k, *v;   /* codes */
   void *ks, *vs; /* (step, base) */

@@ -6,15 +6,16 @@
 namespace {
 
 constexpr size_t kKv4MaxDim = static_cast<size_t>(1) << 31;
+constexpr size_t kKv4MaxSlots = kKv4MaxDim - 8192;  // slots are ints, and a kernel's walk goes up to a block's step past them
 
 int kv4_check(const char* what, const vmlm_kv4* c) {
   if (!c) return fail(VMLM_ERR_ARG, "%s: null cache", what);
   if (c->d != 64 && c->d != 128 && c->d != 256)
     return fail(VMLM_ERR_SHAPE, "%s: head size %zu (64, 128 and 256 are built)", what, c->d);
   if (c->n_kv == 0) return fail(VMLM_ERR_ARG, "%s: no kv heads", what);
-  if (c->n_seq >= kKv4MaxDim || c->n_kv >= kKv4MaxDim || c->cap >= kKv4MaxDim ||
-      c->n_seq * c->n_kv >= kKv4MaxDim)
-    return fail(VMLM_ERR_SHAPE, "%s: n_seq * n_kv and cap must be < 2^31", what);
+  if (c->n_seq >= kKv4MaxDim || c->n_kv >= kKv4MaxDim || c->n_seq * c->n_kv >= kKv4MaxDim)
+    return fail(VMLM_ERR_SHAPE, "%s: n_seq * n_kv must be < 2^31", what);
+  if (c->cap > kKv4MaxSlots) return fail(VMLM_ERR_SHAPE, "%s: cap must be at most 2^31 - 8192", what);
   if (c->n_seq > 0 && c->cap > 0) {
     if (!c->k || !c->v || !c->ks || !c->vs) return fail(VMLM_ERR_ARG, "%s: null pointer in the cache", what);
     if (!aligned16(c->k) || !aligned16(c->v) || !aligned16(c->ks) || !aligned16(c->vs))
@@ -325,7 +326,7 @@ int vmlm_kv4_read_dev(const vmlm_kv4* cache, const int32_t* start, const int32_t
   std::lock_guard<std::recursive_mutex> lk(g_mu);
   const char* what = "kv4_read_dev";
   VMLM_TRY(kv4_check(what, cache));
-  if (count >= kKv4MaxDim) return fail(VMLM_ERR_SHAPE, "%s: count must be < 2^31", what);
+  if (count > kKv4MaxSlots) return fail(VMLM_ERR_SHAPE, "%s: count must be at most 2^31 - 8192", what);
   if (count == 0 || cache->n_seq == 0) return VMLM_OK;
   if (!start || !end || !k || !v) return fail(VMLM_ERR_ARG, "%s: null pointer", what);
   if (!aligned16(k) || !aligned16(v)) return fail(VMLM_ERR_ARG, "%s: k and v must start on a 16-byte boundary", what);
@@ -390,6 +391,8 @@ int vmlm_kv4_evict_dev(const vmlm_kv4* src, const vmlm_kv4* dst, const float* w,
   if (src->n_seq != dst->n_seq || src->n_kv != dst->n_kv || src->d != dst->d)
     return fail(VMLM_ERR_SHAPE, "%s: the two caches differ in n_seq, n_kv or d", what);
   if (keep > dst->cap) return fail(VMLM_ERR_SHAPE, "%s: keep is %zu, dst holds %zu slots", what, keep, dst->cap);
+  if (keep * (src->d / 32) > kKv4MaxSlots)
+    return fail(VMLM_ERR_SHAPE, "%s: keep * d / 32 must be at most 2^31 - 8192", what);
   if (first > keep || recent > keep - first)
     return fail(VMLM_ERR_ARG, "%s: first + recent is above keep (%zu + %zu, %zu)", what, first, recent, keep);
   if (src->n_seq == 0) return VMLM_OK;

@@ -104,6 +104,26 @@ def test_attention_refuses_sizes_whose_product_wraps():
     assert rc == 2 and "n_seq * m * n_q" in msg
 
 
+def test_refuses_slots_that_a_step_would_carry_past_32_bits():
+    """A kernel's walk steps by a tile or by a block of threads from slots below cap, and by units of 32 columns over what an
+    eviction keeps."""
+    T = 1 << 40
+
+    def cache(**kw):
+        return _cache(**{**dict(k=T, v=2 * T, ks=3 * T, vs=4 * T, n_kv=1), **kw})
+
+    for cap in ((1 << 31) - 1, (1 << 31) - 8191):
+        c = cache(cap=cap)
+        rc, msg = _rc("vmlm_kv4_attn_dev", ctypes.byref(c), 4096, 64, 4096, 1 << 28, 64, 1, 1, 0.125, None, None, None)
+        assert rc == 2 and "cap" in msg
+        assert _rc("vmlm_kv4_read_dev", ctypes.byref(c), 4096, 4096, 1, 4096, 4096, None)[0] == 2
+    assert _rc("vmlm_kv4_read_dev", ctypes.byref(cache()), 4096, 4096, (1 << 31) - 1, 4096, 4096, None)[0] == 2
+    for d, keep in ((64, 1 << 30), (128, 1 << 29), (256, 1 << 28)):
+        s, t = cache(cap=keep + 8, d=d), cache(k=5 * T, v=6 * T, ks=7 * T, vs=8 * T, cap=keep, d=d)
+        rc, msg = _rc("vmlm_kv4_evict_dev", ctypes.byref(s), ctypes.byref(t), 9 * T, 10 * T, keep, 0, 0, 11 * T, None, 12 * T, None)
+        assert rc == 2 and "keep" in msg
+
+
 # ------------------------------------------------- aliased buffers
 
 def test_eviction_refuses_outputs_that_overlap():
