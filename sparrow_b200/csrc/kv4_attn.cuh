@@ -42,7 +42,7 @@ struct Kv4Attn {
   const float* w_in;
   float* w_out;
   float* score;       // [n_seq][n_kv][chunks][kept_rows][cap]: log2 of the unnormalised weights (w_out only)
-  float* lse;         // [n_seq][n_kv][rows]: log2 of their sum
+  float2* norm;       // [n_seq][n_kv][rows]: what is added to a score to be the exponent of a weight, 1 / the weights' sum
   float* part;        // two partial results a CTA: m, l, O of a chunk of rows
   int2* split;        // [n_seq][n_kv][chunks]: the first CTA of an item and how many have a part of it (one: the output is there)
   float scale2;       // scale * log2(e)
@@ -325,15 +325,16 @@ __device__ __forceinline__ void attn_join(float& m, float& l, float& v, float pm
   l = fmaf(l, f, pl * fp), v = fmaf(v, f, pv * fp), m = mm;
 }
 
-// A query row's token; its place in q and in the output; where its log2 sum goes.
+// A query row's token; its place in q and in the output; where its maximum and sum go.
 __device__ __forceinline__ int attn_token(const Kv4Attn& p, int row) { return p.m == 1 ? 0 : row / p.group; }
 template <int D>
 __device__ __forceinline__ long long attn_row_at(const Kv4Attn& p, const AttnRun& s, int row, long long ld) {
   const int t = attn_token(p, row);
   return (static_cast<long long>(s.b) * p.m + t) * ld + static_cast<long long>(s.head * p.group + row - t * p.group) * D;
 }
-__device__ __forceinline__ void attn_put_lse(const Kv4Attn& p, const Kv4View& c, const AttnRun& s, int row, float m, float l) {
-  p.lse[(static_cast<long long>(s.b) * c.n_kv + s.head) * p.rows + row] = m - kAttnShift + log2f(l);
+__device__ __forceinline__ void attn_put_norm(const Kv4Attn& p, const Kv4View& c, const AttnRun& s, int row, float m, float inv) {
+  // not the log of the sum: nothing is lost between two large numbers, and a row without a weight gives every slot 0
+  p.norm[(static_cast<long long>(s.b) * c.n_kv + s.head) * p.rows + row] = make_float2(kAttnShift - m, inv);
 }
 
 // An item's first run says which CTAs have parts of it: shares of `each` tiles, one more for the first `extra` CTAs.
@@ -477,7 +478,7 @@ __global__ void __launch_bounds__(attn_warps(D, NT) * 32, 1) kv4_attn_kernel(con
   auto first_row = [&](const AttnRun& s) { return (static_cast<long long>(s.b) * c.n_kv + s.head) * c.cap; };
   auto token = [&](int row) { return attn_token(p, row); };
   auto row_at = [&](const AttnRun& s, int row, long long ld) { return attn_row_at<D>(p, s, row, ld); };
-  auto put_lse = [&](const AttnRun& s, int row, float m, float l) { attn_put_lse(p, c, s, row, m, l); };
+  auto put_norm = [&](const AttnRun& s, int row, float m, float inv) { attn_put_norm(p, c, s, row, m, inv); };
 
   if (lane < 2) s_state[2 * warp + lane] = 0;
   __syncwarp();
@@ -787,8 +788,7 @@ __global__ void __launch_bounds__(attn_warps(D, NT) * 32, 1) kv4_attn_kernel(con
         #pragma unroll
         for (int r4 = 0; r4 < 4; ++r4) {
           const int r = nt * 4 + r4;
-          const float f = __shfl_sync(0xffffffffu, inv, r4), tp = __shfl_sync(0xffffffffu, top[nt], r4),
-                      sm = __shfl_sync(0xffffffffu, sum[nt], r4);
+          const float f = __shfl_sync(0xffffffffu, inv, r4), tp = __shfl_sync(0xffffffffu, top[nt], r4);
           if (r0 + r >= p.rows) continue;
           float* to = p.out + row_at(run, r0 + r, p.ldo);
           #pragma unroll
@@ -797,7 +797,7 @@ __global__ void __launch_bounds__(attn_warps(D, NT) * 32, 1) kv4_attn_kernel(con
             attn_place<D>(x + lane, ti, h, g);
             to[x + lane] = fr[((ti * 2 + h) * NT + nt) * 32 + g * 4 + r4] * f;
           }
-          if (kW && lane == 0) put_lse(run, r0 + r, tp, sm);
+          if (kW && lane == 0) put_norm(run, r0 + r, tp, f);
         }
       }
       if (lane == 0) p.split[run.b * walk.hc_count + run.hc] = make_int2(cta, 1);
@@ -858,7 +858,7 @@ __global__ void __launch_bounds__(attn_warps(D, NT) * 32, 1) kv4_attn_kernel(con
       if (!final_here)
         part[row] = m, part[RC + row] = l;
       else if (kW && it.r0 + row < p.rows)
-        put_lse(it, it.r0 + row, m, l);
+        put_norm(it, it.r0 + row, m, inv);
     }
     __syncwarp();
     if ((parts >> lane & 1) != 0) from[__popc(parts & ((1u << lane) - 1u))] = s_from[lane];
@@ -954,7 +954,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(const Kv4Attn
   for (int j = 0; j < 4; ++j) {
     if (r + j >= rows) continue;
     p.out[attn_row_at<D>(p, it, it.r0 + r + j, p.ldo) + col] = l[j] != 0.f ? v[j] / l[j] : 0.f;
-    if (kW && col == 0) attn_put_lse(p, c, it, it.r0 + r + j, m[j], l[j]);
+    if (kW && col == 0) attn_put_norm(p, c, it, it.r0 + r + j, m[j], l[j] != 0.f ? 1.f / l[j] : 0.f);
   }
 }
 
@@ -966,7 +966,7 @@ constexpr int kWeightThreads = 256, kWeightFewRows = 8;
 
 template <int kWeightSlots>
 __global__ void __launch_bounds__(kWeightThreads) kv4_weights_kernel(const Kv4Attn p, const Kv4View c, int blocks) {
-  __shared__ float s_lse[kWeightThreads];
+  __shared__ float2 s_norm[kWeightThreads];
   pdl_wait_prior();
   pdl_launch_dependents();
   const int tid = threadIdx.x, bh = blockIdx.x / blocks, b = bh / c.n_kv;
@@ -988,15 +988,19 @@ __global__ void __launch_bounds__(kWeightThreads) kv4_weights_kernel(const Kv4At
   for (int chunk = 0, r0 = 0; chunk < p.chunks; ++chunk, r0 += p.chunk_rows) {  // at most 80 rows
     const int rows = min(p.chunk_rows, p.rows - r0);
     __syncthreads();
-    if (tid < rows) s_lse[tid] = p.lse[static_cast<long long>(bh) * p.rows + r0 + tid];
+    if (tid < rows) s_norm[tid] = p.norm[static_cast<long long>(bh) * p.rows + r0 + tid];
     __syncthreads();
     const float* s = p.score + (static_cast<long long>(bh) * p.chunks + chunk) * p.kept_rows * c.cap + j0 + tid;
-    #pragma unroll 4
+    constexpr int kAhead = kWeightSlots == 1 ? 4 : 8;  // rows in flight; the other way round the two calls take 59.8 and 35.1 us
+    #pragma unroll kAhead
     for (int r = 0; r < rows; ++r) {
-      const float lse = s_lse[r];
+      const float2 norm = s_norm[r];
       #pragma unroll
-      for (int i = 0; i < kWeightSlots; ++i)
-        if (r0 + r >= skip[i]) got[i] += ex2(__ldg(s + i * kWeightThreads) - lse);
+      for (int i = 0; i < kWeightSlots; ++i) {
+        float score = -INFINITY;
+        if (r0 + r >= skip[i]) score = __ldg(s + i * kWeightThreads);
+        got[i] = fmaf(ex2(score + norm.x), norm.y, got[i]);
+      }
       s += c.cap;
     }
   }

@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, 1) kv4_attn_rows_kernel(const
         part[r] = s_max[r], part[RC + r] = l;
       } else {
         s_fac[r] = l != 0.f ? 1.f / l : 0.f;
-        if (kW && r < rows) attn_put_lse(p, c, run, run.r0 + r, s_max[r], l);
+        if (kW && r < rows) attn_put_norm(p, c, run, run.r0 + r, s_max[r], s_fac[r]);
       }
     }
     if (!whole) {

@@ -165,9 +165,9 @@ int kv4_prepare_attn(Ctx* ctx, Kv4Attn* p, const Kv4View& v, int nt, int d, int 
     if (static_cast<double>(heads) * p->chunks * p->kept_rows * static_cast<double>(v.cap) > 2.5e11)
       return fail(VMLM_ERR_SHAPE, "kv4_attn_dev: the scores of a call with w_out take %.3g bytes",
                   4.0 * static_cast<double>(heads) * p->chunks * p->kept_rows * static_cast<double>(v.cap));
-    VMLM_TRY(ensure(ctx->kv4_lse, heads * p->rows * 4));
+    VMLM_TRY(ensure(ctx->kv4_norm, heads * p->rows * sizeof(float2)));
     VMLM_TRY(ensure(ctx->kv4_score, heads * p->chunks * p->kept_rows * static_cast<size_t>(v.cap) * 4));
-    p->lse = static_cast<float*>(ctx->kv4_lse.p);
+    p->norm = static_cast<float2*>(ctx->kv4_norm.p);
     p->score = static_cast<float*>(ctx->kv4_score.p);
   }
   return VMLM_OK;

@@ -162,8 +162,8 @@ struct Ctx {
   DevBuf h_a, h_c, h_w, h_s, h_acc, h_b, h_g;  // host-API staging
   DevBuf xn;  // RMSNorm-fused Q8 calls: the normalised activations [M][K]
   // attention over a 4-bit cache: the CTAs' partial results, which of them an
-  // item has, scores and log2 of each row's sum
-  DevBuf kv4_part, kv4_split, kv4_score, kv4_lse;
+  // item has, scores, and each row's maximum and sum
+  DevBuf kv4_part, kv4_split, kv4_score, kv4_norm;
   DevBuf grp_planes;  // grouped Q8 batches in planes mode: every problem's planes, exponents and flags
   // host-pointer calls pipelined by row chunks: copies in and out on streams of
   // their own, ordered against the compute stream by events
@@ -2180,7 +2180,7 @@ int vmlm_shutdown(void) {
     for (DevBuf* b : {&c->act, &c->small, &c->slots, &c->counters, &c->shard_done, &c->sync, &c->norm_terms,
                       &c->norm_dirty, &c->norm_flags, &c->f32_ta, &c->f32_tb, &c->f32_da, &c->f32_db, &c->f32_nfa,
                       &c->f32_nfb, &c->f32_nft, &c->f32_flags, &c->h_a, &c->h_c, &c->h_w, &c->h_s, &c->h_acc, &c->h_b, &c->h_g, &c->xn,
-                      &c->grp_planes, &c->kv4_part, &c->kv4_split, &c->kv4_score, &c->kv4_lse})
+                      &c->grp_planes, &c->kv4_part, &c->kv4_split, &c->kv4_score, &c->kv4_norm})
       release(*b);
     cudaFree(c->err);
     cudaFreeHost(c->err_host);

@@ -289,3 +289,45 @@ def test_attention_hidden_values_that_are_not_finite(kernels, d, group, m, n_seq
             if weights:
                 tol = ((2 * ds + 2.0 ** -18)[:, None] * p).sum(0) + 2.0 ** -22 * p.sum(0) + 1e-12
                 assert (np.abs(w_out[b, h].cpu().numpy()[:n] - p.sum(0)) <= tol).all(), (b, h)
+
+
+# ------------------------------------------------- scores at the end of the f32 range
+
+#: d, query heads a kv head, sequences, kv heads, slots: one to sixteen rows a warp, items shared by warps and by CTAs, the
+#: kernel for many rows of 256
+SCORE_CASES = [(64, 1, 1, 2, 50), (64, 12, 1, 1, 6000), (128, 4, 2, 2, 333), (128, 7, 1, 1, 9000), (256, 2, 1, 2, 700),
+               (256, 32, 8, 2, 3000)]
+
+
+def _one_sign(d, group, n_seq, n_kv, n, size, scale):
+    """Attention with weights where every key is positive and every query has the sign of `size`, so that all scores have
+    it, and one slot of each head is far ahead of the others (by more than a thousandth of the scores). Returns the output
+    [n_seq, n_kv, group, d], the weight that was added [n_seq, n_kv, n], and the slot and its values [n_seq, n_kv, d]."""
+    torch = _torch()
+    rng = np.random.default_rng(d + n)
+    host, _ = _random_cache(rng, n_seq, n_kv, n, d, [n] * n_seq)
+    (kc, ks, kb), (vc, vs, vb) = host
+    ks[:], kb[:] = rng.uniform(0.1, 2.0, ks.shape).astype(np.float16), np.float16(0.5)
+    best = rng.integers(0, n - 1, (n_seq, n_kv))
+    for b in range(n_seq):
+        for h in range(n_kv):
+            ks[b, h, best[b, h]] = np.float16(5.0 if size * scale > 0 else 0.0)
+    cache = K.Kv4Cache(_up(kc[..., 0::2] | (kc[..., 1::2] << 4)), _up(vc[..., 0::2] | (vc[..., 1::2] << 4)),
+                       _up(np.stack((ks, kb), -1)), _up(np.stack((vs, vb), -1)))
+    q = (size * rng.uniform(0.5, 1.0, (n_seq, n_kv * group * d))).astype(np.float32)
+    out = torch.full((n_seq, n_kv * group * d), 7.0, device="cuda")
+    w = torch.full((n_seq, n_kv, n), 7.0, device="cuda")
+    st = torch.cuda.current_stream()
+    K.kv4_attn_dev(cache, _up(q), _up(np.full(n_seq, n, np.int32)), out, 1, n_kv * group, scale, w_out=w, stream=st)
+    K.sync(st)
+    v = np_values(vc, vs, vb)
+    return (out.cpu().numpy().reshape(n_seq, n_kv, group, d), w.cpu().numpy(), best,
+            np.take_along_axis(v, best[..., None, None], 2)[:, :, 0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", SCORE_CASES)
+def test_attention_scores_of_minus_infinity(kernels, case):
+    """Every score overflows to -inf: nothing is left to weigh, for the output and for the weights alike."""
+    out, w, _, _ = _one_sign(*case, size=-3e38, scale=1.0)
+    assert (out == 0).all() and (w == 0).all()
