@@ -45,7 +45,8 @@ struct Kv4Attn {
   float2* norm;       // [n_seq][n_kv][rows]: what is added to a score to be the exponent of a weight, 1 / the weights' sum
   float* part;        // two partial results a CTA: m, l, O of a chunk of rows
   int2* split;        // [n_seq][n_kv][chunks]: the first CTA of an item and how many have a part of it (one: the output is there)
-  float scale2;       // scale * log2(e)
+  float scale_m;      // scale * log2(e) = scale_m * 2^scale_e, 1 <= |scale_m| < 2 (or 0, or not finite)
+  int scale_e;
   int m, n_q, group, rows;  // rows = m * group query rows a kv head
   int chunks, chunk_rows;   // in chunks of a multiple of 4
   int kept_rows;            // of a chunk among the kept scores: chunk_rows and what a kernel rounds them up to
@@ -55,8 +56,13 @@ struct Kv4Attn {
 };
 
 constexpr int kAttnStageBytes = 5120;    // 4096 values of K and of V with their steps and bases
-constexpr float kAttnShift = 14.f;       // weights are held as 2^14 times their value: their halves keep 2^-39 of the largest
-constexpr float kAttnSlack = 1.f;        // a running maximum may lag by this (log2): 2^15 is still a half
+// A row's weights are 2^(score - top), in log2 units. top is the integer from 13 to 14 below the running maximum, so the largest
+// weight lies between 2^13 and 2^14 and halves keep 2^-38 of it, or up to 2^15, still a half, before top is moved. Integers,
+// so that differences of tops, and what one part's weights are multiplied by to join another's, are exact; and where
+// scores are so large (2^24) that f32 has no such integer, top is rounded up: a weight then is smaller, never above 2^15.
+constexpr float kAttnBelow = 14.f, kAttnRoom = 15.f;
+__device__ __forceinline__ float attn_top(float best) { return __fadd_ru(ceilf(best), -kAttnBelow); }
+__device__ __forceinline__ float attn_limit(float top) { return __fadd_rd(top, kAttnRoom); }  // scores above it move top
 constexpr int kAttnAlone = 4;            // tiles a warp up to which a CTA may take an item alone
 
 // Warps of the one CTA on an SM. A chunk of rows takes D/8 registers a four rows
@@ -161,12 +167,11 @@ __device__ __forceinline__ float kv4_weight(uint32_t hi, uint32_t lo, int odd) {
   return odd ? __high2float(bits_h2(hi)) + __high2float(bits_h2(lo)) : __low2float(bits_h2(hi)) + __low2float(bits_h2(lo));
 }
 
-// A query row as B fragments of its halves, a power of two apart from the row so
-// that its largest value lies in [1, 2), with the scale's sign in it. Lane (gid,
-// tig) has columns tig * D/4 .. of row gid / 2 of four: hi for even gid, lo for
-// odd. Returns what a score has to be multiplied by to be in log2 units.
+// A query row as B fragments of its halves: the row times the scale, a power of two apart from that so that its largest value
+// lies in [1, 4). Lane (gid, tig) has columns tig * D/4 .. of row gid / 2 of four: hi for even gid, lo for odd. Returns the
+// power of two that a score has to be multiplied by to be in log2 units, exactly.
 template <int D>
-__device__ __forceinline__ float attn_query(const float* src, bool vec, float scale2, uint32_t (&qb)[D / 16][2]) {
+__device__ __forceinline__ float attn_query(const float* src, bool vec, float scale_m, int scale_e, uint32_t (&qb)[D / 16][2]) {
   const int gid = (threadIdx.x & 31) >> 2, tig = threadIdx.x & 3;
   float x[D / 4];
   if (src) {
@@ -181,7 +186,7 @@ __device__ __forceinline__ float attn_query(const float* src, bool vec, float sc
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
   const int e = min(max(static_cast<int>((__float_as_uint(top) >> 23) & 255) - 127, -120), 120);
-  const float down = copysignf(__uint_as_float(static_cast<uint32_t>(127 - e) << 23), scale2);
+  const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23) * scale_m;
   #pragma unroll
   for (int w = 0; w < D / 32; ++w) {
     #pragma unroll
@@ -193,7 +198,7 @@ __device__ __forceinline__ float attn_query(const float* src, bool vec, float sc
     }
   }
   // not 0, or a hidden slot's -inf would become a NaN
-  return fmaxf(__uint_as_float(static_cast<uint32_t>(127 + e) << 23) * fabsf(scale2), 1e-37f);
+  return __uint_as_float(static_cast<uint32_t>(min(max(e + scale_e, -126), 127) + 127) << 23);
 }
 
 // Where a slot's 16-byte chunk c of codes lies in its row in shared memory: the
@@ -333,8 +338,8 @@ __device__ __forceinline__ long long attn_row_at(const Kv4Attn& p, const AttnRun
   return (static_cast<long long>(s.b) * p.m + t) * ld + static_cast<long long>(s.head * p.group + row - t * p.group) * D;
 }
 __device__ __forceinline__ void attn_put_norm(const Kv4Attn& p, const Kv4View& c, const AttnRun& s, int row, float m, float inv) {
-  // not the log of the sum: nothing is lost between two large numbers, and a row without a weight gives every slot 0
-  p.norm[(static_cast<long long>(s.b) * c.n_kv + s.head) * p.rows + row] = make_float2(kAttnShift - m, inv);
+  // not the log of the sum: a row without a weight gives every slot 0, and weights are what the output was made with
+  p.norm[(static_cast<long long>(s.b) * c.n_kv + s.head) * p.rows + row] = make_float2(-m, inv);
 }
 
 // An item's first run says which CTAs have parts of it: shares of `each` tiles, one more for the first `extra` CTAs.
@@ -519,7 +524,7 @@ __global__ void __launch_bounds__(attn_warps(D, NT) * 32, 1) kv4_attn_kernel(con
     #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int r = r0 + nt * 4 + (gid >> 1), rt = r0 + nt * 4 + tig;
-      const float up = attn_query<D>(r < p.rows ? p.q + row_at(run, r, p.ldq) : nullptr, p.vec, p.scale2, qb[nt]);
+      const float up = attn_query<D>(r < p.rows ? p.q + row_at(run, r, p.ldq) : nullptr, p.vec, p.scale_m, p.scale_e, qb[nt]);
       sc[nt] = __shfl_sync(0xffffffffu, up, 8 * tig);
       vis[nt] = rt < p.rows ? run.n - (p.m - 1 - token(rt)) : 0;
     }
@@ -627,23 +632,22 @@ __global__ void __launch_bounds__(attn_warps(D, NT) * 32, 1) kv4_attn_kernel(con
         #pragma unroll
         for (int u = 0; u < ST; ++u) best = fmaxf(best, fmaxf(s[u][0][nt], s[u][1][nt]));
         best *= sc[nt];
-        if (__any_sync(0xffffffffu, best > top[nt] + kAttnSlack)) {
+        if (__any_sync(0xffffffffu, best > attn_limit(top[nt]))) {
           best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 4));
           best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 8));
           best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 16));
-          best = fmaxf(best, top[nt]);
+          best = fmaxf(attn_top(best), top[nt]);
           const float f = ex2(top[nt] - best);
           top[nt] = best;
           sum[nt] *= f;
           #pragma unroll
           for (int i = 0; i < OT; ++i) o[i][0][nt] *= f, o[i][1][nt] *= f;
         }
-        const float off = kAttnShift - top[nt];
         #pragma unroll
         for (int u = 0; u < ST; ++u) {
           #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float e = ex2(fmaf(s[u][h][nt], sc[nt], off));
+            const float e = ex2(fmaf(s[u][h][nt], sc[nt], -top[nt]));
             sum[nt] += e;
             const float big = __uint_as_float(__float_as_uint(e) & 0xFFFFE000u);
             pb[u][nt][h] = transpose8x8(h2_bits(__floats2half2_rn(big, e - big)));

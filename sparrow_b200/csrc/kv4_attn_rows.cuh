@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, 1) kv4_attn_rows_kernel(const
     for (int nt = warp; nt < NT; nt += kRowsWarps) {
       const int r = nt * 4 + (gid >> 1);
       uint32_t qb[2 * KW][2];
-      const float up = attn_query<D>(r < rows ? p.q + attn_row_at<D>(p, run, run.r0 + r, p.ldq) : nullptr, p.vec, p.scale2, qb);
+      const float up = attn_query<D>(r < rows ? p.q + attn_row_at<D>(p, run, run.r0 + r, p.ldq) : nullptr, p.vec, p.scale_m, p.scale_e, qb);
       #pragma unroll
       for (int w = 0; w < KW; ++w)
         qs[(nt * KW + w) * 32 + lane] = make_uint4(qb[2 * w][0], qb[2 * w][1], qb[2 * w + 1][0], qb[2 * w + 1][1]);
@@ -151,13 +151,13 @@ __global__ void __launch_bounds__(kRowsWarps * 32, 1) kv4_attn_rows_kernel(const
       }
     }
     const int n0 = share * NG;  // the first four of rows of this warp's scores
-    // of a row: what a score is multiplied by, kAttnShift - its maximum so far, the score from which that has grown
-    float sc[NG], off[NG], grow[NG], sum[NG];
+    // of a row: what a score is multiplied by, its top so far, the score from which that moves
+    float sc[NG], top[NG], grow[NG], sum[NG];
     const int all_see = run.n - (p.m - 1 - attn_token(p, run.r0));  // slots that every row sees (rows that are not there: any)
     __syncthreads();
     #pragma unroll
     for (int i = 0; i < NG; ++i)
-      sc[i] = s_scale[(n0 + i) * 4 + tig], off[i] = kAttnShift + 1e30f, grow[i] = -3e38f, sum[i] = 0.f;
+      sc[i] = s_scale[(n0 + i) * 4 + tig], top[i] = -1e30f, grow[i] = -3e38f, sum[i] = 0.f;
     float o[2][NT];
     #pragma unroll
     for (int i = 0; i < NT; ++i) o[0][i] = o[1][i] = 0.f;
@@ -245,10 +245,9 @@ __global__ void __launch_bounds__(kRowsWarps * 32, 1) kv4_attn_rows_kernel(const
         #pragma unroll
         for (int i = 0; i < NG; ++i) {
           const int r = (n0 + i) * 4 + tig;
-          const float best = fmaxf(fmaxf(fmaxf(s_max[r], s_max[RC + r]), fmaxf(s_max[2 * RC + r], s_max[3 * RC + r])),
-                                   kAttnShift - off[i]);
-          const float now = kAttnShift - best, f = ex2(now - off[i]);
-          off[i] = now, grow[i] = best > -1e30f ? (best + kAttnSlack) / sc[i] : -3e38f, sum[i] *= f;
+          const float best = fmaxf(fmaxf(s_max[r], s_max[RC + r]), fmaxf(s_max[2 * RC + r], s_max[3 * RC + r]));
+          const float now = fmaxf(attn_top(best), top[i]), f = ex2(top[i] - now);
+          top[i] = now, grow[i] = now > -1e30f ? attn_limit(now) / sc[i] : -3e38f, sum[i] *= f;
           if (st == 0 && gid == 0) s_fac[r] = f;
         }
         if (st == 0 && lane == 0) s_grown[parity][share] = 1;
@@ -258,7 +257,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, 1) kv4_attn_rows_kernel(const
         uint32_t pb[2];
         #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float e = ex2(fmaf(s[h][i], sc[i], off[i]));
+          const float e = ex2(fmaf(s[h][i], sc[i], -top[i]));
           sum[i] += e;
           const float big = __uint_as_float(__float_as_uint(e) & 0xFFFFE000u);
           pb[h] = transpose8x8(h2_bits(__floats2half2_rn(big, e - big)));
@@ -347,7 +346,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, 1) kv4_attn_rows_kernel(const
       const int r = (n0 + i) * 4 + tig;
       if (gid == 0) {
         s_sum[st * RC + r] = sum[i];
-        if (st == 0) s_max[r] = kAttnShift - off[i];
+        if (st == 0) s_max[r] = top[i];
       }
     }
     __syncthreads();

@@ -371,7 +371,9 @@ int vmlm_kv4_attn_dev(const vmlm_kv4* cache, const float* q, size_t ldq, const i
   cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
   Kv4Attn p = {};
   p.q = q, p.out = out, p.ldq = ldq, p.ldo = ldo, p.len = len, p.w_in = w_in, p.w_out = w_out;
-  p.scale2 = scale * 1.44269504088896340736f;
+  int e = 0;
+  p.scale_m = static_cast<float>(2 * std::frexp(scale * 1.44269504088896340736, &e));
+  p.scale_e = std::isfinite(scale) ? e - 1 : 0;
   p.m = static_cast<int>(m), p.n_q = static_cast<int>(n_q);
   p.group = static_cast<int>(n_q / cache->n_kv);
   p.rows = p.m * p.group;

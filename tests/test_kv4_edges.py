@@ -331,3 +331,31 @@ def test_attention_scores_of_minus_infinity(kernels, case):
     """Every score overflows to -inf: nothing is left to weigh, for the output and for the weights alike."""
     out, w, _, _ = _one_sign(*case, size=-3e38, scale=1.0)
     assert (out == 0).all() and (w == 0).all()
+
+
+def _check_one_slot(case, size, scale):
+    """The slot in front has all of the weight: its lead is above 2^-10 of the scores, and ds below 2^-16 of them."""
+    d, group = case[:2]
+    out, w, best, v = _one_sign(*case, size=size, scale=scale)
+    assert (np.abs(out - v[:, :, None]) <= 2.0 ** -18 * np.abs(v).max()).all()
+    for b in range(w.shape[0]):
+        for h in range(w.shape[1]):
+            want = np.zeros(w.shape[2])
+            want[best[b, h]] = group
+            assert (np.abs(w[b, h] - want) <= 2.0 ** -18 * want).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", SCORE_CASES)
+@pytest.mark.parametrize("size", [3e3, 1e5, 3e6, 1e8, 1e12, 1e30, -3e5, -1e8])
+def test_attention_scores_of_any_size(kernels, case, size):
+    """Scores whose neighbours in f32 lie further apart than a weight's room to grow."""
+    _check_one_slot(case, size, 0.125)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", SCORE_CASES)
+def test_attention_with_a_scale_that_is_no_number(kernels, case):
+    """softmax(NaN) is NaN, in the output and in the weights."""
+    out, w, _, _ = _one_sign(*case, size=1.0, scale=float("nan"))
+    assert np.isnan(out).all() and np.isnan(w).all()
