@@ -140,27 +140,19 @@ __device__ __forceinline__ uint32_t kv4_pair(uint32_t u, uint32_t mul, __half2 s
 }
 
 // Values of slots that some rows of a chunk see and others do not. A hidden slot's weight is 0, but 0 times a NaN or an
-// infinity is NaN, and a product takes a slot's values for all rows: slots whose values are not finite (of one group of 32
-// columns; judged by the smallest and the largest code's value) leave the product, and the rows that see them get them
-// by scalar operations. This is looked for only in tiles that a row of the chunk sees in part.
-__device__ __forceinline__ bool kv4_infinite(__half2 step, __half2 base) {  // of the low half
-  const uint32_t lo = h2_bits(__hfma2(__float2half2_rn(16.f), step, base)), hi = h2_bits(__hfma2(__float2half2_rn(31.f), step, base));
-  return (lo & 0x7C00u) == 0x7C00u || (hi & 0x7C00u) == 0x7C00u;
+// infinity is NaN, and a product takes a slot's values for all rows: where values of one slot and group of 32 columns are
+// not finite (judged by the smallest and the largest code's), their step and base become zeros in shared memory, and the
+// rows that see them get them by scalar operations once the tile is done. This is looked for only in tiles that a row of
+// the chunk sees in part, and there first by a test that all usual values pass: a step below 1024, a base below 32768.
+__device__ __forceinline__ bool kv4_large(uint32_t sb) { return (((sb & 0x7FFF7FFFu) + 0x08001C00u) & 0x80008000u) != 0; }
+__device__ __forceinline__ bool kv4_infinite(uint32_t sb) {
+  const __half2 step = __low2half2(bits_h2(sb)), base = __high2half2(bits_h2(sb));
+  const uint32_t x = h2_bits(__hfma2(__floats2half2_rn(16.f, 31.f), step, base)) & 0x7C007C00u;
+  return (x & 0x7C00u) == 0x7C00u || x >> 16 == 0x7C00u;
 }
-// Bits 15 and 31: whether any of the pairs seen so far may be so: a step of 1024 or a base of 32768 and more.
-__device__ __forceinline__ uint32_t kv4_large(uint32_t seen, __half2 steps, __half2 bases) {
-  return seen | ((h2_bits(steps) & 0x7FFF7FFFu) + 0x1C001C00u) | ((h2_bits(bases) & 0x7FFF7FFFu) + 0x08000800u);
-}
-// Two slots' steps and bases (halves of a register each), made zero where they are not finite and `from` (0 for both, 1 for
-// the second, 2 for none) allows it: the values become zeros. Returns which, as bits 0 and 1.
-__device__ __forceinline__ uint32_t kv4_take_out(__half2& step, __half2& base, int from) {
-  const bool a = from <= 0 && kv4_infinite(step, base), b = from <= 1 && kv4_infinite(__lowhigh2highlow(step), __lowhigh2highlow(base));
-  const uint32_t keep = (a ? 0u : 0xFFFFu) | (b ? 0u : 0xFFFF0000u);
-  step = bits_h2(h2_bits(step) & keep), base = bits_h2(h2_bits(base) & keep);
-  return (a ? 1u : 0u) | (b ? 2u : 0u);
-}
-__device__ __forceinline__ float kv4_value(uint32_t word, int nibble, __half2 sb) {
-  return __half2float(__hfma(__float2half_rn(16.f + static_cast<float>(word >> 4 * nibble & 15u)), __low2half(sb), __high2half(sb)));
+__device__ __forceinline__ float kv4_value(uint32_t word, int nibble, uint32_t sb) {
+  const __half2 x = bits_h2(sb);
+  return __half2float(__hfma(__float2half_rn(16.f + static_cast<float>(word >> 4 * nibble & 15u)), __low2half(x), __high2half(x)));
 }
 // A weight from its halves: slot `odd` of two in the fragments of a row's hi and lo.
 __device__ __forceinline__ float kv4_weight(uint32_t hi, uint32_t lo, int odd) {
@@ -547,6 +539,18 @@ __global__ void __launch_bounds__(attn_warps(D, NT) * 32, 1) kv4_attn_kernel(con
       __syncwarp();
       const unsigned char* st = ring + stage * kAttnStageBytes;
       const int left = run.s1 - at;
+      bool unsafe = false;
+      if (kSeveral && all_see < run.n && at + TS > all_see) {  // a row may not see slots that others do
+        uint32_t* sb = reinterpret_cast<uint32_t*>(ring + stage * kAttnStageBytes + 4608 + lane * 16);
+        const uint4 x = *reinterpret_cast<const uint4*>(sb);
+        unsafe = __any_sync(0xffffffffu, kv4_large(x.x) || kv4_large(x.y) || kv4_large(x.z) || kv4_large(x.w));
+        if (unsafe) {
+          #pragma unroll 1
+          for (int i = 0; i < 4; ++i)
+            if ((lane * 4 + i) / (D / 32) >= all_see - at && kv4_infinite(sb[i])) sb[i] = 0;
+          __syncwarp();
+        }
+      }
       // scores (times sc: in log2 units)
       float s[ST][2][NT];
       #pragma unroll
@@ -679,48 +683,6 @@ __global__ void __launch_bounds__(attn_warps(D, NT) * 32, 1) kv4_attn_kernel(con
           bas[u][h] = bits_h2(__byte_perm(x, y, 0x7632));
         }
       }
-      bool unsafe = false;
-      if (kSeveral && all_see < run.n && at + TS > all_see) {  // a row may not see slots that others do
-        uint32_t large = 0;
-        #pragma unroll
-        for (int u = 0; u < ST; ++u) large = kv4_large(kv4_large(large, stp[u][0], bas[u][0]), stp[u][1], bas[u][1]);
-        unsafe = __any_sync(0xffffffffu, large & 0x80008000u);
-      }
-      if (__builtin_expect(unsafe, 0)) {
-        uint32_t out_of[(TS + 31) / 32] = {};
-        #pragma unroll
-        for (int u = 0; u < ST; ++u)
-          #pragma unroll
-          for (int h = 0; h < 2; ++h)
-            out_of[u / 2] |= kv4_take_out(stp[u][h], bas[u][h], all_see - at - (u * 16 + h * 8 + 2 * tig)) << (u % 2 * 16 + h * 8 + 2 * tig);
-        #pragma unroll
-        for (int i = 0; i < (TS + 31) / 32; ++i) {
-          #pragma unroll 1
-          for (uint32_t bad = __reduce_or_sync(0xffffffffu, out_of[i]); bad; bad &= bad - 1) {
-            const int in = __ffs(bad) - 1, slot = 32 * i + in;
-            const __half2 sb = *reinterpret_cast<const __half2*>(st + 4608 + slot * (D / 8) + gid * VW / 4 * 4);
-            const bool mine = kv4_infinite(__low2half2(sb), __high2half2(sb));
-            const uint32_t* words = reinterpret_cast<const uint32_t*>(
-                st + 2048 + slot * (D / 2) + attn_swizzle<D>(slot, v_in / 16) * 16 + v_in % 16);
-            #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              uint32_t both = 0;
-              #pragma unroll
-              for (int x = 0; x < 4 && 2 * i + x / 2 < ST; ++x)  // eights of a word of slots (an index would put pb into memory)
-                both |= pb[2 * i + x / 2][nt][x % 2] & -static_cast<uint32_t>(in / 8 == x);
-              const int from = 8 * tig + in % 8 / 2;
-              const uint32_t hi = __shfl_sync(0xffffffffu, both, from), lo = __shfl_sync(0xffffffffu, both, from + 4);
-              if (!mine || at + slot >= vis[nt]) continue;
-              const float w = kv4_weight(hi, lo, in & 1);
-              #pragma unroll
-              for (int t = 0; t < OT; ++t)
-                #pragma unroll
-                for (int h = 0; h < 2; ++h)
-                  o[t][h][nt] += w * kv4_value(words[VW == 1 ? 0 : t / 8 * 2 + h], VW == 1 ? 4 * h + t : t % 8, sb);
-            }
-          }
-        }
-      }
       // Tiles 2 y and 2 y + 1 are the low and the high nibbles of one byte of the words: d = 64, columns 8 gid + n and
       // 8 gid + 4 + n of the lane's word (n = tile); else columns n of words 2 w and 2 w + 1 of the lane's words
       // (tile = 8 w + n).
@@ -759,6 +721,31 @@ __global__ void __launch_bounds__(attn_warps(D, NT) * 32, 1) kv4_attn_kernel(con
           for (int nt = 0; nt < NT; ++nt) {
             o[2 * y + z][0][nt] += acc[z][nt][0] + acc[z][nt][1];
             o[2 * y + z][1][nt] += acc[z][nt][2] + acc[z][nt][3];
+          }
+        }
+      }
+      if (unsafe) {  // what was taken out of the products
+        #pragma unroll 1
+        for (int slot = max(all_see - at, 0); slot < min(left, TS); ++slot) {
+          const uint32_t sb = __ldg(c.vs + (row0 + at + slot) * (D / kKv4Group) + gid * VW / 4);
+          const bool mine = kv4_infinite(sb);
+          if (!__any_sync(0xffffffffu, mine)) continue;
+          const uint32_t* words = reinterpret_cast<const uint32_t*>(
+              st + 2048 + slot * (D / 2) + attn_swizzle<D>(slot, v_in / 16) * 16 + v_in % 16);
+          #pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            uint32_t both = 0;  // not pb[slot ..]: an index would put it into memory
+            #pragma unroll
+            for (int x = 0; x < 2 * ST; ++x) both |= pb[x / 2][nt][x % 2] & -static_cast<uint32_t>(slot / 8 == x);
+            const int from = 8 * tig + slot % 8 / 2;
+            const uint32_t hi = __shfl_sync(0xffffffffu, both, from), lo = __shfl_sync(0xffffffffu, both, from + 4);
+            if (!mine || at + slot >= vis[nt]) continue;
+            const float w = kv4_weight(hi, lo, slot & 1);
+            #pragma unroll
+            for (int t = 0; t < OT; ++t)
+              #pragma unroll
+              for (int h = 0; h < 2; ++h)
+                o[t][h][nt] += w * kv4_value(words[VW == 1 ? 0 : t / 8 * 2 + h], VW == 1 ? 4 * h + t : t % 8, sb);
           }
         }
       }

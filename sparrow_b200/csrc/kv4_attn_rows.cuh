@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, 1) kv4_attn_rows_kernel(const
   float* s_sum = s_fac + RC;                                                        // [4][RC]
   float* s_scale = s_sum + 4 * RC;                                                  // [RC]
   int* s_see = reinterpret_cast<int*>(s_scale + RC);                                // [RC]: slots that a row sees
-  __shared__ int s_grown[2][4];  // a part's maxima grew in a tile: by the tile's parity
+  __shared__ int s_grown[2][5];  // by a tile's parity: a part's maxima grew; values were taken out of the products (4)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int gid = lane >> 2, tig = lane & 3;
   const int st = warp & 3, share = warp >> 2;           // scores: slots 16 st .., fours share * NG ..
@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, 1) kv4_attn_rows_kernel(const
   fetch(row0 + run.s0, run.s1 - run.s0, 0);
   cp_async_commit();
   int stage = 0, parity = 0;
-  if (tid < 8) s_grown[tid >> 2][tid & 3] = 0;
+  if (tid < 10) s_grown[tid / 5][tid % 5] = 0;
 
   while (true) {
     const bool more = walk.next(nxt);
@@ -171,6 +171,11 @@ __global__ void __launch_bounds__(kRowsWarps * 32, 1) kv4_attn_rows_kernel(const
       cp_async_commit();
       const unsigned char* tile = smem + stage * kStage;
       const int left = run.s1 - at;
+      const bool partly = all_see < run.n && at + TS > all_see;  // a row may not see slots that others do
+      if (partly) {
+        uint32_t* sb = reinterpret_cast<uint32_t*>(smem + stage * kStage + kVsAt) + tid;
+        if (kv4_large(*sb) && tid / (D / 32) >= all_see - at && kv4_infinite(*sb)) *sb = 0, s_grown[parity][4] = 1;
+      }
 
       // scores of 16 slots and a part of the rows
       float acc[NG][4];
@@ -277,19 +282,16 @@ __global__ void __launch_bounds__(kRowsWarps * 32, 1) kv4_attn_rows_kernel(const
           }
         }
       }
-      if (tid < 4) s_grown[parity ^ 1][tid] = 0;  // read last before this tile's first barrier
+      if (tid < 5) s_grown[parity ^ 1][tid] = 0;  // read last before this tile's first barrier
       // Tile 8 w + n is columns n of words 2 w and 2 w + 1 of the lane's; odd tiles are high nibbles.
-      uint32_t a[4][4], out_of[2] = {};
-      const bool partly = all_see < run.n && at + TS > all_see;  // a row may not see slots that others do
+      uint32_t a[4][4];
       #pragma unroll
       for (int u = 0; u < 4; ++u) {
         #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const unsigned char* pc = tile + vs_at + (u * 16 + h * 8) * (D / 8);
           const uint32_t x = *reinterpret_cast<const uint32_t*>(pc), y = *reinterpret_cast<const uint32_t*>(pc + D / 8);
-          __half2 step = bits_h2(__byte_perm(x, y, 0x5410)), base = bits_h2(__byte_perm(x, y, 0x7632));
-          if (partly)
-            out_of[u / 2] |= kv4_take_out(step, base, all_see - at - (u * 16 + h * 8 + 2 * tig)) << (u % 2 * 16 + h * 8 + 2 * tig);
+          const __half2 step = bits_h2(__byte_perm(x, y, 0x5410)), base = bits_h2(__byte_perm(x, y, 0x7632));
           #pragma unroll
           for (int z = 0; z < 2; ++z) {
             const int byte = ot % 8 / 2, off = (u * 16 + h * 8) * (D / 2) + (ot / 8 * 2 + z) * 4;
@@ -313,24 +315,20 @@ __global__ void __launch_bounds__(kRowsWarps * 32, 1) kv4_attn_rows_kernel(const
         }
         o[0][i] += d[0] + d[1], o[1][i] += d[2] + d[3];
       }
-      if (partly) {
+      if (partly && s_grown[parity][4]) {
         #pragma unroll 1
-        for (int k = 0; k < 2; ++k) {
-          #pragma unroll 1
-          for (uint32_t bad = __reduce_or_sync(0xffffffffu, k ? out_of[1] : out_of[0]); bad; bad &= bad - 1) {
-            const int slot = 32 * k + __ffs(bad) - 1;
-            const __half2 sb = *reinterpret_cast<const __half2*>(tile + kVsAt + slot * (D / 8) + gid * VW / 4 * 4);
-            if (!kv4_infinite(__low2half2(sb), __high2half2(sb))) continue;
-            const uint32_t* words = reinterpret_cast<const uint32_t*>(
-                tile + kVAt + slot * (D / 2) + attn_swizzle<D>(slot, v_in / 16) * 16 + v_in % 16) + ot / 8 * 2;
-            const float v0 = kv4_value(words[0], ot % 8, sb), v1 = kv4_value(words[1], ot % 8, sb);
-            const uint32_t* from = reinterpret_cast<const uint32_t*>(ps + slot / 16 * NT * 32 + 8 * tig + slot % 8 / 2) + slot / 8 % 2;
-            #pragma unroll
-            for (int i = 0; i < NT; ++i) {
-              if (at + slot >= s_see[i * 4 + tig]) continue;
-              const float w = kv4_weight(from[i * 64], from[i * 64 + 8], slot & 1);
-              o[0][i] += w * v0, o[1][i] += w * v1;
-            }
+        for (int slot = max(all_see - at, 0); slot < min(left, TS); ++slot) {
+          const uint32_t sb = __ldg(c.vs + (row0 + at + slot) * (D / kKv4Group) + gid * VW / 4);
+          if (!kv4_infinite(sb)) continue;
+          const uint32_t* words = reinterpret_cast<const uint32_t*>(
+              tile + kVAt + slot * (D / 2) + attn_swizzle<D>(slot, v_in / 16) * 16 + v_in % 16) + ot / 8 * 2;
+          const float v0 = kv4_value(words[0], ot % 8, sb), v1 = kv4_value(words[1], ot % 8, sb);
+          const uint32_t* from = reinterpret_cast<const uint32_t*>(ps + slot / 16 * NT * 32 + 8 * tig + slot % 8 / 2) + slot / 8 % 2;
+          #pragma unroll
+          for (int i = 0; i < NT; ++i) {
+            if (at + slot >= s_see[i * 4 + tig]) continue;
+            const float w = kv4_weight(from[i * 64], from[i * 64 + 8], slot & 1);
+            o[0][i] += w * v0, o[1][i] += w * v1;
           }
         }
       }
