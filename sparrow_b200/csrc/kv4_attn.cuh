@@ -61,6 +61,7 @@ constexpr int kAttnStageBytes = 5120;    // 4096 values of K and of V with their
 // so that differences of tops, and what one part's weights are multiplied by to join another's, are exact; and where
 // scores are so large (2^24) that f32 has no such integer, top is rounded up: a weight then is smaller, never above 2^15.
 constexpr float kAttnBelow = 14.f, kAttnRoom = 15.f;
+constexpr float kAttnNone = -3.402823466e38f;  // of no scores: finite, so that what joins parts is a number
 __device__ __forceinline__ float attn_top(float best) { return __fadd_ru(ceilf(best), -kAttnBelow); }
 __device__ __forceinline__ float attn_limit(float top) { return __fadd_rd(top, kAttnRoom); }  // scores above it move top
 constexpr int kAttnAlone = 4;            // tiles a warp up to which a CTA may take an item alone
@@ -525,7 +526,7 @@ __global__ void __launch_bounds__(attn_warps(D, NT) * 32, 1) kv4_attn_kernel(con
     float top[NT], sum[NT], o[OT][2][NT];
     #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      top[nt] = -1e30f, sum[nt] = 0.f;
+      top[nt] = kAttnNone, sum[nt] = 0.f;
       #pragma unroll
       for (int i = 0; i < OT; ++i) o[i][0][nt] = 0.f, o[i][1][nt] = 0.f;
     }
@@ -833,7 +834,7 @@ __global__ void __launch_bounds__(attn_warps(D, NT) * 32, 1) kv4_attn_kernel(con
     int* from = s_at + warp * 32;         // [part]
     if (parts >> lane & 1) from[__popc(parts & ((1u << lane) - 1u))] = lane;
     __syncwarp();
-    float m = -1e30f, l = 0.f;
+    float m = kAttnNone, l = 0.f;
     for (int i = group; i < count; i += kGroups) m = fmaxf(m, ml[(from[i] * RC + row) * 2]);
     #pragma unroll
     for (int x = kRowLanes; x < 32; x *= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
@@ -902,7 +903,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(const Kv4Attn
   AttnRun it;
   it.b = b, it.head = hc / p.chunks, it.r0 = (hc - it.head * p.chunks) * p.chunk_rows;
   const int rows = min(p.chunk_rows, p.rows - it.r0);
-  float m[4] = {-1e30f, -1e30f, -1e30f, -1e30f}, l[4] = {}, v[4] = {};
+  float m[4] = {kAttnNone, kAttnNone, kAttnNone, kAttnNone}, l[4] = {}, v[4] = {};
   constexpr int kAhead = 5;
   #pragma unroll 1
   for (int k0 = warp; k0 < s.y; k0 += kAhead * kJoinWarps) {

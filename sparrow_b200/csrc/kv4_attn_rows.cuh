@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, 1) kv4_attn_rows_kernel(const
     __syncthreads();
     #pragma unroll
     for (int i = 0; i < NG; ++i)
-      sc[i] = s_scale[(n0 + i) * 4 + tig], top[i] = -1e30f, grow[i] = -3e38f, sum[i] = 0.f;
+      sc[i] = s_scale[(n0 + i) * 4 + tig], top[i] = kAttnNone, grow[i] = -INFINITY, sum[i] = 0.f;
     float o[2][NT];
     #pragma unroll
     for (int i = 0; i < NT; ++i) o[0][i] = o[1][i] = 0.f;
@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, 1) kv4_attn_rows_kernel(const
           const int r = (n0 + i) * 4 + tig;
           const float best = fmaxf(fmaxf(s_max[r], s_max[RC + r]), fmaxf(s_max[2 * RC + r], s_max[3 * RC + r]));
           const float now = fmaxf(attn_top(best), top[i]), f = ex2(top[i] - now);
-          top[i] = now, grow[i] = now > -1e30f ? attn_limit(now) / sc[i] : -3e38f, sum[i] *= f;
+          top[i] = now, grow[i] = now > kAttnNone ? attn_limit(now) / sc[i] : -INFINITY, sum[i] *= f;
           if (st == 0 && gid == 0) s_fac[r] = f;
         }
         if (st == 0 && lane == 0) s_grown[parity][share] = 1;

@@ -359,3 +359,11 @@ def test_attention_with_a_scale_that_is_no_number(kernels, case):
     """softmax(NaN) is NaN, in the output and in the weights."""
     out, w, _, _ = _one_sign(*case, size=1.0, scale=float("nan"))
     assert np.isnan(out).all() and np.isnan(w).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", SCORE_CASES)
+@pytest.mark.parametrize("size", [-1e28, -1e30, -3e33])
+def test_attention_scores_far_below_zero(kernels, case, size):
+    """Scores down to -1e37: the largest of them still leads."""
+    _check_one_slot(case, size, 0.125)
