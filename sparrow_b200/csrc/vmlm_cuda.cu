@@ -91,8 +91,7 @@ struct DevBuf {
 int ensure(DevBuf& b, size_t bytes) {
   if (bytes == 0) bytes = 16;
   if (b.bytes >= bytes) return VMLM_OK;
-  size_t nb = b.bytes * 2 > bytes ? b.bytes * 2 : bytes;
-  nb = (nb + 255) & ~static_cast<size_t>(255);
+  const size_t had = b.bytes;
   if (b.p && b.captured != g_captured) {
     try {
       b.kept.emplace_back(b.p, b.bytes);
@@ -104,8 +103,20 @@ int ensure(DevBuf& b, size_t bytes) {
   }
   b.p = nullptr;
   b.bytes = 0;
-  VMLM_CUDA(cudaMalloc(&b.p, nb));
-  b.bytes = nb;
+  // Twice the old size, so that growing stays rare, or what is needed where that does not fit.
+  for (size_t want : {std::max(2 * had, bytes), bytes}) {
+    want = (want + 255) & ~static_cast<size_t>(255);
+    const cudaError_t e = cudaMalloc(&b.p, want);
+    if (e == cudaSuccess) {
+      b.bytes = want;
+      break;
+    }
+    b.p = nullptr;
+    cudaGetLastError();
+    if (e != cudaErrorMemoryAllocation || want - bytes < 256)
+      return fail(e == cudaErrorMemoryAllocation ? VMLM_ERR_OOM : VMLM_ERR_CUDA, "a workspace of %zu bytes: %s", bytes,
+                  cudaGetErrorString(e));
+  }
   b.captured = g_captured;
   return VMLM_OK;
 }

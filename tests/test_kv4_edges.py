@@ -367,3 +367,42 @@ def test_attention_with_a_scale_that_is_no_number(kernels, case):
 def test_attention_scores_far_below_zero(kernels, case, size):
     """Scores down to -1e37: the largest of them still leads."""
     _check_one_slot(case, size, 0.125)
+
+
+# ------------------------------------------------- workspaces
+
+@pytest.mark.gpu
+def test_workspace_grows_into_what_is_left(kernels):
+    """A call that needs a little more workspace than the one before it runs where that fits, although twice the old size
+    (what the library asks for, so that growing stays rare) does not."""
+    torch = _torch()
+    rng = np.random.default_rng(3)
+    d, n_seq, n_kv, group, cap = 64, 2, 4, 4, 4000
+    m = 512
+    _, cache = _random_cache(rng, n_seq, n_kv, cap, d, [cap] * n_seq, bad=False)
+    st = torch.cuda.current_stream()
+    w = torch.zeros((n_seq, n_kv, cap), device="cuda")
+    lens = _up(np.full(n_seq, cap, np.int32))
+
+    def call(m):
+        q = torch.ones((n_seq * m, n_kv * group * d), device="cuda")
+        out = torch.empty_like(q)
+        K.kv4_attn_dev(cache, q, lens, out, m, n_kv * group, 0.1, w_out=w, stream=st)
+        K.sync(st)
+        return out
+
+    K.sync(st)
+    K.shutdown()  # the workspaces of earlier tests go
+    K.init(0)
+    call(m)  # scores: 2 * 4 * 2048 rows * 4000 slots * 4 bytes = 262 MB
+    torch.cuda.empty_cache()
+    need = n_seq * n_kv * (m + 64) * group * cap * 4
+    free = torch.cuda.mem_get_info()[0]
+    old = n_seq * n_kv * m * group * cap * 4
+    held = torch.empty(free + old - need - (96 << 20), dtype=torch.uint8, device="cuda")  # all but what is needed and 96 MB
+    try:
+        out = call(m + 64)
+        assert torch.isfinite(out).all()
+    finally:
+        del held
+        torch.cuda.empty_cache()
