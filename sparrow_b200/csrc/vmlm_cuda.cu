@@ -92,31 +92,37 @@ int ensure(DevBuf& b, size_t bytes) {
   if (bytes == 0) bytes = 16;
   if (b.bytes >= bytes) return VMLM_OK;
   const size_t had = b.bytes;
-  if (b.p && b.captured != g_captured) {
+  const bool keep = b.p && b.captured != g_captured;
+  if (keep) {
     try {
-      b.kept.emplace_back(b.p, b.bytes);
+      b.kept.reserve(b.kept.size() + 1);
     } catch (const std::bad_alloc&) {
       return fail(VMLM_ERR_OOM, "no host memory");
     }
   } else if (b.p) {
     VMLM_CUDA(cudaFree(b.p));
+    b.p = nullptr;
+    b.bytes = 0;
   }
-  b.p = nullptr;
-  b.bytes = 0;
-  // Twice the old size, so that growing stays rare, or what is needed where that does not fit.
+  // Twice the old size, so that growing stays rare, or what is needed where that does not fit. A buffer that is to be kept
+  // stays in use if neither can be had (inside a capture nothing can).
+  void* p = nullptr;
+  size_t got = 0;
   for (size_t want : {std::max(2 * had, bytes), bytes}) {
     want = (want + 255) & ~static_cast<size_t>(255);
-    const cudaError_t e = cudaMalloc(&b.p, want);
+    const cudaError_t e = cudaMalloc(&p, want);
     if (e == cudaSuccess) {
-      b.bytes = want;
+      got = want;
       break;
     }
-    b.p = nullptr;
     cudaGetLastError();
     if (e != cudaErrorMemoryAllocation || want - bytes < 256)
       return fail(e == cudaErrorMemoryAllocation ? VMLM_ERR_OOM : VMLM_ERR_CUDA, "a workspace of %zu bytes: %s", bytes,
                   cudaGetErrorString(e));
   }
+  if (keep) b.kept.emplace_back(b.p, b.bytes);
+  b.p = p;
+  b.bytes = got;
   b.captured = g_captured;
   return VMLM_OK;
 }
@@ -1295,7 +1301,8 @@ int run_bf16_norm(Ctx* c, const float* a, const uint16_t* b, float* out, int M, 
                   cudaStream_t st, const Bf16Plan* force = nullptr) {
   const size_t tbytes = static_cast<size_t>(3) * M * kp * 2;
   if (M != c->norm_m || kp != c->norm_kp) {
-    // a new layout: planes and dirty bits start over at zero
+    // a new layout: planes and dirty bits start over at zero (and none holds if that fails)
+    c->norm_m = -1;
     VMLM_TRY(ensure(c->norm_terms, tbytes));
     VMLM_TRY(ensure(c->norm_dirty, static_cast<size_t>(M)));
     VMLM_CUDA(cudaMemsetAsync(c->norm_terms.p, 0, tbytes, st));
@@ -1379,7 +1386,8 @@ int run_f32(Ctx* c, const float* a, const float* b, float* out, int M, int N, in
   const int kp = static_cast<int>(cdiv(K, 64) * 64);  // a k-block never runs into the next term
   const size_t ta_bytes = static_cast<size_t>(3) * M * kp * 2, tb_bytes = static_cast<size_t>(3) * N * kp * 2;
   if (M != c->f32_m || N != c->f32_n || kp != c->f32_kp) {
-    // a new layout: planes and dirty bits start over at zero
+    // a new layout: planes and dirty bits start over at zero (and none holds if that fails)
+    c->f32_m = -1;
     VMLM_TRY(ensure(c->f32_ta, ta_bytes));
     VMLM_TRY(ensure(c->f32_tb, tb_bytes));
     VMLM_TRY(ensure(c->f32_da, static_cast<size_t>(M)));

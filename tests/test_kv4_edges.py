@@ -406,3 +406,63 @@ def test_workspace_grows_into_what_is_left(kernels):
     finally:
         del held
         torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", ["bf16", "f32", "attention"])
+def test_a_call_that_cannot_grow_leaves_the_workspace(kernels, what):
+    """A larger call inside a capture is an error, and calls of the old size go on as before, behind a graph that holds the
+    workspace and without one."""
+    torch = _torch()
+    K.sync()
+    K.shutdown()
+    K.init(0)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+    n, k = 256, 512
+    _, cache = _random_cache(np.random.default_rng(1), 2, 4, 600, 64, [600] * 2, bad=False)
+    length = _up(np.array([600, 77], np.int32))
+    wb = (torch.randn((n, k), generator=g, device="cuda") * 0.05).to(torch.bfloat16)
+    wf = wb.float()
+
+    def make(m):
+        if what == "attention":
+            q = torch.randn((2 * m, 4 * 64), generator=g, device="cuda")
+            out, w = torch.empty_like(q), torch.zeros((2, 4, 600), device="cuda")
+            return [out, w], lambda st: K.kv4_attn_dev(cache, q, length, out, m, 4, 0.1, w_out=w, stream=st)
+        x, y = torch.randn((m, k), generator=g, device="cuda"), torch.empty((m, n), device="cuda")
+        if what == "bf16":
+            return [y], lambda st: K.gemm_nt_bf16_dev(x, wb, y, m, n, k, stream=st)
+        return [y], lambda st: K.gemm_nt_f32_dev(x, wf, y, m, n, k, stream=st)
+
+    cuda = ctypes.CDLL("libcuda.so.1")
+    outs, step = make(200)
+    _, larger = make(4000)
+    st = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    step(st)
+    K.sync(st)
+    ref = [x.clone() for x in outs]
+    for held in (False, True):
+        if held:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=st):
+                step(st)
+                step(st)
+        handle, made = ctypes.c_void_p(st.cuda_stream), ctypes.c_void_p()
+        assert cuda.cuStreamBeginCapture_v2(handle, 1) == 0  # of this thread
+        with pytest.raises(VmlmError):
+            larger(st)
+        assert cuda.cuStreamEndCapture(handle, ctypes.byref(made)) == 901 and not made.value  # the capture is void
+        torch.cuda.synchronize()
+        for _ in range(2):
+            for x in outs:
+                x.zero_()
+            torch.cuda.synchronize()
+            step(st)
+            K.sync(st)
+            assert all(torch.equal(x, r) for x, r in zip(outs, ref))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, r) for x, r in zip(outs, ref))
+    del graph
