@@ -344,7 +344,8 @@ VMLM_API int vmlm_qk_norm_rope_dev(const float *q, size_t ldq, const float *k, s
 /* The same for q (n_q = 0: none) and k, and the m new tokens of each sequence
  * (rows b * m + t) written to slots len[b] + t in 4 bits, v as it is. len is
  * not changed; len[b] < 0 marks an idle sequence, for which nothing is
- * written to the cache. A slot behind cap is not written and is reported by
+ * written to the cache; its queries are written where their positions lie in the
+ * table, and no position outside it is reported. A slot behind cap is not written and is reported by
  * vmlm_sync. qo may be q (same stride) and may share no other memory with q, k
  * or v. */
 VMLM_API int vmlm_kv4_append_dev(const vmlm_kv4 *cache, const float *q, size_t ldq, float *qo, size_t ldqo,

@@ -252,7 +252,8 @@ __global__ void __launch_bounds__(256, 4) kv4_rows_kernel(const Kv4Rows p, const
   if (p.cos_t) {
     const long long row = __ldg(p.pos + tok);
     if (row < 0 || row >= p.n_pos) {
-      if (lane == 0) atomicCAS(err, 0, kDevRopePos);
+      // an idle sequence has no position
+      if (lane == 0 && !(kCache && __ldg(p.len + tok / static_cast<uint32_t>(p.m)) < 0)) atomicCAS(err, 0, kDevRopePos);
       return;
     }
     const float *ct = p.cos_t + row * half, *st = p.sin_t + row * half;

@@ -11,7 +11,7 @@ import pytest
 
 import sparrow_b200.kernels as K
 from sparrow_b200._lib import VmlmError
-from test_kv4 import EPS, _cache, _random_cache, _rc, _torch, _up, np_attention, np_values
+from test_kv4 import EPS, _cache, _random_cache, _rc, _tables, _torch, _up, np_attention, np_norm_rope, np_values
 
 
 # ------------------------------------------------- captured steps
@@ -466,3 +466,37 @@ def test_a_call_that_cannot_grow_leaves_the_workspace(kernels, what):
     torch.cuda.synchronize()
     assert all(torch.equal(x, r) for x, r in zip(outs, ref))
     del graph
+
+
+# ------------------------------------------------- idle sequences
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_append_asks_no_position_of_an_idle_sequence(kernels, d):
+    """Positions that follow the lengths, as a decode step has them: -1 for an idle sequence is no error, and one outside
+    the table of a sequence in use is one all the same."""
+    torch = _torch()
+    rng = np.random.default_rng(d)
+    n_seq, n_kv, cap = 4, 2, 9
+    _, cache = _random_cache(rng, n_seq, n_kv, cap, d, [cap] * n_seq, bad=False)
+    x = rng.standard_normal((n_seq, 3 * n_kv * d)).astype(np.float32)
+    length = np.array([3, -1, 8, -7], np.int32)
+    tc, ts = _tables(cap, d)
+    before = cache.k.clone()
+    xd, g = _up(x), _up(np.ones(d, np.float32))
+    qo = torch.full((n_seq, n_kv * d), 7.0, device="cuda")
+    st = torch.cuda.current_stream()
+
+    def append(pos):
+        K.kv4_append_dev(cache, xd[:, n_kv * d:2 * n_kv * d], xd[:, 2 * n_kv * d:], _up(length), 1, q=xd[:, :n_kv * d], qo=qo,
+                         n_q=n_kv, gq=g, gk=g, eps=EPS, rope=K.Rope(_up(tc), _up(ts), _up(pos)), stream=st)
+        K.sync(st)
+
+    append(length)
+    got = qo.cpu().numpy()
+    ref = np_norm_rope(x[[0, 2], :n_kv * d].reshape(2, n_kv, d), np.ones(d, np.float32), tc[[3, 8]], ts[[3, 8]], False)
+    assert np.abs(got[[0, 2]].reshape(ref.shape) - ref).max() < 1e-5 and (got[[1, 3]] == 7).all()
+    assert torch.equal(cache.k[[1, 3]], before[[1, 3]]) and not torch.equal(cache.k[0, :, 3], before[0, :, 3])
+    with pytest.raises(VmlmError) as e:
+        append(np.array([3, -1, 9, -1], np.int32))
+    assert e.value.status == 8 and "position" in str(e.value)
