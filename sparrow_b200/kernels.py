@@ -432,11 +432,13 @@ _F32 = None  # torch.float32, once a tensor of it has been seen
 def _rows_ptr(x, rows, width, name):
     """(address, row stride) of a [rows, >= width] float32 CUDA tensor whose rows may be slices of wider ones."""
     global _F32
-    if x.dtype is not _F32:
-        if _dtype_name(x.dtype) != "float32":
+    try:
+        if not x.is_cuda or (x.dtype is not _F32 and _dtype_name(x.dtype) != "float32"):
             raise ValueError(f"{name}: expected a float32 CUDA tensor")
-        _F32 = x.dtype
-    if x.dim() != 2 or not x.is_cuda:
+    except AttributeError:
+        raise ValueError(f"{name}: expected a float32 CUDA tensor, got {type(x).__name__}") from None
+    _F32 = x.dtype
+    if x.dim() != 2:
         raise ValueError(f"{name}: expected a CUDA tensor of rows")
     (n, w), (ld, step) = x.shape, x.stride()
     if n < rows or w < width or (step != 1 and w > 1):
@@ -448,9 +450,12 @@ def _ptr(x, dtype_name, count, name):
     """_dev_ptr for the calls of a decode step, whose host time counts: a plain address."""
     if x is None or isinstance(x, int):
         return x
-    if not x.is_cuda or _dtype_name(x.dtype) != dtype_name or x.numel() < count or not x.is_contiguous():
-        return _dev_ptr(x, dtype_name, count, name)  # says what is wrong
-    return x.data_ptr()
+    try:
+        if x.is_cuda and _dtype_name(x.dtype) == dtype_name and x.numel() >= count and x.is_contiguous():
+            return x.data_ptr()
+    except AttributeError:
+        pass
+    return _dev_ptr(x, dtype_name, count, name)  # says what is wrong
 
 
 class Rope:

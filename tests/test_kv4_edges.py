@@ -500,3 +500,20 @@ def test_append_asks_no_position_of_an_idle_sequence(kernels, d):
     with pytest.raises(VmlmError) as e:
         append(np.array([3, -1, 9, -1], np.int32))
     assert e.value.status == 8 and "position" in str(e.value)
+
+
+# ------------------------------------------------- what is no tensor on the GPU
+
+@pytest.mark.parametrize("bad", [None, np.zeros((1, 64), np.float32), [0.0] * 64, 1.5])
+def test_python_says_which_argument_is_no_cuda_tensor(bad):
+    from types import SimpleNamespace
+    c = SimpleNamespace(n_seq=1, n_kv=1, cap=4, d=64, ref=None)
+    for call in (lambda: K.kv4_attn_dev(c, bad, 8, bad, 1, 1, 0.1), lambda: K.kv4_append_dev(c, bad, bad, 8, 1),
+                 lambda: K.qk_norm_rope_dev(bad, None, None, None, EPS, None, bad, None, 1, 1, 0, 64)):
+        with pytest.raises(ValueError, match="^[qk]: expected a float32 CUDA tensor"):
+            call()
+    if bad is not None:
+        with pytest.raises(ValueError, match="^start: "):
+            K.kv4_read_dev(c, bad, 8, 1, 16, 16)
+        with pytest.raises(ValueError, match="^w: "):
+            K.kv4_evict_dev(c, c, bad, 8, 1, 0, 0, 8, None, 8)
