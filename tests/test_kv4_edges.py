@@ -11,7 +11,7 @@ import pytest
 
 import sparrow_b200.kernels as K
 from sparrow_b200._lib import VmlmError
-from test_kv4 import EPS, _cache, _random_cache, _rc, _tables, _torch, _up, np_attention, np_norm_rope, np_values
+from test_kv4 import EPS, _cache, _random_cache, _rc, _tables, _torch, _up, np_attention, np_keep, np_norm_rope, np_values
 
 
 # ------------------------------------------------- captured steps
@@ -517,3 +517,45 @@ def test_python_says_which_argument_is_no_cuda_tensor(bad):
             K.kv4_read_dev(c, bad, 8, 1, 16, 16)
         with pytest.raises(ValueError, match="^w: "):
             K.kv4_evict_dev(c, c, bad, 8, 1, 0, 0, 8, None, 8)
+
+
+# ------------------------------------------------- eviction from shares that outgrow shared memory
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["spread", "ties", "late"])
+def test_eviction_keys_read_again(kernels, kind):
+    """More heads than SMs, so that one CTA has all of a head: 24576 of its keys lie in shared memory and those behind are
+    read again in every pass. Lengths on both sides of that, ties across it, all of the weight behind it."""
+    torch = _torch()
+    rng = np.random.default_rng(len(kind))
+    n_seq, n_kv, d, cap, keep, first, recent = 150, 1, 64, 24700, 300, 4, 20
+    lens = rng.integers(24570, cap + 1, n_seq).astype(np.int32)
+    lens[:6] = [24576, 24577, 24575, cap, 300, 0]
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+    codes = lambda n: [torch.randint(0, 256, (n_seq, n_kv, n, d // 2), generator=g, device="cuda", dtype=torch.uint8)  # noqa: E731
+                       for _ in range(2)]
+    scales = lambda n: [torch.randn((n_seq, n_kv, n, d // 32, 2), generator=g, device="cuda").half() for _ in range(2)]  # noqa: E731
+    src, dst = K.Kv4Cache(*codes(cap), *scales(cap)), K.Kv4Cache(*codes(keep), *scales(keep))
+    w = rng.random((n_seq, n_kv, cap)).astype(np.float32)
+    if kind == "ties":
+        w = np.where(w < 0.995, 0.0, np.where(np.arange(cap) < 24500, np.float32(0.5), np.float32(0.25))).astype(np.float32)
+        w[:, :, 24560:24600] = 0.25
+    elif kind == "late":
+        w[:, :, :24570] *= 1e-6
+    idx = torch.empty((n_seq, n_kv, keep), dtype=torch.int32, device="cuda")
+    w_out = torch.empty((n_seq, n_kv, keep), device="cuda")
+    len_out = torch.empty(n_seq, dtype=torch.int32, device="cuda")
+    st = torch.cuda.current_stream()
+    K.kv4_evict_dev(src, dst, _up(w), _up(lens), keep, first, recent, idx, w_out, len_out, stream=st)
+    K.sync(st)
+    assert np.array_equal(len_out.cpu().numpy(), np.minimum(lens, keep))
+    ix, wo = idx.cpu().numpy()[:, 0], w_out.cpu().numpy()[:, 0]
+    for b in range(n_seq):
+        at = np_keep(w[b, 0], int(lens[b]), keep, first, recent)
+        assert np.array_equal(ix[b, :len(at)], at) and (ix[b, len(at):] == -1).all(), b
+        assert np.array_equal(wo[b, :len(at)], w[b, 0, at]) and (wo[b, len(at):] == 0).all(), b
+        t = torch.from_numpy(at).cuda()
+        for x, y in ((src.k, dst.k), (src.v, dst.v), (src.ks.view(torch.int16), dst.ks.view(torch.int16)),
+                     (src.vs.view(torch.int16), dst.vs.view(torch.int16))):
+            assert torch.equal(y[b, 0, :len(at)], x[b, 0, t]), b
