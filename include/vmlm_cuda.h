@@ -364,17 +364,22 @@ VMLM_API int vmlm_kv4_read_dev(const vmlm_kv4 *cache, const int32_t *start, cons
  * out, n_q heads, n_q / n_kv of them to a kv head): token t sees the slots
  * j < len[b] - (m - 1 - t), len[b] counting the m tokens themselves.
  * A slot that a token does not see has no part in its output, whatever bits it
- * holds (a NaN among the newest values reaches the tokens that see it).
+ * holds; a NaN or an infinity in a value reaches the tokens that see it, as
+ * one of the two.
  *   out = sum_j p_j v_j, p = softmax(scale * q . k_j); no visible slot: zeros.
  * With w_out ([n_seq][n_kv][cap]), the weight that each slot received is
  * accumulated: w_out[j] = w_in[j] + the sum of p_j over the tokens and the kv
  * head's query heads for j < len[b] (w_in counts as 0 for the m newest slots
  * and where it is NULL; w_in and w_out may be the same). Other slots of w_out
  * are not written. out may not overlap q. A len above cap is taken as cap and reported by vmlm_sync.
- * Sums are f32; products with cached values are exact. With w_out the call
- * holds n_seq * n_kv * cap scores a query row of a kv head in workspace
- * (f32; rows rounded up to a multiple of 4): a prompt's last tokens are a
- * cheaper source of weights than all of them. */
+ * Sums are f32. Queries are held as two halves (22 bits of a row's largest
+ * value), softmax weights as two (21 bits, and down to 2^-38 of a row's
+ * largest); products of these with cached values are exact. With w_out the call
+ * holds n_seq * n_kv * cap scores a query row of a kv head in workspace (f32;
+ * rows rounded up to even chunks of a multiple of 4, for 25 rows and more of
+ * d = 256 to chunks of 32, 48, 64 or 80): a prompt's last tokens are a cheaper
+ * source of weights than all of them. Every chunk of rows walks all slots of
+ * its sequence, those that none of its tokens sees too. */
 VMLM_API int vmlm_kv4_attn_dev(const vmlm_kv4 *cache, const float *q, size_t ldq, const int32_t *len, float *out,
                                size_t ldo, size_t m, size_t n_q, float scale, const float *w_in, float *w_out,
                                void *stream);

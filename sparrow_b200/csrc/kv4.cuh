@@ -8,9 +8,9 @@
 // (step, base) of two halves, step in the low one. A code c stands for
 //     half(step * (16 + c) + base),
 // one rounding. 16 + c because a nibble placed in the top four mantissa bits of
-// the half 16.0 (0x4C00) is the half 16 + c: unpacking costs a shift and one
-// LOP3 for two values, and one HFMA2 makes them the halves that the tensor
-// cores take, so a product with a cached value is exact. Rounding the value
+// the half 16.0 (0x4C00) is the half 16 + c: unpacking costs a LOP3 and a shift or
+// a multiply-add for two values, and one HFMA2 makes them the halves that the
+// tensor cores take, so a product with a cached value is exact. Rounding the value
 // to a half costs at most 2^-11 of it, where half a code step is about 1/30 of
 // the group's range; halves for step and base make 5 bits a value in all.
 //
@@ -216,8 +216,10 @@ __device__ __forceinline__ void load4(const float* p, bool vec, float* x) {
 // Bound by HBM (each value is read once and written once) and nearly as much by
 // instructions: the root and the tree count for 256 / d rows, the token's table
 // rows and addresses for all steps. While a step is computed the next one's rows
-// are on their way. 2047 tokens of 40 heads of 128, half rotated: 19.5 us, 4.3 TB/s;
-// 8191 tokens written to a cache: 86 us, 4.5 TB/s.
+// are on their way. 2047 tokens of 40 heads of 128, half rotated: 19.4 us, 4.3 TB/s
+// (47% of issue slots); 8191 tokens of 48 heads written to a cache: 77 us, 4.6 TB/s
+// (62%). In both the warps wait for loads most often (2.4 of 8 to 11 warp-cycles an
+// instruction), then for fixed latencies and shuffles.
 template <int D, bool kCache>
 __global__ void __launch_bounds__(256, 4) kv4_rows_kernel(const Kv4Rows p, const Kv4View c,
                                                                        int* __restrict__ err) {
@@ -378,8 +380,8 @@ __device__ __forceinline__ void kv4_unpack(uint32_t w, __half2 step, __half2 bas
 
 // Values as halves: a thread takes code words (8 columns) of K and of V. Rows
 // start[b] + i, i < count; a row at or behind end[b] reads as zeros. Bound by
-// the halves it writes (4 d bytes a slot against 1.25 d read). Grid: (words,
-// n_seq * n_kv).
+// the halves it writes (4 d bytes a slot against 1.25 d read): 64 heads of 4096 rows
+// of 128 take 29 us, 6.0 TB/s. Grid: (words, n_seq * n_kv).
 constexpr int kReadWords = 2;  // of K, and as many of V, that a thread has in flight
 
 template <int D>
@@ -442,7 +444,9 @@ constexpr int kEvictThreads = 1024;
 constexpr int kEvictMaxCluster = 8;
 constexpr int kEvictBins = 2048;   // 11 bits a pass of the radix select: 11, 11, 10
 constexpr int kEvictKeys = 24 * 1024;  // keys that a CTA's shared memory holds, two CTAs on an SM
-constexpr int kEvictShare = 4096;      // slots a CTA from which a cluster is made larger (1024: 36 heads of 1100 take 16.5 us, not 12.4)
+// Slots a CTA from which a cluster is made larger. 8 heads of 16384 slots take 24.1 us with 4096, 25.7 with 2048, 29.6 with
+// 8192; 32 heads of 8192: 22.9, 24.3, 26.2; 16 heads of 6000: 16.2, 16.7, 15.3.
+constexpr int kEvictShare = 4096;
 
 // Shared memory: a histogram, the scans' words, the CTA's keys (and later its kept slots).
 __host__ __device__ constexpr int evict_smem_bytes(int keys) { return kEvictBins * 4 + 256 + keys * 4; }
@@ -503,7 +507,8 @@ __device__ __forceinline__ void cluster_sync() {
 // Then every CTA knows what it keeps and where its first kept slot goes, and
 // moves its rows. Bound by HBM for long caches (4 bytes a slot, 2.5 d a kept
 // one), by the passes' barriers for short ones: 36 heads of 1100 slots of 64, 512
-// kept, 12.4 us; 64 heads of up to 32768 slots of 128, 4096 kept, 79 us.
+// kept, 9.9 us; 64 heads of up to 32768 slots of 128, 4096 kept, 49 us, where warps
+// wait for loads and barriers in turn and DRAM is busy 24% of the time.
 template <int D>
 __global__ void __launch_bounds__(kEvictThreads, 2)
     kv4_evict_kernel(const Kv4Evict p, const Kv4View src, const Kv4View dst, int* __restrict__ err) {

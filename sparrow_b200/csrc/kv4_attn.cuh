@@ -19,14 +19,14 @@
 //   scores  S^T[slot][row]  = K[slot][d] . q[d][row]     A rows: slots
 //   output  O^T[d][row]     = V^T[d][slot] . P[slot][row] A rows: columns of V
 // V^T comes without a transpose: A's register holds one column of two slots,
-// and one PRMT pairs the halves of two slots' code words, after which a shift
-// and a LOP3 give both slots' nibbles of one column. Which column of V is which
+// and one PRMT pairs the bytes of two slots' code words, after which a LOP3 and
+// a multiply-add give both slots' nibbles of one column. Which column of V is which
 // row of A, and which column of K and q is which k, is free, and chosen so that
 // each lane takes whole words. S^T leaves the tensor core with a row's hi and lo
 // sums in one lane; P goes back through movmatrix, an 8 x 8 transpose.
 //
-// Measured: 8 kv heads of 4 rows, d = 128, 131071 slots: 41.2 us = 4.1 TB/s of codes; 48 ragged sequences of up to 8192
-// slots: 55.8 us = 4.5 TB/s; 36 heads of one row, d = 64, 777 slots: 8.4 us, of which 2 are the launch and the loads'
+// Measured: 8 kv heads of 4 rows, d = 128, 131071 slots: 41.3 us = 4.1 TB/s of codes; 48 ragged sequences of up to 8192
+// slots: 56.2 us = 4.5 TB/s; 36 heads of one row, d = 64, 777 slots: 8.3 us, of which 2 are the launch and the loads'
 // latency most of the rest. With few rows the loads in flight bound it (two tiles a warp), with many the instructions of
 // the softmax: about 25 for two scores a lane.
 #pragma once
@@ -222,7 +222,9 @@ struct AttnRun {
 
 // The shares are counted in units: an item is its tiles, and before them `cost` units for what a run costs besides
 // (its queries and its result), so that short items do not gather in one share.
-constexpr int kAttnRunCost = 2;  // of a warp here: 48 ragged sequences take 55.8 us, with 1 56.6
+// Of a warp here. 16 ragged sequences of up to 4000 slots, 8 x 8 heads of 128: 28.5 us with 1, 23.9 with 2, 23.4 with 3; 64 of
+// up to 1000, 2 x 4 heads of 256: 19.6, 18.0, 17.8; 200 of up to 600, 8 heads of 64: 23.6, 23.9, 25.2.
+constexpr int kAttnRunCost = 2;
 
 template <int TS, int kCost>
 struct AttnWalk {
@@ -952,8 +954,9 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(const Kv4Attn
 
 // The weights that slots received, from the kept scores and the rows' sums: a thread has kWeightSlots slots, 256 apart, of
 // a kv head. Bound by the scores' reads (4 bytes a row and slot): four slots keep enough of them in flight for few rows (8 x
-// 8 heads of 4 rows, up to 16384 slots: the call takes 33.4 us, 3 less than with one slot), one slot makes enough blocks
-// where many rows do that (72 heads of 33 rows, 4097 slots: the call takes 56 us, 7 less than with four).
+// 8 heads of 4 rows, up to 16384 slots: the call takes 32.8 us, with one slot 35.1), one slot makes enough blocks where many
+// rows do that (8 x 8 heads of 16 rows, up to 4096 slots: 23.3 us, with four 25.3). At 8 rows they are close: 28.8 with four
+// and 28.7 with one for 8 x 8 heads of up to 8192 slots, 26.4 and 25.8 for 16 x 8 of up to 2000; at 12, 37.6 and 35.9.
 constexpr int kWeightThreads = 256, kWeightFewRows = 8;
 
 template <int kWeightSlots>

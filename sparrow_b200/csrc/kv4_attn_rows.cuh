@@ -10,7 +10,7 @@
 //   weights  to shared memory as B fragments, with a maximum shared by the tile
 //   output   each warp its 16 columns of V, V unpacked once, all slots, all rows
 // Three barriers a tile. What bounds it is the latency between them, with four
-// warps a scheduler (38% of issue slots, mma.sync 21% active; 80 rows over 16 ragged
+// warps a scheduler (35% of issue slots, mma.sync 21% active; 80 rows over 16 ragged
 // caches of up to 3001 slots take 46 us), then mma.sync (one m16n8k16 in two cycles an SM: 64 slots take
 // d * rows / 8 of them) and the B fragments' reads from shared memory (256 bytes
 // for one).

@@ -213,7 +213,9 @@ int kv4_launch_attn_rows(Ctx* ctx, Kv4Attn p, const Kv4View& v, cudaStream_t st)
 // its registers hold, in even chunks (16 x 8 heads of 8192 slots, 12 rows: 42 us as 12, 53 as 8 + 4). d = 256 holds 4
 // rows; there a CTA shares what it unpacks if rows and tiles a CTA are many: with 8 heads of 8192 slots and 16 sequences,
 // 28 rows take 412 us so and 435 by fours, 80 rows 743 and 1333, 20 rows 405 and 313; 80 rows over 16 ragged caches of
-// up to 3001 slots take 46 us and 53, over 32 of 1024 (3.5 tiles a CTA) 67 and 58. Its chunks of 80 rows leave too few
+// up to 3001 slots take 46 us and 53, over 32 of 1024 (3.5 tiles a CTA) 67 and 58, over 64 ragged ones of up to 1024 79 and
+// 80 (all full 108 and 105). The tiles are those of cap, which the host knows, not of the lengths: over 8 ragged caches of up
+// to 3001 slots (2.5 tiles a CTA) it would win by 29 against 34, over 8 full ones it ties (43). Its chunks of 80 rows leave too few
 // CTAs work below twice as many tiles (the ragged caches: 47.6 us as one chunk).
 template <int D, bool kW>
 int kv4_pick_attn(Ctx* ctx, const Kv4Attn& p, const Kv4View& v, cudaStream_t st) {
