@@ -559,3 +559,18 @@ def test_eviction_keys_read_again(kernels, kind):
         for x, y in ((src.k, dst.k), (src.v, dst.v), (src.ks.view(torch.int16), dst.ks.view(torch.int16)),
                      (src.vs.view(torch.int16), dst.vs.view(torch.int16))):
             assert torch.equal(y[b, 0, :len(at)], x[b, 0, t]), b
+
+
+# ------------------------------------------------- the example
+
+def test_decode_example_refuses_what_cannot_fit():
+    import importlib.util
+    import os
+
+    from conftest import ROOT
+    spec = importlib.util.spec_from_file_location("kv4_decode", os.path.join(ROOT, "examples", "kv4_decode.py"))
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    for bad in (dict(prompt=49, cap=48), dict(prompt=10, cap=48, keep=48), dict(tokens=0), dict(prompt=0)):
+        with pytest.raises(ValueError, match="the prompt has to fit"):
+            example.run(**bad)
