@@ -992,9 +992,9 @@ __global__ void __launch_bounds__(kWeightThreads) kv4_weights_kernel(const Kv4At
       const float2 norm = s_norm[r];
       #pragma unroll
       for (int i = 0; i < kWeightSlots; ++i) {
-        float score = -INFINITY;
-        if (r0 + r >= skip[i]) score = __ldg(s + i * kWeightThreads);
-        got[i] = fmaf(ex2(score + norm.x), norm.y, got[i]);
+        const bool sees = r0 + r >= skip[i];
+        const float score = sees ? __ldg(s + i * kWeightThreads) : 0.f, sum = fmaf(ex2(score + norm.x), norm.y, got[i]);
+        got[i] = sees ? sum : got[i];  // not 0 times what may be a NaN
       }
       s += c.cap;
     }

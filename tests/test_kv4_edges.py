@@ -574,3 +574,34 @@ def test_decode_example_refuses_what_cannot_fit():
     for bad in (dict(prompt=49, cap=48), dict(prompt=10, cap=48, keep=48), dict(tokens=0), dict(prompt=0)):
         with pytest.raises(ValueError, match="the prompt has to fit"):
             example.run(**bad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,group,m,n_seq,n_kv,cap", [(64, 1, 3, 1, 2, 300), (64, 2, 9, 2, 2, 2500), (128, 4, 4, 2, 2, 700),
+                                                      (256, 1, 5, 1, 2, 90), (256, 16, 5, 8, 2, 3000)])
+def test_weights_of_slots_that_a_query_of_nan_does_not_see(kernels, d, group, m, n_seq, n_kv, cap):
+    """The first token's query is NaN: its outputs are, and the weights of the slots that it sees; the newer tokens have
+    their outputs, and their own slots the weights that they give them."""
+    torch = _torch()
+    rng = np.random.default_rng(d + m)
+    host, cache = _random_cache(rng, n_seq, n_kv, cap, d, [cap] * n_seq)
+    q = rng.standard_normal((n_seq * m, n_kv * group * d)).astype(np.float32)
+    q[0::m] = np.nan
+    out = torch.empty((n_seq * m, n_kv * group * d), device="cuda")
+    w = torch.zeros((n_seq, n_kv, cap), device="cuda")
+    st = torch.cuda.current_stream()
+    K.kv4_attn_dev(cache, _up(q), _up(np.full(n_seq, cap, np.int32)), out, m, n_kv * group, 0.1, w_out=w, stream=st)
+    K.sync(st)
+    got, w = out.cpu().numpy().reshape(n_seq, m, n_kv, group, d), w.cpu().numpy()
+    assert np.isnan(got[:, 0]).all() and np.isnan(w[:, :, :cap - m + 1]).all()
+    q = q.reshape(n_seq, m, n_kv, group, d).astype(np.float64)
+    seen = np.repeat(cap - (m - 1 - np.arange(1, m)), group)
+    for b in range(n_seq):
+        for h in range(n_kv):
+            k, v = (np_values(c[b, h], s[b, h], x[b, h]) for c, s, x in host)
+            ref, p, ds = np_attention(q[b, 1:, h].reshape(-1, d), k, v, seen, 0.1)
+            y = got[b, 1:, h].reshape(-1, d)
+            assert (np.abs(y - ref) <= ((2 * ds + 2.0 ** -18) * np.abs(v).max())[:, None]).all(), (b, h)
+            new = slice(cap - m + 1, cap)
+            tol = ((2 * ds + 2.0 ** -18)[:, None] * p[:, new]).sum(0) + 2.0 ** -22 * p[:, new].sum(0) + 1e-12
+            assert (np.abs(w[b, h, new] - p[:, new].sum(0)) <= tol).all(), (b, h)
