@@ -142,7 +142,7 @@ __device__ __forceinline__ uint32_t kv4_pair(uint32_t u, uint32_t mul, __half2 s
 
 // Values of slots that some rows of a chunk see and others do not. A hidden slot's weight is 0, but 0 times a NaN or an
 // infinity is NaN, and a product takes a slot's values for all rows: where values of one slot and group of 32 columns are
-// not finite (judged by the smallest and the largest code's), their step and base become zeros in shared memory, and the
+// not finite (as the smallest and the largest code have it), their step and base become zeros in shared memory, and the
 // rows that see them get them by scalar operations once the tile is done. This is looked for only in tiles that a row of
 // the chunk sees in part, and there first by a test that all usual values pass: a step below 1024, a base below 32768.
 __device__ __forceinline__ bool kv4_large(uint32_t sb) { return (((sb & 0x7FFF7FFFu) + 0x08001C00u) & 0x80008000u) != 0; }
